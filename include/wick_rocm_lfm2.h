@@ -101,6 +101,54 @@ int wick_rocm_attention_prefill_quantize_q8_0(wick_rocm_ctx *ctx, const float *d
                                               const float *d_v_cache, int8_t *d_out_q, float *d_out_scales, uint32_t pos0, uint32_t n,
                                               uint32_t max_seq, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim);
 
+/* ---- a KV cache held in 4 bits ----
+ * 4.5 bits a value: 14 % of the memory of f32 rows and 28 % of that of f16 rows, for contexts whose caches are what fills the device or
+ * what a step waits for.  The reference's counterpart is its compressed cache (wick/src/turboquant.rs, 3-bit keys and 2-bit values with
+ * rotations and codebooks); this one holds plain blocks, like the weights.
+ *
+ * A cache of max_seq rows (n_kv_heads heads of head_dim values; 32, 64, 128 or 256) is one buffer of wick_rocm_kv_q4_bytes(...)
+ * bytes (0: not such a shape), 16-byte aligned: the quants, [n_kv_heads][max_seq][head_dim / 8] 32-bit words of 8 consecutive values
+ * each, value 2 i in bits 4 i .. and value 2 i + 1 in bits 16 + 4 i .., and behind them the scales, [n_kv_heads][max_seq]
+ * [head_dim / 32] f16, one to a block of 32 values.  A value stands for (nibble - 8) * scale.
+ *
+ * wick_rocm_kv_q4_append: rows row .. row + n - 1 (or *d_row .., those past the cache are dropped) of both caches from the normed and rotated keys and the values
+ * of n tokens (token j's heads at j * kv_stride floats, kv_stride % 4 == 0, 16-byte aligned).  Per block, with m its value of largest
+ * magnitude (the positive one of two): d = m / -8, n_i = min(15, trunc(x_i * (1 / d) + 8.5)) in f32, and the scale f16(d) is held; a
+ * block whose scale rounds to 0 is held as zeros (scale +0), one with a value that is not finite or beyond +-65504 as NaN.
+ * wick_rocm_kv_q4_read: rows row .. row + n - 1 of one cache as floats (out_stride a token, % 4 == 0, 16-byte aligned). */
+size_t wick_rocm_kv_q4_bytes(uint32_t max_seq, uint32_t n_kv_heads, uint32_t head_dim);
+int wick_rocm_kv_q4_append(wick_rocm_ctx *ctx, const float *d_k, const float *d_v, uint32_t kv_stride, void *d_k_cache, void *d_v_cache, uint32_t row,
+                           const uint32_t *d_row, uint32_t n, uint32_t max_seq, uint32_t n_kv_heads, uint32_t head_dim);
+int wick_rocm_kv_q4_read(wick_rocm_ctx *ctx, const void *d_cache, float *d_out, uint32_t out_stride, uint32_t row, uint32_t n, uint32_t max_seq,
+                         uint32_t n_kv_heads, uint32_t head_dim);
+
+/* wick_rocm_attention_decode and wick_rocm_attention_prefill over such caches, f32 in and out and f32-accurate: the queries, the softmax
+ * weights and all sums keep their bits, only the cached values have four.  Decode: rows [0, seq_len) or [0, *d_pos]; seq_len 0 gives zeros.
+ * d_weights (may be null): [n_kv_heads][max_seq] floats to which every row's softmax weights are added, over the head's query heads
+ * and all tokens, in an order of their own that is the same in every run: what a row has gathered, for wick_rocm_kv_q4_evict.  Rows appended anew
+ * start from what the array holds for them (the caller clears it once, an eviction clears what it frees).
+ * d_scratch: wick_rocm_attention_q4_scratch_floats(n, ...) floats (n = 1 for decode; of a longer n than the call's: fine), 16-byte
+ * aligned, contents need not be kept; calls that may run at the same time need one each.  d_q, d_out and caches 16-byte aligned, strides multiples of 4.
+ * A row held as NaN gives NaN to every token that sees it, and to no other. */
+size_t wick_rocm_attention_q4_scratch_floats(uint32_t n, uint32_t max_seq, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, int with_weights);
+int wick_rocm_attention_decode_q4(wick_rocm_ctx *ctx, const float *d_q, const void *d_k_cache, const void *d_v_cache, float *d_out, float *d_weights,
+                                  float *d_scratch, uint32_t seq_len, const uint32_t *d_pos, uint32_t max_seq, uint32_t n_heads, uint32_t n_kv_heads,
+                                  uint32_t head_dim);
+int wick_rocm_attention_prefill_q4(wick_rocm_ctx *ctx, const float *d_q, uint32_t q_stride, const void *d_k_cache, const void *d_v_cache, float *d_out,
+                                   uint32_t out_stride, float *d_weights, float *d_scratch, uint32_t pos0, uint32_t n, uint32_t max_seq, uint32_t n_heads,
+                                   uint32_t n_kv_heads, uint32_t head_dim);
+
+/* Makes room in such caches by what their rows have gathered, where wick_rocm_kv_shift drops a fixed range: for every KV head on its own, of rows
+ * [n_keep, seq_len - n_recent) the n_drop ones of least weight leave (of equal ones the lower row; NaN counts as least), the others
+ * move together in their order, in place.  Quants, scales and weights move as they are and keys keep the rotation of the position they
+ * came from: nothing is rounded again, and the caller goes on counting positions (for the rotation) while rows are counted anew from
+ * seq_len - n_drop.  d_kept ([n_kv_heads][seq_len - n_drop]): the old row of every one that stayed.  Cache rows from seq_len - n_drop on
+ * are left as they were, their weights cleared up to seq_len.  n_drop > 0, n_keep + n_recent + n_drop <= seq_len.  d_scratch:
+ * wick_rocm_kv_q4_evict_scratch_floats(...) floats (may be null where that is 0). */
+size_t wick_rocm_kv_q4_evict_scratch_floats(uint32_t seq_len, uint32_t n_kv_heads);
+int wick_rocm_kv_q4_evict(wick_rocm_ctx *ctx, void *d_k_cache, void *d_v_cache, float *d_weights, uint32_t *d_kept, float *d_scratch, uint32_t seq_len,
+                          uint32_t n_keep, uint32_t n_recent, uint32_t n_drop, uint32_t max_seq, uint32_t n_kv_heads, uint32_t head_dim);
+
 /* The attention block between the Q/K/V projections and the output projection: what wick_rocm_qk_norm_rope followed
  * by wick_rocm_attention_decode compute (wick/src/model/lfm2.rs:783-1006), bit for bit, with the norm, the rotation and
  * the KV append folded into the attention kernel (every workgroup norms and rotates its own query heads and the new key, one

@@ -143,6 +143,129 @@ int wick_rocm_attention_prefill_quantize_q8_0(wick_rocm_ctx* ctx, const float* d
     return e == hipSuccess ? WICK_ROCM_OK : fail_hip(ctx, e, "attention_prefill_quantize launch");
 }
 
+// ---- the KV cache held in 4 bits ----
+
+}  // extern "C"
+
+namespace {
+
+constexpr uint32_t kQ4MaxRows = 1u << 30;
+
+// What every call on such caches asks of their shape and place; null: nothing is wrong.
+const char* q4_shape(uint32_t max_seq, uint32_t n_kv_heads, uint32_t head_dim) {
+    if (head_dim != 32u && head_dim != 64u && head_dim != 128u && head_dim != 256u) return "kv_q4: head_dim must be 32, 64, 128 or 256";
+    if (n_kv_heads == 0 || n_kv_heads > 65535u) return "kv_q4: n_kv_heads must be 1 .. 65535";
+    if (max_seq == 0 || max_seq > kQ4MaxRows) return "kv_q4: max_seq must be 1 .. 2^30";
+    return nullptr;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t wick_rocm_kv_q4_bytes(uint32_t max_seq, uint32_t n_kv_heads, uint32_t head_dim) {
+    return q4_shape(max_seq, n_kv_heads, head_dim) ? 0 : kv_q4_bytes(max_seq, n_kv_heads, head_dim);
+}
+
+int wick_rocm_kv_q4_append(wick_rocm_ctx* ctx, const float* d_k, const float* d_v, uint32_t kv_stride, void* d_k_cache, void* d_v_cache, uint32_t row,
+                           const uint32_t* d_row, uint32_t n, uint32_t max_seq, uint32_t n_kv_heads, uint32_t head_dim) {
+    WR_ENTER(ctx);
+    if (const char* wrong = q4_shape(max_seq, n_kv_heads, head_dim)) return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, wrong);
+    if (!d_k || !d_v || !d_k_cache || !d_v_cache) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_q4_append: null device pointer");
+    if (kv_stride < (uint64_t)n_kv_heads * head_dim || kv_stride % 4u != 0)
+        return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, "kv_q4_append: kv_stride must cover n_kv_heads * head_dim and be a multiple of 4");
+    if (misaligned(d_k, 16) || misaligned(d_v, 16) || misaligned(d_k_cache, 16) || misaligned(d_v_cache, 16))
+        return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_q4_append: keys, values and caches must be 16-byte aligned");
+    if (n > max_seq || (!d_row && (uint64_t)row + n > max_seq)) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_q4_append: rows beyond the cache");
+    hipError_t e = launch_kv_q4_append(d_k, d_v, kv_stride, d_k_cache, d_v_cache, row, d_row, n, max_seq, n_kv_heads, head_dim, ctx->launch());
+    return e == hipSuccess ? WICK_ROCM_OK : fail_hip(ctx, e, "kv_q4_append launch");
+}
+
+int wick_rocm_kv_q4_read(wick_rocm_ctx* ctx, const void* d_cache, float* d_out, uint32_t out_stride, uint32_t row, uint32_t n, uint32_t max_seq,
+                         uint32_t n_kv_heads, uint32_t head_dim) {
+    WR_ENTER(ctx);
+    if (const char* wrong = q4_shape(max_seq, n_kv_heads, head_dim)) return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, wrong);
+    if (!d_cache || !d_out) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_q4_read: null device pointer");
+    if (out_stride < (uint64_t)n_kv_heads * head_dim || out_stride % 4u != 0)
+        return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, "kv_q4_read: out_stride must cover n_kv_heads * head_dim and be a multiple of 4");
+    if (misaligned(d_cache, 16) || misaligned(d_out, 16)) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_q4_read: cache and output must be 16-byte aligned");
+    if ((uint64_t)row + n > max_seq) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_q4_read: rows beyond the cache");
+    hipError_t e = launch_kv_q4_read(d_cache, d_out, out_stride, row, n, max_seq, n_kv_heads, head_dim, ctx->launch());
+    return e == hipSuccess ? WICK_ROCM_OK : fail_hip(ctx, e, "kv_q4_read launch");
+}
+
+size_t wick_rocm_attention_q4_scratch_floats(uint32_t n, uint32_t max_seq, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, int with_weights) {
+    if (q4_shape(max_seq, n_kv_heads, head_dim) || n_heads == 0 || n_heads % n_kv_heads != 0) return 0;
+    return attention_q4_scratch_floats(n, max_seq, n_heads, n_kv_heads, head_dim, with_weights != 0);
+}
+
+}  // extern "C"
+
+// n tokens at rows pos0 .. (or *d_pos ..); what both public forms check alike.
+static int attention_q4(wick_rocm_ctx* ctx, const float* d_q, uint32_t q_stride, const void* d_k_cache, const void* d_v_cache, float* d_out, uint32_t out_stride,
+                        float* d_weights, float* d_scratch, uint32_t pos0, const uint32_t* d_pos, uint32_t n, uint32_t max_seq, uint32_t n_heads,
+                        uint32_t n_kv_heads, uint32_t head_dim) {
+    if (n_heads == 0 || n_heads % n_kv_heads != 0) return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, "attention_q4: n_kv_heads must divide n_heads");
+    if (q_stride < (uint64_t)n_heads * head_dim || out_stride < (uint64_t)n_heads * head_dim || q_stride % 4u != 0 || out_stride % 4u != 0 ||
+        (uint64_t)n * n_heads > kQ4MaxRows)
+        return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, "attention_q4: strides must cover n_heads * head_dim and be multiples of 4, n * n_heads at most 2^30");
+    if (!d_q || !d_k_cache || !d_v_cache || !d_out || (!d_scratch && attention_q4_scratch_floats(n, max_seq, n_heads, n_kv_heads, head_dim, d_weights != nullptr)))
+        return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "attention_q4: null device pointer");
+    if (misaligned(d_q, 16) || misaligned(d_k_cache, 16) || misaligned(d_v_cache, 16) || misaligned(d_out, 16) || misaligned(d_scratch, 16) || misaligned(d_weights, 4))
+        return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "attention_q4: q, caches, output and scratch must be 16-byte aligned");
+    const float scale = 1.0f / sqrtf((float)head_dim);  // wick/src/model/lfm2.rs:862
+    hipError_t e = launch_attention_q4(d_q, q_stride, d_k_cache, d_v_cache, d_out, out_stride, d_weights, d_scratch, pos0, d_pos, n, max_seq, n_heads,
+                                       n_kv_heads, head_dim, scale, ctx->launch());
+    return e == hipSuccess ? WICK_ROCM_OK : fail_hip(ctx, e, "attention_q4 launch");
+}
+
+extern "C" {
+
+int wick_rocm_attention_decode_q4(wick_rocm_ctx* ctx, const float* d_q, const void* d_k_cache, const void* d_v_cache, float* d_out, float* d_weights,
+                                  float* d_scratch, uint32_t seq_len, const uint32_t* d_pos, uint32_t max_seq, uint32_t n_heads, uint32_t n_kv_heads,
+                                  uint32_t head_dim) {
+    WR_ENTER(ctx);
+    if (const char* wrong = q4_shape(max_seq, n_kv_heads, head_dim)) return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, wrong);
+    if (!d_pos && seq_len > max_seq) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "attention_q4: seq_len beyond the cache");
+    if ((uint64_t)n_heads * head_dim > UINT32_MAX - 3u) return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, "attention_q4: too many heads");
+    if (!d_pos && seq_len == 0) {  // no row to attend over
+        if (!d_out) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "attention_q4: null device pointer");
+        hipError_t e = launch_fill_zero(d_out, (size_t)n_heads * head_dim, ctx->launch());
+        return e == hipSuccess ? WICK_ROCM_OK : fail_hip(ctx, e, "attention_q4 launch");
+    }
+    return attention_q4(ctx, d_q, n_heads * head_dim, d_k_cache, d_v_cache, d_out, n_heads * head_dim, d_weights, d_scratch, seq_len - 1u, d_pos, 1,
+                        max_seq, n_heads, n_kv_heads, head_dim);
+}
+
+int wick_rocm_attention_prefill_q4(wick_rocm_ctx* ctx, const float* d_q, uint32_t q_stride, const void* d_k_cache, const void* d_v_cache, float* d_out,
+                                   uint32_t out_stride, float* d_weights, float* d_scratch, uint32_t pos0, uint32_t n, uint32_t max_seq, uint32_t n_heads,
+                                   uint32_t n_kv_heads, uint32_t head_dim) {
+    WR_ENTER(ctx);
+    if (const char* wrong = q4_shape(max_seq, n_kv_heads, head_dim)) return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, wrong);
+    if ((uint64_t)pos0 + n > max_seq) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "attention_q4: positions beyond the cache");
+    return attention_q4(ctx, d_q, q_stride, d_k_cache, d_v_cache, d_out, out_stride, d_weights, d_scratch, pos0, nullptr, n, max_seq, n_heads, n_kv_heads,
+                        head_dim);
+}
+
+size_t wick_rocm_kv_q4_evict_scratch_floats(uint32_t seq_len, uint32_t n_kv_heads) { return kv_q4_evict_scratch_floats(seq_len, n_kv_heads); }
+
+int wick_rocm_kv_q4_evict(wick_rocm_ctx* ctx, void* d_k_cache, void* d_v_cache, float* d_weights, uint32_t* d_kept, float* d_scratch, uint32_t seq_len,
+                          uint32_t n_keep, uint32_t n_recent, uint32_t n_drop, uint32_t max_seq, uint32_t n_kv_heads, uint32_t head_dim) {
+    WR_ENTER(ctx);
+    if (const char* wrong = q4_shape(max_seq, n_kv_heads, head_dim)) return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, wrong);
+    if (n_drop == 0) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_q4_evict: n_drop must be > 0");
+    if (seq_len > max_seq || (uint64_t)n_keep + n_recent + n_drop > seq_len)
+        return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_q4_evict: rows out of bounds (n_keep + n_recent + n_drop > seq_len, or seq_len beyond the cache)");
+    if (!d_k_cache || !d_v_cache || !d_weights || !d_kept || (!d_scratch && kv_q4_evict_scratch_floats(seq_len, n_kv_heads)))
+        return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_q4_evict: null device pointer");
+    if (d_k_cache == d_v_cache) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_q4_evict: keys and values are one cache");
+    if (misaligned(d_k_cache, 16) || misaligned(d_v_cache, 16) || misaligned(d_scratch, 16) || misaligned(d_weights, 4) || misaligned(d_kept, 4))
+        return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_q4_evict: caches and scratch must be 16-byte aligned");
+    hipError_t e = launch_kv_q4_evict(d_k_cache, d_v_cache, d_weights, d_kept, d_scratch, seq_len, n_keep, n_recent, n_drop, max_seq, n_kv_heads, head_dim,
+                                      ctx->launch());
+    return e == hipSuccess ? WICK_ROCM_OK : fail_hip(ctx, e, "kv_q4_evict launch");
+}
+
 int wick_rocm_ffn_gate_up_silu_quantize_applies(const wick_rocm_weight* w_gate, const wick_rocm_weight* w_up, uint32_t n) {
     if (!w_gate || !w_up || !w_gate->d_gemm || !w_up->d_gemm) return 0;
     if (w_gate->type != w_up->type || (w_gate->type != kTypeQ4_0 && w_gate->type != kTypeQ8_0)) return 0;

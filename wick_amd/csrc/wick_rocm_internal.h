@@ -271,6 +271,21 @@ hipError_t launch_argmax_final(const unsigned long long* d_partial, uint32_t n_p
 hipError_t launch_set_step(uint32_t* d_token, uint32_t token, uint32_t* d_pos, uint32_t pos, const Launch& L, const uint8_t* d_embd = nullptr,
                            int embd_type = 0, uint32_t embd_m = 0, uint32_t embd_k = 0, float* d_embd_out = nullptr, RopeTable rope = {});
 
+// The KV cache held in 4 bits (kv_q4.hip): head_dim 32 / 64 / 128 / 256.
+size_t kv_q4_bytes(uint32_t max_seq, uint32_t n_kv_heads, uint32_t head_dim);
+hipError_t launch_kv_q4_append(const float* d_k, const float* d_v, uint32_t kv_stride, void* d_k_cache, void* d_v_cache, uint32_t row, const uint32_t* d_row,
+                               uint32_t n, uint32_t max_seq, uint32_t n_kv_heads, uint32_t head_dim, const Launch& L);
+hipError_t launch_kv_q4_read(const void* d_cache, float* d_out, uint32_t out_stride, uint32_t row, uint32_t n, uint32_t max_seq, uint32_t n_kv_heads,
+                             uint32_t head_dim, const Launch& L);
+// n tokens at rows pos0 .. (or *d_pos ..) whose keys and values are in the caches already, each over the rows up to its own.  d_weights null: not gathered.
+size_t attention_q4_scratch_floats(uint32_t n, uint32_t max_seq, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, bool weights);
+hipError_t launch_attention_q4(const float* d_q, uint32_t q_stride, const void* d_k_cache, const void* d_v_cache, float* d_out, uint32_t out_stride,
+                               float* d_weights, float* d_scratch, uint32_t pos0, const uint32_t* d_pos, uint32_t n, uint32_t max_seq, uint32_t n_heads,
+                               uint32_t n_kv_heads, uint32_t head_dim, float scale, const Launch& L);
+size_t kv_q4_evict_scratch_floats(uint32_t seq_len, uint32_t n_kv_heads);
+hipError_t launch_kv_q4_evict(void* d_k_cache, void* d_v_cache, float* d_weights, uint32_t* d_kept, float* d_scratch, uint32_t seq_len, uint32_t n_keep,
+                              uint32_t n_recent, uint32_t n_drop, uint32_t max_seq, uint32_t n_kv_heads, uint32_t head_dim, const Launch& L);
+
 // n at and above which gemm_q8 uses the MFMA kernel (when k % 128 == 0): the counterpart of GEMM_MIN_N = 16
 // (wick/src/model/metal_lfm2.rs:18-21), set where the two routes cross on this GPU.  The multi-token GEMV streams the weight
 // once per group of four tokens; the narrow MFMA kernel streams it once and computes 16 token columns at a time.  A 1024 x 1024

@@ -45,6 +45,14 @@ _SIGNATURES = {
     "wick_rocm_lm_head_greedy_f32": (C.c_int, [_P, _P, _P, _P, _F, _P, _P, _P, _P]),
     "wick_rocm_rmsnorm_quantize_q8_0": (C.c_int, [_P, _P, _P, _U32, _U32, _U32, _F, _P, _P]),
     "wick_rocm_silu_mul_quantize_q8_0": (C.c_int, [_P, _P, _P, _U32, _U32, _P, _P]),
+    "wick_rocm_kv_q4_bytes": (C.c_size_t, [_U32, _U32, _U32]),
+    "wick_rocm_kv_q4_append": (C.c_int, [_P, _P, _P, _U32, _P, _P, _U32, _P, _U32, _U32, _U32, _U32]),
+    "wick_rocm_kv_q4_read": (C.c_int, [_P, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32]),
+    "wick_rocm_attention_q4_scratch_floats": (C.c_size_t, [_U32, _U32, _U32, _U32, _U32, C.c_int]),
+    "wick_rocm_attention_decode_q4": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _U32, _P, _U32, _U32, _U32, _U32]),
+    "wick_rocm_attention_prefill_q4": (C.c_int, [_P, _P, _U32, _P, _P, _P, _U32, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32]),
+    "wick_rocm_kv_q4_evict_scratch_floats": (C.c_size_t, [_U32, _U32]),
+    "wick_rocm_kv_q4_evict": (C.c_int, [_P, _P, _P, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32, _U32]),
     "wick_rocm_lfm2_load": (C.c_int, [_P, _P, _U32, C.POINTER(_P)]),
     "wick_rocm_lfm2_load_kv": (C.c_int, [_P, _P, _U32, C.c_int, C.POINTER(_P)]),
     "wick_rocm_lfm2_kv_dtype": (C.c_int, [_P]),
@@ -97,6 +105,19 @@ def attention_scratch_floats(max_seq: int, n_heads: int, head_dim: int) -> int:
 
 def attention_block_scratch_bytes(max_seq: int, n_heads: int, head_dim: int) -> int:
     return int(_lib().wick_rocm_attention_block_scratch_bytes(max_seq, n_heads, head_dim))
+
+
+def kv_q4_bytes(max_seq: int, n_kv_heads: int, head_dim: int) -> int:
+    """Bytes of one cache (keys or values) held in 4 bits."""
+    return int(_lib().wick_rocm_kv_q4_bytes(max_seq, n_kv_heads, head_dim))
+
+
+def attention_q4_scratch_floats(n: int, max_seq: int, n_heads: int, n_kv_heads: int, head_dim: int, weights: bool = False) -> int:
+    return int(_lib().wick_rocm_attention_q4_scratch_floats(n, max_seq, n_heads, n_kv_heads, head_dim, int(weights)))
+
+
+def kv_q4_evict_scratch_floats(seq_len: int, n_kv_heads: int) -> int:
+    return int(_lib().wick_rocm_kv_q4_evict_scratch_floats(seq_len, n_kv_heads))
 
 
 def rope_theta_scale(head_dim: int, freq_base: float) -> float:
@@ -153,6 +174,34 @@ class Lfm2Ops:
         """encode_attention_prefill with the result written as Q8_0 blocks (the out projection's input)."""
         self.ctx._check(self._l.wick_rocm_attention_prefill_quantize_q8_0(self.ctx._h, _ptr(q), q_stride, _ptr(k_cache), _ptr(v_cache), _ptr(out_q),
                                                                           _ptr(out_scales), pos0, n, max_seq, n_heads, n_kv_heads, head_dim))
+
+    def encode_kv_q4_append(self, k, v, kv_stride: int, k_cache, v_cache, row: int, n: int, max_seq: int, n_kv_heads: int, head_dim: int,
+                            d_row=None) -> None:
+        """Rows row .. of both 4-bit caches from n tokens' normed and rotated keys and their values."""
+        self.ctx._check(self._l.wick_rocm_kv_q4_append(self.ctx._h, _ptr(k), _ptr(v), kv_stride, _ptr(k_cache), _ptr(v_cache), row, _ptr(d_row), n,
+                                                       max_seq, n_kv_heads, head_dim))
+
+    def encode_kv_q4_read(self, cache, out, out_stride: int, row: int, n: int, max_seq: int, n_kv_heads: int, head_dim: int) -> None:
+        """Rows row .. row + n - 1 of a 4-bit cache as floats."""
+        self.ctx._check(self._l.wick_rocm_kv_q4_read(self.ctx._h, _ptr(cache), _ptr(out), out_stride, row, n, max_seq, n_kv_heads, head_dim))
+
+    def encode_attention_q4(self, q, k_cache, v_cache, out, scratch, seq_len: int, max_seq: int, n_heads: int, n_kv_heads: int, head_dim: int,
+                            weights=None, d_pos=None) -> None:
+        """encode_attention over 4-bit caches; weights: what the rows' softmax weights are added to."""
+        self.ctx._check(self._l.wick_rocm_attention_decode_q4(self.ctx._h, _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(weights), _ptr(scratch),
+                                                              seq_len, _ptr(d_pos), max_seq, n_heads, n_kv_heads, head_dim))
+
+    def encode_attention_prefill_q4(self, q, q_stride: int, k_cache, v_cache, out, out_stride: int, scratch, pos0: int, n: int, max_seq: int,
+                                    n_heads: int, n_kv_heads: int, head_dim: int, weights=None) -> None:
+        """encode_attention_prefill over 4-bit caches."""
+        self.ctx._check(self._l.wick_rocm_attention_prefill_q4(self.ctx._h, _ptr(q), q_stride, _ptr(k_cache), _ptr(v_cache), _ptr(out), out_stride,
+                                                               _ptr(weights), _ptr(scratch), pos0, n, max_seq, n_heads, n_kv_heads, head_dim))
+
+    def encode_kv_q4_evict(self, k_cache, v_cache, weights, kept, scratch, seq_len: int, n_keep: int, n_recent: int, n_drop: int, max_seq: int,
+                           n_kv_heads: int, head_dim: int) -> None:
+        """The n_drop rows of least weight leave both 4-bit caches, each head's own; kept: the old rows of those that stay."""
+        self.ctx._check(self._l.wick_rocm_kv_q4_evict(self.ctx._h, _ptr(k_cache), _ptr(v_cache), _ptr(weights), _ptr(kept), _ptr(scratch), seq_len, n_keep,
+                                                      n_recent, n_drop, max_seq, n_kv_heads, head_dim))
 
     def encode_conv1d_seq(self, proj, buffer, conv_weight, out, hidden: int, kernel_size: int, n: int) -> None:
         """The gated short convolution of n prompt tokens (proj [n][3*hidden] -> out [n][hidden]), then the rolling state."""
