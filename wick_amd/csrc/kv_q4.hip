@@ -1,12 +1,6 @@
-// The KV cache held in 4 bits: rows appended and read back, attention of one token and of a prompt over it, eviction of the rows
-// that have gathered the least attention weight.
-//
-// A cache of max_seq rows of n_kv_heads heads is two planes: the quants, [n_kv_heads][max_seq][head_dim / 8] words of 8 consecutive
-// values, and behind them the scales, [n_kv_heads][max_seq][head_dim / 32] f16, one to a block of 32 values; a value stands for
-// (nibble - 8) * scale.  A head's rows lie one behind the other, so that a workgroup, which attends over one head, reads whole
-// cache lines of its own head alone and evicts rows of each head on their own.  Value 2 i of a word is nibble i of its lower half and
-// value 2 i + 1 nibble i of the upper: (w >> 4 i) & 0x000f000f is a pair of neighbours, which two more instructions turn into halves.
-#include "wick_rocm_device.h"
+// The KV cache held in 4 bits (its layout: kv_q4_device.h): rows appended and read back, eviction of the rows that have gathered
+// the least attention weight.
+#include "kv_q4_device.h"
 #include "wick_rocm_internal.h"
 
 namespace wick_rocm {
@@ -14,20 +8,6 @@ namespace wick_rocm {
 namespace {
 
 constexpr float kQ4Largest = 65504.0f;  // of a value that a block can hold: eight times its scale is an f16, whatever product takes it
-
-// A cache's planes from the buffer that holds both.
-struct Q4Cache {
-    uint32_t* quants;
-    uint16_t* scales;
-};
-__host__ __device__ __forceinline__ Q4Cache q4_planes(void* cache, uint32_t max_seq, uint32_t n_kv_heads, uint32_t head_dim) {
-    uint8_t* const p = static_cast<uint8_t*>(cache);
-    return {reinterpret_cast<uint32_t*>(p), reinterpret_cast<uint16_t*>(p + (size_t)n_kv_heads * max_seq * (head_dim / 2))};
-}
-
-__device__ __forceinline__ float q4_value(uint32_t w, uint32_t i, float scale) {  // value i of a word: exact
-    return (float)((int)(w >> (4u * (i >> 1) + 16u * (i & 1u)) & 15u) - 8) * scale;
-}
 
 // ---- append, read back ---------------------------------------------------------------------
 // A block's scale is its value of largest magnitude over -8 (the positive one of two), so that this value is held as it is up to
@@ -99,90 +79,6 @@ __global__ __launch_bounds__(256) void kv_q4_read_kernel(const void* p, float* _
 #pragma unroll
     for (int e = 0; e < 8; e += 4)
         *reinterpret_cast<float4*>(to + e) = make_float4(q4_value(q, e, d), q4_value(q, e + 1, d), q4_value(q, e + 2, d), q4_value(q, e + 3, d));
-}
-
-// ---- attention ------------------------------------------------------------------------------
-struct Q4AttentionArgs {
-    const float* q;      // [n][q_stride]
-    const void* k_cache;
-    const void* v_cache;
-    float* out;          // [n][out_stride]
-    float* rows;         // {maximum, 1 / sum} of every (token, head)'s softmax, for the weights; may be null
-    float* weights;      // [n_kv_heads][max_seq]
-    const uint32_t* d_pos;
-    uint32_t pos0, n, q_stride, out_stride, max_seq, n_heads, n_kv_heads, head_dim;
-    float scale;
-};
-
-// One (token, head) per workgroup, rows in chunks of 256 with a running maximum and sum.
-__global__ __launch_bounds__(256) void attention_q4_kernel(Q4AttentionArgs a) {
-    __shared__ float q[256], p[256], red[256];
-    const uint32_t j = blockIdx.x / a.n_heads, h = blockIdx.x % a.n_heads, c = h / (a.n_heads / a.n_kv_heads), hd = a.head_dim, words = hd / 8u, tid = threadIdx.x;
-    const uint64_t sees = (uint64_t)(a.d_pos ? *a.d_pos : a.pos0) + j + 1u;
-    const uint32_t seq = (uint32_t)(sees < a.max_seq ? sees : a.max_seq);
-    const Q4Cache k = q4_planes(const_cast<void*>(a.k_cache), a.max_seq, a.n_kv_heads, hd), v = q4_planes(const_cast<void*>(a.v_cache), a.max_seq, a.n_kv_heads, hd);
-    const size_t first = (size_t)c * a.max_seq;
-    if (tid < hd) q[tid] = a.q[(size_t)j * a.q_stride + (size_t)h * hd + tid] * a.scale;
-    float m = -__builtin_inff(), l = 0.0f, o = 0.0f;
-    for (uint32_t t0 = 0; t0 < seq; t0 += 256u) {
-        __syncthreads();
-        const uint32_t t = t0 + tid, nt = seq - t0 < 256u ? seq - t0 : 256u;
-        float s = -__builtin_inff();
-        if (t < seq) {
-            s = 0.0f;
-            for (uint32_t w = 0; w < words; w++) {
-                const uint32_t bits = k.quants[(first + t) * words + w];
-                const float d = f16_bits_to_f32(k.scales[(first + t) * (words / 4u) + w / 4u]);
-                for (uint32_t e = 0; e < 8u; e++) s += q[8u * w + e] * q4_value(bits, e, d);
-                s += 0.0f * f16_bits_to_f32(v.scales[(first + t) * (words / 4u) + w / 4u]);  // (a row of values held as NaN)
-            }
-        }
-        red[tid] = s;
-        __syncthreads();
-        for (uint32_t off = 128; off; off >>= 1) {
-            if (tid < off) red[tid] = fmaxf(red[tid], red[tid + off]);
-            __syncthreads();
-        }
-        const float m_new = fmaxf(m, red[0]);
-        __syncthreads();
-        p[tid] = t < seq ? expf(s - m_new) : 0.0f;
-        red[tid] = p[tid];
-        __syncthreads();
-        for (uint32_t off = 128; off; off >>= 1) {
-            if (tid < off) red[tid] += red[tid + off];
-            __syncthreads();
-        }
-        const float rescale = expf(m - m_new);
-        l = l * rescale + red[0], o *= rescale, m = m_new;
-        if (tid < hd)
-            for (uint32_t i = 0; i < nt; i++)
-                o += p[i] * q4_value(v.quants[(first + t0 + i) * words + tid / 8u], tid % 8u, f16_bits_to_f32(v.scales[(first + t0 + i) * (words / 4u) + tid / 32u]));
-    }
-    if (tid < hd) a.out[(size_t)j * a.out_stride + (size_t)h * hd + tid] = seq ? o / l : 0.0f;
-    if (a.rows && tid == 0) a.rows[2u * blockIdx.x] = m, a.rows[2u * blockIdx.x + 1u] = 1.0f / l;
-}
-
-// What each row of a KV head has gathered, one lane a row: the tokens and heads in their order.
-__global__ __launch_bounds__(256) void attention_q4_weights_kernel(Q4AttentionArgs a) {
-    const uint32_t c = blockIdx.y, t = blockIdx.x * 256u + threadIdx.x, hd = a.head_dim, words = hd / 8u, group = a.n_heads / a.n_kv_heads;
-    const uint32_t pos0 = a.d_pos ? *a.d_pos : a.pos0;
-    const uint64_t sees = (uint64_t)pos0 + a.n;
-    if (t >= sees || t >= a.max_seq) return;
-    const Q4Cache k = q4_planes(const_cast<void*>(a.k_cache), a.max_seq, a.n_kv_heads, hd);
-    const size_t at = (size_t)c * a.max_seq + t;
-    float sum = 0.0f;
-    for (uint32_t j = t > pos0 ? t - pos0 : 0u; j < a.n; j++)
-        for (uint32_t h = c * group; h < (c + 1u) * group; h++) {
-            float s = 0.0f;
-            for (uint32_t w = 0; w < words; w++) {
-                const uint32_t bits = k.quants[at * words + w];
-                const float d = f16_bits_to_f32(k.scales[at * (words / 4u) + w / 4u]);
-                for (uint32_t e = 0; e < 8u; e++) s += a.q[(size_t)j * a.q_stride + (size_t)h * hd + 8u * w + e] * a.scale * q4_value(bits, e, d);
-            }
-            const float* const row = a.rows + 2u * ((size_t)j * a.n_heads + h);
-            sum += expf(s - row[0]) * row[1];
-        }
-    a.weights[at] += sum;
 }
 
 // ---- eviction -------------------------------------------------------------------------------
@@ -307,22 +203,6 @@ hipError_t launch_kv_q4_read(const void* d_cache, float* d_out, uint32_t out_str
     const uint64_t threads = (uint64_t)n_kv_heads * n * (head_dim / 8u);
     return launch_kernel(L, kFamOther, kv_q4_read_kernel, dim3((uint32_t)((threads + 255) / 256)), dim3(256), d_cache, d_out, out_stride, row, n, max_seq,
                          n_kv_heads, head_dim);
-}
-
-size_t attention_q4_scratch_floats(uint32_t n, uint32_t max_seq, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, bool weights) {
-    (void)max_seq, (void)n_kv_heads, (void)head_dim;
-    return weights ? 2 * (size_t)n * n_heads : 0;
-}
-
-hipError_t launch_attention_q4(const float* d_q, uint32_t q_stride, const void* d_k_cache, const void* d_v_cache, float* d_out, uint32_t out_stride,
-                               float* d_weights, float* d_scratch, uint32_t pos0, const uint32_t* d_pos, uint32_t n, uint32_t max_seq, uint32_t n_heads,
-                               uint32_t n_kv_heads, uint32_t head_dim, float scale, const Launch& L) {
-    if (n == 0) return hipSuccess;
-    const Q4AttentionArgs a{d_q, d_k_cache, d_v_cache, d_out, d_weights ? d_scratch : nullptr, d_weights, d_pos, pos0, n, q_stride, out_stride,
-                            max_seq, n_heads, n_kv_heads, head_dim, scale};
-    hipError_t e = launch_kernel(L, kFamOther, attention_q4_kernel, dim3(n * n_heads), dim3(256), a);
-    if (e == hipSuccess && d_weights) e = launch_kernel(L, kFamOther, attention_q4_weights_kernel, dim3((max_seq + 255u) / 256u, n_kv_heads), dim3(256), a);
-    return e;
 }
 
 size_t kv_q4_evict_scratch_floats(uint32_t seq_len, uint32_t n_kv_heads) {

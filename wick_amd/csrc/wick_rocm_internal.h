@@ -271,7 +271,7 @@ hipError_t launch_argmax_final(const unsigned long long* d_partial, uint32_t n_p
 hipError_t launch_set_step(uint32_t* d_token, uint32_t token, uint32_t* d_pos, uint32_t pos, const Launch& L, const uint8_t* d_embd = nullptr,
                            int embd_type = 0, uint32_t embd_m = 0, uint32_t embd_k = 0, float* d_embd_out = nullptr, RopeTable rope = {});
 
-// The KV cache held in 4 bits (kv_q4.hip): head_dim 32 / 64 / 128 / 256.
+// The KV cache held in 4 bits (kv_q4.hip, attention_q4.hip): head_dim 32 / 64 / 128 / 256.
 size_t kv_q4_bytes(uint32_t max_seq, uint32_t n_kv_heads, uint32_t head_dim);
 hipError_t launch_kv_q4_append(const float* d_k, const float* d_v, uint32_t kv_stride, void* d_k_cache, void* d_v_cache, uint32_t row, const uint32_t* d_row,
                                uint32_t n, uint32_t max_seq, uint32_t n_kv_heads, uint32_t head_dim, const Launch& L);
