@@ -1,13 +1,13 @@
 // Attention over KV caches held in 4 bits (kv_q4_device.h), on the f16 matrix cores at f32 accuracy.
 //
 // With G = n_heads / n_kv_heads, the query heads of KV head c over n tokens are n G rows, row r = token r / G, head c G + r % G:
-// all of them read the same keys and values, and row r sees rows [0, pos0 + r / G] of the cache.  A workgroup takes 16 WQ of them and
-// walks the cache in tiles of 32 WK rows: wave (wq, wk) multiplies 16 query rows with 32 rows of each tile, on
-// v_mfma_f32_16x16x32_f16, both products transposed:
-//   S^T[key][row] = sum_d K[key][d] Q[row][d]    lane l is left with keys 4 (l / 16) + i of row l % 16, twice (16 keys each);
+// all of them read the same keys and values, and row r sees rows [0, pos0 + r / G] of the cache.  A workgroup takes 32 WQ of them and
+// walks the cache in tiles of 32 WK rows: wave (wq, wk) multiplies 32 query rows with 32 rows of each tile, on
+// v_mfma_f32_32x32x16_f16, both products transposed:
+//   S^T[key][row] = sum_d K[key][d] Q[row][d]    lane l is left with keys 8 (i / 4) + 4 (l / 32) + i % 4 of row l % 32;
 //   O^T[d][row]  += sum_key V[key][d] P[key][row]   whose B operand is, per lane, consecutive K steps of one row: the weights as they
 //                                                   are in the lane's registers (an MFMA's K steps are in any order, so both
-//                                                   operands agree that slot j of lane group g is key 4 g + j, or 12 + 4 g + j from j = 4 on).
+//                                                   operands agree on which key a lane's slot is).
 // Accuracy: a cached value, four bits times an f16 scale, is the sum of two halves exactly (hi = f16(n d), lo = f16(n d - hi), 15 bits
 // in all); a query, scaled by a power of two to below 1, and a softmax weight, times 2^12, are split into two halves that keep 22 bits.
 // a b = a_hi b_hi + a_hi b_lo + a_lo b_hi: each product of halves is exact, sums are f32's, what is dropped is below 2^-22.
@@ -20,10 +20,11 @@ namespace wick_rocm {
 
 namespace {
 
-constexpr float kWeightScale = 4096.0f;    // of the softmax weights in front of their split, so that small ones keep their bits
+constexpr float kWeightBits = 12.0f;       // softmax weights are taken times 2^12, so that small ones keep their bits in the split
 constexpr uint32_t kMaxSplits = 64;        // workgroups that share the rows of the cache among them
-constexpr uint32_t kSplitSlots = 512;      // split launches have no more workgroups than this, or one split
-constexpr uint32_t kMostRows = 64;         // query rows of a workgroup at the most
+constexpr uint32_t kCus = 256;
+constexpr uint32_t kSplitSlots = 2 * kCus; // split launches have no more workgroups than this
+constexpr uint32_t kMostRows = 128;        // query rows of a workgroup at the most
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct Q4AttentionArgs {
@@ -32,10 +33,11 @@ struct Q4AttentionArgs {
     const void* v_cache;
     float* out;      // [n][out_stride]
     float* parts;    // records of the splits, [n * n_heads][splits][4 + head_dim]: {maximum, sum, -, -, values}
-    float* stats;    // {maximum, 1 / sum} of every (token, head)'s softmax (in powers of two), for the weights; may be null
+    float* stats;    // {maximum (as a power of two), 1 / (sum 2^12)} of every (token, head)'s softmax, for the weights; may be null
     float* weights;  // [n_kv_heads][max_seq]
     const uint32_t* d_pos;
     uint32_t pos0, n, q_stride, out_stride, max_seq, n_heads, n_kv_heads, splits;
+    uint32_t first_blocks;  // blocks of query rows that are taken in descending order
     float scale;
 };
 
@@ -47,60 +49,86 @@ __device__ __forceinline__ uint32_t sees(const Q4AttentionArgs& a, uint32_t base
 // Splits that a workgroup of `tiles` tiles has in earnest: with the position on the device the host does not know.
 __device__ __forceinline__ uint32_t used_splits(uint32_t splits, uint32_t tiles) { return min(splits, tiles); }
 
-// Eight values of a word as two planes of halves.
+// Eight values of a word as two planes of halves.  (The mask in a scalar and the offset's bits in a vector register: one instruction takes both.)
 __device__ __forceinline__ void dequantize(uint32_t w, _Float16 scale, h8& hi, h8& lo) {
     const h2 d = {scale, scale}, offset = {(_Float16)1032.0f, (_Float16)1032.0f};
+    uint32_t mask = 0x000f000fu, bits = 0x64006400u;
+    asm("" : "+s"(mask), "+v"(bits));
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const h2 n = __builtin_bit_cast(h2, ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u) - offset;  // 1024 + nibble, exact
+        const h2 n = __builtin_bit_cast(h2, ((w >> (4 * i)) & mask) | bits) - offset;  // 1024 + nibble, exact
         const h2 h = n * d, l = __builtin_elementwise_fma(n, d, -h);
         hi[2 * i] = h[0], hi[2 * i + 1] = h[1], lo[2 * i] = l[0], lo[2 * i + 1] = l[1];
     }
 }
 
-// 16 query rows as the B operand of the first product: dims 32 s + 8 g .. + 7 of row l16, times 2^-e (the row's largest below 1), and
+// Four f32 values as two planes: a pair at a time, then one instruction a value (y * 1 - hi, rounded to a half; the compiler does not see the 1 and cannot
+// make two instructions of it).
+__device__ __forceinline__ void split_halves(const v4f& y, h4& hi, h4& lo) {
+    float one = 1.0f;
+    asm("" : "+s"(one));
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+        const h2 h = __builtin_convertvector((v2f{y[i], y[i + 1]}), h2);
+        hi[i] = h[0], hi[i + 1] = h[1];
+        lo[i] = (_Float16)__builtin_fmaf(y[i], one, -(float)h[0]), lo[i + 1] = (_Float16)__builtin_fmaf(y[i + 1], one, -(float)h[1]);
+    }
+}
+
+__device__ __forceinline__ float halves_max(float v) {  // over lanes l, l ^ 32
+    const uint32_t b = __float_as_uint(v);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float halves_sum(float v) {
+    const uint32_t b = __float_as_uint(v);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// 32 query rows as the B operand of the first product: dims 16 s + 8 h .. + 7 of row l32, times 2^-e (the row's largest below 1), and
 // the factor that turns a product into a power of two.
 template <int HD>
 struct Queries {
-    h8 hi[HD / 32], lo[HD / 32];
+    h8 hi[HD / 16], lo[HD / 16];
     float factor;
-    __device__ __forceinline__ void load(const Q4AttentionArgs& a, uint32_t r, uint32_t c, uint32_t group, uint32_t g) {
-        const float* const p = a.q + (size_t)(r / group) * a.q_stride + (size_t)(c * group + r % group) * HD + 8u * g;
-        v4f x[HD / 16];
+    __device__ __forceinline__ void load(const Q4AttentionArgs& a, uint32_t r, uint32_t c, uint32_t group, uint32_t h) {
+        const float* const p = a.q + (size_t)(r / group) * a.q_stride + (size_t)(c * group + r % group) * HD + 8u * h;
+        v4f x[HD / 8];
         float top = 0.0f;
 #pragma unroll
-        for (int s = 0; s < HD / 32; s++)
+        for (int s = 0; s < HD / 16; s++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                x[2 * s + i] = *reinterpret_cast<const v4f*>(p + 32 * s + 4 * i);
+                x[2 * s + i] = *reinterpret_cast<const v4f*>(p + 16 * s + 4 * i);
 #pragma unroll
                 for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(x[2 * s + i][e]));
             }
-        const int e = __builtin_amdgcn_frexp_expf(groups_max(top));
+        const int e = __builtin_amdgcn_frexp_expf(halves_max(top));
         factor = __builtin_amdgcn_ldexpf(a.scale * kLog2e, e);
 #pragma unroll
-        for (int s = 0; s < HD / 32; s++) {
-            h4 h[2], l[2];
+        for (int s = 0; s < HD / 16; s++) {
+            h4 u[2], l[2];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 v4f y;
 #pragma unroll
                 for (int k = 0; k < 4; k++) y[k] = __builtin_amdgcn_ldexpf(x[2 * s + i][k], -e);
-                split_f16(y, h[i], l[i]);
+                split_halves(y, u[i], l[i]);
             }
-            hi[s] = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7), lo[s] = __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3, 4, 5, 6, 7);
+            hi[s] = __builtin_shufflevector(u[0], u[1], 0, 1, 2, 3, 4, 5, 6, 7), lo[s] = __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
 };
 
 // A tile of the cache in LDS: keys as rows of halves with 16 bytes between them (conflict-free reads of 16 bytes), values with piece p of 16 bytes of
-// a row at p ^ swizzle(row), so that the 16 rows that a transposing read touches spread over the banks.
+// a row at p ^ swizzle(row), so that the 4 rows of 32 bytes that 16 lanes of a transposing read touch are on different banks.
 template <int HD, int KT>
 struct Tile {
     static constexpr int LD = HD + 8;
     _Float16 k[2][KT][LD];
     _Float16 v[2][KT][HD];
-    static __device__ __forceinline__ uint32_t swizzle(uint32_t row) { return HD >= 64 ? row & 7u : row >> 1 & 3u; }
+    static __device__ __forceinline__ uint32_t swizzle(uint32_t row) { return HD >= 64 ? (row & 3u) << 1 | (row >> 2 & 1u) : row & 2u; }
 };
 
 // A thread's share of a tile as loaded: P pieces of W words of one block of one row, of keys and of values.
@@ -113,30 +141,31 @@ struct Raw {
     uint16_t kd[P], vd[P];
 };
 
-template <int HD, int WQ, int WK>
-__global__ __launch_bounds__(64 * WQ * WK) void attention_q4_kernel(Q4AttentionArgs a) {
-    constexpr int KT = 32 * WK, NT = 64 * WQ * WK, SLABS = HD / 32, CS = HD / 16, kWords = KT * HD / 8 / NT, W = kWords < 4 ? kWords : 4, P = kWords / W;
-    constexpr int kStates = 2 + HD / 4;
+template <int HD, int WQ, int WK, int PER_CU>
+__global__ __launch_bounds__(64 * WQ * WK, PER_CU * WQ * WK / 4) void attention_q4_kernel(Q4AttentionArgs a) {
+    constexpr int KT = 32 * WK, NT = 64 * WQ * WK, SLABS = HD / 16, DT = HD / 32, kWords = KT * HD / 8 / NT, W = kWords < 4 ? kWords : 4, P = kWords / W;
+    constexpr int kStates = 2 + HD / 2;
+    constexpr uint32_t RB = 32 * WQ;  // query rows of a workgroup
     static_assert(kWords >= 1 && W * P * NT == KT * HD / 8, "every thread moves the same number of words");
     using Share = Raw<W, P>;
     using T = Tile<HD, KT>;
-    constexpr bool TWO = 2 * sizeof(T) <= 160 * 1024;
+    constexpr bool TWO = 2 * sizeof(T) * PER_CU <= 160 * 1024;
     constexpr size_t kTiles = (TWO ? 2 : 1) * sizeof(T), kStateBytes = sizeof(float) * kStates * 64 * WQ * (WK - 1);
     __shared__ __align__(16) uint8_t smem[kTiles > kStateBytes ? kTiles : kStateBytes];
     T* const tiles = reinterpret_cast<T*>(smem);
-    const uint32_t group = a.n_heads / a.n_kv_heads, rows = a.n * group, blocks = (rows + 16u * WQ - 1u) / (16u * WQ);
-    // Workgroups go to the eight XCDs in turn: a KV head's share an L2 where there are eight of them.  Those with the most to see first.
-    const uint32_t c = blockIdx.x % a.n_kv_heads, split = blockIdx.x / a.n_kv_heads % a.splits, block = blocks - 1u - blockIdx.x / a.n_kv_heads / a.splits;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, l16 = lane & 15u, g = lane >> 4;
+    const uint32_t group = a.n_heads / a.n_kv_heads, rows = a.n * group, blocks = (rows + RB - 1u) / RB;
+    // Workgroups go to the eight XCDs in turn: a KV head's share an L2 where there are eight of them.  Those with the most to see first; where all of them are on
+    // the GPU at once, two a CU, the second half the other way round, so that a CU's two have as much together as any other's.
+    const uint32_t c = blockIdx.x % a.n_kv_heads, split = blockIdx.x / a.n_kv_heads % a.splits, nth = blockIdx.x / a.n_kv_heads / a.splits;
+    const uint32_t block = PER_CU == 2 && nth >= a.first_blocks ? nth - a.first_blocks : blocks - 1u - nth;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, l32 = lane & 31u, h = lane >> 5, l16 = lane & 15u;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6)), wq = wave / WK, wk = wave % WK;
-    const uint32_t base = first_row(a), r0 = block * 16u * WQ + 16u * wq;
-    const uint32_t wg_last = sees(a, base, block * 16u * WQ + 16u * WQ - 1u, rows, group), n_tiles = wg_last / KT + 1u, used = used_splits(a.splits, n_tiles);
+    const uint32_t base = first_row(a), r0 = block * RB + 32u * wq;
+    const uint32_t wg_last = sees(a, base, block * RB + RB - 1u, rows, group), n_tiles = wg_last / KT + 1u, used = used_splits(a.splits, n_tiles);
     if (split >= used) return;
     const uint32_t t_first = (uint32_t)((uint64_t)n_tiles * split / used), t_end = (uint32_t)((uint64_t)n_tiles * (split + 1u) / used);
     const bool active = r0 < rows;
-    const uint32_t r = min(r0 + l16, rows - 1u), mine = sees(a, base, r, rows, group), wave_first = sees(a, base, r0, rows, group), wave_last = sees(a, base, r0 + 15u, rows, group);
-    Queries<HD> q;
-    q.load(a, r, c, group, g);
+    const uint32_t r = min(r0 + l32, rows - 1u), mine = sees(a, base, r, rows, group), wave_first = sees(a, base, r0, rows, group), wave_last = sees(a, base, r0 + 31u, rows, group);
 
     const Q4Cache kc = q4_planes(const_cast<void*>(a.k_cache), a.max_seq, a.n_kv_heads, HD), vc = q4_planes(const_cast<void*>(a.v_cache), a.max_seq, a.n_kv_heads, HD);
     const size_t first = (size_t)c * a.max_seq;
@@ -170,88 +199,94 @@ __global__ __launch_bounds__(64 * WQ * WK) void attention_q4_kernel(Q4AttentionA
             }
         }
     };
-    // V^T rows (dims) 16 cc + l16, keys 32 wk + 16 u + 4 g ..: the 16 lanes of a lane group point at 4 keys x 16 dims, lane i at key i / 4 and dims
-    // 4 (i % 4) .. of them, and the read hands every lane four keys of one dim.
-    const uint32_t vkey = 32u * wk + 4u * g + (l16 >> 2);
-    const auto read_v = [&](const T& t, int plane, int cc) {
+    // V^T rows (dims) 32 i + l32, keys 16 s + 8 u + 4 h ..: the 16 lanes of a group point at 4 keys x 16 dims, lane j at key j / 4 and dims
+    // 4 (j % 4) .. of them, and the read hands every lane four keys of one dim.
+    const uint32_t vkey = 32u * wk + 4u * h + (l16 >> 2), vpiece = 2u * (lane >> 4 & 1u) + (l16 >> 1 & 1u);
+    const auto read_v = [&](const T& t, int plane, int i, int s) {
         typedef short s4 __attribute__((ext_vector_type(4)));
         typedef __attribute__((address_space(3))) s4* lds_s4;
-        const _Float16* const p = &t.v[plane][vkey][8u * ((2u * cc + (l16 >> 1 & 1u)) ^ T::swizzle(vkey)) + 4u * (l16 & 1u)];
+        const _Float16* const p = &t.v[plane][vkey][8u * ((4u * i + vpiece) ^ T::swizzle(vkey)) + 4u * (l16 & 1u)] + 16 * s * HD;  // (keys 8 apart swizzle alike)
         const h4 a0 = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p));
-        const h4 a1 = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + 16 * HD)));  // (keys 16 apart swizzle alike)
+        const h4 a1 = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + 8 * HD)));
         return h8{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
     };
 
-    v4f o[CS];
+    Queries<HD> q;
+    v16f o[DT];
 #pragma unroll
-    for (int i = 0; i < CS; i++) o[i] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < DT; i++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[i][e] = 0.0f;
     float m_run = -__builtin_inff(), l_run = 0.0f;
     const auto attend = [&](const T& t, uint32_t t0) {
         const uint32_t key0 = t0 + 32u * wk;
         if (!active || key0 > wave_last) return;
-        v4f sc[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
+        v16f sc;
+#pragma unroll
+        for (int e = 0; e < 16; e++) sc[e] = 0.0f;
 #pragma unroll
         for (int s = 0; s < SLABS; s++) {
-            h8 kh[2], kl[2];
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                kh[u] = *reinterpret_cast<const h8*>(&t.k[0][32u * wk + 16 * u + l16][32 * s + 8 * g]);
-                kl[u] = *reinterpret_cast<const h8*>(&t.k[1][32u * wk + 16 * u + l16][32 * s + 8 * g]);
-            }
-#pragma unroll
-            for (int u = 0; u < 2; u++) sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl[u], q.hi[s], sc[u], 0, 0, 0);
-#pragma unroll
-            for (int u = 0; u < 2; u++) sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[u], q.lo[s], sc[u], 0, 0, 0);
-#pragma unroll
-            for (int u = 0; u < 2; u++) sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[u], q.hi[s], sc[u], 0, 0, 0);
+            const h8 kh = *reinterpret_cast<const h8*>(&t.k[0][32u * wk + l32][16 * s + 8 * h]), kl = *reinterpret_cast<const h8*>(&t.k[1][32u * wk + l32][16 * s + 8 * h]);
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, q.hi[s], sc, 0, 0, 0);
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, q.lo[s], sc, 0, 0, 0);
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, q.hi[s], sc, 0, 0, 0);
         }
+        h8 vh = read_v(t, 0, 0, 0), vl = read_v(t, 1, 0, 0);  // (on its way while the softmax runs)
         if (key0 + 31u > wave_first) {  // some query row does not see all of the keys
 #pragma unroll
-            for (int u = 0; u < 2; u++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (key0 + 16u * u + 4u * g + i > mine) sc[u][i] = -__builtin_inff();
+            for (int e = 0; e < 16; e++)
+                if (key0 + 8u * (e >> 2) + 4u * h + (e & 3) > mine) sc[e] = -__builtin_inff();
         }
-        float top = -__builtin_inff();
+        float top = sc[0];
 #pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) top = fmaxf(top, sc[u][i]);
-        const float m_new = fmaxf(m_run, groups_max(top) * q.factor), m_sub = m_new == -__builtin_inff() ? 0.0f : m_new;
+        for (int e = 1; e < 16; e++) top = fmaxf(top, sc[e]);
+        const float m_new = fmaxf(m_run, halves_max(top) * q.factor), m_sub = m_new == -__builtin_inff() ? 0.0f : m_new;
         float alpha = 1.0f;
         if (__builtin_amdgcn_ballot_w64(m_new > m_run) != 0) {  // else every factor is one (or acts on zeros)
             alpha = __builtin_amdgcn_exp2f(m_run - m_sub);
             m_run = m_new;
 #pragma unroll
-            for (int i = 0; i < CS; i++) o[i] *= alpha;
+            for (int i = 0; i < DT; i++) o[i] *= alpha;
         }
+        const float shift = m_sub - kWeightBits;
         float sum = 0.0f;
-        h4 hi[2], lo[2];
+        h8 ph[2], pl[2];
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            v4f w;
+        for (int s = 0; s < 2; s++) {
+            h4 hi[2], lo[2];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][i], q.factor, -m_sub));
-                sum += w[i];
+            for (int u = 0; u < 2; u++) {
+                v4f w;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * s + 4 * u + i], q.factor, -shift));
+                    sum += w[i];
+                }
+                split_halves(w, hi[u], lo[u]);
             }
-            split_f16<(int)kWeightScale>(w, hi[u], lo[u]);
+            ph[s] = __builtin_shufflevector(hi[0], hi[1], 0, 1, 2, 3, 4, 5, 6, 7), pl[s] = __builtin_shufflevector(lo[0], lo[1], 0, 1, 2, 3, 4, 5, 6, 7);
         }
         l_run = __builtin_fmaf(l_run, alpha, sum);
-        const h8 ph = __builtin_shufflevector(hi[0], hi[1], 0, 1, 2, 3, 4, 5, 6, 7), pl = __builtin_shufflevector(lo[0], lo[1], 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-        for (int i = 0; i < CS; i++) {
-            const h8 vh = read_v(t, 0, i), vl = read_v(t, 1, i);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph, o[i], 0, 0, 0);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl, o[i], 0, 0, 0);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph, o[i], 0, 0, 0);
-        }
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int i = 0; i < DT; i++) {
+                h8 next_h = vh, next_l = vl;
+                const int next = DT * s + i + 1;
+                if (next < 2 * DT) next_h = read_v(t, 0, next % DT, next / DT), next_l = read_v(t, 1, next % DT, next / DT);
+                __builtin_amdgcn_sched_barrier(0);
+                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[s], o[i], 0, 0, 0);
+                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[s], o[i], 0, 0, 0);
+                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[s], o[i], 0, 0, 0);
+                vh = next_h, vl = next_l;
+            }
     };
 
     // Tile t sits in LDS and t + 1 is on its way in registers: behind the arithmetic of tile t it goes where tile t - 1 was (or t, where there is no
     // room for two, behind a barrier more) and t + 2 is requested.
     Share raw;
     fetch(t_first, raw);
+    q.load(a, r, c, group, h);
     store(tiles[0], raw);
     if (t_first + 1u < t_end) fetch(t_first + 1u, raw);
     __syncthreads();
@@ -266,16 +301,16 @@ __global__ __launch_bounds__(64 * WQ * WK) void attention_q4_kernel(Q4AttentionA
         __syncthreads();
     }
 
-    l_run = groups_sum(l_run);
+    l_run = halves_sum(l_run);
     if constexpr (WK > 1) {  // the waves of other keys hand their states to the first
         float* const state = reinterpret_cast<float*>(smem) + (size_t)wq * (WK - 1) * kStates * 64u + lane;
         if (wk != 0) {
             float* const to = state + (size_t)(wk - 1u) * kStates * 64u;
             to[0] = m_run, to[64] = l_run;
 #pragma unroll
-            for (int i = 0; i < CS; i++)
+            for (int i = 0; i < DT; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) to[(2 + 4 * i + e) * 64] = o[i][e];
+                for (int e = 0; e < 16; e++) to[(2 + 16 * i + e) * 64] = o[i][e];
         }
         __syncthreads();
         if (wk != 0) return;
@@ -285,36 +320,40 @@ __global__ __launch_bounds__(64 * WQ * WK) void attention_q4_kernel(Q4AttentionA
         float f = __builtin_amdgcn_exp2f(m_run - m_sub);
         l_run *= f;
 #pragma unroll
-        for (int i = 0; i < CS; i++) o[i] *= f;
+        for (int i = 0; i < DT; i++) o[i] *= f;
         for (int k = 0; k < WK - 1; k++) {
             const float* const from = state + k * kStates * 64;
             f = __builtin_amdgcn_exp2f(from[0] - m_sub);
             l_run = __builtin_fmaf(from[64], f, l_run);
 #pragma unroll
-            for (int i = 0; i < CS; i++)
+            for (int i = 0; i < DT; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) o[i][e] = __builtin_fmaf(from[(2 + 4 * i + e) * 64], f, o[i][e]);
+                for (int e = 0; e < 16; e++) o[i][e] = __builtin_fmaf(from[(2 + 16 * i + e) * 64], f, o[i][e]);
         }
         m_run = m_all;
     }
-    if (r0 + l16 >= rows) return;
-    // register e of o[i] holds dim 16 i + 4 g + e of row l16
+    if (r0 + l32 >= rows) return;
+    // register e of o[i] holds dim 32 i + 8 (e / 4) + 4 h + e % 4 of row l32
     const uint32_t token = r / group, head = c * group + r % group;
+    float* to;
+    float inverse = 1.0f;
     if (a.splits == 1u) {
-        float* const to = a.out + (size_t)token * a.out_stride + (size_t)head * HD + 4u * g;
-        const float inverse = __fdiv_rn(1.0f / kWeightScale, l_run);
-#pragma unroll
-        for (int i = 0; i < CS; i++) *reinterpret_cast<v4f*>(to + 16 * i) = o[i] * inverse;
-        if (a.stats && g == 0) {
+        to = a.out + (size_t)token * a.out_stride + (size_t)head * HD;
+        inverse = __fdiv_rn(1.0f, l_run);
+        if (a.stats && h == 0) {
             float* const st = a.stats + 2u * ((size_t)token * a.n_heads + head);
-            st[0] = m_run, st[1] = __fdiv_rn(1.0f, l_run);
+            st[0] = m_run, st[1] = inverse;
         }
-        return;
+    } else {
+        to = a.parts + (((size_t)token * a.n_heads + head) * a.splits + split) * (HD + 4);
+        if (h == 0) to[0] = m_run, to[1] = l_run;
+        to += 4;
     }
-    float* const to = a.parts + (((size_t)token * a.n_heads + head) * a.splits + split) * (HD + 4);
-    if (g == 0) to[0] = m_run, to[1] = l_run;
 #pragma unroll
-    for (int i = 0; i < CS; i++) *reinterpret_cast<v4f*>(to + 4 + 16 * i + 4 * g) = o[i];
+    for (int i = 0; i < DT; i++)
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            *reinterpret_cast<v4f*>(to + 32 * i + 8 * k + 4 * h) = v4f{o[i][4 * k], o[i][4 * k + 1], o[i][4 * k + 2], o[i][4 * k + 3]} * inverse;
 }
 
 // The splits of one (token, head) merged: a wave turns their (maximum, sum) pairs into weights, then every thread sums its share of the values.
@@ -332,8 +371,8 @@ __global__ __launch_bounds__(256) void attention_q4_merge_kernel(Q4AttentionArgs
         const float m = wave_max_f32(m_i), m_sub = m == -__builtin_inff() ? 0.0f : m, w = __builtin_amdgcn_exp2f(m_i - m_sub), l = wave_sum_f32(l_i * w);
         weights[tid] = w;
         if (tid == 0) {
-            inverse = __fdiv_rn(1.0f / kWeightScale, l);
-            if (a.stats) a.stats[2u * at] = m, a.stats[2u * at + 1u] = __fdiv_rn(1.0f, l);
+            inverse = __fdiv_rn(1.0f, l);
+            if (a.stats) a.stats[2u * at] = m, a.stats[2u * at + 1u] = inverse;
         }
     }
     __syncthreads();
@@ -348,14 +387,14 @@ __global__ __launch_bounds__(256) void attention_q4_merge_kernel(Q4AttentionArgs
 }
 
 // What 64 rows of a KV head have gathered: the scores once more, now that every softmax's maximum and sum is known, and their weights added
-// up over the query rows -- 16 of them at a time and wave, kept apart by lane and wave and added in one order at the end.
+// up over the query rows -- 32 of them at a time and wave, kept apart by lane and wave and added in one order at the end.
 template <int HD, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void attention_q4_weights_kernel(Q4AttentionArgs a) {
-    constexpr int KT = 64, LD = HD + 8, SLABS = HD / 32, U = KT / 16;
+    constexpr int KT = 64, LD = HD + 8, SLABS = HD / 16, U = KT / 32;
     __shared__ __align__(16) _Float16 keys[2][KT][LD];
     __shared__ float sums[WAVES][KT];
     const uint32_t c = blockIdx.y, key0 = blockIdx.x * KT, group = a.n_heads / a.n_kv_heads, rows = a.n * group;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, l16 = lane & 15u, g = lane >> 4, wave = tid >> 6;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, l32 = lane & 31u, h = lane >> 5, wave = tid >> 6;
     const uint32_t base = first_row(a), last = sees(a, base, rows - 1u, rows, group);
     if (key0 > last) return;
     const Q4Cache kc = q4_planes(const_cast<void*>(a.k_cache), a.max_seq, a.n_kv_heads, HD), vc = q4_planes(const_cast<void*>(a.v_cache), a.max_seq, a.n_kv_heads, HD);
@@ -369,39 +408,43 @@ __global__ __launch_bounds__(64 * WAVES) void attention_q4_weights_kernel(Q4Atte
         *reinterpret_cast<h8*>(&keys[0][row][8u * word]) = hi, *reinterpret_cast<h8*>(&keys[1][row][8u * word]) = lo;
     }
     __syncthreads();
-    v4f acc[U];
+    v16f acc[U];
 #pragma unroll
-    for (int u = 0; u < U; u++) acc[u] = v4f{0.f, 0.f, 0.f, 0.f};
-    const uint32_t r_first = key0 > base ? (key0 - base) * group / 16u * 16u : 0u;  // rows in front of it see none of the keys
-    for (uint32_t r0 = r_first + 16u * wave; r0 < rows; r0 += 16u * WAVES) {
-        const uint32_t r = min(r0 + l16, rows - 1u), mine = sees(a, base, r, rows, group);
+    for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) acc[u][e] = 0.0f;
+    const uint32_t r_first = key0 > base ? (key0 - base) * group / 32u * 32u : 0u;  // rows in front of it see none of the keys
+    for (uint32_t r0 = r_first + 32u * wave; r0 < rows; r0 += 32u * WAVES) {
+        const uint32_t r = min(r0 + l32, rows - 1u), mine = sees(a, base, r, rows, group);
         Queries<HD> q;
-        q.load(a, r, c, group, g);
+        q.load(a, r, c, group, h);
         const float* const st = a.stats + 2u * ((size_t)(r / group) * a.n_heads + c * group + r % group);
-        const float m = st[0] == -__builtin_inff() ? 0.0f : st[0], inverse = r0 + l16 < rows ? st[1] : 0.0f;
+        const float shift = (st[0] == -__builtin_inff() ? 0.0f : st[0]) - kWeightBits, inverse = st[1];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            v4f sc = {0.f, 0.f, 0.f, 0.f};
+            v16f sc;
+#pragma unroll
+            for (int e = 0; e < 16; e++) sc[e] = 0.0f;
 #pragma unroll
             for (int s = 0; s < SLABS; s++) {
-                const h8 kh = *reinterpret_cast<const h8*>(&keys[0][16 * u + l16][32 * s + 8 * g]), kl = *reinterpret_cast<const h8*>(&keys[1][16 * u + l16][32 * s + 8 * g]);
-                sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, q.hi[s], sc, 0, 0, 0);
-                sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, q.lo[s], sc, 0, 0, 0);
-                sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, q.hi[s], sc, 0, 0, 0);
+                const h8 kh = *reinterpret_cast<const h8*>(&keys[0][32 * u + l32][16 * s + 8 * h]), kl = *reinterpret_cast<const h8*>(&keys[1][32 * u + l32][16 * s + 8 * h]);
+                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, q.hi[s], sc, 0, 0, 0);
+                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, q.lo[s], sc, 0, 0, 0);
+                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, q.hi[s], sc, 0, 0, 0);
             }
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], q.factor, -m)) * inverse;
-                acc[u][i] += key0 + 16u * u + 4u * g + i > mine || r0 + l16 >= rows ? 0.0f : w;
+            for (int e = 0; e < 16; e++) {
+                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], q.factor, -shift)) * inverse;
+                acc[u][e] += key0 + 32u * u + 8u * (e >> 2) + 4u * h + (e & 3) > mine || r0 + l32 >= rows ? 0.0f : w;
             }
         }
     }
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float w = group_sum<16>(acc[u][i]);
-            if (l16 == 0) sums[wave][16 * u + 4 * g + i] = w;
+        for (int e = 0; e < 16; e++) {
+            const float w = group_sum<32>(acc[u][e]);
+            if (l32 == 0) sums[wave][32 * u + 8 * (e >> 2) + 4 * h + (e & 3)] = w;
         }
     __syncthreads();
     if (tid < KT && key0 + tid <= last) {
@@ -411,16 +454,18 @@ __global__ __launch_bounds__(64 * WAVES) void attention_q4_weights_kernel(Q4Atte
     }
 }
 
-// The workgroup's shape for `rows` query rows of a KV head.
-template <int HD, int WQ, int WK>
+template <int HD, int WQ, int WK, int PER_CU>
 hipError_t launch_tiles(Q4AttentionArgs a, const Launch& L) {
-    const uint32_t rows = a.n * (a.n_heads / a.n_kv_heads), base = a.n_kv_heads * ((rows + 16u * WQ - 1u) / (16u * WQ));
+    constexpr uint32_t RB = 32 * WQ, KT = 32 * WK;
+    const uint32_t rows = a.n * (a.n_heads / a.n_kv_heads), base = a.n_kv_heads * ((rows + RB - 1u) / RB);
     const uint64_t seen = a.d_pos ? a.max_seq : (uint64_t)a.pos0 + a.n;
-    const uint32_t tiles = (uint32_t)((seen + 32u * WK - 1u) / (32u * WK)), room = kSplitSlots / base;
-    a.splits = room < 2u ? 1u : (room < tiles ? room : tiles);
+    const uint32_t tiles = (uint32_t)((seen + KT - 1u) / KT), room = kCus * PER_CU / base, most = rows <= 32u ? tiles : (tiles + 2u) / 3u;
+    a.splits = room < 2u ? 1u : (room < most ? room : most);
     if (a.splits > kMaxSplits) a.splits = kMaxSplits;
-    hipError_t e = launch_kernel(L, kFamOther, attention_q4_kernel<HD, WQ, WK>, dim3(base * a.splits), dim3(64 * WQ * WK), a);
-    if (e == hipSuccess && a.splits > 1u) e = launch_kernel(L, kFamOther, attention_q4_merge_kernel<HD>, dim3(a.n * a.n_heads), dim3(256), a, 16u * WQ, 32u * WK);
+    const uint32_t blocks = base / a.n_kv_heads;
+    a.first_blocks = base * a.splits > kCus && base * a.splits <= 2u * kCus ? (kCus + a.n_kv_heads * a.splits - 1u) / (a.n_kv_heads * a.splits) : blocks;
+    hipError_t e = launch_kernel(L, kFamOther, attention_q4_kernel<HD, WQ, WK, PER_CU>, dim3(base * a.splits), dim3(64 * WQ * WK), a);
+    if (e == hipSuccess && a.splits > 1u) e = launch_kernel(L, kFamOther, attention_q4_merge_kernel<HD>, dim3(a.n * a.n_heads), dim3(256), a, RB, KT);
     return e;
 }
 
@@ -428,14 +473,14 @@ template <int HD>
 hipError_t launch_head_dim(const Q4AttentionArgs& a, const Launch& L) {
     const uint32_t rows = a.n * (a.n_heads / a.n_kv_heads);
     hipError_t e;
-    if constexpr (HD == 32) e = launch_tiles<HD, 2, 2>(a, L);
-    else if constexpr (HD == 256) e = launch_tiles<HD, 4, 1>(a, L);
-    else if (rows <= 16u) e = launch_tiles<HD, 1, HD == 64 ? 4 : 2>(a, L);
-    else e = launch_tiles<HD, 4, 2>(a, L);
+    if constexpr (HD == 32) e = launch_tiles<HD, 2, 2, 4>(a, L);
+    else if constexpr (HD == 64) e = rows <= 32u ? launch_tiles<HD, 1, 4, 1>(a, L) : launch_tiles<HD, 4, 2, 2>(a, L);
+    else if constexpr (HD == 128) e = rows <= 32u ? launch_tiles<HD, 1, 2, 1>(a, L) : launch_tiles<HD, 4, 2, 1>(a, L);
+    else e = launch_tiles<HD, 4, 1, 1>(a, L);
     if (e != hipSuccess || !a.weights) return e;
     const uint64_t seen = a.d_pos ? a.max_seq : (uint64_t)a.pos0 + a.n;
     const dim3 grid((uint32_t)((seen + 63) / 64), a.n_kv_heads);
-    return rows <= 16u ? launch_kernel(L, kFamOther, attention_q4_weights_kernel<HD, 1>, grid, dim3(64), a)
+    return rows <= 32u ? launch_kernel(L, kFamOther, attention_q4_weights_kernel<HD, 1>, grid, dim3(64), a)
                        : launch_kernel(L, kFamOther, attention_q4_weights_kernel<HD, 8>, grid, dim3(512), a);
 }
 
@@ -457,7 +502,7 @@ hipError_t launch_attention_q4(const float* d_q, uint32_t q_stride, const void* 
                                uint32_t n_kv_heads, uint32_t head_dim, float scale, const Launch& L) {
     if (n == 0) return hipSuccess;
     const Q4AttentionArgs a{d_q, d_k_cache, d_v_cache, d_out, d_scratch, d_weights ? d_scratch + part_floats(n, n_heads, head_dim) : nullptr, d_weights, d_pos,
-                            pos0, n, q_stride, out_stride, max_seq, n_heads, n_kv_heads, 1, scale};
+                            pos0, n, q_stride, out_stride, max_seq, n_heads, n_kv_heads, 1, 0, scale};
     switch (head_dim) {
         case 32: return launch_head_dim<32>(a, L);
         case 64: return launch_head_dim<64>(a, L);
