@@ -106,7 +106,7 @@ int wick_rocm_attention_prefill_quantize_q8_0(wick_rocm_ctx *ctx, const float *d
  * what a step waits for.  The reference's counterpart is its compressed cache (wick/src/turboquant.rs, 3-bit keys and 2-bit values with
  * rotations and codebooks); this one holds plain blocks, like the weights.
  *
- * A cache of max_seq rows (n_kv_heads heads of head_dim values; 32, 64, 128 or 256) is one buffer of wick_rocm_kv_q4_bytes(...)
+ * A cache of max_seq rows (at most 2^24; n_kv_heads heads of head_dim values; 32, 64, 128 or 256) is one buffer of wick_rocm_kv_q4_bytes(...)
  * bytes (0: not such a shape), 16-byte aligned: the quants, [n_kv_heads][max_seq][head_dim / 8] 32-bit words of 8 consecutive values
  * each, value 2 i in bits 4 i .. and value 2 i + 1 in bits 16 + 4 i .., and behind them the scales, [n_kv_heads][max_seq]
  * [head_dim / 32] f16, one to a block of 32 values.  A value stands for (nibble - 8) * scale.

@@ -78,7 +78,7 @@ int main() {
         {"head_dim 0", kShape, [](Call& a) { a.hd = 0; }},          {"head_dim 48", kShape, [](Call& a) { a.hd = 48; }},
         {"head_dim 96", kShape, [](Call& a) { a.hd = 96; }},        {"head_dim 512", kShape, [](Call& a) { a.hd = 512; }},
         {"no KV heads", kShape, [](Call& a) { a.n_kv = 0; }},       {"too many KV heads", kShape, [](Call& a) { a.n_kv = 1u << 16; }},
-        {"no rows", kShape, [](Call& a) { a.max_seq = 0; }},        {"too many rows", kShape, [](Call& a) { a.max_seq = (1u << 30) + 1; }},
+        {"no rows", kShape, [](Call& a) { a.max_seq = 0; }},        {"too many rows", kShape, [](Call& a) { a.max_seq = (1u << 24) + 1; }},
     };
     const auto with = [&](std::vector<Wrong> more) {
         more.insert(more.end(), shape.begin(), shape.end());
@@ -154,7 +154,7 @@ int main() {
     const long before = fake_hip::launches;
     if (append(ctx, none) || read(ctx, none) || prefill(ctx, none) || fake_hip::launches != before) failures++, std::printf("no tokens\n");
     if (wick_rocm_kv_q4_bytes(100, 3, 64) != 100 * 3 * 36 || wick_rocm_kv_q4_bytes(100, 3, 48) || wick_rocm_kv_q4_bytes(0, 3, 64) ||
-        wick_rocm_kv_q4_bytes(1u << 30, 8, 256) != (size_t)8 * 144 << 30)
+        wick_rocm_kv_q4_bytes(1u << 24, 8, 256) != (size_t)8 * 144 << 24 || wick_rocm_kv_q4_bytes((1u << 24) + 1, 8, 256))
         failures++, std::printf("bytes\n");
     // the scratch of many tokens serves fewer
     for (uint32_t hd : {32u, 64u, 128u, 256u})

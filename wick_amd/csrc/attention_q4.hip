@@ -49,17 +49,19 @@ __device__ __forceinline__ uint32_t sees(const Q4AttentionArgs& a, uint32_t base
 // Splits that a workgroup of `tiles` tiles has in earnest: with the position on the device the host does not know.
 __device__ __forceinline__ uint32_t used_splits(uint32_t splits, uint32_t tiles) { return min(splits, tiles); }
 
-// Eight values of a word as two planes of halves.  (The mask in a scalar and the offset's bits in a vector register: one instruction takes both.)
-__device__ __forceinline__ void dequantize(uint32_t w, _Float16 scale, h8& hi, h8& lo) {
+// Eight values of a word as two planes of halves, a pair at a time.  (The mask in a scalar and the offset's bits in a vector register: one instruction
+// takes both.)
+__device__ __forceinline__ void dequantize_pair(uint32_t w, _Float16 scale, int i, h8& hi, h8& lo) {
     const h2 d = {scale, scale}, offset = {(_Float16)1032.0f, (_Float16)1032.0f};
     uint32_t mask = 0x000f000fu, bits = 0x64006400u;
     asm("" : "+s"(mask), "+v"(bits));
+    const h2 n = __builtin_bit_cast(h2, ((w >> (4 * i)) & mask) | bits) - offset;  // 1024 + nibble, exact
+    const h2 h = n * d, l = __builtin_elementwise_fma(n, d, -h);
+    hi[2 * i] = h[0], hi[2 * i + 1] = h[1], lo[2 * i] = l[0], lo[2 * i + 1] = l[1];
+}
+__device__ __forceinline__ void dequantize(uint32_t w, _Float16 scale, h8& hi, h8& lo) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const h2 n = __builtin_bit_cast(h2, ((w >> (4 * i)) & mask) | bits) - offset;  // 1024 + nibble, exact
-        const h2 h = n * d, l = __builtin_elementwise_fma(n, d, -h);
-        hi[2 * i] = h[0], hi[2 * i + 1] = h[1], lo[2 * i] = l[0], lo[2 * i + 1] = l[1];
-    }
+    for (int i = 0; i < 4; i++) dequantize_pair(w, scale, i, hi, lo);
 }
 
 // Four f32 values as two planes: a pair at a time, then one instruction a value (y * 1 - hi, rounded to a half; the compiler does not see the 1 and cannot
@@ -121,23 +123,25 @@ struct Queries {
     }
 };
 
-// A tile of the cache in LDS: keys as rows of halves with 16 bytes between them (conflict-free reads of 16 bytes), values with piece p of 16 bytes of
-// a row at p ^ swizzle(row), so that the 4 rows of 32 bytes that 16 lanes of a transposing read touch are on different banks.
+// A tile of the cache in LDS, two planes of halves: keys as rows with 16 bytes between them (conflict-free reads of 16 bytes), values with piece p of
+// 16 bytes of a row at p ^ swizzle(row), so that the 4 rows of 32 bytes that 16 lanes of a transposing read touch are on different banks.
 template <int HD, int KT>
-struct Tile {
-    static constexpr int LD = HD + 8;
-    _Float16 k[2][KT][LD];
-    _Float16 v[2][KT][HD];
+struct KeyTile {
+    _Float16 h[2][KT][HD + 8];
+};
+template <int HD, int KT>
+struct ValueTile {
+    _Float16 h[2][KT][HD];
     static __device__ __forceinline__ uint32_t swizzle(uint32_t row) { return HD >= 64 ? (row & 3u) << 1 | (row >> 2 & 1u) : row & 2u; }
 };
 
-// A thread's share of a tile as loaded: P pieces of W words of one block of one row, of keys and of values.
+// A thread's share of a tile of keys or of values as loaded: P pieces of W words of one block of one row, and the block's scales.
 template <int W, int P>
 struct Raw {
     struct __attribute__((aligned(4 * W))) Words {
         uint32_t w[W];
     };
-    Words k[P], v[P];
+    Words w[P];
     uint16_t kd[P], vd[P];
 };
 
@@ -148,11 +152,11 @@ __global__ __launch_bounds__(64 * WQ * WK, PER_CU * WQ * WK / 4) void attention_
     constexpr uint32_t RB = 32 * WQ;  // query rows of a workgroup
     static_assert(kWords >= 1 && W * P * NT == KT * HD / 8, "every thread moves the same number of words");
     using Share = Raw<W, P>;
-    using T = Tile<HD, KT>;
-    constexpr bool TWO = 2 * sizeof(T) * PER_CU <= 160 * 1024;
-    constexpr size_t kTiles = (TWO ? 2 : 1) * sizeof(T), kStateBytes = sizeof(float) * kStates * 64 * WQ * (WK - 1);
+    using VT = ValueTile<HD, KT>;
+    constexpr size_t kTiles = 2 * (sizeof(KeyTile<HD, KT>) + sizeof(VT)), kStateBytes = sizeof(float) * kStates * 64 * WQ * (WK - 1);
     __shared__ __align__(16) uint8_t smem[kTiles > kStateBytes ? kTiles : kStateBytes];
-    T* const tiles = reinterpret_cast<T*>(smem);
+    KeyTile<HD, KT>* const k_tile = reinterpret_cast<KeyTile<HD, KT>*>(smem);
+    VT* const v_tile = reinterpret_cast<VT*>(smem + 2 * sizeof(KeyTile<HD, KT>));
     const uint32_t group = a.n_heads / a.n_kv_heads, rows = a.n * group, blocks = (rows + RB - 1u) / RB;
     // Workgroups go to the eight XCDs in turn: a KV head's share an L2 where there are eight of them.  Those with the most to see first; where all of them are on
     // the GPU at once, two a CU, the second half the other way round, so that a CU's two have as much together as any other's.
@@ -164,48 +168,62 @@ __global__ __launch_bounds__(64 * WQ * WK, PER_CU * WQ * WK / 4) void attention_
     const uint32_t wg_last = sees(a, base, block * RB + RB - 1u, rows, group), n_tiles = wg_last / KT + 1u, used = used_splits(a.splits, n_tiles);
     if (split >= used) return;
     const uint32_t t_first = (uint32_t)((uint64_t)n_tiles * split / used), t_end = (uint32_t)((uint64_t)n_tiles * (split + 1u) / used);
-    const bool active = r0 < rows;
-    const uint32_t r = min(r0 + l32, rows - 1u), mine = sees(a, base, r, rows, group), wave_first = sees(a, base, r0, rows, group), wave_last = sees(a, base, r0 + 31u, rows, group);
+    const uint32_t r = min(r0 + l32, rows - 1u), mine = sees(a, base, r, rows, group), wave_first = sees(a, base, r0, rows, group);
 
     const Q4Cache kc = q4_planes(const_cast<void*>(a.k_cache), a.max_seq, a.n_kv_heads, HD), vc = q4_planes(const_cast<void*>(a.v_cache), a.max_seq, a.n_kv_heads, HD);
     const size_t first = (size_t)c * a.max_seq;
-    // Rows past the last one that any query row sees repeat it (their weights are zero).
-    const auto fetch = [&](uint32_t t, Share& x) {
+    // The tiles from t_first on, one behind the other, by offsets into what the workgroup's rows see of each plane: a read behind it gives zeros (whose weights
+    // the mask makes zeros).
+    const uint32_t from = t_first * KT, seen = wg_last + 1u - from;
+    const auto plane = [&](const void* p, uint32_t row_bytes) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(static_cast<const uint8_t*>(p)) + (first + from) * row_bytes, 0, (int)(seen * row_bytes), 0x27000);
+    };
+    const auto kq = plane(kc.quants, HD / 2), vq = plane(vc.quants, HD / 2), ks = plane(kc.scales, HD / 16), vs = plane(vc.scales, HD / 16);
+    uint32_t q_at[P], s_at[P];  // of this thread's pieces in the tile that is requested next
+#pragma unroll
+    for (int p = 0; p < P; p++) q_at[p] = (p * NT + tid) * W * 4u, s_at[p] = (p * NT + tid) * W / 4u * 2u;
+    const auto fetch = [&](Share& x, bool keys) {
 #pragma unroll
         for (int p = 0; p < P; p++) {
-            const uint32_t i = (p * NT + tid) * W, word = i % (HD / 8);
-            const size_t at = first + min(t * KT + i / (HD / 8), wg_last);
-            x.k[p] = *reinterpret_cast<const typename Share::Words*>(kc.quants + at * (HD / 8) + word);
-            x.v[p] = *reinterpret_cast<const typename Share::Words*>(vc.quants + at * (HD / 8) + word);
-            x.kd[p] = kc.scales[at * (HD / 32) + word / 4u], x.vd[p] = vc.scales[at * (HD / 32) + word / 4u];
+            if constexpr (W == 1) x.w[p].w[0] = __builtin_amdgcn_raw_buffer_load_b32(keys ? kq : vq, q_at[p], 0, 0);
+            if constexpr (W == 2) x.w[p] = __builtin_bit_cast(typename Share::Words, __builtin_amdgcn_raw_buffer_load_b64(keys ? kq : vq, q_at[p], 0, 0));
+            if constexpr (W == 4) x.w[p] = __builtin_bit_cast(typename Share::Words, __builtin_amdgcn_raw_buffer_load_b128(keys ? kq : vq, q_at[p], 0, 0));
+            x.vd[p] = __builtin_amdgcn_raw_buffer_load_b16(vs, s_at[p], 0, 0);
+            if (keys) x.kd[p] = __builtin_amdgcn_raw_buffer_load_b16(ks, s_at[p], 0, 0);
         }
     };
+    const auto next_tile = [&] {
+#pragma unroll
+        for (int p = 0; p < P; p++) q_at[p] += KT * HD / 2, s_at[p] += KT * HD / 16;
+    };
     // Values that are not finite would reach the rows that do not see them (0 times NaN): they are taken as zeros and their keys as NaN, whose scores the
-    // mask replaces.
-    const auto store = [&](T& t, const Share& x) {
-#pragma unroll
-        for (int p = 0; p < P; p++) {
-            const uint32_t i = (p * NT + tid) * W, row = i / (HD / 8), word = i % (HD / 8);
-            const _Float16 vd = __builtin_bit_cast(_Float16, x.vd[p]);
-            const _Float16 poison = vd * (_Float16)0.0f, kd = __builtin_bit_cast(_Float16, x.kd[p]) + poison, vs = poison == poison ? vd : (_Float16)0.0f;
-#pragma unroll
-            for (int e = 0; e < W; e++) {
-                h8 hi, lo;
-                dequantize(x.k[p].w[e], kd, hi, lo);
-                *reinterpret_cast<h8*>(&t.k[0][row][8u * (word + e)]) = hi, *reinterpret_cast<h8*>(&t.k[1][row][8u * (word + e)]) = lo;
-                dequantize(x.v[p].w[e], vs, hi, lo);
-                const uint32_t at = 8u * ((word + e) ^ T::swizzle(row));
-                *reinterpret_cast<h8*>(&t.v[0][row][at]) = hi, *reinterpret_cast<h8*>(&t.v[1][row][at]) = lo;
-            }
+    // mask replaces.  A thread's share is unpacked and stored in kSteps steps, a pair of values each.
+    constexpr int kSteps = 4 * kWords;
+    h8 step_hi, step_lo;
+    _Float16 step_scale;
+    const auto store_step = [&](int buffer, const Share& x, bool keys, int step) {
+        const int p = step / 4 / W, e = step / 4 % W;
+        const uint32_t i = (p * NT + tid) * W, row = i / (HD / 8), word = i % (HD / 8) + e;
+        if (step % (4 * W) == 0) {
+            const _Float16 vd = __builtin_bit_cast(_Float16, x.vd[p]), poison = vd * (_Float16)0.0f;
+            step_scale = keys ? __builtin_bit_cast(_Float16, x.kd[p]) + poison : poison == poison ? vd : (_Float16)0.0f;
         }
+        dequantize_pair(x.w[p].w[e], step_scale, step % 4, step_hi, step_lo);
+        if (step % 4 != 3) return;
+        _Float16* const hi = keys ? &k_tile[buffer].h[0][row][8u * word] : &v_tile[buffer].h[0][row][8u * (word ^ VT::swizzle(row))];
+        *reinterpret_cast<h8*>(hi) = step_hi, *reinterpret_cast<h8*>(hi + (keys ? KT * (HD + 8) : KT * HD)) = step_lo;
+    };
+    const auto store = [&](int buffer, const Share& x, bool keys) {
+#pragma unroll
+        for (int step = 0; step < kSteps; step++) store_step(buffer, x, keys, step);
     };
     // V^T rows (dims) 32 i + l32, keys 16 s + 8 u + 4 h ..: the 16 lanes of a group point at 4 keys x 16 dims, lane j at key j / 4 and dims
     // 4 (j % 4) .. of them, and the read hands every lane four keys of one dim.
     const uint32_t vkey = 32u * wk + 4u * h + (l16 >> 2), vpiece = 2u * (lane >> 4 & 1u) + (l16 >> 1 & 1u);
-    const auto read_v = [&](const T& t, int plane, int i, int s) {
+    const auto read_v = [&](int buffer, int plane, int i, int s) {
         typedef short s4 __attribute__((ext_vector_type(4)));
         typedef __attribute__((address_space(3))) s4* lds_s4;
-        const _Float16* const p = &t.v[plane][vkey][8u * ((4u * i + vpiece) ^ T::swizzle(vkey)) + 4u * (l16 & 1u)] + 16 * s * HD;  // (keys 8 apart swizzle alike)
+        const _Float16* const p = &v_tile[buffer].h[plane][vkey][8u * ((4u * i + vpiece) ^ VT::swizzle(vkey)) + 4u * (l16 & 1u)] + 16 * s * HD;  // (keys 8 apart swizzle alike)
         const h4 a0 = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p));
         const h4 a1 = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + 8 * HD)));
         return h8{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
@@ -217,88 +235,128 @@ __global__ __launch_bounds__(64 * WQ * WK, PER_CU * WQ * WK / 4) void attention_
     for (int i = 0; i < DT; i++)
 #pragma unroll
         for (int e = 0; e < 16; e++) o[i][e] = 0.0f;
-    float m_run = -__builtin_inff(), l_run = 0.0f;
-    const auto attend = [&](const T& t, uint32_t t0) {
-        const uint32_t key0 = t0 + 32u * wk;
-        if (!active || key0 > wave_last) return;
-        v16f sc;
-#pragma unroll
-        for (int e = 0; e < 16; e++) sc[e] = 0.0f;
-#pragma unroll
-        for (int s = 0; s < SLABS; s++) {
-            const h8 kh = *reinterpret_cast<const h8*>(&t.k[0][32u * wk + l32][16 * s + 8 * h]), kl = *reinterpret_cast<const h8*>(&t.k[1][32u * wk + l32][16 * s + 8 * h]);
-            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, q.hi[s], sc, 0, 0, 0);
-            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, q.lo[s], sc, 0, 0, 0);
-            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, q.hi[s], sc, 0, 0, 0);
-        }
-        h8 vh = read_v(t, 0, 0, 0), vl = read_v(t, 1, 0, 0);  // (on its way while the softmax runs)
+    float m_run = -__builtin_inff(), l_run = 0.0f, top;  // (top: of a row's scores of the tile at hand)
+    // One tile's arithmetic, with the scores of the next tile (in the other buffer) and the unpacking of what is stored next in between: a wave's matrix
+    // instructions run beside its vector instructions where they take turns in its program, so they do, in this very order.  (A wave that sees none of the tile's
+    // keys goes along: the workgroup's barriers wait for the others anyway.)
+    const auto attend = [&](int buffer, uint32_t t, v16f& sc, v16f& next, const Share& kraw, const Share& vraw) {
+        const uint32_t key0 = t * KT + 32u * wk;
         if (key0 + 31u > wave_first) {  // some query row does not see all of the keys
 #pragma unroll
             for (int e = 0; e < 16; e++)
                 if (key0 + 8u * (e >> 2) + 4u * h + (e & 3) > mine) sc[e] = -__builtin_inff();
-        }
-        float top = sc[0];
+            top = sc[0];
 #pragma unroll
-        for (int e = 1; e < 16; e++) top = fmaxf(top, sc[e]);
-        const float m_new = fmaxf(m_run, halves_max(top) * q.factor), m_sub = m_new == -__builtin_inff() ? 0.0f : m_new;
-        float alpha = 1.0f;
+            for (int e = 1; e < 16; e++) top = fmaxf(top, sc[e]);
+            top = halves_max(top);
+        }
+        const _Float16* const keys = &k_tile[buffer ^ 1].h[0][32u * wk + l32][8 * h];  // (behind the last tile: whatever is there, for nobody)
+        const auto key = [&](int plane, int s) { return *reinterpret_cast<const h8*>(keys + plane * (KT * (HD + 8)) + 16 * s); };
+        // operands are read kAhead slabs (three matrix instructions each) before their use: as long as LDS takes to answer
+        constexpr int kAhead = HD == 64 ? 3 : 2;
+        h8 kl[SLABS], kh[SLABS], vl[2 * DT], vh[2 * DT];
+#pragma unroll
+        for (int s = 0; s < kAhead && s < SLABS; s++) kl[s] = key(1, s), kh[s] = key(0, s);
+        const float m_new = fmaxf(m_run, top * q.factor), m_sub = m_new == -__builtin_inff() ? 0.0f : m_new;
         if (__builtin_amdgcn_ballot_w64(m_new > m_run) != 0) {  // else every factor is one (or acts on zeros)
-            alpha = __builtin_amdgcn_exp2f(m_run - m_sub);
-            m_run = m_new;
+            const float alpha = __builtin_amdgcn_exp2f(m_run - m_sub);
+            m_run = m_new, l_run *= alpha;
 #pragma unroll
             for (int i = 0; i < DT; i++) o[i] *= alpha;
         }
         const float shift = m_sub - kWeightBits;
-        float sum = 0.0f;
-        h8 ph[2], pl[2];
+        h4 hi[4], lo[4];
+        v4f w[4];
+        const auto softmax_step = [&](int step) {  // 12 of them: the exponentials of four weights two steps ahead of their split
+            if (step % 3 == 0) {
 #pragma unroll
-        for (int s = 0; s < 2; s++) {
-            h4 hi[2], lo[2];
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                v4f w;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * s + 4 * u + i], q.factor, -shift));
-                    sum += w[i];
-                }
-                split_halves(w, hi[u], lo[u]);
+                for (int i = 0; i < 4; i++) w[step / 3][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[4 * (step / 3) + i], q.factor, -shift));
+            } else if (step % 3 == 1) {
+                l_run += (w[step / 3][0] + w[step / 3][1]) + (w[step / 3][2] + w[step / 3][3]);
+            } else {
+                split_halves(w[step / 3], hi[step / 3], lo[step / 3]);
             }
-            ph[s] = __builtin_shufflevector(hi[0], hi[1], 0, 1, 2, 3, 4, 5, 6, 7), pl[s] = __builtin_shufflevector(lo[0], lo[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        };
+#pragma unroll
+        for (int e = 0; e < 16; e++) next[e] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 3 * SLABS; i++) {
+            const int s = i / 3, then = s + kAhead;
+            if (i % 3 == 0) next = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl[s], q.hi[s], next, 0, 0, 0);
+            if (i % 3 == 1) next = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[s], q.lo[s], next, 0, 0, 0);
+            if (i % 3 == 2) next = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[s], q.hi[s], next, 0, 0, 0);
+            if (i % 3 == 0 && then < SLABS) kl[then] = key(1, then), kh[then] = key(0, then);
+            if (i % 3 == 0 && then >= SLABS && then - SLABS < 2 * DT) vl[then - SLABS] = read_v(buffer, 1, (then - SLABS) % DT, (then - SLABS) / DT), vh[then - SLABS] = read_v(buffer, 0, (then - SLABS) % DT, (then - SLABS) / DT);
+#pragma unroll
+            for (int step = 12 * i / (3 * SLABS); step < 12 * (i + 1) / (3 * SLABS); step++) softmax_step(step);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        l_run = __builtin_fmaf(l_run, alpha, sum);
+        const h8 ph[2] = {__builtin_shufflevector(hi[0], hi[1], 0, 1, 2, 3, 4, 5, 6, 7), __builtin_shufflevector(hi[2], hi[3], 0, 1, 2, 3, 4, 5, 6, 7)};
+        const h8 pl[2] = {__builtin_shufflevector(lo[0], lo[1], 0, 1, 2, 3, 4, 5, 6, 7), __builtin_shufflevector(lo[2], lo[3], 0, 1, 2, 3, 4, 5, 6, 7)};
 #pragma unroll
-        for (int s = 0; s < 2; s++)
+        for (int i = 0; i < 6 * DT; i++) {
+            const int n = i / 3, d = n % DT, s = n / DT, then = n + kAhead;
+            if (i % 3 == 0) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl[n], ph[s], o[d], 0, 0, 0);
+            if (i % 3 == 1) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh[n], pl[s], o[d], 0, 0, 0);
+            if (i % 3 == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh[n], ph[s], o[d], 0, 0, 0);
+            if (i % 3 == 0 && then < 2 * DT) vl[then] = read_v(buffer, 1, then % DT, then / DT), vh[then] = read_v(buffer, 0, then % DT, then / DT);
 #pragma unroll
-            for (int i = 0; i < DT; i++) {
-                h8 next_h = vh, next_l = vl;
-                const int next = DT * s + i + 1;
-                if (next < 2 * DT) next_h = read_v(t, 0, next % DT, next / DT), next_l = read_v(t, 1, next % DT, next / DT);
-                __builtin_amdgcn_sched_barrier(0);
-                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[s], o[i], 0, 0, 0);
-                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[s], o[i], 0, 0, 0);
-                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[s], o[i], 0, 0, 0);
-                vh = next_h, vl = next_l;
+            for (int step = 2 * kSteps * i / (6 * DT); step < 2 * kSteps * (i + 1) / (6 * DT); step++) {
+                if (step < kSteps) store_step(buffer ^ 1, vraw, false, step);
+                else store_step(buffer, kraw, true, step - kSteps);
             }
+            if (i == 6 * DT - 2) {  // the next tile's maximum, if it needs no mask
+                top = next[0];
+#pragma unroll
+                for (int e = 1; e < 16; e++) top = fmaxf(top, next[e]);
+            }
+            if (i == 6 * DT - 1) top = halves_max(top);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
 
-    // Tile t sits in LDS and t + 1 is on its way in registers: behind the arithmetic of tile t it goes where tile t - 1 was (or t, where there is no
-    // room for two, behind a barrier more) and t + 2 is requested.
-    Share raw;
-    fetch(t_first, raw);
+    // While the arithmetic of tile t runs, the values of t and the keys of t + 1 sit in LDS; the values of t + 1 and the keys of t + 2 are in registers and
+    // go where those of t - 1 and t were; behind them the next are requested.  (Requests past the end repeat the last row.)
+    Share kraw, vraw;
+    v16f sc[2];
+    fetch(kraw, true);
+    fetch(vraw, false);
+    next_tile();
     q.load(a, r, c, group, h);
-    store(tiles[0], raw);
-    if (t_first + 1u < t_end) fetch(t_first + 1u, raw);
+    store(0, kraw, true);
+    fetch(kraw, true);
+    store(0, vraw, false);
+    fetch(vraw, false);
+    next_tile();
+    store(1, kraw, true);
+    fetch(kraw, true);
     __syncthreads();
-    for (uint32_t t = t_first; t < t_end; t++) {
-        const uint32_t at = TWO ? (t - t_first) & 1u : 0u;
-        attend(tiles[at], t * KT);
-        if (t + 1u < t_end) {
-            if (!TWO) __syncthreads();
-            store(tiles[TWO ? at ^ 1u : 0u], raw);
-            if (t + 2u < t_end) fetch(t + 2u, raw);
-        }
+#pragma unroll
+    for (int e = 0; e < 16; e++) sc[0][e] = 0.0f;
+#pragma unroll
+    for (int s = 0; s < SLABS; s++) {
+        const h8 kh = *reinterpret_cast<const h8*>(&k_tile[0].h[0][32u * wk + l32][16 * s + 8 * h]), kl = *reinterpret_cast<const h8*>(&k_tile[0].h[1][32u * wk + l32][16 * s + 8 * h]);
+        sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, q.hi[s], sc[0], 0, 0, 0);
+        sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, q.lo[s], sc[0], 0, 0, 0);
+        sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, q.hi[s], sc[0], 0, 0, 0);
+    }
+    top = sc[0][0];
+#pragma unroll
+    for (int e = 1; e < 16; e++) top = fmaxf(top, sc[0][e]);
+    top = halves_max(top);
+    __syncthreads();
+    const auto tile = [&](int buffer, uint32_t t) {
+        attend(buffer, t, sc[buffer], sc[buffer ^ 1], kraw, vraw);
+        fetch(vraw, false);  // (of tile t + 2, and keys of t + 3)
+        next_tile();
+        fetch(kraw, true);
         __syncthreads();
+    };
+    for (uint32_t t = t_first;; t += 2u) {
+        tile(0, t);
+        if (t + 1u >= t_end) break;
+        tile(1, t + 1u);
+        if (t + 2u >= t_end) break;
     }
 
     l_run = halves_sum(l_run);
@@ -473,8 +531,8 @@ template <int HD>
 hipError_t launch_head_dim(const Q4AttentionArgs& a, const Launch& L) {
     const uint32_t rows = a.n * (a.n_heads / a.n_kv_heads);
     hipError_t e;
-    if constexpr (HD == 32) e = launch_tiles<HD, 2, 2, 4>(a, L);
-    else if constexpr (HD == 64) e = rows <= 32u ? launch_tiles<HD, 1, 4, 1>(a, L) : launch_tiles<HD, 4, 2, 2>(a, L);
+    if constexpr (HD == 32) e = launch_tiles<HD, 2, 2, 2>(a, L);
+    else if constexpr (HD == 64) e = rows <= 32u ? launch_tiles<HD, 1, 4, 1>(a, L) : launch_tiles<HD, 4, 2, 1>(a, L);
     else if constexpr (HD == 128) e = rows <= 32u ? launch_tiles<HD, 1, 2, 1>(a, L) : launch_tiles<HD, 4, 2, 1>(a, L);
     else e = launch_tiles<HD, 4, 1, 1>(a, L);
     if (e != hipSuccess || !a.weights) return e;

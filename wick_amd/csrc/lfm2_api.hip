@@ -149,13 +149,14 @@ int wick_rocm_attention_prefill_quantize_q8_0(wick_rocm_ctx* ctx, const float* d
 
 namespace {
 
-constexpr uint32_t kQ4MaxRows = 1u << 30;
+constexpr uint32_t kQ4MaxRows = 1u << 24;    // a head's rows are within 32-bit offsets
+constexpr uint32_t kQ4MaxQueries = 1u << 30;
 
 // What every call on such caches asks of their shape and place; null: nothing is wrong.
 const char* q4_shape(uint32_t max_seq, uint32_t n_kv_heads, uint32_t head_dim) {
     if (head_dim != 32u && head_dim != 64u && head_dim != 128u && head_dim != 256u) return "kv_q4: head_dim must be 32, 64, 128 or 256";
     if (n_kv_heads == 0 || n_kv_heads > 65535u) return "kv_q4: n_kv_heads must be 1 .. 65535";
-    if (max_seq == 0 || max_seq > kQ4MaxRows) return "kv_q4: max_seq must be 1 .. 2^30";
+    if (max_seq == 0 || max_seq > kQ4MaxRows) return "kv_q4: max_seq must be 1 .. 2^24";
     return nullptr;
 }
 
@@ -207,7 +208,7 @@ static int attention_q4(wick_rocm_ctx* ctx, const float* d_q, uint32_t q_stride,
                         uint32_t n_kv_heads, uint32_t head_dim) {
     if (n_heads == 0 || n_heads % n_kv_heads != 0) return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, "attention_q4: n_kv_heads must divide n_heads");
     if (q_stride < (uint64_t)n_heads * head_dim || out_stride < (uint64_t)n_heads * head_dim || q_stride % 4u != 0 || out_stride % 4u != 0 ||
-        (uint64_t)n * n_heads > kQ4MaxRows)
+        (uint64_t)n * n_heads > kQ4MaxQueries)
         return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, "attention_q4: strides must cover n_heads * head_dim and be multiples of 4, n * n_heads at most 2^30");
     if (!d_q || !d_k_cache || !d_v_cache || !d_out || (!d_scratch && attention_q4_scratch_floats(n, max_seq, n_heads, n_kv_heads, head_dim, d_weights != nullptr)))
         return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "attention_q4: null device pointer");
