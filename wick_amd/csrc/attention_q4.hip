@@ -414,34 +414,305 @@ __global__ __launch_bounds__(64 * WQ * WK, PER_CU * WQ * WK / 4) void attention_
             *reinterpret_cast<v4f*>(to + 32 * i + 8 * k + 4 * h) = v4f{o[i][4 * k], o[i][4 * k + 1], o[i][4 * k + 2], o[i][4 * k + 3]} * inverse;
 }
 
-// The splits of one (token, head) merged: a wave turns their (maximum, sum) pairs into weights, then every thread sums its share of the values.
-template <int HD>
-__global__ __launch_bounds__(256) void attention_q4_merge_kernel(Q4AttentionArgs a, uint32_t wg_rows, uint32_t tile) {
-    constexpr uint32_t Q = HD / 4, G = 256 / Q;
-    __shared__ float weights[kMaxSplits], inverse;
-    __shared__ __align__(16) v4f sums[256];
-    const uint32_t at = blockIdx.x, token = at / a.n_heads, head = at % a.n_heads, tid = threadIdx.x, d = tid % Q, grp = tid / Q;
-    const uint32_t group = a.n_heads / a.n_kv_heads, rows = a.n * group, r = token * group + head % group;
+// The splits of a (token, head) merged, by G groups of HD / 4 lanes that share the splits among them (G = 1: no exchange, for launches of many rows).
+// Everything is requested at once: a record's values do not wait for its maximum.
+template <int HD, int G>
+__device__ __forceinline__ void merge_splits(const Q4AttentionArgs& a, uint32_t wg_rows, uint32_t tile) {
+    constexpr uint32_t Q = HD / 4, RPB = 256 / (Q * G), kBatch = 4;  // rows of a workgroup
+    __shared__ __align__(16) v4f sums[G > 1 ? 256 : 1];
+    __shared__ float2 states[G > 1 ? 256 / Q : 1];
+    const uint32_t tid = threadIdx.x, d = tid % Q, grp = tid / Q % G, at = blockIdx.x * RPB + tid / (Q * G);
+    if (G == 1 && at >= a.n * a.n_heads) return;  // (else a workgroup is whole: RPB divides, see the launch)
+    const uint32_t token = at / a.n_heads, head = at % a.n_heads, group = a.n_heads / a.n_kv_heads, rows = a.n * group, r = token * group + head % group;
     const uint32_t used = used_splits(a.splits, sees(a, first_row(a), r / wg_rows * wg_rows + wg_rows - 1u, rows, group) / tile + 1u);
     const float* const parts = a.parts + (size_t)at * a.splits * (HD + 4);
-    if (tid < 64u) {
-        const float m_i = tid < used ? parts[(size_t)tid * (HD + 4)] : -__builtin_inff(), l_i = tid < used ? parts[(size_t)tid * (HD + 4) + 1] : 0.0f;
-        const float m = wave_max_f32(m_i), m_sub = m == -__builtin_inff() ? 0.0f : m, w = __builtin_amdgcn_exp2f(m_i - m_sub), l = wave_sum_f32(l_i * w);
-        weights[tid] = w;
-        if (tid == 0) {
-            inverse = __fdiv_rn(1.0f, l);
-            if (a.stats) a.stats[2u * at] = m, a.stats[2u * at + 1u] = inverse;
+    float m = -__builtin_inff(), l = 0.0f;
+    v4f o = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t i0 = grp; i0 < used; i0 += G * kBatch) {
+        float2 ml[kBatch];
+        v4f v[kBatch];
+#pragma unroll
+        for (uint32_t b = 0; b < kBatch; b++) {
+            const float* const rec = parts + (size_t)min(i0 + b * G, used - 1u) * (HD + 4);
+            ml[b] = *reinterpret_cast<const float2*>(rec), v[b] = *reinterpret_cast<const v4f*>(rec + 4 + 4 * d);
+        }
+        float top = m;
+#pragma unroll
+        for (uint32_t b = 0; b < kBatch; b++) top = fmaxf(top, ml[b].x);
+        const float sub = top == -__builtin_inff() ? 0.0f : top, f = __builtin_amdgcn_exp2f(m - sub);
+        l *= f, o *= f, m = top;
+#pragma unroll
+        for (uint32_t b = 0; b < kBatch; b++) {
+            const float w = i0 + b * G < used ? __builtin_amdgcn_exp2f(ml[b].x - sub) : 0.0f;
+            if (i0 + b * G < used) l = __builtin_fmaf(ml[b].y, w, l), o += v[b] * w;
         }
     }
-    __syncthreads();
-    v4f o = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t i = grp; i < used; i += G) o += *reinterpret_cast<const v4f*>(parts + (size_t)i * (HD + 4) + 4 + 4 * d) * weights[i];
-    sums[tid] = o;
-    __syncthreads();
-    if (tid < Q) {
-        for (uint32_t i = 1; i < G; i++) o += sums[i * Q + tid];
-        *reinterpret_cast<v4f*>(a.out + (size_t)token * a.out_stride + (size_t)head * HD + 4u * tid) = o * inverse;
+    if constexpr (G > 1) {
+        sums[tid] = o;
+        if (d == 0) states[tid / Q] = make_float2(m, l);
+        __syncthreads();
+        if (grp != 0) return;
+        float top = m;
+#pragma unroll
+        for (uint32_t i = 1; i < G; i++) top = fmaxf(top, states[tid / Q + i].x);
+        const float sub = top == -__builtin_inff() ? 0.0f : top, f = __builtin_amdgcn_exp2f(m - sub);
+        l *= f, o *= f, m = top;
+#pragma unroll
+        for (uint32_t i = 1; i < G; i++) {
+            const float2 st = states[tid / Q + i];
+            const float w = __builtin_amdgcn_exp2f(st.x - sub);
+            l = __builtin_fmaf(st.y, w, l), o += sums[tid + i * Q] * w;
+        }
     }
+    const float inverse = __fdiv_rn(1.0f, l);
+    if (a.stats && d == 0) a.stats[2u * at] = m, a.stats[2u * at + 1u] = inverse;
+    *reinterpret_cast<v4f*>(a.out + (size_t)token * a.out_stride + (size_t)head * HD + 4u * d) = o * inverse;
+}
+template <int HD, int G>
+__global__ __launch_bounds__(256) void attention_q4_merge_kernel(Q4AttentionArgs a, uint32_t wg_rows, uint32_t tile) {
+    merge_splits<HD, G>(a, wg_rows, tile);
+}
+
+// ---- few query rows ----
+// Up to 16 query rows of a KV head (the heads of one token, of a few tokens) per workgroup, and a part of the cache to each of its waves, 32 rows
+// at a time, on v_mfma_f32_16x16x32_f16.  Nothing is shared but the states at the end: a lane loads the words of a key row that it multiplies (lane group g
+// HD / 32 of them from word g HD / 32 on, the order of an MFMA's K steps being free), values go through LDS of the wave's own to be transposed.
+struct FewArgs {
+    Q4AttentionArgs at;
+    float* scores;  // [n_heads][max_seq], of one token's heads in powers of two, for the weights; may be null
+};
+constexpr uint32_t kFewRows = 16, kFewWaves = 4, kFewKeys = 32;
+
+template <int HD>
+__global__ __launch_bounds__(64 * kFewWaves) void attention_q4_few_kernel(FewArgs args) {
+    const Q4AttentionArgs& a = args.at;
+    constexpr int SLABS = HD / 32, CS = HD / 16, kStates = 2 + HD / 4, kLoad = SLABS < 4 ? SLABS : 4, kLoads = SLABS / kLoad;  // words a load, loads a row
+    using VT = ValueTile<HD, (int)kFewKeys>;
+    constexpr size_t kValues = sizeof(VT) * kFewWaves, kStateBytes = sizeof(float) * kStates * 64 * (kFewWaves - 1);
+    __shared__ __align__(16) uint8_t smem[kValues > kStateBytes ? kValues : kStateBytes];
+    const uint32_t group = a.n_heads / a.n_kv_heads, rows = a.n * group;
+    const uint32_t c = blockIdx.x % a.n_kv_heads, split = blockIdx.x / a.n_kv_heads % a.splits, r0 = blockIdx.x / a.n_kv_heads / a.splits * kFewRows;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, l16 = lane & 15u, g = lane >> 4, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+    const uint32_t base = first_row(a), last = sees(a, base, r0 + kFewRows - 1u, rows, group), used = used_splits(a.splits, last / (kFewKeys * kFewWaves) + 1u);
+    if (split >= used) return;
+    const uint32_t units = last / kFewKeys + 1u, nth = split * kFewWaves + wave;
+    const uint32_t u_first = (uint32_t)((uint64_t)units * nth / (used * kFewWaves)), u_end = (uint32_t)((uint64_t)units * (nth + 1u) / (used * kFewWaves));
+    const uint32_t r = min(r0 + l16, rows - 1u), mine = sees(a, base, r, rows, group), first_sees = sees(a, base, r0, rows, group);
+    const uint32_t token = r / group, head = c * group + r % group;
+    VT& v_tile = reinterpret_cast<VT*>(smem)[wave];
+
+    const Q4Cache kc = q4_planes(const_cast<void*>(a.k_cache), a.max_seq, a.n_kv_heads, HD), vc = q4_planes(const_cast<void*>(a.v_cache), a.max_seq, a.n_kv_heads, HD);
+    const size_t first = (size_t)c * a.max_seq;
+    const auto plane = [&](const void* p, uint32_t row_bytes) {  // (a read behind the last row gives zeros, whose weights the mask makes zeros)
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(static_cast<const uint8_t*>(p)) + first * row_bytes, 0, (int)((last + 1u) * row_bytes), 0x27000);
+    };
+    const auto kq = plane(kc.quants, HD / 2), vq = plane(vc.quants, HD / 2), ks = plane(kc.scales, HD / 16), vs = plane(vc.scales, HD / 16);
+    struct Unit {  // this lane's words of keys l16 and 16 + l16, and of those values
+        struct __attribute__((aligned(4 * kLoad))) Words {
+            uint32_t w[kLoad];
+        };
+        Words k[2][kLoads], v[2][kLoads];
+        uint16_t kd[2][kLoads], vd[2][kLoads];
+    };
+    const auto load = [&](decltype(kq) from, uint32_t at) {
+        if constexpr (kLoad == 1) return __builtin_bit_cast(typename Unit::Words, __builtin_amdgcn_raw_buffer_load_b32(from, at, 0, 0));
+        else if constexpr (kLoad == 2) return __builtin_bit_cast(typename Unit::Words, __builtin_amdgcn_raw_buffer_load_b64(from, at, 0, 0));
+        else return __builtin_bit_cast(typename Unit::Words, __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, 0));
+    };
+    const auto fetch = [&](uint32_t unit, Unit& x) {
+#pragma unroll
+        for (uint32_t u = 0; u < 2; u++)
+#pragma unroll
+            for (uint32_t i = 0; i < kLoads; i++) {
+                const uint32_t row = unit * kFewKeys + 16u * u + l16, word = g * SLABS + i * kLoad;
+                x.k[u][i] = load(kq, row * (HD / 2) + 4u * word), x.v[u][i] = load(vq, row * (HD / 2) + 4u * word);
+                x.kd[u][i] = __builtin_amdgcn_raw_buffer_load_b16(ks, row * (HD / 16) + word / 4u * 2u, 0, 0);
+                x.vd[u][i] = __builtin_amdgcn_raw_buffer_load_b16(vs, row * (HD / 16) + word / 4u * 2u, 0, 0);
+            }
+    };
+    Unit now, then;
+    fetch(u_first, now);
+
+    // the query rows: dims 8 (g SLABS + s) .. of row l16 in slab s, times 2^-e
+    h8 qh[SLABS], ql[SLABS];
+    float factor;
+    {
+        const float* const p = a.q + (size_t)token * a.q_stride + (size_t)head * HD + 8u * SLABS * g;
+        v4f x[2 * SLABS];
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2 * SLABS; i++) {
+            x[i] = *reinterpret_cast<const v4f*>(p + 4 * i);
+#pragma unroll
+            for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(x[i][e]));
+        }
+        const int e = __builtin_amdgcn_frexp_expf(groups_max(top));
+        factor = __builtin_amdgcn_ldexpf(a.scale * kLog2e, e);
+#pragma unroll
+        for (int s = 0; s < SLABS; s++) {
+            h4 u[2], l[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                v4f y;
+#pragma unroll
+                for (int k = 0; k < 4; k++) y[k] = __builtin_amdgcn_ldexpf(x[2 * s + i][k], -e);
+                split_halves(y, u[i], l[i]);
+            }
+            qh[s] = __builtin_shufflevector(u[0], u[1], 0, 1, 2, 3, 4, 5, 6, 7), ql[s] = __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+    // V^T rows (dims) 16 i + l16, keys 4 g .. and 16 + 4 g ..: the 16 lanes of a group point at 4 keys x 16 dims, lane j at key j / 4 and dims 4 (j % 4) .. of them
+    const uint32_t vkey = 4u * g + (l16 >> 2), vpiece = l16 >> 1 & 1u;
+    const auto read_v = [&](int half, int i) {
+        typedef short s4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s4* lds_s4;
+        const _Float16* const p = &v_tile.h[half][vkey][8u * ((2u * i + vpiece) ^ VT::swizzle(vkey)) + 4u * (l16 & 1u)];  // (keys 16 apart swizzle alike)
+        const h4 a0 = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p));
+        const h4 a1 = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + 16 * HD)));
+        return h8{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
+    };
+    v4f o[CS];
+#pragma unroll
+    for (int i = 0; i < CS; i++) o[i] = v4f{0.f, 0.f, 0.f, 0.f};
+    float m_run = -__builtin_inff(), l_run = 0.0f;
+    for (uint32_t unit = u_first; unit < u_end; unit++) {
+        fetch(unit + 1u, then);  // (of the last one: for nobody)
+        const uint32_t key0 = unit * kFewKeys;
+        v4f sc[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            sc[u] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < SLABS; s++) {
+                const _Float16 vd = __builtin_bit_cast(_Float16, now.vd[u][s / kLoad]), poison = vd * (_Float16)0.0f;  // (see attention_q4_kernel)
+                const _Float16 kd = __builtin_bit_cast(_Float16, now.kd[u][s / kLoad]) + poison, vds = poison == poison ? vd : (_Float16)0.0f;
+                h8 hi, lo;
+                dequantize(now.k[u][s / kLoad].w[s % kLoad], kd, hi, lo);
+                sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, qh[s], sc[u], 0, 0, 0);
+                sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, ql[s], sc[u], 0, 0, 0);
+                sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, qh[s], sc[u], 0, 0, 0);
+                dequantize(now.v[u][s / kLoad].w[s % kLoad], vds, hi, lo);
+                const uint32_t row = 16u * u + l16, at = 8u * ((g * SLABS + s) ^ VT::swizzle(row));
+                *reinterpret_cast<h8*>(&v_tile.h[0][row][at]) = hi, *reinterpret_cast<h8*>(&v_tile.h[1][row][at]) = lo;
+            }
+        }
+        if (args.scores && r0 + l16 < rows) {
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t key = key0 + 16u * u + 4u * g + e;
+                    if (key <= mine) args.scores[(size_t)head * a.max_seq + key] = sc[u][e] * factor;
+                }
+        }
+        if (key0 + kFewKeys - 1u > first_sees) {
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (key0 + 16u * u + 4u * g + e > mine) sc[u][e] = -__builtin_inff();
+        }
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) top = fmaxf(top, sc[u][e]);
+        const float m_new = fmaxf(m_run, groups_max(top) * factor), m_sub = m_new == -__builtin_inff() ? 0.0f : m_new;
+        if (__builtin_amdgcn_ballot_w64(m_new > m_run) != 0) {
+            const float alpha = __builtin_amdgcn_exp2f(m_run - m_sub);
+            m_run = m_new, l_run *= alpha;
+#pragma unroll
+            for (int i = 0; i < CS; i++) o[i] *= alpha;
+        }
+        const float shift = m_sub - kWeightBits;
+        h4 hi[2], lo[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            v4f w;
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][e], factor, -shift));
+            l_run += (w[0] + w[1]) + (w[2] + w[3]);
+            split_halves(w, hi[u], lo[u]);
+        }
+        const h8 ph = __builtin_shufflevector(hi[0], hi[1], 0, 1, 2, 3, 4, 5, 6, 7), pl = __builtin_shufflevector(lo[0], lo[1], 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+        for (int i = 0; i < CS; i++) {
+            const h8 vh = read_v(0, i), vl = read_v(1, i);
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph, o[i], 0, 0, 0);
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl, o[i], 0, 0, 0);
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph, o[i], 0, 0, 0);
+        }
+        now = then;
+    }
+    l_run = groups_sum(l_run);
+    __syncthreads();  // (the states go where the values were)
+    float* const state = reinterpret_cast<float*>(smem) + lane;
+    if (wave != 0) {
+        float* const to = state + (size_t)(wave - 1u) * kStates * 64u;
+        to[0] = m_run, to[64] = l_run;
+#pragma unroll
+        for (int i = 0; i < CS; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) to[(2 + 4 * i + e) * 64] = o[i][e];
+    }
+    __syncthreads();
+    if (wave != 0) return;
+    float m_all = m_run;
+#pragma unroll
+    for (uint32_t k = 0; k < kFewWaves - 1u; k++) m_all = fmaxf(m_all, state[k * kStates * 64]);
+    const float m_sub = m_all == -__builtin_inff() ? 0.0f : m_all;
+    float f = __builtin_amdgcn_exp2f(m_run - m_sub);
+    l_run *= f;
+#pragma unroll
+    for (int i = 0; i < CS; i++) o[i] *= f;
+#pragma unroll
+    for (uint32_t k = 0; k < kFewWaves - 1u; k++) {
+        const float* const from = state + k * kStates * 64;
+        f = __builtin_amdgcn_exp2f(from[0] - m_sub);
+        l_run = __builtin_fmaf(from[64], f, l_run);
+#pragma unroll
+        for (int i = 0; i < CS; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[i][e] = __builtin_fmaf(from[(2 + 4 * i + e) * 64], f, o[i][e]);
+    }
+    if (r0 + l16 >= rows) return;
+    float* to;
+    float inverse = 1.0f;
+    if (a.splits == 1u) {
+        to = a.out + (size_t)token * a.out_stride + (size_t)head * HD;
+        inverse = __fdiv_rn(1.0f, l_run);
+        if (a.stats && g == 0) {
+            float* const st = a.stats + 2u * ((size_t)token * a.n_heads + head);
+            st[0] = m_all, st[1] = inverse;
+        }
+    } else {
+        to = a.parts + (((size_t)token * a.n_heads + head) * a.splits + split) * (HD + 4);
+        if (g == 0) to[0] = m_all, to[1] = l_run;
+        to += 4;
+    }
+#pragma unroll
+    for (int i = 0; i < CS; i++) *reinterpret_cast<v4f*>(to + 16 * i + 4 * g) = o[i] * inverse;  // register e of o[i] holds dim 16 i + 4 g + e of row l16
+}
+
+// One token's splits merged and, in workgroups of their own, its weights added to what the rows have gathered: from the scores that the launch before left, with
+// each head's maximum and sum worked out from its splits once more.
+template <int HD>
+__global__ __launch_bounds__(256) void attention_q4_finish_kernel(FewArgs args) {
+    const Q4AttentionArgs& a = args.at;
+    if (blockIdx.x < a.n_heads) return merge_splits<HD, 1024 / HD>(a, kFewRows, kFewKeys * kFewWaves);
+    const uint32_t group = a.n_heads / a.n_kv_heads, nth = blockIdx.x - a.n_heads, c = nth % a.n_kv_heads, t = nth / a.n_kv_heads * 256u + threadIdx.x, lane = threadIdx.x & 63u;
+    const uint32_t last = first_row(a), used = used_splits(a.splits, last / (kFewKeys * kFewWaves) + 1u);
+    if (t - threadIdx.x > last) return;
+    const uint32_t at = min(t, last);
+    float sum = 0.0f;
+    for (uint32_t h = c * group; h < (c + 1u) * group; h++) {
+        const float* const parts = a.parts + (size_t)h * a.splits * (HD + 4);
+        const float score = args.scores[(size_t)h * a.max_seq + at];
+        const float m_i = lane < used ? parts[(size_t)lane * (HD + 4)] : -__builtin_inff(), l_i = lane < used ? parts[(size_t)lane * (HD + 4) + 1] : 0.0f;
+        const float m = wave_max_f32(m_i), m_sub = m == -__builtin_inff() ? 0.0f : m, l = wave_sum_f32(l_i * __builtin_amdgcn_exp2f(m_i - m_sub));
+        sum += __fdiv_rn(__builtin_amdgcn_exp2f(score - m_sub + kWeightBits), l);
+    }
+    if (t <= last) a.weights[(size_t)c * a.max_seq + t] += sum;
 }
 
 // What 64 rows of a KV head have gathered: the scores once more, now that every softmax's maximum and sum is known, and their weights added
@@ -523,20 +794,32 @@ hipError_t launch_tiles(Q4AttentionArgs a, const Launch& L) {
     const uint32_t blocks = base / a.n_kv_heads;
     a.first_blocks = base * a.splits > kCus && base * a.splits <= 2u * kCus ? (kCus + a.n_kv_heads * a.splits - 1u) / (a.n_kv_heads * a.splits) : blocks;
     hipError_t e = launch_kernel(L, kFamOther, attention_q4_kernel<HD, WQ, WK, PER_CU>, dim3(base * a.splits), dim3(64 * WQ * WK), a);
-    if (e == hipSuccess && a.splits > 1u) e = launch_kernel(L, kFamOther, attention_q4_merge_kernel<HD>, dim3(a.n * a.n_heads), dim3(256), a, RB, KT);
-    return e;
+    if (e != hipSuccess || a.splits == 1u) return e;
+    const uint32_t merged = a.n * a.n_heads;
+    return a.splits > 8u ? launch_kernel(L, kFamOther, attention_q4_merge_kernel<HD, 1024 / HD>, dim3(merged), dim3(256), a, RB, KT)
+                         : launch_kernel(L, kFamOther, attention_q4_merge_kernel<HD, 1>, dim3((merged + 1024u / HD - 1u) / (1024u / HD)), dim3(256), a, RB, KT);
 }
 
 template <int HD>
-hipError_t launch_head_dim(const Q4AttentionArgs& a, const Launch& L) {
+hipError_t launch_head_dim(const Q4AttentionArgs& a, float* d_scores, const Launch& L) {
     const uint32_t rows = a.n * (a.n_heads / a.n_kv_heads);
+    const uint64_t seen = a.d_pos ? a.max_seq : (uint64_t)a.pos0 + a.n;
     hipError_t e;
-    if constexpr (HD == 32) e = launch_tiles<HD, 2, 2, 2>(a, L);
-    else if constexpr (HD == 64) e = rows <= 32u ? launch_tiles<HD, 1, 4, 1>(a, L) : launch_tiles<HD, 4, 2, 1>(a, L);
-    else if constexpr (HD == 128) e = rows <= 32u ? launch_tiles<HD, 1, 2, 1>(a, L) : launch_tiles<HD, 4, 2, 1>(a, L);
+    if (rows <= kFewRows) {
+        FewArgs f{a, a.n == 1u && a.weights ? d_scores : nullptr};
+        const uint32_t base = a.n_kv_heads, span = kFewKeys * kFewWaves, most = (uint32_t)((seen + span - 1u) / span), room = kSplitSlots / base;
+        f.at.splits = room < 2u ? 1u : (room < most ? room : most);
+        if (f.at.splits > kMaxSplits) f.at.splits = kMaxSplits;
+        e = launch_kernel(L, kFamOther, attention_q4_few_kernel<HD>, dim3(base * f.at.splits), dim3(64 * kFewWaves), f);
+        if (e != hipSuccess) return e;
+        if (f.scores && f.at.splits > 1u)
+            return launch_kernel(L, kFamOther, attention_q4_finish_kernel<HD>, dim3(a.n_heads + a.n_kv_heads * (uint32_t)((seen + 255u) / 256u)), dim3(256), f);
+        if (f.at.splits > 1u) e = launch_kernel(L, kFamOther, attention_q4_merge_kernel<HD, 1024 / HD>, dim3(a.n * a.n_heads), dim3(256), f.at, kFewRows, span);
+    } else if constexpr (HD == 32) e = launch_tiles<HD, 2, 2, 2>(a, L);
+    else if constexpr (HD == 64) e = launch_tiles<HD, 4, 2, 1>(a, L);
+    else if constexpr (HD == 128) e = launch_tiles<HD, 4, 2, 1>(a, L);
     else e = launch_tiles<HD, 4, 1, 1>(a, L);
     if (e != hipSuccess || !a.weights) return e;
-    const uint64_t seen = a.d_pos ? a.max_seq : (uint64_t)a.pos0 + a.n;
     const dim3 grid((uint32_t)((seen + 63) / 64), a.n_kv_heads);
     return rows <= 32u ? launch_kernel(L, kFamOther, attention_q4_weights_kernel<HD, 1>, grid, dim3(64), a)
                        : launch_kernel(L, kFamOther, attention_q4_weights_kernel<HD, 8>, grid, dim3(512), a);
@@ -551,21 +834,22 @@ size_t part_floats(uint32_t n, uint32_t n_heads, uint32_t head_dim) {
 }  // namespace
 
 size_t attention_q4_scratch_floats(uint32_t n, uint32_t max_seq, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, bool weights) {
-    (void)max_seq, (void)n_kv_heads;
-    return part_floats(n, n_heads, head_dim) + (weights ? 2 * (size_t)n * n_heads : 0);
+    (void)n_kv_heads;
+    return part_floats(n, n_heads, head_dim) + (weights ? 2 * (size_t)n * n_heads + (size_t)n_heads * max_seq : 0);  // records, statistics, a token's scores
 }
 
 hipError_t launch_attention_q4(const float* d_q, uint32_t q_stride, const void* d_k_cache, const void* d_v_cache, float* d_out, uint32_t out_stride,
                                float* d_weights, float* d_scratch, uint32_t pos0, const uint32_t* d_pos, uint32_t n, uint32_t max_seq, uint32_t n_heads,
                                uint32_t n_kv_heads, uint32_t head_dim, float scale, const Launch& L) {
     if (n == 0) return hipSuccess;
-    const Q4AttentionArgs a{d_q, d_k_cache, d_v_cache, d_out, d_scratch, d_weights ? d_scratch + part_floats(n, n_heads, head_dim) : nullptr, d_weights, d_pos,
+    float *const d_stats = d_scratch + part_floats(n, n_heads, head_dim), *const d_scores = d_stats + 2 * (size_t)n * n_heads;
+    const Q4AttentionArgs a{d_q, d_k_cache, d_v_cache, d_out, d_scratch, d_weights ? d_stats : nullptr, d_weights, d_pos,
                             pos0, n, q_stride, out_stride, max_seq, n_heads, n_kv_heads, 1, 0, scale};
     switch (head_dim) {
-        case 32: return launch_head_dim<32>(a, L);
-        case 64: return launch_head_dim<64>(a, L);
-        case 128: return launch_head_dim<128>(a, L);
-        default: return launch_head_dim<256>(a, L);
+        case 32: return launch_head_dim<32>(a, d_scores, L);
+        case 64: return launch_head_dim<64>(a, d_scores, L);
+        case 128: return launch_head_dim<128>(a, d_scores, L);
+        default: return launch_head_dim<256>(a, d_scores, L);
     }
 }
 
