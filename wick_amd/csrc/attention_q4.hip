@@ -21,7 +21,7 @@ namespace wick_rocm {
 namespace {
 
 constexpr float kWeightBits = 12.0f;       // softmax weights are taken times 2^12, so that small ones keep their bits in the split
-constexpr uint32_t kMaxSplits = 64;        // workgroups that share the rows of the cache among them
+constexpr uint32_t kMaxSplits = 96;        // workgroups that share the rows of the cache among them
 constexpr uint32_t kCus = 256;
 constexpr uint32_t kSplitSlots = 2 * kCus; // split launches have no more workgroups than this
 constexpr uint32_t kMostRows = 128;        // query rows of a workgroup at the most
@@ -481,22 +481,28 @@ struct FewArgs {
     Q4AttentionArgs at;
     float* scores;  // [n_heads][max_seq], of one token's heads in powers of two, for the weights; may be null
 };
-constexpr uint32_t kFewRows = 16, kFewWaves = 4, kFewKeys = 32;
+constexpr uint32_t kFewRows = 16, kFewKeys = 32;
+template <int HD>
+constexpr uint32_t kFewWaves = 4;
+template <int HD>
+constexpr uint32_t kFewSlots = kCus * (HD <= 64 ? 2 : HD == 128 ? 3 : 1);  // workgroups that the GPU has at once
 
 template <int HD>
-__global__ __launch_bounds__(64 * kFewWaves) void attention_q4_few_kernel(FewArgs args) {
+__global__ __launch_bounds__(64 * kFewWaves<HD>, HD <= 64 ? 4 : HD == 128 ? 3 : 1) void attention_q4_few_kernel(FewArgs args) {
     const Q4AttentionArgs& a = args.at;
+    constexpr uint32_t kWaves = kFewWaves<HD>;
     constexpr int SLABS = HD / 32, CS = HD / 16, kStates = 2 + HD / 4, kLoad = SLABS < 4 ? SLABS : 4, kLoads = SLABS / kLoad;  // words a load, loads a row
-    using VT = ValueTile<HD, (int)kFewKeys>;
-    constexpr size_t kValues = sizeof(VT) * kFewWaves, kStateBytes = sizeof(float) * kStates * 64 * (kFewWaves - 1);
+    constexpr int TD = HD < 64 ? HD : 64, PARTS = HD / TD, SP = SLABS / PARTS;  // dims in LDS at a time, words of a lane in them
+    using VT = ValueTile<TD, (int)kFewKeys>;
+    constexpr size_t kValues = sizeof(VT) * kWaves, kStateBytes = sizeof(float) * kStates * 64 * kWaves;
     __shared__ __align__(16) uint8_t smem[kValues > kStateBytes ? kValues : kStateBytes];
     const uint32_t group = a.n_heads / a.n_kv_heads, rows = a.n * group;
     const uint32_t c = blockIdx.x % a.n_kv_heads, split = blockIdx.x / a.n_kv_heads % a.splits, r0 = blockIdx.x / a.n_kv_heads / a.splits * kFewRows;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, l16 = lane & 15u, g = lane >> 4, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
-    const uint32_t base = first_row(a), last = sees(a, base, r0 + kFewRows - 1u, rows, group), used = used_splits(a.splits, last / (kFewKeys * kFewWaves) + 1u);
+    const uint32_t base = first_row(a), last = sees(a, base, r0 + kFewRows - 1u, rows, group), used = used_splits(a.splits, last / (kFewKeys * kWaves) + 1u);
     if (split >= used) return;
-    const uint32_t units = last / kFewKeys + 1u, nth = split * kFewWaves + wave;
-    const uint32_t u_first = (uint32_t)((uint64_t)units * nth / (used * kFewWaves)), u_end = (uint32_t)((uint64_t)units * (nth + 1u) / (used * kFewWaves));
+    const uint32_t units = last / kFewKeys + 1u, nth = split * kWaves + wave;
+    const uint32_t u_first = (uint32_t)((uint64_t)units * nth / (used * kWaves)), u_end = (uint32_t)((uint64_t)units * (nth + 1u) / (used * kWaves));
     const uint32_t r = min(r0 + l16, rows - 1u), mine = sees(a, base, r, rows, group), first_sees = sees(a, base, r0, rows, group);
     const uint32_t token = r / group, head = c * group + r % group;
     VT& v_tile = reinterpret_cast<VT*>(smem)[wave];
@@ -530,8 +536,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void attention_q4_few_kernel(FewArg
                 x.vd[u][i] = __builtin_amdgcn_raw_buffer_load_b16(vs, row * (HD / 16) + word / 4u * 2u, 0, 0);
             }
     };
-    Unit now, then;
-    fetch(u_first, now);
+    Unit units_ahead[2];
+    fetch(u_first, units_ahead[0]);
 
     // the query rows: dims 8 (g SLABS + s) .. of row l16 in slab s, times 2^-e
     h8 qh[SLABS], ql[SLABS];
@@ -561,21 +567,35 @@ __global__ __launch_bounds__(64 * kFewWaves) void attention_q4_few_kernel(FewArg
             qh[s] = __builtin_shufflevector(u[0], u[1], 0, 1, 2, 3, 4, 5, 6, 7), ql[s] = __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
-    // V^T rows (dims) 16 i + l16, keys 4 g .. and 16 + 4 g ..: the 16 lanes of a group point at 4 keys x 16 dims, lane j at key j / 4 and dims 4 (j % 4) .. of them
+    // V^T rows 16 i + l16 of the part that is in LDS (dims HD / 4 i + 16 part + l16 of the head), keys 4 g .. and 16 + 4 g ..: the 16 lanes of a group point at
+    // 4 keys x 16 dims, lane j at key j / 4 and dims 4 (j % 4) .. of them.
     const uint32_t vkey = 4u * g + (l16 >> 2), vpiece = l16 >> 1 & 1u;
     const auto read_v = [&](int half, int i) {
         typedef short s4 __attribute__((ext_vector_type(4)));
         typedef __attribute__((address_space(3))) s4* lds_s4;
         const _Float16* const p = &v_tile.h[half][vkey][8u * ((2u * i + vpiece) ^ VT::swizzle(vkey)) + 4u * (l16 & 1u)];  // (keys 16 apart swizzle alike)
         const h4 a0 = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p));
-        const h4 a1 = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + 16 * HD)));
+        const h4 a1 = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + 16 * TD)));
         return h8{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
+    };
+    const auto write_v = [&](const Unit& x, int part) {
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int i = 0; i < SP; i++) {
+                const int s = part * SP + i;
+                const _Float16 vd = __builtin_bit_cast(_Float16, x.vd[u][s / kLoad]), poison = vd * (_Float16)0.0f;
+                h8 hi, lo;
+                dequantize(x.v[u][s / kLoad].w[s % kLoad], poison == poison ? vd : (_Float16)0.0f, hi, lo);
+                const uint32_t row = 16u * u + l16, at = 8u * ((g * SP + i) ^ VT::swizzle(row));
+                *reinterpret_cast<h8*>(&v_tile.h[0][row][at]) = hi, *reinterpret_cast<h8*>(&v_tile.h[1][row][at]) = lo;
+            }
     };
     v4f o[CS];
 #pragma unroll
     for (int i = 0; i < CS; i++) o[i] = v4f{0.f, 0.f, 0.f, 0.f};
     float m_run = -__builtin_inff(), l_run = 0.0f;
-    for (uint32_t unit = u_first; unit < u_end; unit++) {
+    const auto attend = [&](uint32_t unit, const Unit& now, Unit& then) {
         fetch(unit + 1u, then);  // (of the last one: for nobody)
         const uint32_t key0 = unit * kFewKeys;
         v4f sc[2];
@@ -584,18 +604,15 @@ __global__ __launch_bounds__(64 * kFewWaves) void attention_q4_few_kernel(FewArg
             sc[u] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int s = 0; s < SLABS; s++) {
-                const _Float16 vd = __builtin_bit_cast(_Float16, now.vd[u][s / kLoad]), poison = vd * (_Float16)0.0f;  // (see attention_q4_kernel)
-                const _Float16 kd = __builtin_bit_cast(_Float16, now.kd[u][s / kLoad]) + poison, vds = poison == poison ? vd : (_Float16)0.0f;
+                const _Float16 poison = __builtin_bit_cast(_Float16, now.vd[u][s / kLoad]) * (_Float16)0.0f;  // (see attention_q4_kernel)
                 h8 hi, lo;
-                dequantize(now.k[u][s / kLoad].w[s % kLoad], kd, hi, lo);
+                dequantize(now.k[u][s / kLoad].w[s % kLoad], __builtin_bit_cast(_Float16, now.kd[u][s / kLoad]) + poison, hi, lo);
                 sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, qh[s], sc[u], 0, 0, 0);
                 sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, ql[s], sc[u], 0, 0, 0);
                 sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, qh[s], sc[u], 0, 0, 0);
-                dequantize(now.v[u][s / kLoad].w[s % kLoad], vds, hi, lo);
-                const uint32_t row = 16u * u + l16, at = 8u * ((g * SLABS + s) ^ VT::swizzle(row));
-                *reinterpret_cast<h8*>(&v_tile.h[0][row][at]) = hi, *reinterpret_cast<h8*>(&v_tile.h[1][row][at]) = lo;
             }
         }
+        write_v(now, 0);
         if (args.scores && r0 + l16 < rows) {
 #pragma unroll
             for (int u = 0; u < 2; u++)
@@ -636,19 +653,30 @@ __global__ __launch_bounds__(64 * kFewWaves) void attention_q4_few_kernel(FewArg
         }
         const h8 ph = __builtin_shufflevector(hi[0], hi[1], 0, 1, 2, 3, 4, 5, 6, 7), pl = __builtin_shufflevector(lo[0], lo[1], 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-        for (int i = 0; i < CS; i++) {
-            const h8 vh = read_v(0, i), vl = read_v(1, i);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph, o[i], 0, 0, 0);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl, o[i], 0, 0, 0);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph, o[i], 0, 0, 0);
+        for (int part = 0; part < PARTS; part++) {
+            if (part > 0) write_v(now, part);
+#pragma unroll
+            for (int i = 0; i < TD / 16; i++) {
+                const h8 vh = read_v(0, i), vl = read_v(1, i);
+                const int d = PARTS * i + part;
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph, o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl, o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph, o[d], 0, 0, 0);
+            }
         }
-        now = then;
+    };
+    for (uint32_t unit = u_first; unit < u_end; unit += 2u) {
+        attend(unit, units_ahead[0], units_ahead[1]);
+        if (unit + 1u >= u_end) break;
+        attend(unit + 1u, units_ahead[1], units_ahead[0]);
     }
     l_run = groups_sum(l_run);
-    __syncthreads();  // (the states go where the values were)
-    float* const state = reinterpret_cast<float*>(smem) + lane;
-    if (wave != 0) {
-        float* const to = state + (size_t)(wave - 1u) * kStates * 64u;
+    // The waves' states side by side (where the values were), then every wave merges its share of the values.
+    constexpr int kShare = HD / 4 < (int)kWaves ? 1 : HD / 4 / (int)kWaves;
+    __syncthreads();
+    float* const states = reinterpret_cast<float*>(smem) + lane;
+    {
+        float* const to = states + wave * (kStates * 64u);
         to[0] = m_run, to[64] = l_run;
 #pragma unroll
         for (int i = 0; i < CS; i++)
@@ -656,42 +684,40 @@ __global__ __launch_bounds__(64 * kFewWaves) void attention_q4_few_kernel(FewArg
             for (int e = 0; e < 4; e++) to[(2 + 4 * i + e) * 64] = o[i][e];
     }
     __syncthreads();
-    if (wave != 0) return;
-    float m_all = m_run;
+    if (wave * kShare >= HD / 4 || r0 + l16 >= rows) return;
+    float m = -__builtin_inff(), l = 0.0f, sums[kShare];
 #pragma unroll
-    for (uint32_t k = 0; k < kFewWaves - 1u; k++) m_all = fmaxf(m_all, state[k * kStates * 64]);
-    const float m_sub = m_all == -__builtin_inff() ? 0.0f : m_all;
-    float f = __builtin_amdgcn_exp2f(m_run - m_sub);
-    l_run *= f;
+    for (uint32_t k = 0; k < kWaves; k++) m = fmaxf(m, states[k * (kStates * 64u)]);
+    const float m_sub = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
-    for (int i = 0; i < CS; i++) o[i] *= f;
+    for (int i = 0; i < kShare; i++) sums[i] = 0.0f;
 #pragma unroll
-    for (uint32_t k = 0; k < kFewWaves - 1u; k++) {
-        const float* const from = state + k * kStates * 64;
-        f = __builtin_amdgcn_exp2f(from[0] - m_sub);
-        l_run = __builtin_fmaf(from[64], f, l_run);
+    for (uint32_t k = 0; k < kWaves; k++) {
+        const float* const from = states + k * (kStates * 64u);
+        const float f = __builtin_amdgcn_exp2f(from[0] - m_sub);
+        l = __builtin_fmaf(from[64], f, l);
 #pragma unroll
-        for (int i = 0; i < CS; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) o[i][e] = __builtin_fmaf(from[(2 + 4 * i + e) * 64], f, o[i][e]);
+        for (int i = 0; i < kShare; i++) sums[i] = __builtin_fmaf(from[(2 + kShare * wave + i) * 64u], f, sums[i]);
     }
-    if (r0 + l16 >= rows) return;
     float* to;
     float inverse = 1.0f;
     if (a.splits == 1u) {
         to = a.out + (size_t)token * a.out_stride + (size_t)head * HD;
-        inverse = __fdiv_rn(1.0f, l_run);
-        if (a.stats && g == 0) {
+        inverse = __fdiv_rn(1.0f, l);
+        if (a.stats && g == 0 && wave == 0) {
             float* const st = a.stats + 2u * ((size_t)token * a.n_heads + head);
-            st[0] = m_all, st[1] = inverse;
+            st[0] = m, st[1] = inverse;
         }
     } else {
         to = a.parts + (((size_t)token * a.n_heads + head) * a.splits + split) * (HD + 4);
-        if (g == 0) to[0] = m_all, to[1] = l_run;
+        if (g == 0 && wave == 0) to[0] = m, to[1] = l;
         to += 4;
     }
 #pragma unroll
-    for (int i = 0; i < CS; i++) *reinterpret_cast<v4f*>(to + 16 * i + 4 * g) = o[i] * inverse;  // register e of o[i] holds dim 16 i + 4 g + e of row l16
+    for (int i = 0; i < kShare; i++) {  // value j of a lane is dim 16 (j / 4) + 4 g + j % 4 of row l16
+        const uint32_t j = kShare * wave + i;
+        to[16u * (j >> 2) + 4u * g + (j & 3u)] = sums[i] * inverse;
+    }
 }
 
 // One token's splits merged and, in workgroups of their own, its weights added to what the rows have gathered: from the scores that the launch before left, with
@@ -699,17 +725,27 @@ __global__ __launch_bounds__(64 * kFewWaves) void attention_q4_few_kernel(FewArg
 template <int HD>
 __global__ __launch_bounds__(256) void attention_q4_finish_kernel(FewArgs args) {
     const Q4AttentionArgs& a = args.at;
-    if (blockIdx.x < a.n_heads) return merge_splits<HD, 1024 / HD>(a, kFewRows, kFewKeys * kFewWaves);
+    if (blockIdx.x < a.n_heads) return merge_splits<HD, 1024 / HD>(a, kFewRows, kFewKeys * kFewWaves<HD>);
     const uint32_t group = a.n_heads / a.n_kv_heads, nth = blockIdx.x - a.n_heads, c = nth % a.n_kv_heads, t = nth / a.n_kv_heads * 256u + threadIdx.x, lane = threadIdx.x & 63u;
-    const uint32_t last = first_row(a), used = used_splits(a.splits, last / (kFewKeys * kFewWaves) + 1u);
+    const uint32_t last = first_row(a), used = used_splits(a.splits, last / (kFewKeys * kFewWaves<HD>) + 1u);
     if (t - threadIdx.x > last) return;
+    constexpr uint32_t kPerLane = (kMaxSplits + 63u) / 64u;
     const uint32_t at = min(t, last);
     float sum = 0.0f;
     for (uint32_t h = c * group; h < (c + 1u) * group; h++) {
         const float* const parts = a.parts + (size_t)h * a.splits * (HD + 4);
         const float score = args.scores[(size_t)h * a.max_seq + at];
-        const float m_i = lane < used ? parts[(size_t)lane * (HD + 4)] : -__builtin_inff(), l_i = lane < used ? parts[(size_t)lane * (HD + 4) + 1] : 0.0f;
-        const float m = wave_max_f32(m_i), m_sub = m == -__builtin_inff() ? 0.0f : m, l = wave_sum_f32(l_i * __builtin_amdgcn_exp2f(m_i - m_sub));
+        float m_i[kPerLane], l_i[kPerLane], top = -__builtin_inff(), l = 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < kPerLane; i++) {
+            const uint32_t nth_split = lane + 64u * i;
+            m_i[i] = nth_split < used ? parts[(size_t)nth_split * (HD + 4)] : -__builtin_inff(), l_i[i] = nth_split < used ? parts[(size_t)nth_split * (HD + 4) + 1] : 0.0f;
+            top = fmaxf(top, m_i[i]);
+        }
+        const float m = wave_max_f32(top), m_sub = m == -__builtin_inff() ? 0.0f : m;
+#pragma unroll
+        for (uint32_t i = 0; i < kPerLane; i++) l = __builtin_fmaf(l_i[i], __builtin_amdgcn_exp2f(m_i[i] - m_sub), l);
+        l = wave_sum_f32(l);
         sum += __fdiv_rn(__builtin_amdgcn_exp2f(score - m_sub + kWeightBits), l);
     }
     if (t <= last) a.weights[(size_t)c * a.max_seq + t] += sum;
@@ -807,10 +843,10 @@ hipError_t launch_head_dim(const Q4AttentionArgs& a, float* d_scores, const Laun
     hipError_t e;
     if (rows <= kFewRows) {
         FewArgs f{a, a.n == 1u && a.weights ? d_scores : nullptr};
-        const uint32_t base = a.n_kv_heads, span = kFewKeys * kFewWaves, most = (uint32_t)((seen + span - 1u) / span), room = kSplitSlots / base;
+        const uint32_t base = a.n_kv_heads, span = kFewKeys * kFewWaves<HD>, most = (uint32_t)((seen + span - 1u) / span), room = kFewSlots<HD> / base;
         f.at.splits = room < 2u ? 1u : (room < most ? room : most);
         if (f.at.splits > kMaxSplits) f.at.splits = kMaxSplits;
-        e = launch_kernel(L, kFamOther, attention_q4_few_kernel<HD>, dim3(base * f.at.splits), dim3(64 * kFewWaves), f);
+        e = launch_kernel(L, kFamOther, attention_q4_few_kernel<HD>, dim3(base * f.at.splits), dim3(64 * kFewWaves<HD>), f);
         if (e != hipSuccess) return e;
         if (f.scores && f.at.splits > 1u)
             return launch_kernel(L, kFamOther, attention_q4_finish_kernel<HD>, dim3(a.n_heads + a.n_kv_heads * (uint32_t)((seen + 255u) / 256u)), dim3(256), f);
