@@ -12,6 +12,8 @@
 // in all); a query, scaled by a power of two to below 1, and a softmax weight, times 2^12, are split into two halves that keep 22 bits.
 // a b = a_hi b_hi + a_hi b_lo + a_lo b_hi: each product of halves is exact, sums are f32's, what is dropped is below 2^-22.
 // (One half for the weights or the queries would be off by 2^-12 of each: 100 times what f32 sums are.)
+#include <algorithm>
+
 #include "attention_device.h"
 #include "kv_q4_device.h"
 #include "wick_rocm_internal.h"
@@ -92,22 +94,24 @@ __device__ __forceinline__ float halves_sum(float v) {
 // the factor that turns a product into a power of two.
 template <int HD>
 struct Queries {
+    struct Raw {
+        v4f x[HD / 8];
+        __device__ __forceinline__ void request(const Q4AttentionArgs& a, uint32_t r, uint32_t c, uint32_t group, uint32_t h) {
+            const float* const p = a.q + (size_t)(r / group) * a.q_stride + (size_t)(c * group + r % group) * HD + 8u * h;
+#pragma unroll
+            for (int i = 0; i < HD / 8; i++) x[i] = *reinterpret_cast<const v4f*>(p + 16 * (i / 2) + 4 * (i % 2));
+        }
+    };
     h8 hi[HD / 16], lo[HD / 16];
     float factor;
-    __device__ __forceinline__ void load(const Q4AttentionArgs& a, uint32_t r, uint32_t c, uint32_t group, uint32_t h) {
-        const float* const p = a.q + (size_t)(r / group) * a.q_stride + (size_t)(c * group + r % group) * HD + 8u * h;
-        v4f x[HD / 8];
+    __device__ __forceinline__ void take(const Raw& raw, float scale) {
         float top = 0.0f;
 #pragma unroll
-        for (int s = 0; s < HD / 16; s++)
+        for (int i = 0; i < HD / 8; i++)
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                x[2 * s + i] = *reinterpret_cast<const v4f*>(p + 16 * s + 4 * i);
-#pragma unroll
-                for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(x[2 * s + i][e]));
-            }
+            for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(raw.x[i][e]));
         const int e = __builtin_amdgcn_frexp_expf(halves_max(top));
-        factor = __builtin_amdgcn_ldexpf(a.scale * kLog2e, e);
+        factor = __builtin_amdgcn_ldexpf(scale * kLog2e, e);
 #pragma unroll
         for (int s = 0; s < HD / 16; s++) {
             h4 u[2], l[2];
@@ -115,7 +119,7 @@ struct Queries {
             for (int i = 0; i < 2; i++) {
                 v4f y;
 #pragma unroll
-                for (int k = 0; k < 4; k++) y[k] = __builtin_amdgcn_ldexpf(x[2 * s + i][k], -e);
+                for (int k = 0; k < 4; k++) y[k] = __builtin_amdgcn_ldexpf(raw.x[2 * s + i][k], -e);
                 split_halves(y, u[i], l[i]);
             }
             hi[s] = __builtin_shufflevector(u[0], u[1], 0, 1, 2, 3, 4, 5, 6, 7), lo[s] = __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3, 4, 5, 6, 7);
@@ -322,7 +326,11 @@ __global__ __launch_bounds__(64 * WQ * WK, PER_CU * WQ * WK / 4) void attention_
     fetch(kraw, true);
     fetch(vraw, false);
     next_tile();
-    q.load(a, r, c, group, h);
+    {
+        typename Queries<HD>::Raw raw;
+        raw.request(a, r, c, group, h);
+        q.take(raw, a.scale);
+    }
     store(0, kraw, true);
     fetch(kraw, true);
     store(0, vraw, false);
@@ -481,23 +489,21 @@ struct FewArgs {
     Q4AttentionArgs at;
     float* scores;  // [n_heads][max_seq], of one token's heads in powers of two, for the weights; may be null
 };
-constexpr uint32_t kFewRows = 16, kFewKeys = 32;
-template <int HD>
-constexpr uint32_t kFewWaves = 4;
+constexpr uint32_t kFewRows = 16, kFewKeys = 32, kFewWaves = 4;
 template <int HD>
 constexpr uint32_t kFewSlots = kCus * (HD <= 64 ? 2 : HD == 128 ? 3 : 1);  // workgroups that the GPU has at once
 
 template <int HD>
-__global__ __launch_bounds__(64 * kFewWaves<HD>, HD <= 64 ? 4 : HD == 128 ? 3 : 1) void attention_q4_few_kernel(FewArgs args) {
+__global__ __launch_bounds__(64 * kFewWaves, HD <= 64 ? 4 : HD == 128 ? 3 : 1) void attention_q4_few_kernel(FewArgs args) {
     const Q4AttentionArgs& a = args.at;
-    constexpr uint32_t kWaves = kFewWaves<HD>;
+    constexpr uint32_t kWaves = kFewWaves;
     constexpr int SLABS = HD / 32, CS = HD / 16, kStates = 2 + HD / 4, kLoad = SLABS < 4 ? SLABS : 4, kLoads = SLABS / kLoad;  // words a load, loads a row
     constexpr int TD = HD < 64 ? HD : 64, PARTS = HD / TD, SP = SLABS / PARTS;  // dims in LDS at a time, words of a lane in them
     using VT = ValueTile<TD, (int)kFewKeys>;
     constexpr size_t kValues = sizeof(VT) * kWaves, kStateBytes = sizeof(float) * kStates * 64 * kWaves;
     __shared__ __align__(16) uint8_t smem[kValues > kStateBytes ? kValues : kStateBytes];
     const uint32_t group = a.n_heads / a.n_kv_heads, rows = a.n * group;
-    const uint32_t c = blockIdx.x % a.n_kv_heads, split = blockIdx.x / a.n_kv_heads % a.splits, r0 = blockIdx.x / a.n_kv_heads / a.splits * kFewRows;
+    const uint32_t c = blockIdx.x % a.n_kv_heads, split = blockIdx.x / a.n_kv_heads % a.splits, r0 = ((rows + kFewRows - 1u) / kFewRows - 1u - blockIdx.x / a.n_kv_heads / a.splits) * kFewRows;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, l16 = lane & 15u, g = lane >> 4, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
     const uint32_t base = first_row(a), last = sees(a, base, r0 + kFewRows - 1u, rows, group), used = used_splits(a.splits, last / (kFewKeys * kWaves) + 1u);
     if (split >= used) return;
@@ -701,7 +707,7 @@ __global__ __launch_bounds__(64 * kFewWaves<HD>, HD <= 64 ? 4 : HD == 128 ? 3 : 
     }
     float* to;
     float inverse = 1.0f;
-    if (a.splits == 1u) {
+    if (a.splits == 1u && !args.scores) {
         to = a.out + (size_t)token * a.out_stride + (size_t)head * HD;
         inverse = __fdiv_rn(1.0f, l);
         if (a.stats && g == 0 && wave == 0) {
@@ -725,9 +731,9 @@ __global__ __launch_bounds__(64 * kFewWaves<HD>, HD <= 64 ? 4 : HD == 128 ? 3 : 
 template <int HD>
 __global__ __launch_bounds__(256) void attention_q4_finish_kernel(FewArgs args) {
     const Q4AttentionArgs& a = args.at;
-    if (blockIdx.x < a.n_heads) return merge_splits<HD, 1024 / HD>(a, kFewRows, kFewKeys * kFewWaves<HD>);
+    if (blockIdx.x < a.n_heads) return merge_splits<HD, 1024 / HD>(a, kFewRows, kFewKeys * kFewWaves);
     const uint32_t group = a.n_heads / a.n_kv_heads, nth = blockIdx.x - a.n_heads, c = nth % a.n_kv_heads, t = nth / a.n_kv_heads * 256u + threadIdx.x, lane = threadIdx.x & 63u;
-    const uint32_t last = first_row(a), used = used_splits(a.splits, last / (kFewKeys * kFewWaves<HD>) + 1u);
+    const uint32_t last = first_row(a), used = used_splits(a.splits, last / (kFewKeys * kFewWaves) + 1u);
     if (t - threadIdx.x > last) return;
     constexpr uint32_t kPerLane = (kMaxSplits + 63u) / 64u;
     const uint32_t at = min(t, last);
@@ -751,17 +757,26 @@ __global__ __launch_bounds__(256) void attention_q4_finish_kernel(FewArgs args) 
     if (t <= last) a.weights[(size_t)c * a.max_seq + t] += sum;
 }
 
-// What 64 rows of a KV head have gathered: the scores once more, now that every softmax's maximum and sum is known, and their weights added
-// up over the query rows -- 32 of them at a time and wave, kept apart by lane and wave and added in one order at the end.
-template <int HD, int WAVES>
+// What 32 U rows of a KV head have gathered: the scores once more, now that every softmax's maximum and sum is known, and their weights added
+// up over the query rows -- 32 of them at a time and wave, the next ones on their way meanwhile, kept apart by lane and wave and added in one order at the end.
+template <int HD, int WAVES, int U>
 __global__ __launch_bounds__(64 * WAVES) void attention_q4_weights_kernel(Q4AttentionArgs a) {
-    constexpr int KT = 64, LD = HD + 8, SLABS = HD / 16, U = KT / 32;
+    constexpr int KT = 32 * U, LD = HD + 8, SLABS = HD / 16;
     __shared__ __align__(16) _Float16 keys[2][KT][LD];
     __shared__ float sums[WAVES][KT];
     const uint32_t c = blockIdx.y, key0 = blockIdx.x * KT, group = a.n_heads / a.n_kv_heads, rows = a.n * group;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, l32 = lane & 31u, h = lane >> 5, wave = tid >> 6;
     const uint32_t base = first_row(a), last = sees(a, base, rows - 1u, rows, group);
     if (key0 > last) return;
+    const uint32_t r_first = key0 > base ? (key0 - base) * group / 32u * 32u : 0u;  // rows in front of it see none of the keys
+    typename Queries<HD>::Raw raw;
+    float2 stat;
+    const auto request = [&](uint32_t r0) {  // (of rows past the last: the last one's, for nobody)
+        const uint32_t r = min(r0 + l32, rows - 1u);
+        raw.request(a, r, c, group, h);
+        stat = *reinterpret_cast<const float2*>(a.stats + 2u * ((size_t)(r / group) * a.n_heads + c * group + r % group));
+    };
+    request(r_first + 32u * wave);
     const Q4Cache kc = q4_planes(const_cast<void*>(a.k_cache), a.max_seq, a.n_kv_heads, HD), vc = q4_planes(const_cast<void*>(a.v_cache), a.max_seq, a.n_kv_heads, HD);
     const size_t first = (size_t)c * a.max_seq;
     for (uint32_t i = tid; i < KT * HD / 8; i += 64 * WAVES) {
@@ -778,13 +793,12 @@ __global__ __launch_bounds__(64 * WAVES) void attention_q4_weights_kernel(Q4Atte
     for (int u = 0; u < U; u++)
 #pragma unroll
         for (int e = 0; e < 16; e++) acc[u][e] = 0.0f;
-    const uint32_t r_first = key0 > base ? (key0 - base) * group / 32u * 32u : 0u;  // rows in front of it see none of the keys
     for (uint32_t r0 = r_first + 32u * wave; r0 < rows; r0 += 32u * WAVES) {
-        const uint32_t r = min(r0 + l32, rows - 1u), mine = sees(a, base, r, rows, group);
+        const uint32_t mine = sees(a, base, r0 + l32, rows, group);
         Queries<HD> q;
-        q.load(a, r, c, group, h);
-        const float* const st = a.stats + 2u * ((size_t)(r / group) * a.n_heads + c * group + r % group);
-        const float shift = (st[0] == -__builtin_inff() ? 0.0f : st[0]) - kWeightBits, inverse = st[1];
+        q.take(raw, a.scale);
+        const float shift = (stat.x == -__builtin_inff() ? 0.0f : stat.x) - kWeightBits, inverse = stat.y;
+        request(r0 + 32u * WAVES);
 #pragma unroll
         for (int u = 0; u < U; u++) {
             v16f sc;
@@ -814,51 +828,74 @@ __global__ __launch_bounds__(64 * WAVES) void attention_q4_weights_kernel(Q4Atte
     __syncthreads();
     if (tid < KT && key0 + tid <= last) {
         float w = sums[0][tid];
+#pragma unroll
         for (int i = 1; i < WAVES; i++) w += sums[i][tid];
         a.weights[first + key0 + tid] += w;
     }
 }
 
+// Large launches: as many splits as workgroups fit on the GPU, three tiles or more each (a split's state is written and read again).
 template <int HD, int WQ, int WK, int PER_CU>
-hipError_t launch_tiles(Q4AttentionArgs a, const Launch& L) {
+hipError_t launch_tiles(Q4AttentionArgs a, uint64_t seen, const Launch& L) {
     constexpr uint32_t RB = 32 * WQ, KT = 32 * WK;
-    const uint32_t rows = a.n * (a.n_heads / a.n_kv_heads), base = a.n_kv_heads * ((rows + RB - 1u) / RB);
-    const uint64_t seen = a.d_pos ? a.max_seq : (uint64_t)a.pos0 + a.n;
-    const uint32_t tiles = (uint32_t)((seen + KT - 1u) / KT), room = kCus * PER_CU / base, most = rows <= 32u ? tiles : (tiles + 2u) / 3u;
-    a.splits = room < 2u ? 1u : (room < most ? room : most);
-    if (a.splits > kMaxSplits) a.splits = kMaxSplits;
-    const uint32_t blocks = base / a.n_kv_heads;
-    a.first_blocks = base * a.splits > kCus && base * a.splits <= 2u * kCus ? (kCus + a.n_kv_heads * a.splits - 1u) / (a.n_kv_heads * a.splits) : blocks;
-    hipError_t e = launch_kernel(L, kFamOther, attention_q4_kernel<HD, WQ, WK, PER_CU>, dim3(base * a.splits), dim3(64 * WQ * WK), a);
+    const uint32_t rows = a.n * (a.n_heads / a.n_kv_heads), blocks = (rows + RB - 1u) / RB, base = a.n_kv_heads * blocks;
+    const uint32_t room = kCus * PER_CU / base, most = (uint32_t)((seen + 3u * KT - 1u) / (3u * KT));
+    a.splits = std::min({std::max(room, 1u), most, kMaxSplits});
+    const uint32_t per_block = a.n_kv_heads * a.splits;
+    a.first_blocks = base * a.splits > kCus && base * a.splits <= 2u * kCus ? (kCus + per_block - 1u) / per_block : blocks;
+    const hipError_t e = launch_kernel(L, kFamOther, attention_q4_kernel<HD, WQ, WK, PER_CU>, dim3(base * a.splits), dim3(64 * WQ * WK), a);
     if (e != hipSuccess || a.splits == 1u) return e;
     const uint32_t merged = a.n * a.n_heads;
     return a.splits > 8u ? launch_kernel(L, kFamOther, attention_q4_merge_kernel<HD, 1024 / HD>, dim3(merged), dim3(256), a, RB, KT)
                          : launch_kernel(L, kFamOther, attention_q4_merge_kernel<HD, 1>, dim3((merged + 1024u / HD - 1u) / (1024u / HD)), dim3(256), a, RB, KT);
 }
 
+// Small ones: workgroups of 16 query rows and as many splits as fill the GPU, down to a unit of keys for each wave.
+template <int HD>
+hipError_t launch_few(FewArgs f, uint64_t seen, const Launch& L) {
+    const Q4AttentionArgs& a = f.at;
+    constexpr uint32_t kSpan = kFewKeys * kFewWaves;
+    const uint32_t rows = a.n * (a.n_heads / a.n_kv_heads), base = a.n_kv_heads * ((rows + kFewRows - 1u) / kFewRows);
+    f.at.splits = std::min({std::max(kFewSlots<HD> / base, 1u), (uint32_t)((seen + kSpan - 1u) / kSpan), kMaxSplits});
+    const hipError_t e = launch_kernel(L, kFamOther, attention_q4_few_kernel<HD>, dim3(base * a.splits), dim3(64 * kFewWaves), f);
+    if (e != hipSuccess) return e;
+    if (f.scores) return launch_kernel(L, kFamOther, attention_q4_finish_kernel<HD>, dim3(a.n_heads + a.n_kv_heads * (uint32_t)((seen + 255u) / 256u)), dim3(256), f);
+    return a.splits == 1u ? e : launch_kernel(L, kFamOther, attention_q4_merge_kernel<HD, 1024 / HD>, dim3(a.n * a.n_heads), dim3(256), a, kFewRows, kSpan);
+}
+
+// Which kernel: the one for few rows wastes nothing on them and fills the GPU with little work, the tiled one reads and unpacks the cache for up to eight
+// times as many rows at once.  Up to 64 rows of a KV head the first is as fast or faster at any length (heads of 64 values, 32 query heads, 8 KV heads, in us:
+// 32 rows behind 100000 47 against 81, 64 behind 60000 55 and 55, 96 behind 60000 82 and 57), and with more rows up to some 2^29 of (query row, key,
+// value) products: 555 tokens of 16 heads 9.9 against 17.1, 64 tokens behind 4000 22.7 and 22.8, 1000 tokens of 32 heads 30.2 and 29.1, 2002 of them
+// 95 and 65; heads of 32 values, 1400 tokens of 16 heads 18.9 and 19.9, 2000 32.8 and 27.5; of 128, 64 tokens of 16 heads behind 4000 25.4 and 27.5, 300
+// behind 1000 33.5 and 31.4; of 256, 500 tokens of 8 heads behind 500 35 and 43, 1000 behind 1000 103 and 82.
 template <int HD>
 hipError_t launch_head_dim(const Q4AttentionArgs& a, float* d_scores, const Launch& L) {
     const uint32_t rows = a.n * (a.n_heads / a.n_kv_heads);
-    const uint64_t seen = a.d_pos ? a.max_seq : (uint64_t)a.pos0 + a.n;
+    const uint64_t seen = a.d_pos ? a.max_seq : (uint64_t)a.pos0 + a.n, products = (uint64_t)a.n * a.n_heads * (seen - a.n / 2u) * HD;
     hipError_t e;
-    if (rows <= kFewRows) {
-        FewArgs f{a, a.n == 1u && a.weights ? d_scores : nullptr};
-        const uint32_t base = a.n_kv_heads, span = kFewKeys * kFewWaves<HD>, most = (uint32_t)((seen + span - 1u) / span), room = kFewSlots<HD> / base;
-        f.at.splits = room < 2u ? 1u : (room < most ? room : most);
-        if (f.at.splits > kMaxSplits) f.at.splits = kMaxSplits;
-        e = launch_kernel(L, kFamOther, attention_q4_few_kernel<HD>, dim3(base * f.at.splits), dim3(64 * kFewWaves<HD>), f);
-        if (e != hipSuccess) return e;
-        if (f.scores && f.at.splits > 1u)
-            return launch_kernel(L, kFamOther, attention_q4_finish_kernel<HD>, dim3(a.n_heads + a.n_kv_heads * (uint32_t)((seen + 255u) / 256u)), dim3(256), f);
-        if (f.at.splits > 1u) e = launch_kernel(L, kFamOther, attention_q4_merge_kernel<HD, 1024 / HD>, dim3(a.n * a.n_heads), dim3(256), f.at, kFewRows, span);
-    } else if constexpr (HD == 32) e = launch_tiles<HD, 2, 2, 2>(a, L);
-    else if constexpr (HD == 64) e = launch_tiles<HD, 4, 2, 1>(a, L);
-    else if constexpr (HD == 128) e = launch_tiles<HD, 4, 2, 1>(a, L);
-    else e = launch_tiles<HD, 4, 1, 1>(a, L);
+    if (rows <= 64u || products <= 1ull << 29) {
+        float* const scores = a.n == 1u && a.weights ? d_scores : nullptr;
+        e = launch_few<HD>(FewArgs{a, scores}, seen, L);
+        if (scores) return e;
+    } else if constexpr (HD == 32) {
+        e = launch_tiles<HD, 2, 2, 2>(a, seen, L);
+    } else if constexpr (HD <= 128) {
+        // Where every CU has a block of rows of its own, two workgroups of half the keys a CU (2048 tokens behind 6144 of 16 heads of 128 values 344 us
+        // against 365, 4000 tokens of 32 heads of 64 values 225 against 237), else one (500 behind 2000 of those 43 against 45).
+        const bool many = a.n_kv_heads * ((rows + 127u) / 128u) >= kCus;
+        e = many ? launch_tiles<HD, 4, 1, 2>(a, seen, L) : launch_tiles<HD, 4, 2, 1>(a, seen, L);
+    } else {
+        e = launch_tiles<HD, 4, 1, 1>(a, seen, L);
+    }
     if (e != hipSuccess || !a.weights) return e;
-    const dim3 grid((uint32_t)((seen + 63) / 64), a.n_kv_heads);
-    return rows <= 32u ? launch_kernel(L, kFamOther, attention_q4_weights_kernel<HD, 1>, grid, dim3(64), a)
-                       : launch_kernel(L, kFamOther, attention_q4_weights_kernel<HD, 8>, grid, dim3(512), a);
+    const uint32_t wide = (uint32_t)((seen + 63u) / 64u);
+    if constexpr (HD <= 128) {  // (of 256 values: the next rows do not fit into the registers)
+        constexpr int kWaves = HD <= 64 ? 16 : 8;
+        if (wide * a.n_kv_heads < kCus)
+            return launch_kernel(L, kFamOther, attention_q4_weights_kernel<HD, kWaves, 1>, dim3((uint32_t)((seen + 31u) / 32u), a.n_kv_heads), dim3(64 * kWaves), a);
+    }
+    return launch_kernel(L, kFamOther, attention_q4_weights_kernel<HD, 8, 2>, dim3(wide, a.n_kv_heads), dim3(512), a);
 }
 
 // Floats of the splits' records: what a split launch has at most, for any number of tokens up to n.
