@@ -167,8 +167,13 @@ PROMPTS = [  # head_dim, heads, KV heads, first row, tokens, rows behind them, f
 ]
 
 
-@pytest.mark.parametrize("weights", [False, True])
-@pytest.mark.parametrize("hd,heads,n_kv,pos0,n,behind,pad", PROMPTS)
+LARGE = [  # more than 64 rows of a KV head and 2^29 products: the tiled kernels, split over few and many workgroups, one and two workgroups a CU
+    (64, 16, 4, 1777, 333, 0, 0), (64, 32, 8, 0, 1030, 3, 0), (64, 2, 1, 66000, 65, 0, 0), (64, 12, 4, 900, 701, 5, 4), (128, 6, 2, 2222, 301, 0, 8),
+    (128, 16, 4, 7, 2050, 0, 0), (256, 3, 1, 1300, 500, 40, 0), (32, 8, 8, 1000, 1500, 0, 0), (32, 24, 2, 20001, 67, 0, 0),
+]
+
+
+@pytest.mark.parametrize("hd,heads,n_kv,pos0,n,behind,pad,weights", [(*p, w) for p in PROMPTS for w in (False, True)] + [(*p, True) for p in LARGE])
 def test_attention_of_a_prompt(ctx, ops, dev, hd, heads, n_kv, pos0, n, behind, pad, weights):
     max_seq, stride = pos0 + n + behind, heads * hd + pad
     k, v = filled(n, max_seq, n_kv, hd, pos0 + n)
@@ -192,7 +197,8 @@ def test_attention_of_a_prompt(ctx, ops, dev, hd, heads, n_kv, pos0, n, behind, 
         assert np.array_equal(got, w0)
 
 
-@pytest.mark.parametrize("hd,heads,n_kv,pos0,n", [(64, 4, 2, 0, 100), (128, 2, 1, 70, 30), (64, 4, 2, 300, 1), (32, 2, 2, 5, 60), (256, 2, 2, 5, 60)])
+@pytest.mark.parametrize("hd,heads,n_kv,pos0,n", [(64, 4, 2, 0, 100), (128, 2, 1, 70, 30), (64, 4, 2, 300, 1), (32, 2, 2, 5, 60), (256, 2, 2, 5, 60),
+                                                  (64, 8, 2, 1500, 600), (128, 8, 4, 700, 600), (32, 16, 2, 300, 1200), (256, 4, 2, 500, 700)])
 def test_a_row_held_as_nan_is_seen_by_those_that_see_it(ctx, ops, dev, hd, heads, n_kv, pos0, n):
     """Of keys in head 0, of values in the last head: NaN to the tokens from that row on, everything as without it to those before."""
     max_seq, bad = pos0 + n, pos0 + n // 2
@@ -214,30 +220,31 @@ def test_a_row_held_as_nan_is_seen_by_those_that_see_it(ctx, ops, dev, hd, heads
         assert_f32_parity(out[~hit], clean[~hit], "tokens that do not see it")
 
 
+@pytest.mark.parametrize("heads,n_kv,seq,n", [(4, 2, 300, 20), (16, 4, 1200, 700)])
 @pytest.mark.parametrize("factor", [1e-30, 1e-6, 1e4, 3e4])
-def test_queries_of_all_sizes(ctx, ops, dev, factor):
+def test_queries_of_all_sizes(ctx, ops, dev, factor, heads, n_kv, seq, n):
     """Tiny queries weigh all rows alike, huge ones one row alone; both with keys that answer in kind."""
-    hd, heads, n_kv, seq = 64, 4, 2, 300
+    hd = 64
     k, v = R.Cache(seq, n_kv, hd), R.Cache(seq, n_kv, hd)
     k.append(0, normal(1, seq, n_kv, hd) * np.float32(1 / factor if factor > 1 else 1000)), v.append(0, normal(2, seq, n_kv, hd) * np.float32(1e-4))
-    q = (normal(3, 20, heads, hd) * factor).astype(np.float32)
-    scratch, d_out = scratch_for(ctx, dev, 20, seq, heads, n_kv, hd), dev(np.zeros((20, heads, hd), np.float32))
-    ops.encode_attention_prefill_q4(dev(q), heads * hd, dev(k.raw), dev(v.raw), d_out, heads * hd, scratch, seq - 20, 20, seq, heads, n_kv, hd)
-    assert_f32_parity(d_out.download(np.float32, q.size).reshape(q.shape), R.attention(q, k, v, seq - 20)[0], "out")
-    ops.encode_attention_q4(dev(q[19]), dev(k.raw), dev(v.raw), d_out, scratch, seq, seq, heads, n_kv, hd)
-    assert_f32_parity(d_out.download(np.float32, heads * hd).reshape(heads, hd), R.attention(q[19:], k, v, seq - 1)[0][0], "one token")
+    q = (normal(3, n, heads, hd) * factor).astype(np.float32)
+    scratch, d_out = scratch_for(ctx, dev, n, seq, heads, n_kv, hd), dev(np.zeros((n, heads, hd), np.float32))
+    ops.encode_attention_prefill_q4(dev(q), heads * hd, dev(k.raw), dev(v.raw), d_out, heads * hd, scratch, seq - n, n, seq, heads, n_kv, hd)
+    assert_f32_parity(d_out.download(np.float32, q.size).reshape(q.shape), R.attention(q, k, v, seq - n)[0], "out")
+    ops.encode_attention_q4(dev(q[n - 1]), dev(k.raw), dev(v.raw), d_out, scratch, seq, seq, heads, n_kv, hd)
+    assert_f32_parity(d_out.download(np.float32, heads * hd).reshape(heads, hd), R.attention(q[n - 1:], k, v, seq - 1)[0][0], "one token")
 
 
-def test_a_value_that_is_not_finite_stays_with_its_query(ctx, ops, dev):
-    hd, heads, n_kv, n = 64, 4, 2, 50
+@pytest.mark.parametrize("hd,heads,n_kv,n", [(64, 4, 2, 50), (128, 8, 2, 1100)])
+def test_a_value_that_is_not_finite_stays_with_its_query(ctx, ops, dev, hd, heads, n_kv, n):
     k, v = filled(1, n, n_kv, hd, n)
     q = normal(3, n, heads, hd)
     ref = R.attention(q, k, v, 0)[0]
-    q[10, 1, 5], q[30, 2, 60] = np.nan, np.inf
+    q[10, 1, 5], q[n - 20, 2, 60] = np.nan, np.inf
     scratch, d_out = scratch_for(ctx, dev, n, n, heads, n_kv, hd), dev(np.zeros((n, heads, hd), np.float32))
     ops.encode_attention_prefill_q4(dev(q), heads * hd, dev(k.raw), dev(v.raw), d_out, heads * hd, scratch, 0, n, n, heads, n_kv, hd)
     out, hit = d_out.download(np.float32, q.size).reshape(q.shape), np.zeros((n, heads), bool)
-    hit[10, 1] = hit[30, 2] = True
+    hit[10, 1] = hit[n - 20, 2] = True
     assert np.isnan(out[hit]).all()
     assert_f32_parity(out[~hit], ref[~hit], "the others")
 
@@ -358,8 +365,9 @@ def test_a_captured_step_replayed_while_the_position_moves(ctx, ops, dev):
     ctx.graph_destroy(g)
 
 
-def test_results_do_not_change_from_run_to_run(ctx, ops, dev):
-    hd, heads, n_kv, n, pos0 = 64, 16, 4, 300, 500
+@pytest.mark.parametrize("n,pos0", [(300, 500), (700, 500)])
+def test_results_do_not_change_from_run_to_run(ctx, ops, dev, n, pos0):
+    hd, heads, n_kv = 64, 16, 4
     k, v = filled(3, pos0 + n, n_kv, hd, pos0 + n)
     q, d_k, d_v = dev(normal(4, n, heads, hd)), dev(k.raw), dev(v.raw)
     scratch, got = scratch_for(ctx, dev, n, pos0 + n, heads, n_kv, hd, True), []
