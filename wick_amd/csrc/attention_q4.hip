@@ -51,13 +51,13 @@ __device__ __forceinline__ uint32_t sees(const Q4AttentionArgs& a, uint32_t base
 // Splits that a workgroup of `tiles` tiles has in earnest: with the position on the device the host does not know.
 __device__ __forceinline__ uint32_t used_splits(uint32_t splits, uint32_t tiles) { return min(splits, tiles); }
 
-// Eight values of a word as two planes of halves, a pair at a time.  (The mask in a scalar and the offset's bits in a vector register: one instruction
-// takes both.)
+// Eight values of a word as two planes of halves, a pair at a time: nibbles in bits 0 .. 3 of a half are the last bits of 1024 + nibble, in bits 4 .. 7 those of
+// 64 + nibble, so only the upper half of the pairs is shifted.  (The mask in a scalar and the offset's bits in a vector register: one instruction takes both.)
 __device__ __forceinline__ void dequantize_pair(uint32_t w, _Float16 scale, int i, h8& hi, h8& lo) {
-    const h2 d = {scale, scale}, offset = {(_Float16)1032.0f, (_Float16)1032.0f};
-    uint32_t mask = 0x000f000fu, bits = 0x64006400u;
+    const h2 d = {scale, scale}, offset = i & 1 ? h2{(_Float16)72.0f, (_Float16)72.0f} : h2{(_Float16)1032.0f, (_Float16)1032.0f};
+    uint32_t mask = i & 1 ? 0x00f000f0u : 0x000f000fu, bits = i & 1 ? 0x54005400u : 0x64006400u;
     asm("" : "+s"(mask), "+v"(bits));
-    const h2 n = __builtin_bit_cast(h2, ((w >> (4 * i)) & mask) | bits) - offset;  // 1024 + nibble, exact
+    const h2 n = __builtin_bit_cast(h2, ((i < 2 ? w : w >> 8) & mask) | bits) - offset;  // nibble - 8, exact
     const h2 h = n * d, l = __builtin_elementwise_fma(n, d, -h);
     hi[2 * i] = h[0], hi[2 * i + 1] = h[1], lo[2 * i] = l[0], lo[2 * i + 1] = l[1];
 }
