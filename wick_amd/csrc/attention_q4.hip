@@ -53,17 +53,17 @@ __device__ __forceinline__ uint32_t used_splits(uint32_t splits, uint32_t tiles)
 
 // Eight values of a word as two planes of halves, a pair at a time: nibbles in bits 0 .. 3 of a half are the last bits of 1024 + nibble, in bits 4 .. 7 those of
 // 64 + nibble, so only the upper half of the pairs is shifted.  (The mask in a scalar and the offset's bits in a vector register: one instruction takes both.)
-__device__ __forceinline__ void dequantize_pair(uint32_t w, _Float16 scale, int i, h8& hi, h8& lo) {
-    const h2 d = {scale, scale}, offset = i & 1 ? h2{(_Float16)72.0f, (_Float16)72.0f} : h2{(_Float16)1032.0f, (_Float16)1032.0f};
+__device__ __forceinline__ void dequantize_pair(uint32_t w, h2 d, int i, int at, h8& hi, h8& lo) {
+    const h2 offset = i & 1 ? h2{(_Float16)72.0f, (_Float16)72.0f} : h2{(_Float16)1032.0f, (_Float16)1032.0f};
     uint32_t mask = i & 1 ? 0x00f000f0u : 0x000f000fu, bits = i & 1 ? 0x54005400u : 0x64006400u;
     asm("" : "+s"(mask), "+v"(bits));
     const h2 n = __builtin_bit_cast(h2, ((i < 2 ? w : w >> 8) & mask) | bits) - offset;  // nibble - 8, exact
     const h2 h = n * d, l = __builtin_elementwise_fma(n, d, -h);
-    hi[2 * i] = h[0], hi[2 * i + 1] = h[1], lo[2 * i] = l[0], lo[2 * i + 1] = l[1];
+    hi[2 * at] = h[0], hi[2 * at + 1] = h[1], lo[2 * at] = l[0], lo[2 * at + 1] = l[1];
 }
 __device__ __forceinline__ void dequantize(uint32_t w, _Float16 scale, h8& hi, h8& lo) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) dequantize_pair(w, scale, i, hi, lo);
+    for (int i = 0; i < 4; i++) dequantize_pair(w, h2{scale, scale}, i, i, hi, lo);
 }
 
 // Four f32 values as two planes: a pair at a time, then one instruction a value (y * 1 - hi, rounded to a half; the compiler does not see the 1 and cannot
@@ -212,7 +212,7 @@ __global__ __launch_bounds__(64 * WQ * WK, PER_CU * WQ * WK / 4) void attention_
             const _Float16 vd = __builtin_bit_cast(_Float16, x.vd[p]), poison = vd * (_Float16)0.0f;
             step_scale = keys ? __builtin_bit_cast(_Float16, x.kd[p]) + poison : poison == poison ? vd : (_Float16)0.0f;
         }
-        dequantize_pair(x.w[p].w[e], step_scale, step % 4, step_hi, step_lo);
+        dequantize_pair(x.w[p].w[e], h2{step_scale, step_scale}, step % 4, step % 4, step_hi, step_lo);
         if (step % 4 != 3) return;
         _Float16* const hi = keys ? &k_tile[buffer].h[0][row][8u * word] : &v_tile[buffer].h[0][row][8u * (word ^ VT::swizzle(row))];
         *reinterpret_cast<h8*>(hi) = step_hi, *reinterpret_cast<h8*>(hi + (keys ? KT * (HD + 8) : KT * HD)) = step_lo;
@@ -483,8 +483,9 @@ __global__ __launch_bounds__(256) void attention_q4_merge_kernel(Q4AttentionArgs
 
 // ---- few query rows ----
 // Up to 16 query rows of a KV head (the heads of one token, of a few tokens) per workgroup, and a part of the cache to each of its waves, 32 rows
-// at a time, on v_mfma_f32_16x16x32_f16.  Nothing is shared but the states at the end: a lane loads the words of a key row that it multiplies (lane group g
-// HD / 32 of them from word g HD / 32 on, the order of an MFMA's K steps being free), values go through LDS of the wave's own to be transposed.
+// at a time, on v_mfma_f32_16x16x32_f16.  Nothing goes through LDS but the states at the end: a lane loads the words of a key row that it multiplies (lane
+// group g HD / 32 of them from word g HD / 32 on, the order of an MFMA's K steps being free), and of the values one word of eight rows, the rows whose weights it
+// holds: two rows' words are transposed to pairs of one dim's values with one byte permutation each.
 struct FewArgs {
     Q4AttentionArgs at;
     float* scores;  // [n_heads][max_seq], of one token's heads in powers of two, for the weights; may be null
@@ -498,10 +499,9 @@ __global__ __launch_bounds__(64 * kFewWaves, HD <= 64 ? 4 : HD == 128 ? 3 : 1) v
     const Q4AttentionArgs& a = args.at;
     constexpr uint32_t kWaves = kFewWaves;
     constexpr int SLABS = HD / 32, CS = HD / 16, kStates = 2 + HD / 4, kLoad = SLABS < 4 ? SLABS : 4, kLoads = SLABS / kLoad;  // words a load, loads a row
-    constexpr int TD = HD < 64 ? HD : 64, PARTS = HD / TD, SP = SLABS / PARTS;  // dims in LDS at a time, words of a lane in them
-    using VT = ValueTile<TD, (int)kFewKeys>;
-    constexpr size_t kValues = sizeof(VT) * kWaves, kStateBytes = sizeof(float) * kStates * 64 * kWaves;
-    __shared__ __align__(16) uint8_t smem[kValues > kStateBytes ? kValues : kStateBytes];
+    // a value row's words: lane l16 has word l16 % kOctets (and the one kOctets behind it), or as many dims of it as lanes do not share it
+    constexpr int kOctets = HD < 128 ? HD / 8 : 16, kSharers = 16 / kOctets, kMine = HD / 8 / kOctets, kVd = 8 * kMine;
+    __shared__ float smem[kStates * 64 * kWaves];
     const uint32_t group = a.n_heads / a.n_kv_heads, rows = a.n * group;
     const uint32_t c = blockIdx.x % a.n_kv_heads, split = blockIdx.x / a.n_kv_heads % a.splits, r0 = ((rows + kFewRows - 1u) / kFewRows - 1u - blockIdx.x / a.n_kv_heads / a.splits) * kFewRows;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, l16 = lane & 15u, g = lane >> 4, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
@@ -511,7 +511,7 @@ __global__ __launch_bounds__(64 * kFewWaves, HD <= 64 ? 4 : HD == 128 ? 3 : 1) v
     const uint32_t u_first = (uint32_t)((uint64_t)units * nth / (used * kWaves)), u_end = (uint32_t)((uint64_t)units * (nth + 1u) / (used * kWaves));
     const uint32_t r = min(r0 + l16, rows - 1u), mine = sees(a, base, r, rows, group), first_sees = sees(a, base, r0, rows, group);
     const uint32_t token = r / group, head = c * group + r % group;
-    VT& v_tile = reinterpret_cast<VT*>(smem)[wave];
+    const uint32_t octet = l16 % kOctets, sharer = l16 / kOctets;
 
     const Q4Cache kc = q4_planes(const_cast<void*>(a.k_cache), a.max_seq, a.n_kv_heads, HD), vc = q4_planes(const_cast<void*>(a.v_cache), a.max_seq, a.n_kv_heads, HD);
     const size_t first = (size_t)c * a.max_seq;
@@ -519,12 +519,14 @@ __global__ __launch_bounds__(64 * kFewWaves, HD <= 64 ? 4 : HD == 128 ? 3 : 1) v
         return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(static_cast<const uint8_t*>(p)) + first * row_bytes, 0, (int)((last + 1u) * row_bytes), 0x27000);
     };
     const auto kq = plane(kc.quants, HD / 2), vq = plane(vc.quants, HD / 2), ks = plane(kc.scales, HD / 16), vs = plane(vc.scales, HD / 16);
-    struct Unit {  // this lane's words of keys l16 and 16 + l16, and of those values
+    struct Unit {
         struct __attribute__((aligned(4 * kLoad))) Words {
             uint32_t w[kLoad];
         };
-        Words k[2][kLoads], v[2][kLoads];
-        uint16_t kd[2][kLoads], vd[2][kLoads];
+        Words k[2][kLoads];  // of keys l16 and 16 + l16
+        uint32_t kd[2][kLoads];
+        uint32_t v[8][kMine];  // of values 4 g .. and 16 + 4 g ..
+        uint32_t vd[kVd];      // and their scales: of the word's block (heads of 64 values: of both blocks)
     };
     const auto load = [&](decltype(kq) from, uint32_t at) {
         if constexpr (kLoad == 1) return __builtin_bit_cast(typename Unit::Words, __builtin_amdgcn_raw_buffer_load_b32(from, at, 0, 0));
@@ -537,10 +539,24 @@ __global__ __launch_bounds__(64 * kFewWaves, HD <= 64 ? 4 : HD == 128 ? 3 : 1) v
 #pragma unroll
             for (uint32_t i = 0; i < kLoads; i++) {
                 const uint32_t row = unit * kFewKeys + 16u * u + l16, word = g * SLABS + i * kLoad;
-                x.k[u][i] = load(kq, row * (HD / 2) + 4u * word), x.v[u][i] = load(vq, row * (HD / 2) + 4u * word);
-                x.kd[u][i] = __builtin_amdgcn_raw_buffer_load_b16(ks, row * (HD / 16) + word / 4u * 2u, 0, 0);
-                x.vd[u][i] = __builtin_amdgcn_raw_buffer_load_b16(vs, row * (HD / 16) + word / 4u * 2u, 0, 0);
+                x.k[u][i] = load(kq, row * (HD / 2) + 4u * word), x.kd[u][i] = __builtin_amdgcn_raw_buffer_load_b16(ks, row * (HD / 16) + word / 4u * 2u, 0, 0);
             }
+#pragma unroll
+        for (uint32_t j = 0; j < 8; j++)
+#pragma unroll
+            for (uint32_t i = 0; i < kMine; i++) {
+                const uint32_t row = unit * kFewKeys + 16u * (j / 4u) + 4u * g + j % 4u, word = octet + i * kOctets;
+                x.v[j][i] = __builtin_amdgcn_raw_buffer_load_b32(vq, row * (HD / 2) + 4u * word, 0, 0);
+                if constexpr (HD != 64) x.vd[j * kMine + i] = __builtin_amdgcn_raw_buffer_load_b16(vs, row * (HD / 16) + word / 4u * 2u, 0, 0);
+            }
+        if constexpr (HD == 64) {
+#pragma unroll
+            for (uint32_t u = 0; u < 2; u++) {
+                const auto d = __builtin_amdgcn_raw_buffer_load_b128(vs, (unit * kFewKeys + 16u * u + 4u * g) * (HD / 16), 0, 0);
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++) x.vd[4 * u + j] = d[j];
+            }
+        }
     };
     Unit units_ahead[2];
     fetch(u_first, units_ahead[0]);
@@ -573,52 +589,57 @@ __global__ __launch_bounds__(64 * kFewWaves, HD <= 64 ? 4 : HD == 128 ? 3 : 1) v
             qh[s] = __builtin_shufflevector(u[0], u[1], 0, 1, 2, 3, 4, 5, 6, 7), ql[s] = __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
-    // V^T rows 16 i + l16 of the part that is in LDS (dims HD / 4 i + 16 part + l16 of the head), keys 4 g .. and 16 + 4 g ..: the 16 lanes of a group point at
-    // 4 keys x 16 dims, lane j at key j / 4 and dims 4 (j % 4) .. of them.
-    const uint32_t vkey = 4u * g + (l16 >> 2), vpiece = l16 >> 1 & 1u;
-    const auto read_v = [&](int half, int i) {
-        typedef short s4 __attribute__((ext_vector_type(4)));
-        typedef __attribute__((address_space(3))) s4* lds_s4;
-        const _Float16* const p = &v_tile.h[half][vkey][8u * ((2u * i + vpiece) ^ VT::swizzle(vkey)) + 4u * (l16 & 1u)];  // (keys 16 apart swizzle alike)
-        const h4 a0 = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p));
-        const h4 a1 = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + 16 * TD)));
-        return h8{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
-    };
-    const auto write_v = [&](const Unit& x, int part) {
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int i = 0; i < SP; i++) {
-                const int s = part * SP + i;
-                const _Float16 vd = __builtin_bit_cast(_Float16, x.vd[u][s / kLoad]), poison = vd * (_Float16)0.0f;
-                h8 hi, lo;
-                dequantize(x.v[u][s / kLoad].w[s % kLoad], poison == poison ? vd : (_Float16)0.0f, hi, lo);
-                const uint32_t row = 16u * u + l16, at = 8u * ((g * SP + i) ^ VT::swizzle(row));
-                *reinterpret_cast<h8*>(&v_tile.h[0][row][at]) = hi, *reinterpret_cast<h8*>(&v_tile.h[1][row][at]) = lo;
-            }
-    };
+    // bytes of two rows' words that make one: their lower halves or their upper ones, or one byte of each
+    const uint32_t pick = kSharers == 1 ? 0x05040100u : kSharers == 2 ? (sharer ? 0x07060302u : 0x05040100u) : 0x0c040c00u + 0x00010001u * (2u * (sharer & 1u) + (sharer >> 1));
+    const uint32_t pick_scale = octet < 4u ? 0x05040100u : 0x07060302u;
     v4f o[CS];
 #pragma unroll
     for (int i = 0; i < CS; i++) o[i] = v4f{0.f, 0.f, 0.f, 0.f};
     float m_run = -__builtin_inff(), l_run = 0.0f;
-    const auto attend = [&](uint32_t unit, const Unit& now, Unit& then) {
+    const auto attend = [&](uint32_t unit, Unit& now, Unit& then) {
         fetch(unit + 1u, then);  // (of the last one: for nobody)
         const uint32_t key0 = unit * kFewKeys;
+        // Values that are not finite are taken as zeros and their keys as NaN (see attention_q4_kernel): seldom, and then by looking at their scales again.
+        h2 vd[4][kMine], nan = {(_Float16)0.0f, (_Float16)0.0f};
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int i = 0; i < kMine; i++) {
+                uint32_t d;
+                if constexpr (HD == 64) d = __builtin_amdgcn_perm(now.vd[2 * j + 1], now.vd[2 * j], pick_scale);
+                else d = now.vd[(2 * j + 1) * kMine + i] << 16 | now.vd[2 * j * kMine + i];
+                vd[j][i] = __builtin_bit_cast(h2, d);
+                nan = __builtin_elementwise_fma(vd[j][i], h2{(_Float16)0.0f, (_Float16)0.0f}, nan);
+            }
+        if (__builtin_amdgcn_ballot_w64(nan[0] != nan[0] || nan[1] != nan[1]) != 0) {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int i = 0; i < kMine; i++) {
+                    const _Float16 d0 = vd[j][i][0], d1 = vd[j][i][1], zero = (_Float16)0.0f;
+                    vd[j][i] = h2{d0 * zero == zero ? d0 : zero, d1 * zero == zero ? d1 : zero};
+                }
+#pragma unroll
+            for (uint32_t u = 0; u < 2; u++)
+#pragma unroll
+                for (uint32_t i = 0; i < kLoads; i++) {
+                    const uint16_t d = __builtin_amdgcn_raw_buffer_load_b16(vs, (key0 + 16u * u + l16) * (HD / 16) + (g * SLABS + i * kLoad) / 4u * 2u, 0, 0);
+                    if (__builtin_bit_cast(_Float16, d) * (_Float16)0.0f != (_Float16)0.0f) now.kd[u][i] = 0x7e00u;
+                }
+        }
         v4f sc[2];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             sc[u] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int s = 0; s < SLABS; s++) {
-                const _Float16 poison = __builtin_bit_cast(_Float16, now.vd[u][s / kLoad]) * (_Float16)0.0f;  // (see attention_q4_kernel)
                 h8 hi, lo;
-                dequantize(now.k[u][s / kLoad].w[s % kLoad], __builtin_bit_cast(_Float16, now.kd[u][s / kLoad]) + poison, hi, lo);
+                dequantize(now.k[u][s / kLoad].w[s % kLoad], __builtin_bit_cast(_Float16, (uint16_t)now.kd[u][s / kLoad]), hi, lo);
                 sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, qh[s], sc[u], 0, 0, 0);
                 sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, ql[s], sc[u], 0, 0, 0);
                 sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, qh[s], sc[u], 0, 0, 0);
             }
         }
-        write_v(now, 0);
         if (args.scores && r0 + l16 < rows) {
 #pragma unroll
             for (int u = 0; u < 2; u++)
@@ -658,17 +679,25 @@ __global__ __launch_bounds__(64 * kFewWaves, HD <= 64 ? 4 : HD == 128 ? 3 : 1) v
             split_halves(w, hi[u], lo[u]);
         }
         const h8 ph = __builtin_shufflevector(hi[0], hi[1], 0, 1, 2, 3, 4, 5, 6, 7), pl = __builtin_shufflevector(lo[0], lo[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        uint32_t pairs[4][kMine][kSharers == 1 ? 2 : 1];
 #pragma unroll
-        for (int part = 0; part < PARTS; part++) {
-            if (part > 0) write_v(now, part);
+        for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int i = 0; i < TD / 16; i++) {
-                const h8 vh = read_v(0, i), vl = read_v(1, i);
-                const int d = PARTS * i + part;
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph, o[d], 0, 0, 0);
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl, o[d], 0, 0, 0);
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph, o[d], 0, 0, 0);
+            for (int i = 0; i < kMine; i++) {
+                pairs[j][i][0] = __builtin_amdgcn_perm(now.v[2 * j + 1][i], now.v[2 * j][i], pick);
+                if constexpr (kSharers == 1) pairs[j][i][1] = __builtin_amdgcn_perm(now.v[2 * j + 1][i], now.v[2 * j][i], 0x07060302u);
             }
+#pragma unroll
+        for (int d = 0; d < CS; d++) {
+            h8 vh, vl;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if constexpr (kSharers == 1) dequantize_pair(pairs[j][d / 8][d & 1], vd[j][d / 8], d / 2 % 4, j, vh, vl);
+                else dequantize_pair(pairs[j][0][0], vd[j][0], d, j, vh, vl);
+            }
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph, o[d], 0, 0, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl, o[d], 0, 0, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph, o[d], 0, 0, 0);
         }
     };
     for (uint32_t unit = u_first; unit < u_end; unit += 2u) {
@@ -677,10 +706,9 @@ __global__ __launch_bounds__(64 * kFewWaves, HD <= 64 ? 4 : HD == 128 ? 3 : 1) v
         attend(unit + 1u, units_ahead[1], units_ahead[0]);
     }
     l_run = groups_sum(l_run);
-    // The waves' states side by side (where the values were), then every wave merges its share of the values.
-    constexpr int kShare = HD / 4 < (int)kWaves ? 1 : HD / 4 / (int)kWaves;
-    __syncthreads();
-    float* const states = reinterpret_cast<float*>(smem) + lane;
+    // The waves' states side by side, then every wave merges its share of the values: those of MFMA row 4 g + wave.
+    static_assert(kWaves == 4, "an element of a lane's vectors each");
+    float* const states = smem + lane;
     {
         float* const to = states + wave * (kStates * 64u);
         to[0] = m_run, to[64] = l_run;
@@ -690,20 +718,20 @@ __global__ __launch_bounds__(64 * kFewWaves, HD <= 64 ? 4 : HD == 128 ? 3 : 1) v
             for (int e = 0; e < 4; e++) to[(2 + 4 * i + e) * 64] = o[i][e];
     }
     __syncthreads();
-    if (wave * kShare >= HD / 4 || r0 + l16 >= rows) return;
-    float m = -__builtin_inff(), l = 0.0f, sums[kShare];
+    if (r0 + l16 >= rows) return;
+    float m = -__builtin_inff(), l = 0.0f, sums[CS];
 #pragma unroll
     for (uint32_t k = 0; k < kWaves; k++) m = fmaxf(m, states[k * (kStates * 64u)]);
     const float m_sub = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
-    for (int i = 0; i < kShare; i++) sums[i] = 0.0f;
+    for (int i = 0; i < CS; i++) sums[i] = 0.0f;
 #pragma unroll
     for (uint32_t k = 0; k < kWaves; k++) {
         const float* const from = states + k * (kStates * 64u);
         const float f = __builtin_amdgcn_exp2f(from[0] - m_sub);
         l = __builtin_fmaf(from[64], f, l);
 #pragma unroll
-        for (int i = 0; i < kShare; i++) sums[i] = __builtin_fmaf(from[(2 + kShare * wave + i) * 64u], f, sums[i]);
+        for (int i = 0; i < CS; i++) sums[i] = __builtin_fmaf(from[(2 + 4 * i + wave) * 64u], f, sums[i]);
     }
     float* to;
     float inverse = 1.0f;
@@ -719,11 +747,9 @@ __global__ __launch_bounds__(64 * kFewWaves, HD <= 64 ? 4 : HD == 128 ? 3 : 1) v
         if (g == 0 && wave == 0) to[0] = m, to[1] = l;
         to += 4;
     }
+    const uint32_t m_row = 4u * g + wave, first_dim = 8u * (m_row % kOctets) + (kSharers == 1 ? 0u : m_row / kOctets % 2u + 4u * (m_row / kOctets / 2u));
 #pragma unroll
-    for (int i = 0; i < kShare; i++) {  // value j of a lane is dim 16 (j / 4) + 4 g + j % 4 of row l16
-        const uint32_t j = kShare * wave + i;
-        to[16u * (j >> 2) + 4u * g + (j & 3u)] = sums[i] * inverse;
-    }
+    for (int i = 0; i < CS; i++) to[first_dim + (kSharers == 1 ? 8 * kOctets * (i / 8) + i % 8 : 2 * i)] = sums[i] * inverse;
 }
 
 // One token's splits merged and, in workgroups of their own, its weights added to what the rows have gathered: from the scores that the launch before left, with
