@@ -66,6 +66,17 @@ __device__ __forceinline__ void dequantize(uint32_t w, _Float16 scale, h8& hi, h
     for (int i = 0; i < 4; i++) dequantize_pair(w, h2{scale, scale}, i, i, hi, lo);
 }
 
+// The same without a scale: nibble - 8, in one plane, from pairs whose offset's bits the caller has.
+__device__ __forceinline__ h8 nibbles(uint32_t w, uint32_t first_bits, uint32_t second_bits) {
+    uint32_t first = 0x000f000fu, second = 0x00f000f0u;
+    asm("" : "+s"(first), "+s"(second));
+    const h2 a = {(_Float16)1032.0f, (_Float16)1032.0f}, b = {(_Float16)72.0f, (_Float16)72.0f};
+    const uint32_t high = w >> 8;
+    const h2 n[4] = {__builtin_bit_cast(h2, (w & first) | first_bits) - a, __builtin_bit_cast(h2, (w & second) | second_bits) - b,
+                     __builtin_bit_cast(h2, (high & first) | first_bits) - a, __builtin_bit_cast(h2, (high & second) | second_bits) - b};
+    return h8{n[0][0], n[0][1], n[1][0], n[1][1], n[2][0], n[2][1], n[3][0], n[3][1]};
+}
+
 // Four f32 values as two planes: a pair at a time, then one instruction a value (y * 1 - hi, rounded to a half; the compiler does not see the 1 and cannot
 // make two instructions of it).
 __device__ __forceinline__ void split_halves(const v4f& y, h4& hi, h4& lo) {
@@ -492,15 +503,15 @@ struct FewArgs {
 };
 constexpr uint32_t kFewRows = 16, kFewKeys = 32, kFewWaves = 4;
 template <int HD>
-constexpr uint32_t kFewSlots = kCus * (HD <= 64 ? 2 : HD == 128 ? 3 : 1);  // workgroups that the GPU has at once
+constexpr uint32_t kFewSlots = kCus * (HD <= 128 ? 2 : 1);  // workgroups that the GPU has at once
 
 template <int HD>
-__global__ __launch_bounds__(64 * kFewWaves, HD <= 64 ? 4 : HD == 128 ? 3 : 1) void attention_q4_few_kernel(FewArgs args) {
+__global__ __launch_bounds__(64 * kFewWaves, HD == 32 ? 4 : HD <= 128 ? 2 : 1) void attention_q4_few_kernel(FewArgs args) {
     const Q4AttentionArgs& a = args.at;
     constexpr uint32_t kWaves = kFewWaves;
     constexpr int SLABS = HD / 32, CS = HD / 16, kStates = 2 + HD / 4, kLoad = SLABS < 4 ? SLABS : 4, kLoads = SLABS / kLoad;  // words a load, loads a row
     // a value row's words: lane l16 has word l16 % kOctets (and the one kOctets behind it), or as many dims of it as lanes do not share it
-    constexpr int kOctets = HD < 128 ? HD / 8 : 16, kSharers = 16 / kOctets, kMine = HD / 8 / kOctets, kVd = 8 * kMine;
+    constexpr int kOctets = HD < 128 ? HD / 8 : 16, kSharers = 16 / kOctets, kMine = HD / 8 / kOctets, kVd = 8 * kMine, kKd = HD == 32 ? 4 : HD / 16;
     __shared__ float smem[kStates * 64 * kWaves];
     const uint32_t group = a.n_heads / a.n_kv_heads, rows = a.n * group;
     const uint32_t c = blockIdx.x % a.n_kv_heads, split = blockIdx.x / a.n_kv_heads % a.splits, r0 = ((rows + kFewRows - 1u) / kFewRows - 1u - blockIdx.x / a.n_kv_heads / a.splits) * kFewRows;
@@ -524,7 +535,7 @@ __global__ __launch_bounds__(64 * kFewWaves, HD <= 64 ? 4 : HD == 128 ? 3 : 1) v
             uint32_t w[kLoad];
         };
         Words k[2][kLoads];  // of keys l16 and 16 + l16
-        uint32_t kd[2][kLoads];
+        uint32_t kd[2][kKd];   // scales of all blocks of keys 4 g .. and 16 + 4 g .., one row behind the other
         uint32_t v[8][kMine];  // of values 4 g .. and 16 + 4 g ..
         uint32_t vd[kVd];      // and their scales: of the word's block (heads of 64 values: of both blocks)
     };
@@ -539,7 +550,19 @@ __global__ __launch_bounds__(64 * kFewWaves, HD <= 64 ? 4 : HD == 128 ? 3 : 1) v
 #pragma unroll
             for (uint32_t i = 0; i < kLoads; i++) {
                 const uint32_t row = unit * kFewKeys + 16u * u + l16, word = g * SLABS + i * kLoad;
-                x.k[u][i] = load(kq, row * (HD / 2) + 4u * word), x.kd[u][i] = __builtin_amdgcn_raw_buffer_load_b16(ks, row * (HD / 16) + word / 4u * 2u, 0, 0);
+                x.k[u][i] = load(kq, row * (HD / 2) + 4u * word);
+            }
+#pragma unroll
+        for (uint32_t u = 0; u < 2; u++)
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+                const uint32_t at = (unit * kFewKeys + 16u * u + 4u * g) * (HD / 16);
+                if constexpr (HD == 32) x.kd[u][i] = __builtin_amdgcn_raw_buffer_load_b16(ks, at + 2u * i, 0, 0);
+                else if (i < kKd / 4) {
+                    const auto d = __builtin_amdgcn_raw_buffer_load_b128(ks, at + 16u * i, 0, 0);
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; j++) x.kd[u][4 * i + j] = d[j];
+                }
             }
 #pragma unroll
         for (uint32_t j = 0; j < 8; j++)
@@ -558,19 +581,35 @@ __global__ __launch_bounds__(64 * kFewWaves, HD <= 64 ? 4 : HD == 128 ? 3 : 1) v
             }
         }
     };
+    // A lane's words of a key row to one of each block: blocks(w)[s] is word word_of(s) of the row, whatever lane had it.
+    const auto word_of = [&](uint32_t s) { return HD == 32 ? g : HD == 64 ? 4u * s + 2u * (g & 1u) + (g >> 1) : HD == 128 ? 4u * s + g : 4u * (2u * (s & 3u) + (s >> 2)) + g; };
+    const auto blocks = [&](const typename Unit::Words (&x)[kLoads], uint32_t (&w)[SLABS]) {
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) {
+#pragma unroll
+            for (int j = 0; j < kLoad; j++) w[i * kLoad + j] = x[i].w[j];
+            const auto exchange = [&](int j, int k, bool halves) {
+                uint32_t &p = w[i * kLoad + j], &q = w[i * kLoad + k];
+                const auto r = halves ? __builtin_amdgcn_permlane32_swap(p, q, false, false) : __builtin_amdgcn_permlane16_swap(p, q, false, false);
+                p = r[0], q = r[1];
+            };
+            if constexpr (kLoad == 2) exchange(0, 1, true);
+            if constexpr (kLoad == 4) exchange(0, 2, true), exchange(1, 3, true), exchange(0, 1, false), exchange(2, 3, false);
+        }
+    };
     Unit units_ahead[2];
     fetch(u_first, units_ahead[0]);
 
-    // the query rows: dims 8 (g SLABS + s) .. of row l16 in slab s, times 2^-e
+    // the query rows: dims 8 word_of(s) .. of row l16 in slab s, times 2^-e
     h8 qh[SLABS], ql[SLABS];
     float factor;
     {
-        const float* const p = a.q + (size_t)token * a.q_stride + (size_t)head * HD + 8u * SLABS * g;
+        const float* const p = a.q + (size_t)token * a.q_stride + (size_t)head * HD;
         v4f x[2 * SLABS];
         float top = 0.0f;
 #pragma unroll
         for (int i = 0; i < 2 * SLABS; i++) {
-            x[i] = *reinterpret_cast<const v4f*>(p + 4 * i);
+            x[i] = *reinterpret_cast<const v4f*>(p + 8u * word_of(i / 2) + 4 * (i % 2));
 #pragma unroll
             for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(x[i][e]));
         }
@@ -601,6 +640,7 @@ __global__ __launch_bounds__(64 * kFewWaves, HD <= 64 ? 4 : HD == 128 ? 3 : 1) v
         const uint32_t key0 = unit * kFewKeys;
         // Values that are not finite are taken as zeros and their keys as NaN (see attention_q4_kernel): seldom, and then by looking at their scales again.
         h2 vd[4][kMine], nan = {(_Float16)0.0f, (_Float16)0.0f};
+        uint32_t first_bits[2] = {0x64006400u, 0x64006400u}, second_bits[2] = {0x54005400u, 0x54005400u};  // of the keys' nibbles; a NaN's
 #pragma unroll
         for (int j = 0; j < 4; j++)
 #pragma unroll
@@ -622,22 +662,28 @@ __global__ __launch_bounds__(64 * kFewWaves, HD <= 64 ? 4 : HD == 128 ? 3 : 1) v
 #pragma unroll
             for (uint32_t u = 0; u < 2; u++)
 #pragma unroll
-                for (uint32_t i = 0; i < kLoads; i++) {
-                    const uint16_t d = __builtin_amdgcn_raw_buffer_load_b16(vs, (key0 + 16u * u + l16) * (HD / 16) + (g * SLABS + i * kLoad) / 4u * 2u, 0, 0);
-                    if (__builtin_bit_cast(_Float16, d) * (_Float16)0.0f != (_Float16)0.0f) now.kd[u][i] = 0x7e00u;
+                for (uint32_t i = 0; i < HD / 32; i++) {
+                    const uint16_t d = __builtin_amdgcn_raw_buffer_load_b16(vs, (key0 + 16u * u + l16) * (HD / 16) + 2u * i, 0, 0);
+                    if (__builtin_bit_cast(_Float16, d) * (_Float16)0.0f != (_Float16)0.0f) first_bits[u] = second_bits[u] = 0x7e007e00u;
                 }
         }
         v4f sc[2];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            sc[u] = v4f{0.f, 0.f, 0.f, 0.f};
+            uint32_t w[SLABS];
+            blocks(now.k[u], w);
 #pragma unroll
             for (int s = 0; s < SLABS; s++) {
-                h8 hi, lo;
-                dequantize(now.k[u][s / kLoad].w[s % kLoad], __builtin_bit_cast(_Float16, (uint16_t)now.kd[u][s / kLoad]), hi, lo);
-                sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, qh[s], sc[u], 0, 0, 0);
-                sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, ql[s], sc[u], 0, 0, 0);
-                sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, qh[s], sc[u], 0, 0, 0);
+                const h8 k = nibbles(w[s], first_bits[u], second_bits[u]);
+                v4f acc = {0.f, 0.f, 0.f, 0.f};
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[s], acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[s], acc, 0, 0, 0);
+                const int block = HD == 256 ? 2 * (s & 3) + (s >> 2) : s;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float d = (float)__builtin_bit_cast(h2, now.kd[u][HD == 32 ? e : e * (HD / 64) + block / 2])[block & 1];
+                    sc[u][e] = s == 0 ? acc[e] * d : __builtin_fmaf(acc[e], d, sc[u][e]);
+                }
             }
         }
         if (args.scores && r0 + l16 < rows) {
