@@ -66,17 +66,6 @@ __device__ __forceinline__ void dequantize(uint32_t w, _Float16 scale, h8& hi, h
     for (int i = 0; i < 4; i++) dequantize_pair(w, h2{scale, scale}, i, i, hi, lo);
 }
 
-// The same without a scale: nibble - 8, in one plane, from pairs whose offset's bits the caller has.
-__device__ __forceinline__ h8 nibbles(uint32_t w, uint32_t first_bits, uint32_t second_bits) {
-    uint32_t first = 0x000f000fu, second = 0x00f000f0u;
-    asm("" : "+s"(first), "+s"(second));
-    const h2 a = {(_Float16)1032.0f, (_Float16)1032.0f}, b = {(_Float16)72.0f, (_Float16)72.0f};
-    const uint32_t high = w >> 8;
-    const h2 n[4] = {__builtin_bit_cast(h2, (w & first) | first_bits) - a, __builtin_bit_cast(h2, (w & second) | second_bits) - b,
-                     __builtin_bit_cast(h2, (high & first) | first_bits) - a, __builtin_bit_cast(h2, (high & second) | second_bits) - b};
-    return h8{n[0][0], n[0][1], n[1][0], n[1][1], n[2][0], n[2][1], n[3][0], n[3][1]};
-}
-
 // Four f32 values as two planes: a pair at a time, then one instruction a value (y * 1 - hi, rounded to a half; the compiler does not see the 1 and cannot
 // make two instructions of it).
 __device__ __forceinline__ void split_halves(const v4f& y, h4& hi, h4& lo) {
@@ -667,24 +656,43 @@ __global__ __launch_bounds__(64 * kFewWaves, HD == 32 ? 4 : HD <= 128 ? 2 : 1) v
                     if (__builtin_bit_cast(_Float16, d) * (_Float16)0.0f != (_Float16)0.0f) first_bits[u] = second_bits[u] = 0x7e007e00u;
                 }
         }
-        v4f sc[2];
+        // A block's products of 16 keys: the nibbles unpacked one step ahead, between the matrix instructions (in this very order, in which no instruction waits for
+        // the one before it), and scaled two steps behind.
+        v4f sc[2], acc[3];
+        uint32_t w[2][SLABS], n_bits[4];
+        h8 k[2];
+        blocks(now.k[0], w[0]), blocks(now.k[1], w[1]);
+        const auto unpack = [&](int n) {
+            uint32_t first = 0x000f000fu, second = 0x00f000f0u;
+            asm("" : "+s"(first), "+s"(second));
+            const uint32_t x = w[n % 2][n / 2], high = x >> 8, f = first_bits[n % 2], s = second_bits[n % 2];
+            n_bits[0] = (x & first) | f, n_bits[1] = (x & second) | s, n_bits[2] = (high & first) | f, n_bits[3] = (high & second) | s;
+        };
+        const auto center = [&](int n) {
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            uint32_t w[SLABS];
-            blocks(now.k[u], w);
-#pragma unroll
-            for (int s = 0; s < SLABS; s++) {
-                const h8 k = nibbles(w[s], first_bits[u], second_bits[u]);
-                v4f acc = {0.f, 0.f, 0.f, 0.f};
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[s], acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[s], acc, 0, 0, 0);
-                const int block = HD == 256 ? 2 * (s & 3) + (s >> 2) : s;
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float d = (float)__builtin_bit_cast(h2, now.kd[u][HD == 32 ? e : e * (HD / 64) + block / 2])[block & 1];
-                    sc[u][e] = s == 0 ? acc[e] * d : __builtin_fmaf(acc[e], d, sc[u][e]);
-                }
+            for (int i = 0; i < 4; i++) {
+                const h2 x = __builtin_bit_cast(h2, n_bits[i]) - (i & 1 ? h2{(_Float16)72.0f, (_Float16)72.0f} : h2{(_Float16)1032.0f, (_Float16)1032.0f});
+                k[n % 2][2 * i] = x[0], k[n % 2][2 * i + 1] = x[1];
             }
+        };
+        const auto scale = [&](int n) {
+            const int u = n % 2, s = n / 2, block = HD == 256 ? 2 * (s & 3) + (s >> 2) : s;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float d = (float)__builtin_bit_cast(h2, now.kd[u][HD == 32 ? e : e * (HD / 64) + block / 2])[block & 1];
+                sc[u][e] = s == 0 ? acc[n % 3][e] * d : __builtin_fmaf(acc[n % 3][e], d, sc[u][e]);
+            }
+        };
+        unpack(0), center(0);
+#pragma unroll
+        for (int n = 0; n < 2 * SLABS + 2; n++) {
+            if (n < 2 * SLABS) acc[n % 3] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[n % 2], ql[n / 2], v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+            if (n + 1 < 2 * SLABS) unpack(n + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            if (n >= 1 && n <= 2 * SLABS) acc[(n - 1) % 3] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[(n - 1) % 2], qh[(n - 1) / 2], acc[(n - 1) % 3], 0, 0, 0);
+            if (n + 1 < 2 * SLABS) center(n + 1);
+            if (n >= 2) scale(n - 2);
+            __builtin_amdgcn_sched_barrier(0);
         }
         if (args.scores && r0 + l16 < rows) {
 #pragma unroll
@@ -733,17 +741,39 @@ __global__ __launch_bounds__(64 * kFewWaves, HD == 32 ? 4 : HD <= 128 ? 2 : 1) v
                 pairs[j][i][0] = __builtin_amdgcn_perm(now.v[2 * j + 1][i], now.v[2 * j][i], pick);
                 if constexpr (kSharers == 1) pairs[j][i][1] = __builtin_amdgcn_perm(now.v[2 * j + 1][i], now.v[2 * j][i], 0x07060302u);
             }
-#pragma unroll
-        for (int d = 0; d < CS; d++) {
-            h8 vh, vl;
+        // (and the values, likewise)
+        h2 x[4];
+        h8 vh[2], vl[2];
+        const auto unpack_values = [&](int d, int step) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                if constexpr (kSharers == 1) dequantize_pair(pairs[j][d / 8][d & 1], vd[j][d / 8], d / 2 % 4, j, vh, vl);
-                else dequantize_pair(pairs[j][0][0], vd[j][0], d, j, vh, vl);
+                const int i = kSharers == 1 ? d / 2 % 4 : d, oct = kSharers == 1 ? d / 8 : 0;
+                uint32_t mask = i & 1 ? 0x00f000f0u : 0x000f000fu, bits = i & 1 ? 0x54005400u : 0x64006400u;
+                asm("" : "+s"(mask), "+v"(bits));
+                const uint32_t p = pairs[j][oct][kSharers == 1 ? d & 1 : 0];
+                if (step == 0) x[j] = __builtin_bit_cast(h2, ((i < 2 ? p : p >> 8) & mask) | bits);
+                if (step == 1) x[j] -= i & 1 ? h2{(_Float16)72.0f, (_Float16)72.0f} : h2{(_Float16)1032.0f, (_Float16)1032.0f};
+                if (step == 2) {
+                    const h2 h = x[j] * vd[j][oct];
+                    vh[d % 2][2 * j] = h[0], vh[d % 2][2 * j + 1] = h[1];
+                }
+                if (step == 3) {
+                    const h2 l = __builtin_elementwise_fma(x[j], vd[j][oct], h2{-vh[d % 2][2 * j], -vh[d % 2][2 * j + 1]});
+                    vl[d % 2][2 * j] = l[0], vl[d % 2][2 * j + 1] = l[1];
+                }
             }
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph, o[d], 0, 0, 0);
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl, o[d], 0, 0, 0);
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph, o[d], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+#pragma unroll
+        for (int step = 0; step < 4; step++) unpack_values(0, step);
+#pragma unroll
+        for (int d = 0; d < CS; d++) {
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl[d % 2], ph, o[d], 0, 0, 0);
+            if (d + 1 < CS) unpack_values(d + 1, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[d % 2], pl, o[d], 0, 0, 0);
+            if (d + 1 < CS) unpack_values(d + 1, 1), unpack_values(d + 1, 2);
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[d % 2], ph, o[d], 0, 0, 0);
+            if (d + 1 < CS) unpack_values(d + 1, 3);
         }
     };
     for (uint32_t unit = u_first; unit < u_end; unit += 2u) {
