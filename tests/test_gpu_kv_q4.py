@@ -167,9 +167,10 @@ PROMPTS = [  # head_dim, heads, KV heads, first row, tokens, rows behind them, f
 ]
 
 
-LARGE = [  # more than 64 rows of a KV head and 2^29 products: the tiled kernels, split over few and many workgroups, one and two workgroups a CU
+LARGE = [  # more than 64 rows of a KV head, and up to and beyond 12 million pairs of a query and a key: the tiled kernels, split over few and many workgroups, one and two a CU
     (64, 16, 4, 1777, 333, 0, 0), (64, 32, 8, 0, 1030, 3, 0), (64, 2, 1, 66000, 65, 0, 0), (64, 12, 4, 900, 701, 5, 4), (128, 6, 2, 2222, 301, 0, 8),
     (128, 16, 4, 7, 2050, 0, 0), (256, 3, 1, 1300, 500, 40, 0), (32, 8, 8, 1000, 1500, 0, 0), (32, 24, 2, 20001, 67, 0, 0),
+    (64, 16, 4, 1777, 430, 2, 0), (64, 2, 1, 100000, 65, 0, 0), (64, 12, 4, 1300, 701, 5, 4), (128, 6, 2, 3333, 601, 0, 8), (256, 3, 1, 4400, 901, 0, 0),
 ]
 
 
@@ -198,7 +199,8 @@ def test_attention_of_a_prompt(ctx, ops, dev, hd, heads, n_kv, pos0, n, behind, 
 
 
 @pytest.mark.parametrize("hd,heads,n_kv,pos0,n", [(64, 4, 2, 0, 100), (128, 2, 1, 70, 30), (64, 4, 2, 300, 1), (32, 2, 2, 5, 60), (256, 2, 2, 5, 60),
-                                                  (64, 8, 2, 1500, 600), (128, 8, 4, 700, 600), (32, 16, 2, 300, 1200), (256, 4, 2, 500, 700)])
+                                                  (64, 8, 2, 1500, 600), (128, 8, 4, 700, 600), (32, 16, 2, 300, 1200), (256, 4, 2, 500, 700),
+                                                  (64, 16, 2, 1500, 600), (128, 16, 4, 1000, 700), (256, 8, 2, 1700, 800)])
 def test_a_row_held_as_nan_is_seen_by_those_that_see_it(ctx, ops, dev, hd, heads, n_kv, pos0, n):
     """Of keys in head 0, of values in the last head: NaN to the tokens from that row on, everything as without it to those before."""
     max_seq, bad = pos0 + n, pos0 + n // 2
@@ -220,7 +222,7 @@ def test_a_row_held_as_nan_is_seen_by_those_that_see_it(ctx, ops, dev, hd, heads
         assert_f32_parity(out[~hit], clean[~hit], "tokens that do not see it")
 
 
-@pytest.mark.parametrize("heads,n_kv,seq,n", [(4, 2, 300, 20), (16, 4, 1200, 700)])
+@pytest.mark.parametrize("heads,n_kv,seq,n", [(4, 2, 300, 20), (16, 4, 1200, 700), (16, 4, 1600, 900)])
 @pytest.mark.parametrize("factor", [1e-30, 1e-6, 1e4, 3e4])
 def test_queries_of_all_sizes(ctx, ops, dev, factor, heads, n_kv, seq, n):
     """Tiny queries weigh all rows alike, huge ones one row alone; both with keys that answer in kind."""
@@ -235,7 +237,7 @@ def test_queries_of_all_sizes(ctx, ops, dev, factor, heads, n_kv, seq, n):
     assert_f32_parity(d_out.download(np.float32, heads * hd).reshape(heads, hd), R.attention(q[n - 1:], k, v, seq - 1)[0][0], "one token")
 
 
-@pytest.mark.parametrize("hd,heads,n_kv,n", [(64, 4, 2, 50), (128, 8, 2, 1100)])
+@pytest.mark.parametrize("hd,heads,n_kv,n", [(64, 4, 2, 50), (128, 8, 2, 1100), (128, 16, 2, 1400)])
 def test_a_value_that_is_not_finite_stays_with_its_query(ctx, ops, dev, hd, heads, n_kv, n):
     k, v = filled(1, n, n_kv, hd, n)
     q = normal(3, n, heads, hd)
@@ -365,7 +367,7 @@ def test_a_captured_step_replayed_while_the_position_moves(ctx, ops, dev):
     ctx.graph_destroy(g)
 
 
-@pytest.mark.parametrize("n,pos0", [(300, 500), (700, 500)])
+@pytest.mark.parametrize("n,pos0", [(300, 500), (700, 500), (900, 700)])
 def test_results_do_not_change_from_run_to_run(ctx, ops, dev, n, pos0):
     hd, heads, n_kv = 64, 16, 4
     k, v = filled(3, pos0 + n, n_kv, hd, pos0 + n)

@@ -966,25 +966,25 @@ hipError_t launch_few(FewArgs f, uint64_t seen, const Launch& L) {
 }
 
 // Which kernel: the one for few rows wastes nothing on them and fills the GPU with little work, the tiled one reads and unpacks the cache for up to eight
-// times as many rows at once.  Up to 64 rows of a KV head the first is as fast or faster at any length (heads of 64 values, 32 query heads, 8 KV heads, in us:
-// 32 rows behind 100000 47 against 81, 64 behind 60000 55 and 55, 96 behind 60000 82 and 57), and with more rows up to some 2^29 of (query row, key,
-// value) products: 555 tokens of 16 heads 9.9 against 17.1, 64 tokens behind 4000 22.7 and 22.8, 1000 tokens of 32 heads 30.2 and 29.1, 2002 of them
-// 95 and 65; heads of 32 values, 1400 tokens of 16 heads 18.9 and 19.9, 2000 32.8 and 27.5; of 128, 64 tokens of 16 heads behind 4000 25.4 and 27.5, 300
-// behind 1000 33.5 and 31.4; of 256, 500 tokens of 8 heads behind 500 35 and 43, 1000 behind 1000 103 and 82.
+// times as many rows at once.  Up to 64 rows of a KV head the first is as fast or faster at any length (us: 32 query heads of 64 values over 8 KV heads,
+// 32 rows behind 100000 41 against 78, 64 behind 60000 47 and 54, 96 behind 60000 69 and 56; of 32 values over 4, 64 behind 60000 24 and 21), with more
+// rows up to some 12 million pairs of a query and a key: of 64 values, 555 tokens of 16 heads 9.7 and 17.0, 1500 of 6 16.8 and 24.0, 1000 of 32 30.1 and
+// 28.8, 2002 of 32 89 and 63; of 32 values, 1400 of 16 20.0 and 19.6; of 128, 1000 of 8 18.4 and 30.0, 1000 of 32 50.1 and 47.8; of 256, 500 of
+// 8 behind 500 30 and 42, 1000 of 8 behind 1000 84 and 81.
 template <int HD>
 hipError_t launch_head_dim(const Q4AttentionArgs& a, float* d_scores, const Launch& L) {
     const uint32_t rows = a.n * (a.n_heads / a.n_kv_heads);
-    const uint64_t seen = a.d_pos ? a.max_seq : (uint64_t)a.pos0 + a.n, products = (uint64_t)a.n * a.n_heads * (seen - a.n / 2u) * HD;
+    const uint64_t seen = a.d_pos ? a.max_seq : (uint64_t)a.pos0 + a.n, pairs = (uint64_t)a.n * a.n_heads * (seen - a.n / 2u);
     hipError_t e;
-    if (rows <= 64u || products <= 1ull << 29) {
+    if (rows <= 64u || pairs <= 12u << 20) {
         float* const scores = a.n == 1u && a.weights ? d_scores : nullptr;
         e = launch_few<HD>(FewArgs{a, scores}, seen, L);
         if (scores) return e;
     } else if constexpr (HD == 32) {
         e = launch_tiles<HD, 2, 2, 2>(a, seen, L);
     } else if constexpr (HD <= 128) {
-        // Where every CU has a block of rows of its own, two workgroups of half the keys a CU (2048 tokens behind 6144 of 16 heads of 128 values 344 us
-        // against 365, 4000 tokens of 32 heads of 64 values 225 against 237), else one (500 behind 2000 of those 43 against 45).
+        // Where every CU has a block of rows of its own, two workgroups of half the keys a CU (2048 tokens behind 6144 of 16 heads of 128 values 332 us
+        // against 345, 4000 tokens of 32 heads of 64 values 210 against 230), else one (500 behind 2000 of those 43 against 44).
         const bool many = a.n_kv_heads * ((rows + 127u) / 128u) >= kCus;
         e = many ? launch_tiles<HD, 4, 1, 2>(a, seen, L) : launch_tiles<HD, 4, 2, 1>(a, seen, L);
     } else {
