@@ -84,10 +84,13 @@ __global__ __launch_bounds__(256) void kv_q4_read_kernel(const void* p, float* _
 }
 
 // ---- eviction -------------------------------------------------------------------------------
+constexpr uint32_t kStateLine = 32;
 struct Q4EvictArgs {
     void* cache[2];
     float* weights;
-    uint32_t* kept;  // [n_kv_heads][seq_len - n_drop]
+    uint32_t* kept;   // [n_kv_heads][seq_len - n_drop]
+    uint32_t* state;    // [2 n_kv_heads]: segments taken, and a line behind it which of `segments` are in registers
+    uint32_t segments;  // of rows that stay
     uint32_t seq_len, n_keep, n_recent, n_drop, max_seq, n_kv_heads, head_dim;
 };
 
@@ -135,6 +138,7 @@ __global__ __launch_bounds__(kEvictThreads) void kv_q4_select_kernel(Q4EvictArgs
     __shared__ uint32_t hist[kBins + 64], slots[8][kEvictWaves], votes[kVotes], found[2];
     const uint32_t c = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     const uint64_t in_front = (1ull << lane) - 1ull;
+    for (uint32_t i = tid; i < 2u * (kStateLine + a.segments); i += kEvictThreads) a.state[(size_t)c * 2u * (kStateLine + a.segments) + i] = 0u;  // (for the launch behind)
     // (a read behind the last row gives 0, for nobody)
     const auto w = __builtin_amdgcn_make_buffer_rsrc(a.weights + (size_t)c * a.max_seq, 0, (int)(4u * a.seq_len), 0x27000);
     const uint32_t from = a.n_keep, to = a.seq_len - a.n_recent;
@@ -228,71 +232,94 @@ __global__ __launch_bounds__(kEvictThreads) void kv_q4_select_kernel(Q4EvictArgs
     }
 }
 
-// Moves the kept rows of one stream of a head together in place: C neighbouring pieces (of type T) of every row, rows being `stride`
-// pieces.  A row moves down or stays, so chunks of rows are moved in ascending order: nothing that a chunk overwrites is read behind it,
-// and all of the chunk itself has arrived in registers (the barrier) before its first piece is written.  The next chunk's pieces, which
-// lie behind what this one overwrites, are on their way meanwhile, and its rows' numbers before that.  Bound by the latency of a
-// workgroup's chunks, one behind the other, so a row's quants are several streams with a workgroup each: 24576 rows of 8 heads of 64
-// values took 18.2 us, with whole rows 21.4.
-template <typename T, uint32_t C, int PER>
-__device__ __forceinline__ void move_rows(T* base, uint32_t stride, const uint32_t* kept, uint32_t first, uint32_t n) {
-    constexpr uint32_t kChunk = kEvictThreads * PER / C;  // rows
-    const uint32_t row = threadIdx.x / C, piece = threadIdx.x % C;
-    uint32_t at[2][PER];
-    T v[2][PER];
-    const auto rows = [&](uint32_t i0, uint32_t (&r)[PER]) {
-#pragma unroll
-        for (int i = 0; i < PER; i++) r[i] = kept[min(i0 + i * (kEvictThreads / C) + row, n - 1u)];
-    };
-    const auto read = [&](const uint32_t (&r)[PER], T (&x)[PER]) {
-#pragma unroll
-        for (int i = 0; i < PER; i++) x[i] = base[(size_t)r[i] * stride + piece];
-    };
-    const auto write = [&](uint32_t i0, T (&x)[PER]) {
-#pragma unroll
-        for (int i = 0; i < PER; i++) asm volatile("" : "+v"(x[i]));  // (has arrived)
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const uint32_t to = i0 + i * (kEvictThreads / C) + row;
-            if (to < n) base[(size_t)to * stride + piece] = x[i];
-        }
-    };
-    if (first >= n) return;
-    rows(first, at[0]);
-    read(at[0], v[0]);
-    rows(first + kChunk, at[1]);
-    for (uint32_t i0 = first; i0 < n; i0 += 2u * kChunk) {
-        read(at[1], v[1]);  // (past the end: the last row, for nobody)
-        rows(i0 + 2u * kChunk, at[0]);
-        write(i0, v[0]);
-        if (i0 + kChunk >= n) break;
-        read(at[0], v[0]);
-        rows(i0 + 3u * kChunk, at[1]);
-        write(i0 + kChunk, v[1]);
-    }
-}
+// Moves the kept rows together in place, a segment of rows of one head's keys (with the weights) or values per workgroup.  A row moves down or stays: what a
+// segment overwrites is read by itself and by segments in front of it.  So a workgroup reads its rows into registers, tells that it has, waits until the segments
+// in front of it that can have rows in its place (n_drop rows at most) have told so too, and writes.  Every wait ends: segments are taken by a counter, so
+// those in front of one that waits have been taken by workgroups that run already, and these tell before they wait for anybody.  (No order but that of these reads
+// before those writes is asked of the memory: nothing that this launch writes is read in it.)
+// Weights behind the last row that stays are cleared by segments that have nothing to read.
+// Bound by memory latency: taking a segment, its rows' numbers, the rows, the word of the segments in front, one behind the other; 24576 rows of 8 heads of
+// 64 values took 18 us with one workgroup for all rows of a quarter of a head's planes, one chunk of rows behind the other.
+constexpr uint32_t kMoveThreads = 256, kMoveLeast = 256;  // threads; rows of a segment at least
+template <int HD>
+constexpr uint32_t kMoveRows = HD <= 64 ? 512 : 256;  // 16 KiB of quants and more: enough workgroups, and four and more loads of a thread on their way
 
 template <int HD>
-constexpr uint32_t kMovePieces = HD <= 64 ? 1 : 2;  // of 16 bytes, of a row's quants, in a stream
-template <int HD>
-__global__ __launch_bounds__(kEvictThreads) void kv_q4_move_kernel(Q4EvictArgs a) {
+__global__ __launch_bounds__(kMoveThreads) void kv_q4_move_kernel(Q4EvictArgs a) {
     typedef uint32_t Two __attribute__((ext_vector_type(2)));
     typedef uint32_t Four __attribute__((ext_vector_type(4)));
     using Scales = typename std::conditional<HD == 32, uint16_t, typename std::conditional<HD == 64, uint32_t, typename std::conditional<HD == 128, Two, Four>::type>::type>::type;
-    constexpr uint32_t C = kMovePieces<HD>, kPieces = HD / 32, kStreams = kPieces / C;
-    const uint32_t c = blockIdx.x, n = a.seq_len - a.n_drop, first = a.n_keep;  // (rows in front of n_keep stay where they are)
-    const uint32_t* const kept = a.kept + (size_t)c * n;
+    constexpr uint32_t R = kMoveRows<HD>, kPieces = HD / 32, kPer = R * kPieces / kMoveThreads, kRows = R / kMoveThreads;
+    __shared__ uint32_t taken;
+    const uint32_t tid = threadIdx.x;
+    const uint32_t stream = blockIdx.x % (2u * a.n_kv_heads), c = stream >> 1;
+    uint32_t* const state = a.state + (size_t)stream * (kStateLine + a.segments);
+    if (tid == 0) taken = __hip_atomic_fetch_add(state, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    const uint32_t segment = taken;
+    const bool keys = (stream & 1u) == 0;
+    const uint32_t n = a.seq_len - a.n_drop, first = a.n_keep, row0 = first + segment * R;  // (rows in front of n_keep stay where they are)
+    const bool reads = row0 < n;
+    if (!reads && !keys) return;
     const size_t head = (size_t)c * a.max_seq;
-    const Q4Cache cache = q4_planes(blockIdx.y & 1u ? a.cache[1] : a.cache[0], a.max_seq, a.n_kv_heads, HD);
-    if (blockIdx.y < 2u * kStreams) {
-        move_rows<Four, C, 4>(reinterpret_cast<Four*>(cache.quants) + head * kPieces + blockIdx.y / 2u * C, kPieces, kept, first, n);
-    } else if (blockIdx.y < 2u * kStreams + 2u) {
-        move_rows<Scales, 1, 4>(reinterpret_cast<Scales*>(cache.scales) + head, 1u, kept, first, n);
-    } else {
-        move_rows<float, 1, 4>(a.weights + head, 1u, kept, first, n);
-        __syncthreads();  // (the last chunk's reads)
-        for (uint32_t t = n + threadIdx.x; t < a.seq_len; t += kEvictThreads) a.weights[head + t] = 0.0f;
+    const Q4Cache cache = q4_planes(keys ? a.cache[0] : a.cache[1], a.max_seq, a.n_kv_heads, HD);
+    const auto plane = [&](void* p, uint32_t row_bytes, uint32_t rows) { return __builtin_amdgcn_make_buffer_rsrc(p, 0, (int)(rows * row_bytes), 0x27000); };
+    uint32_t* const quants = cache.quants + head * (HD / 8);
+    uint16_t* const scales = cache.scales + head * (HD / 32);
+    Four q[kPer];
+    Scales d[kRows];
+    uint32_t w[kRows];
+    uint32_t* const told = state + kStateLine;
+    if (reads) {
+        // (numbers behind the last row read as 0: a row for nobody)
+        const auto numbers = plane(a.kept + (size_t)c * n, 4, n), from = plane(quants, HD / 2, a.seq_len), scales_from = plane(scales, HD / 16, a.seq_len),
+                   weights_from = plane(a.weights + head, 4, a.seq_len);
+        uint32_t q_row[kPer], row[kRows];
+#pragma unroll
+        for (uint32_t i = 0; i < kPer; i++) q_row[i] = __builtin_amdgcn_raw_buffer_load_b32(numbers, 4u * (row0 + (i * kMoveThreads + tid) / kPieces), 0, 0);
+#pragma unroll
+        for (uint32_t i = 0; i < kRows; i++) row[i] = __builtin_amdgcn_raw_buffer_load_b32(numbers, 4u * (row0 + i * kMoveThreads + tid), 0, 0);
+#pragma unroll
+        for (uint32_t i = 0; i < kPer; i++) q[i] = __builtin_amdgcn_raw_buffer_load_b128(from, q_row[i] * (HD / 2) + (i * kMoveThreads + tid) % kPieces * 16u, 0, 0);
+#pragma unroll
+        for (uint32_t i = 0; i < kRows; i++) {
+            if constexpr (HD == 32) d[i] = __builtin_amdgcn_raw_buffer_load_b16(scales_from, row[i] * 2u, 0, 0);
+            else if constexpr (HD == 64) d[i] = __builtin_amdgcn_raw_buffer_load_b32(scales_from, row[i] * 4u, 0, 0);
+            else if constexpr (HD == 128) d[i] = __builtin_amdgcn_raw_buffer_load_b64(scales_from, row[i] * 8u, 0, 0);
+            else d[i] = __builtin_amdgcn_raw_buffer_load_b128(scales_from, row[i] * 16u, 0, 0);
+            w[i] = keys ? __builtin_amdgcn_raw_buffer_load_b32(weights_from, row[i] * 4u, 0, 0) : 0u;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kPer; i++) asm volatile("" : "+v"(q[i]));  // (has arrived)
+#pragma unroll
+        for (uint32_t i = 0; i < kRows; i++) asm volatile("" : "+v"(d[i]), "+v"(w[i]));
+        __syncthreads();
+        if (tid == 0) __hip_atomic_store(told + segment, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    const uint32_t nearest = min(segment, a.segments), farthest = segment * R > a.n_drop ? (segment * R - a.n_drop) / R : 0u;
+    for (uint32_t i = farthest + tid; i < nearest; i += kMoveThreads)
+        while (__hip_atomic_load(told + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0u) __builtin_amdgcn_s_sleep(1);
+    __syncthreads();
+    if (reads) {
+        const auto to = plane(quants, HD / 2, n), scales_to = plane(scales, HD / 16, n);  // (writes behind the last row are dropped)
+#pragma unroll
+        for (uint32_t i = 0; i < kPer; i++) __builtin_amdgcn_raw_buffer_store_b128(q[i], to, row0 * (HD / 2) + (i * kMoveThreads + tid) * 16u, 0, 0);
+#pragma unroll
+        for (uint32_t i = 0; i < kRows; i++) {
+            const uint32_t row = row0 + i * kMoveThreads + tid;
+            if constexpr (HD == 32) __builtin_amdgcn_raw_buffer_store_b16(d[i], scales_to, row * 2u, 0, 0);
+            else if constexpr (HD == 64) __builtin_amdgcn_raw_buffer_store_b32(d[i], scales_to, row * 4u, 0, 0);
+            else if constexpr (HD == 128) __builtin_amdgcn_raw_buffer_store_b64(d[i], scales_to, row * 8u, 0, 0);
+            else __builtin_amdgcn_raw_buffer_store_b128(d[i], scales_to, row * 16u, 0, 0);
+        }
+    }
+    if (keys) {
+        const auto weights_to = plane(a.weights + head, 4, a.seq_len);
+#pragma unroll
+        for (uint32_t i = 0; i < kRows; i++) {
+            const uint32_t row = row0 + i * kMoveThreads + tid;
+            __builtin_amdgcn_raw_buffer_store_b32(row < n ? w[i] : 0u, weights_to, row * 4u, 0, 0);
+        }
     }
 }
 
@@ -316,24 +343,31 @@ hipError_t launch_kv_q4_read(const void* d_cache, float* d_out, uint32_t out_str
                          n_kv_heads, head_dim);
 }
 
-size_t kv_q4_evict_scratch_floats(uint32_t seq_len, uint32_t n_kv_heads) {
-    (void)seq_len, (void)n_kv_heads;
-    return 0;
+size_t kv_q4_evict_scratch_floats(uint32_t seq_len, uint32_t n_kv_heads) { return 2 * (size_t)n_kv_heads * (kStateLine + (seq_len + kMoveLeast - 1u) / kMoveLeast); }
+
+namespace {
+
+template <int HD>
+hipError_t launch_evict(Q4EvictArgs a, const Launch& L) {
+    constexpr uint32_t R = kMoveRows<HD>;
+    static_assert(R >= kMoveLeast, "the scratch is sized for it");
+    a.segments = (a.seq_len - a.n_drop - a.n_keep + R - 1u) / R;
+    const auto select = a.seq_len <= 4u * kEvictThreads ? kv_q4_select_kernel<4, false> : a.seq_len <= 32u * kEvictThreads ? kv_q4_select_kernel<32, false> : kv_q4_select_kernel<32, true>;
+    const hipError_t e = launch_kernel(L, kFamOther, select, dim3(a.n_kv_heads), dim3(kEvictThreads), a);
+    if (e != hipSuccess) return e;
+    return launch_kernel(L, kFamOther, kv_q4_move_kernel<HD>, dim3(2u * a.n_kv_heads * ((a.seq_len - a.n_keep + R - 1u) / R)), dim3(kMoveThreads), a);
 }
+
+}  // namespace
 
 hipError_t launch_kv_q4_evict(void* d_k_cache, void* d_v_cache, float* d_weights, uint32_t* d_kept, float* d_scratch, uint32_t seq_len, uint32_t n_keep,
                               uint32_t n_recent, uint32_t n_drop, uint32_t max_seq, uint32_t n_kv_heads, uint32_t head_dim, const Launch& L) {
-    (void)d_scratch;
-    const Q4EvictArgs a{{d_k_cache, d_v_cache}, d_weights, d_kept, seq_len, n_keep, n_recent, n_drop, max_seq, n_kv_heads, head_dim};
-    const auto select = seq_len <= 4u * kEvictThreads ? kv_q4_select_kernel<4, false> : seq_len <= 32u * kEvictThreads ? kv_q4_select_kernel<32, false> : kv_q4_select_kernel<32, true>;
-    const hipError_t e = launch_kernel(L, kFamOther, select, dim3(n_kv_heads), dim3(kEvictThreads), a);
-    if (e != hipSuccess) return e;
-    const auto move = [&](auto kernel, uint32_t streams) { return launch_kernel(L, kFamOther, kernel, dim3(n_kv_heads, 2u * streams + 3u), dim3(kEvictThreads), a); };
+    const Q4EvictArgs a{{d_k_cache, d_v_cache}, d_weights, d_kept, reinterpret_cast<uint32_t*>(d_scratch), 0, seq_len, n_keep, n_recent, n_drop, max_seq, n_kv_heads, head_dim};
     switch (head_dim) {
-        case 32: return move(kv_q4_move_kernel<32>, 1 / kMovePieces<32>);
-        case 64: return move(kv_q4_move_kernel<64>, 2 / kMovePieces<64>);
-        case 128: return move(kv_q4_move_kernel<128>, 4 / kMovePieces<128>);
-        default: return move(kv_q4_move_kernel<256>, 8 / kMovePieces<256>);
+        case 32: return launch_evict<32>(a, L);
+        case 64: return launch_evict<64>(a, L);
+        case 128: return launch_evict<128>(a, L);
+        default: return launch_evict<256>(a, L);
     }
 }
 
