@@ -85,10 +85,15 @@ __global__ __launch_bounds__(256) void kv_q4_read_kernel(const void* p, float* _
 
 // ---- eviction -------------------------------------------------------------------------------
 constexpr uint32_t kStateLine = 32;
+struct SelectRecord {  // what a part of a head knows
+    uint32_t prefix, left, smaller_before;  // bits found, keys that share them and leave, keys of the parts in front that are smaller than those
+};
 struct Q4EvictArgs {
     void* cache[2];
     float* weights;
     uint32_t* kept;   // [n_kv_heads][seq_len - n_drop]
+    uint32_t* hists;    // of more than kSelectChunk rows: [2][n_kv_heads][parts][kBins]
+    SelectRecord* records;  // [n_kv_heads][parts]
     uint32_t* state;    // [2 n_kv_heads]: segments taken, and a line behind it which of `segments` are in registers
     uint32_t segments;  // of rows that stay
     uint32_t seq_len, n_keep, n_recent, n_drop, max_seq, n_kv_heads, head_dim;
@@ -101,133 +106,216 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
+// Sum over a wave's lanes up to this one.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved_or_zero(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v += moved_or_zero<0x111, 0xf>(v), v += moved_or_zero<0x112, 0xf>(v), v += moved_or_zero<0x114, 0xf>(v), v += moved_or_zero<0x118, 0xf>(v);  // in rows of 16 lanes
+    v += moved_or_zero<0x142, 0xa>(v);  // the last of a row to the next: rows 1 and 3,
+    v += moved_or_zero<0x143, 0xc>(v);  // and that of the first half to the second
+    return v;
+}
+
 // Sum over the workgroup's threads in front of this one, and over all of them.  `slots`: one per wave, of this call alone.
 constexpr uint32_t kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64;
 __device__ __forceinline__ uint32_t sum_before(uint32_t v, uint32_t* slots, uint32_t& total) {
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    uint32_t sum = v;
-#pragma unroll
-    for (uint32_t off = 1; off < 64u; off <<= 1) {
-        const uint32_t up = __shfl_up(sum, off, 64);
-        if (lane >= off) sum += up;
-    }
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, sum = wave_scan(v);
     if (lane == 63u) slots[wave] = sum;
     __syncthreads();
-    uint32_t front = 0, all = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < kEvictWaves; i++) {
-        const uint32_t s = slots[i];
-        front += i < wave ? s : 0u, all += s;
-    }
-    total = all;
-    return front + sum - v;
+    const uint32_t sums = wave_scan(lane < kEvictWaves ? slots[lane] : 0u);
+    total = (uint32_t)__builtin_amdgcn_readlane((int)sums, 63);
+    const uint32_t w = (uint32_t)__builtin_amdgcn_readfirstlane((int)wave);
+    return sum - v + (w > 0 ? (uint32_t)__builtin_amdgcn_readlane((int)sums, (int)w - 1) : 0u);
 }
 
 // The rows of one KV head that stay, in order.  Of the candidates' keys the n_drop-th smallest is found 11, 11 and 10 bits at a time from the highest, by a
 // histogram of those bits among the keys that share the bits found so far (11 bits are the exponent and two bits behind it: weights spread over
 // many bins, so that a wave's additions seldom meet).  Of those that have just this key the lower rows leave, as many as are still to go.  A wave's 64
 // consecutive rows are one vote: a row's place is the rows that stay in the votes before, which are added up over the workgroup, and those in front of it in its own.
-// Up to 32768 rows are read once and stay in registers (28 us for 8 heads of 32768 rows; read anew for each step 38), longer caches are read anew for each step.
-// Bound by one CU's instructions per head and, for few rows, by the latency of some 20 barriers and as many trips to LDS (3000 rows 7.3 us); 32768 rows
-// took 76 us with bytes for digits, one lane walking the bins and a run of rows to each thread, which writes no whole lines.
-// ROWS: of a thread at a time (3000 rows as 32 a thread: 24 us); LONG: there are more, in chunks.
-template <uint32_t ROWS, bool LONG>
-__global__ __launch_bounds__(kEvictThreads) void kv_q4_select_kernel(Q4EvictArgs a) {
-    constexpr uint32_t kBins = 2048, kChunk = ROWS * kEvictThreads, kVotes = ROWS * kEvictWaves;
-    static_assert(ROWS <= 32 && kVotes <= kEvictThreads, "a bit a row, a thread a vote");
-    __shared__ uint32_t hist[kBins + 64], slots[8][kEvictWaves], votes[kVotes], found[2];
-    const uint32_t c = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
-    const uint64_t in_front = (1ull << lane) - 1ull;
-    for (uint32_t i = tid; i < 2u * (kStateLine + a.segments); i += kEvictThreads) a.state[(size_t)c * 2u * (kStateLine + a.segments) + i] = 0u;  // (for the launch behind)
+// Up to 4096 rows: one workgroup a head, which reads them once; bound by the latency of some 20 barriers and as many trips to LDS (3000 rows of 8 heads 6.4 us).
+// More: the head in parts of a workgroup each, a launch to each digit and one to place the rows, every one of which begins with adding up the parts'
+// histograms of the launch before (32768 rows of 8 heads 4.0 + 5.2 + 5.4 + 6.1 us, each bound by the same latencies; by one workgroup a head 28 us, and more
+// with every row).
+constexpr uint32_t kSelectRows = 4, kSelectChunk = kSelectRows * kEvictThreads, kVotes = kSelectRows * kEvictWaves;  // rows of a thread, of a workgroup at a time
+constexpr uint32_t kBins = 2048, kMaxParts = 32;
+
+__host__ __device__ inline uint32_t select_parts(uint32_t seq_len) {
+    const uint32_t chunks = (seq_len + kSelectChunk - 1u) / kSelectChunk;
+    return chunks < kMaxParts ? chunks : kMaxParts;
+}
+
+constexpr uint32_t digit_shift(int digit) { return digit == 0 ? 21u : digit == 1 ? 10u : 0u; }
+
+struct SelectShared {
+    uint32_t hist[kBins + 64], slots[3][kEvictWaves], votes[2][kVotes], found[2];
+};
+
+struct SelectKeys {
+    uint32_t k[kSelectRows], candidates;  // bit i: row i of this thread may leave
     // (a read behind the last row gives 0, for nobody)
-    const auto w = __builtin_amdgcn_make_buffer_rsrc(a.weights + (size_t)c * a.max_seq, 0, (int)(4u * a.seq_len), 0x27000);
-    const uint32_t from = a.n_keep, to = a.seq_len - a.n_recent;
-    const uint32_t rows = LONG ? a.seq_len : 1u;  // (one chunk)
-    uint32_t keys[ROWS], candidates;  // bit i: row i of this thread may leave
-    const auto load = [&](uint32_t base) {
+    __device__ __forceinline__ void load(const Q4EvictArgs& a, uint32_t c, uint32_t base) {
+        const auto w = __builtin_amdgcn_make_buffer_rsrc(a.weights + (size_t)c * a.max_seq, 0, (int)(4u * a.seq_len), 0x27000);
+        const uint32_t first = base + threadIdx.x - a.n_keep, n = a.seq_len - a.n_recent - a.n_keep;
+#pragma unroll
+        for (uint32_t i = 0; i < kSelectRows; i++) k[i] = __builtin_amdgcn_raw_buffer_load_b32(w, 4u * (base + i * kEvictThreads + threadIdx.x), 0, 0);
         candidates = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < ROWS; i++) keys[i] = __builtin_amdgcn_raw_buffer_load_b32(w, 4u * (base + i * kEvictThreads + tid), 0, 0);
+        for (uint32_t i = 0; i < kSelectRows; i++) candidates |= (uint32_t)(first + i * kEvictThreads < n) << i, k[i] = weight_key(__uint_as_float(k[i]));
+    }
+    __device__ __forceinline__ void count(uint32_t* hist, int digit, uint32_t prefix) const {
+        const uint32_t shift = digit_shift(digit), mask = digit == 2 ? 1023u : 2047u, above = digit == 1 ? 21u : 10u, lane = threadIdx.x & 63u;
 #pragma unroll
-        for (uint32_t i = 0; i < ROWS; i++) {
-            candidates |= (uint32_t)(base + i * kEvictThreads + tid - from < to - from) << i;
-            keys[i] = weight_key(__uint_as_float(keys[i]));
+        for (uint32_t i = 0; i < kSelectRows; i++) {
+            // What does not count goes to a bin of its lane's own (no branch, no two at one address), and so do the lanes that meet the first one: it
+            // adds for all of them (rows that are new have no weight at all).
+            const bool counts = (candidates >> i & 1u) && (digit == 0 || k[i] >> above == prefix >> above);
+            const uint32_t bin = counts ? k[i] >> shift & mask : kBins + lane, first = (uint32_t)__builtin_amdgcn_readfirstlane((int)bin);
+            const uint64_t same = __ballot(bin == first);
+            atomicAdd(&hist[bin == first && lane != 0 ? kBins + lane : bin], lane == 0 ? (uint32_t)__popcll(same) : 1u);
         }
-    };
-    load(0);
+    }
+};
+
+// The bin that the left-th key is in, this thread having the counts of bins 2 tid and 2 tid + 1; `left` becomes how many of that bin's leave.
+__device__ __forceinline__ uint32_t find_bin(SelectShared& s, uint32_t h0, uint32_t h1, uint32_t* slots, uint32_t& left) {
+    uint32_t all;
+    const uint32_t before = sum_before(h0 + h1, slots, all);
+    if (before < left && left <= before + h0 + h1) {  // one thread's (left is at least one and at most how many there are)
+        const bool second = left > before + h0;
+        s.found[0] = 2u * threadIdx.x + second, s.found[1] = before + (second ? h0 : 0u);
+    }
+    __syncthreads();
+    const uint32_t bin = s.found[0];
+    left -= s.found[1];
+    __syncthreads();  // (found is written again)
+    return bin;
+}
+
+// Bit i of every thread is row i's vote: how many have been given before this wave's, in lane 16 i + its number (and `before` in all: those of earlier chunks).
+__device__ __forceinline__ uint32_t count_votes(uint32_t* votes, uint32_t bits, uint32_t& before) {
+    static_assert(kVotes == 64 && kEvictWaves == 16, "one lane a vote");
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    uint32_t counts = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kSelectRows; i++) {
+        const uint32_t n = (uint32_t)__popcll(__ballot(bits >> i & 1u));
+        counts = lane == i ? n : counts;
+    }
+    if (lane < kSelectRows) votes[lane * kEvictWaves + wave] = counts;
+    __syncthreads();
+    const uint32_t n = votes[lane], sum = wave_scan(n), at = sum - n + before;
+    before += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+    return at;
+}
+
+// Of a chunk, the rows whose keys are larger than `key` stay, and of those equal to it all but the first `left` of the head (equal_before: how many there are
+// in front of the chunk; stay_before: rows that stay in front of it).
+__device__ __forceinline__ void place(SelectShared& s, const Q4EvictArgs& a, uint32_t c, const SelectKeys& keys, uint32_t base, uint32_t key, uint32_t left,
+                                      uint32_t& equal_before, uint32_t& stay_before) {
+    const uint32_t tid = threadIdx.x;
+    const uint64_t in_front = (1ull << (tid & 63u)) - 1ull;
+    uint32_t* const kept = a.kept + (size_t)c * (a.seq_len - a.n_drop);
+    uint32_t equal = 0, stays = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kSelectRows; i++) {
+        equal |= (keys.candidates >> i & (uint32_t)(keys.k[i] == key)) << i;
+        stays |= (uint32_t)(base + i * kEvictThreads + tid < a.seq_len && (!(keys.candidates >> i & 1u) || keys.k[i] > key)) << i;
+    }
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+    uint32_t at = count_votes(s.votes[0], equal, equal_before);
+    if (__ballot(equal != 0) != 0) {  // (few waves)
+#pragma unroll
+        for (uint32_t i = 0; i < kSelectRows; i++) {
+            const uint32_t rank = (uint32_t)__builtin_amdgcn_readlane((int)at, (int)(kEvictWaves * i + wave)) + (uint32_t)__popcll(__ballot(equal >> i & 1u) & in_front);
+            stays |= (equal >> i & (uint32_t)(rank >= left)) << i;
+        }
+    }
+    at = count_votes(s.votes[1], stays, stay_before);
+#pragma unroll
+    for (uint32_t i = 0; i < kSelectRows; i++) {
+        const uint64_t vote = __ballot(stays >> i & 1u);
+        const uint32_t to = (uint32_t)__builtin_amdgcn_readlane((int)at, (int)(kEvictWaves * i + wave)) + (uint32_t)__popcll(vote & in_front);
+        if (stays >> i & 1u) kept[to] = base + i * kEvictThreads + tid;
+    }
+}
+
+__device__ __forceinline__ void clear_move_state(const Q4EvictArgs& a, uint32_t c) {  // (for the launch behind)
+    const uint32_t n = 2u * (kStateLine + a.segments);
+    for (uint32_t i = threadIdx.x; i < n; i += kEvictThreads) a.state[(size_t)c * n + i] = 0u;
+}
+
+__global__ __launch_bounds__(kEvictThreads) void kv_q4_select_kernel(Q4EvictArgs a) {
+    __shared__ SelectShared s;
+    const uint32_t c = blockIdx.x, tid = threadIdx.x;
+    clear_move_state(a, c);
+    SelectKeys keys;
+    keys.load(a, c, 0);
     uint32_t prefix = 0, left = a.n_drop;  // bits found so far; how many of the keys that share them leave
 #pragma unroll
     for (int digit = 0; digit < 3; digit++) {
-        const uint32_t shift = digit == 0 ? 21u : digit == 1 ? 10u : 0u, mask = digit == 2 ? 1023u : 2047u, above = digit == 1 ? 21u : 10u;
-        hist[tid] = hist[tid + kEvictThreads] = 0;
+        s.hist[tid] = s.hist[tid + kEvictThreads] = 0;
         __syncthreads();
-        for (uint32_t base = 0; base < rows; base += kChunk) {
-            if (LONG && (digit > 0 || base > 0)) load(base);
-#pragma unroll
-            for (uint32_t i = 0; i < ROWS; i++) {
-                // What does not count goes to a bin of its lane's own (no branch, no two at one address), and so do the lanes that meet the first one: it
-                // adds for all of them (rows that are new have no weight at all).
-                const bool counts = (candidates >> i & 1u) && (digit == 0 || keys[i] >> above == prefix >> above);
-                const uint32_t bin = counts ? keys[i] >> shift & mask : kBins + lane, first = (uint32_t)__builtin_amdgcn_readfirstlane((int)bin);
-                const uint64_t same = __ballot(bin == first);
-                atomicAdd(&hist[bin == first && lane != 0 ? kBins + lane : bin], lane == 0 ? (uint32_t)__popcll(same) : 1u);
-            }
-        }
+        keys.count(s.hist, digit, prefix);
         __syncthreads();
-        const uint32_t h0 = hist[2u * tid], h1 = hist[2u * tid + 1u];
-        uint32_t all;
-        const uint32_t before = sum_before(h0 + h1, slots[digit], all);
-        if (before < left && left <= before + h0 + h1) {  // one thread's (left is at least one and at most how many there are)
-            const bool second = left > before + h0;
-            found[0] = 2u * tid + second, found[1] = before + (second ? h0 : 0u);
-        }
-        __syncthreads();
-        prefix |= found[0] << shift, left -= found[1];
-        __syncthreads();  // (found and hist are written again)
+        prefix |= find_bin(s, s.hist[2u * tid], s.hist[2u * tid + 1u], s.slots[digit], left) << digit_shift(digit);
     }
-    // Bit i of every thread is row i's vote: how many have been given before each wave's, in lane i (and `before` in all: those of earlier chunks).
-    const auto count_votes = [&](uint32_t bits, uint32_t* table, uint32_t* sums, uint32_t& before) {
-        uint32_t counts = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < ROWS; i++) {
-            const uint32_t n = (uint32_t)__popcll(__ballot(bits >> i & 1u));
-            counts = lane == i ? n : counts;
-        }
-        if (lane < ROWS) table[lane * kEvictWaves + wave] = counts;
-        __syncthreads();
-        uint32_t all;
-        const uint32_t sum = sum_before(tid < kVotes ? table[tid] : 0u, sums, all) + before;
-        if (tid < kVotes) table[tid] = sum;
-        before += all;
-        __syncthreads();
-        const uint32_t at = lane < ROWS ? table[lane * kEvictWaves + wave] : 0u;
-        __syncthreads();  // (the table is written again)
-        return at;
-    };
     uint32_t equal_before = 0, stay_before = 0;
-    uint32_t* const kept = a.kept + (size_t)c * (a.seq_len - a.n_drop);
-    for (uint32_t base = 0; base < rows; base += kChunk) {
-        if (LONG) load(base);
-        uint32_t equal = 0, stays = 0;
+    place(s, a, c, keys, 0, prefix, left, equal_before, stay_before);
+}
+
+// STEP 0 .. 2: a part's histogram of that digit; 3: its rows placed.  What a part knows goes from launch to launch in a record of its own.
+template <int STEP>
+__global__ __launch_bounds__(kEvictThreads) void kv_q4_select_part_kernel(Q4EvictArgs a) {
+    __shared__ SelectShared s;
+    const uint32_t parts = gridDim.x, part = blockIdx.x, c = blockIdx.y, tid = threadIdx.x;
+    const uint32_t chunks = (a.seq_len + kSelectChunk - 1u) / kSelectChunk, chunk0 = (uint32_t)((uint64_t)chunks * part / parts), chunk_end = (uint32_t)((uint64_t)chunks * (part + 1u) / parts);
+    const auto hist_of = [&](int step, uint32_t p) { return reinterpret_cast<uint2*>(a.hists + ((size_t)(step & 1) * a.n_kv_heads * parts + (size_t)c * parts + p) * kBins); };
+    SelectRecord& record = a.records[(size_t)c * parts + part];
+    SelectKeys keys;
+    keys.load(a, c, chunk0 * kSelectChunk);
+    uint32_t prefix = 0, left = a.n_drop, smaller_before = 0, equal_before = 0;
+    if constexpr (STEP == 0) {
+        if (part == 0) clear_move_state(a, c);
+    } else {
+        if constexpr (STEP > 1) prefix = record.prefix, left = record.left, smaller_before = record.smaller_before;
+        uint2 sum = {0, 0}, before = {0, 0};  // over all parts, over those in front
+        for (uint32_t p0 = 0; p0 < parts; p0 += 8u) {
+            uint2 h[8];
 #pragma unroll
-        for (uint32_t i = 0; i < ROWS; i++) {
-            equal |= (candidates >> i & (uint32_t)(keys[i] == prefix)) << i;
-            stays |= (uint32_t)(base + i * kEvictThreads + tid < a.seq_len && (!(candidates >> i & 1u) || keys[i] > prefix)) << i;
-        }
-        uint32_t at = count_votes(equal, votes, slots[3], equal_before);
-        if (__ballot(equal != 0) != 0) {  // (few waves)
+            for (uint32_t i = 0; i < 8u; i++) h[i] = hist_of(STEP - 1, min(p0 + i, parts - 1u))[tid];
 #pragma unroll
-            for (uint32_t i = 0; i < ROWS; i++) {
-                const uint32_t rank = (uint32_t)__builtin_amdgcn_readlane((int)at, (int)i) + (uint32_t)__popcll(__ballot(equal >> i & 1u) & in_front);
-                stays |= (equal >> i & (uint32_t)(rank >= left)) << i;
+            for (uint32_t i = 0; i < 8u; i++) {
+                const uint32_t p = p0 + i;
+                if (p < parts) sum.x += h[i].x, sum.y += h[i].y;
+                if (p < part) before.x += h[i].x, before.y += h[i].y;
             }
         }
-        at = count_votes(stays, votes, slots[4], stay_before);
-#pragma unroll
-        for (uint32_t i = 0; i < ROWS; i++) {
-            const uint64_t vote = __ballot(stays >> i & 1u);
-            const uint32_t to = (uint32_t)__builtin_amdgcn_readlane((int)at, (int)i) + (uint32_t)__popcll(vote & in_front);
-            if (stays >> i & 1u) kept[to] = base + i * kEvictThreads + tid;
+        const uint32_t bin = find_bin(s, sum.x, sum.y, s.slots[0], left);
+        prefix |= bin << digit_shift(STEP - 1);
+        uint32_t smaller;
+        (void)sum_before((2u * tid < bin ? before.x : 0u) + (2u * tid + 1u < bin ? before.y : 0u), s.slots[1], smaller);
+        smaller_before += smaller;
+        if constexpr (STEP == 3) (void)sum_before(2u * tid == bin ? before.x : 2u * tid + 1u == bin ? before.y : 0u, s.slots[2], equal_before);
+    }
+    if constexpr (STEP < 3) {
+        if (STEP > 0 && tid == 0) record = {prefix, left, smaller_before};
+        s.hist[tid] = s.hist[tid + kEvictThreads] = 0;
+        __syncthreads();
+        for (uint32_t i = chunk0;;) {
+            keys.count(s.hist, STEP, prefix);
+            if (++i >= chunk_end) break;
+            keys.load(a, c, i * kSelectChunk);
+        }
+        __syncthreads();
+        hist_of(STEP, part)[tid] = make_uint2(s.hist[2u * tid], s.hist[2u * tid + 1u]);
+    } else {
+        uint32_t stay_before = chunk0 * kSelectChunk - smaller_before - min(equal_before, left);
+        for (uint32_t i = chunk0;;) {
+            place(s, a, c, keys, i * kSelectChunk, prefix, left, equal_before, stay_before);
+            if (++i >= chunk_end) break;
+            keys.load(a, c, i * kSelectChunk);
         }
     }
 }
@@ -239,7 +327,8 @@ __global__ __launch_bounds__(kEvictThreads) void kv_q4_select_kernel(Q4EvictArgs
 // before those writes is asked of the memory: nothing that this launch writes is read in it.)
 // Weights behind the last row that stays are cleared by segments that have nothing to read.
 // Bound by memory latency: taking a segment, its rows' numbers, the rows, the word of the segments in front, one behind the other; 24576 rows of 8 heads of
-// 64 values took 18 us with one workgroup for all rows of a quarter of a head's planes, one chunk of rows behind the other.
+// 64 values 12.2 us (18.1 with one workgroup for all rows of a fifth of a head's planes, one chunk of rows behind the other; of one head of 256 values 8.8
+// and 50.6).
 constexpr uint32_t kMoveThreads = 256, kMoveLeast = 256;  // threads; rows of a segment at least
 template <int HD>
 constexpr uint32_t kMoveRows = HD <= 64 ? 512 : 256;  // 16 KiB of quants and more: enough workgroups, and four and more loads of a thread on their way
@@ -343,7 +432,15 @@ hipError_t launch_kv_q4_read(const void* d_cache, float* d_out, uint32_t out_str
                          n_kv_heads, head_dim);
 }
 
-size_t kv_q4_evict_scratch_floats(uint32_t seq_len, uint32_t n_kv_heads) { return 2 * (size_t)n_kv_heads * (kStateLine + (seq_len + kMoveLeast - 1u) / kMoveLeast); }
+// Histograms, records, state of the move.
+static size_t evict_hist_words(uint32_t seq_len, uint32_t n_kv_heads) { return seq_len <= kSelectChunk ? 0 : 2 * (size_t)n_kv_heads * select_parts(seq_len) * kBins; }
+static size_t evict_record_words(uint32_t seq_len, uint32_t n_kv_heads) {
+    return seq_len <= kSelectChunk ? 0 : (size_t)n_kv_heads * select_parts(seq_len) * (sizeof(SelectRecord) / 4);
+}
+size_t kv_q4_evict_scratch_floats(uint32_t seq_len, uint32_t n_kv_heads) {
+    return evict_hist_words(seq_len, n_kv_heads) + evict_record_words(seq_len, n_kv_heads) +
+           2 * (size_t)n_kv_heads * (kStateLine + (seq_len + kMoveLeast - 1u) / kMoveLeast);
+}
 
 namespace {
 
@@ -352,8 +449,13 @@ hipError_t launch_evict(Q4EvictArgs a, const Launch& L) {
     constexpr uint32_t R = kMoveRows<HD>;
     static_assert(R >= kMoveLeast, "the scratch is sized for it");
     a.segments = (a.seq_len - a.n_drop - a.n_keep + R - 1u) / R;
-    const auto select = a.seq_len <= 4u * kEvictThreads ? kv_q4_select_kernel<4, false> : a.seq_len <= 32u * kEvictThreads ? kv_q4_select_kernel<32, false> : kv_q4_select_kernel<32, true>;
-    const hipError_t e = launch_kernel(L, kFamOther, select, dim3(a.n_kv_heads), dim3(kEvictThreads), a);
+    hipError_t e = hipSuccess;
+    if (a.seq_len <= kSelectChunk) {
+        e = launch_kernel(L, kFamOther, kv_q4_select_kernel, dim3(a.n_kv_heads), dim3(kEvictThreads), a);
+    } else {
+        for (const auto step : {kv_q4_select_part_kernel<0>, kv_q4_select_part_kernel<1>, kv_q4_select_part_kernel<2>, kv_q4_select_part_kernel<3>})
+            if (e == hipSuccess) e = launch_kernel(L, kFamOther, step, dim3(select_parts(a.seq_len), a.n_kv_heads), dim3(kEvictThreads), a);
+    }
     if (e != hipSuccess) return e;
     return launch_kernel(L, kFamOther, kv_q4_move_kernel<HD>, dim3(2u * a.n_kv_heads * ((a.seq_len - a.n_keep + R - 1u) / R)), dim3(kMoveThreads), a);
 }
@@ -362,7 +464,9 @@ hipError_t launch_evict(Q4EvictArgs a, const Launch& L) {
 
 hipError_t launch_kv_q4_evict(void* d_k_cache, void* d_v_cache, float* d_weights, uint32_t* d_kept, float* d_scratch, uint32_t seq_len, uint32_t n_keep,
                               uint32_t n_recent, uint32_t n_drop, uint32_t max_seq, uint32_t n_kv_heads, uint32_t head_dim, const Launch& L) {
-    const Q4EvictArgs a{{d_k_cache, d_v_cache}, d_weights, d_kept, reinterpret_cast<uint32_t*>(d_scratch), 0, seq_len, n_keep, n_recent, n_drop, max_seq, n_kv_heads, head_dim};
+    uint32_t *const hists = reinterpret_cast<uint32_t*>(d_scratch), *const records = hists + evict_hist_words(seq_len, n_kv_heads),
+             *const state = records + evict_record_words(seq_len, n_kv_heads);
+    const Q4EvictArgs a{{d_k_cache, d_v_cache}, d_weights, d_kept, hists, reinterpret_cast<SelectRecord*>(records), state, 0, seq_len, n_keep, n_recent, n_drop, max_seq, n_kv_heads, head_dim};
     switch (head_dim) {
         case 32: return launch_evict<32>(a, L);
         case 64: return launch_evict<64>(a, L);
