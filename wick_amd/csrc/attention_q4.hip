@@ -12,6 +12,9 @@
 // in all); a query, scaled by a power of two to below 1, and a softmax weight, times 2^12, are split into two halves that keep 22 bits.
 // a b = a_hi b_hi + a_hi b_lo + a_lo b_hi: each product of halves is exact, sums are f32's, what is dropped is below 2^-22.
 // (One half for the weights or the queries would be off by 2^-12 of each: 100 times what f32 sums are.)
+// Bound by the matrix and vector instructions of a unit of 32 rows and 32 keys (heads of 64: 24 matrix instructions of 32 cycles and 920 cycles of vector ones, of
+// the softmax above all, in 2060 cycles): 2002 tokens of 32 heads over 8 of 64 60 us, 2048 behind 6144 of 16 heads over 4 of 128 311 us (three products at 1160
+// TFLOP/s; power).
 #include <algorithm>
 
 #include "attention_device.h"
@@ -485,7 +488,10 @@ __global__ __launch_bounds__(256) void attention_q4_merge_kernel(Q4AttentionArgs
 // Up to 16 query rows of a KV head (the heads of one token, of a few tokens) per workgroup, and a part of the cache to each of its waves, 32 rows
 // at a time, on v_mfma_f32_16x16x32_f16.  Nothing goes through LDS but the states at the end: a lane loads the words of a key row that it multiplies (lane
 // group g HD / 32 of them from word g HD / 32 on, the order of an MFMA's K steps being free), and of the values one word of eight rows, the rows whose weights it
-// holds: two rows' words are transposed to pairs of one dim's values with one byte permutation each.
+// holds: two rows' words are transposed to pairs of one dim's values with one byte permutation each.  Keys are multiplied as nibbles less 8, one exact half, a
+// block's 32 dims at a time, and the block's scale is taken into the sum: two products of halves instead of three.
+// Bound at long context by the loads and the unpacking, which overlap in part: one token of 32 heads over 8 of 128 behind 128000 rows (147 MB) 41 us, its
+// loads alone 26; with values through LDS and both planes of the keys 45.  At short context by two or three round trips to memory: 16 heads over 9000 rows 7.2 us.
 struct FewArgs {
     Q4AttentionArgs at;
     float* scores;  // [n_heads][max_seq], of one token's heads in powers of two, for the weights; may be null
@@ -829,7 +835,7 @@ __global__ __launch_bounds__(64 * kFewWaves, HD == 32 ? 4 : HD <= 128 ? 2 : 1) v
 }
 
 // One token's splits merged and, in workgroups of their own, its weights added to what the rows have gathered: from the scores that the launch before left, with
-// each head's maximum and sum worked out from its splits once more.
+// each head's maximum and sum worked out from its splits once more.  (9001 rows of 16 heads 3.6 us: a launch and two round trips.)
 template <int HD>
 __global__ __launch_bounds__(256) void attention_q4_finish_kernel(FewArgs args) {
     const Q4AttentionArgs& a = args.at;
@@ -861,6 +867,8 @@ __global__ __launch_bounds__(256) void attention_q4_finish_kernel(FewArgs args) 
 
 // What 32 U rows of a KV head have gathered: the scores once more, now that every softmax's maximum and sum is known, and their weights added
 // up over the query rows -- 32 of them at a time and wave, the next ones on their way meanwhile, kept apart by lane and wave and added in one order at the end.
+// Bound by vector instructions, most of which split the queries, anew in every workgroup: 555 tokens of 16 heads 12.7 us (64 rows and 8 waves a workgroup 17.2:
+// 72 workgroups, and no queries under way).
 template <int HD, int WAVES, int U>
 __global__ __launch_bounds__(64 * WAVES) void attention_q4_weights_kernel(Q4AttentionArgs a) {
     constexpr int KT = 32 * U, LD = HD + 8, SLABS = HD / 16;
