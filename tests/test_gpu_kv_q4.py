@@ -221,6 +221,9 @@ def test_a_row_held_as_nan_is_seen_by_those_that_see_it(ctx, ops, dev, hd, heads
     assert np.isnan(out[hit]).all()
     if not hit.all():
         assert_f32_parity(out[~hit], clean[~hit], "tokens that do not see it")
+    got = d_w.download(np.float32, n_kv * max_seq).reshape(n_kv, max_seq)
+    assert np.isnan(got[[0, n_kv - 1]]).all()  # (the last token sees every row)
+    assert_f32_parity(got[1:n_kv - 1], R.gathered(p, n_kv)[1:n_kv - 1], "weights of the other heads") if n_kv > 2 else None
 
 
 @pytest.mark.parametrize("heads,n_kv,seq,n", [(4, 2, 300, 20), (16, 4, 1200, 700), (16, 4, 1600, 900)])

@@ -865,83 +865,149 @@ __global__ __launch_bounds__(256) void attention_q4_finish_kernel(FewArgs args) 
     if (t <= last) a.weights[(size_t)c * a.max_seq + t] += sum;
 }
 
-// What 32 U rows of a KV head have gathered: the scores once more, now that every softmax's maximum and sum is known, and their weights added
-// up over the query rows -- 32 of them at a time and wave, the next ones on their way meanwhile, kept apart by lane and wave and added in one order at the end.
-// Bound by vector instructions, most of which split the queries, anew in every workgroup: 555 tokens of 16 heads 12.7 us (64 rows and 8 waves a workgroup 17.2:
-// 72 workgroups, and no queries under way).
-template <int HD, int WAVES, int U>
-__global__ __launch_bounds__(64 * WAVES) void attention_q4_weights_kernel(Q4AttentionArgs a) {
-    constexpr int KT = 32 * U, LD = HD + 8, SLABS = HD / 16;
-    __shared__ __align__(16) _Float16 keys[2][KT][LD];
-    __shared__ float sums[WAVES][KT];
-    const uint32_t c = blockIdx.y, key0 = blockIdx.x * KT, group = a.n_heads / a.n_kv_heads, rows = a.n * group;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, l32 = lane & 31u, h = lane >> 5, wave = tid >> 6;
+// What rows of a KV head have gathered over a prompt: the scores once more, now that every softmax's maximum and sum is known, and their weights added
+// up over the query rows.  Every wave keeps 32 keys as matrix operands in registers; the workgroup walks query rows in blocks of 32 that it splits into
+// halves once for its four waves, through LDS, the next block's on their way meanwhile.  The rows are shared out among `shares` workgroups, whose sums the next launch adds.
+// All sums in one order.  Bound by vector instructions (exponentials, and the queries' split: a block is split in every workgroup that sees it) and, for few
+// rows, by latency: 555 tokens of 16 heads over 8 of 64 7.4 and 4.5 us for the addition, 1500 of 32 heads 26, 4000 of them 138, 500 of 16 over 4 of 128 9.5 (keys
+// in LDS, the queries split by every wave for itself: 12.7, 54, 257 and 37).  128 keys a workgroup: with 256 and eight waves behind one barrier 9.9, 38, 190 and 17.
+constexpr uint32_t kWeightKeys = 128, kMaxShares = 16;
+template <int HD>
+constexpr uint32_t kWeightSlots = kCus * (HD <= 64 ? 4 : HD == 128 ? 3 : 2);  // workgroups that the GPU has at once
+constexpr uint32_t kWeightSums = 4 * kCus * kWeightKeys;  // that the shares of a launch leave at most: no more workgroups than those
+
+template <int HD>
+__global__ __launch_bounds__(256, kWeightSlots<HD> / kCus) void attention_q4_weights_kernel(Q4AttentionArgs a, float* sums, uint32_t shares, uint32_t stride) {
+    constexpr int SLABS = HD / 16, V = HD / 32;  // four values, of a thread's share of a query row
+    struct Block {
+        _Float16 q[2][32][HD + 8];
+        v4f row[32];  // {factor, shift, 1 / sum, -}
+    };
+    __shared__ __align__(16) Block blocks[2];
+    const uint32_t c = blockIdx.x % a.n_kv_heads, share = blockIdx.x / a.n_kv_heads % shares, key0 = blockIdx.x / a.n_kv_heads / shares * kWeightKeys;
+    const uint32_t group = a.n_heads / a.n_kv_heads, rows = a.n * group;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, l32 = lane & 31u, h = lane >> 5, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
     const uint32_t base = first_row(a), last = sees(a, base, rows - 1u, rows, group);
     if (key0 > last) return;
-    const uint32_t r_first = key0 > base ? (key0 - base) * group / 32u * 32u : 0u;  // rows in front of it see none of the keys
-    typename Queries<HD>::Raw raw;
-    float2 stat;
-    const auto request = [&](uint32_t r0) {  // (of rows past the last: the last one's, for nobody)
-        const uint32_t r = min(r0 + l32, rows - 1u);
-        raw.request(a, r, c, group, h);
-        stat = *reinterpret_cast<const float2*>(a.stats + 2u * ((size_t)(r / group) * a.n_heads + c * group + r % group));
+    const uint32_t r_first = key0 > base ? (key0 - base) * group / 32u : 0u, r_end = (rows + 31u) / 32u;  // blocks; rows in front see none of the keys
+    const uint32_t b_first = r_first + (uint32_t)((uint64_t)(r_end - r_first) * share / shares), b_end = r_first + (uint32_t)((uint64_t)(r_end - r_first) * (share + 1u) / shares);
+
+    // this thread's share of a block of query rows: V times four values, 32 apart, of row tid / 8
+    const uint32_t q_row = tid >> 3, q_at = 4u * (tid & 7u);
+    struct {
+        v4f x[V];
+        float2 stat;
+    } raw;
+    // (its token and head one block after the other, without a division)
+    uint32_t token = (32u * b_first + q_row) / group, of_group = (32u * b_first + q_row) % group;
+    const uint32_t tokens_on = 32u / group, rows_on = 32u % group;
+    const auto request = [&] {  // (of rows past the last: the last one's, for nobody)
+        const uint32_t at = min(token, a.n - 1u), head = c * group + (token < a.n ? of_group : group - 1u);
+        token += tokens_on, of_group += rows_on;
+        if (of_group >= group) of_group -= group, token++;
+        const float* const p = a.q + (size_t)at * a.q_stride + (size_t)head * HD + q_at;
+#pragma unroll
+        for (int i = 0; i < V; i++) raw.x[i] = *reinterpret_cast<const v4f*>(p + 32 * i);
+        raw.stat = *reinterpret_cast<const float2*>(a.stats + 2u * ((size_t)at * a.n_heads + head));
     };
-    request(r_first + 32u * wave);
-    const Q4Cache kc = q4_planes(const_cast<void*>(a.k_cache), a.max_seq, a.n_kv_heads, HD), vc = q4_planes(const_cast<void*>(a.v_cache), a.max_seq, a.n_kv_heads, HD);
-    const size_t first = (size_t)c * a.max_seq;
-    for (uint32_t i = tid; i < KT * HD / 8; i += 64 * WAVES) {
-        const uint32_t row = i / (HD / 8), word = i % (HD / 8);
-        const size_t at = first + min(key0 + row, last);
-        const _Float16 poison = __builtin_bit_cast(_Float16, vc.scales[at * (HD / 32) + word / 4u]) * (_Float16)0.0f;  // (as its token's sum has it)
-        h8 hi, lo;
-        dequantize(kc.quants[at * (HD / 8) + word], __builtin_bit_cast(_Float16, kc.scales[at * (HD / 32) + word / 4u]) + poison, hi, lo);
-        *reinterpret_cast<h8*>(&keys[0][row][8u * word]) = hi, *reinterpret_cast<h8*>(&keys[1][row][8u * word]) = lo;
+    const auto store = [&](Block& to, uint32_t b) {
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(raw.x[i][e]));
+        const int e = __builtin_amdgcn_frexp_expf(group_max8(top));
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            v4f y;
+            h4 hi, lo;
+#pragma unroll
+            for (int k = 0; k < 4; k++) y[k] = __builtin_amdgcn_ldexpf(raw.x[i][k], -e);
+            split_halves(y, hi, lo);
+            *reinterpret_cast<h4*>(&to.q[0][q_row][q_at + 32 * i]) = hi, *reinterpret_cast<h4*>(&to.q[1][q_row][q_at + 32 * i]) = lo;
+        }
+        if ((tid & 7u) == 0)
+            to.row[q_row] = v4f{__builtin_amdgcn_ldexpf(a.scale * kLog2e, e), (raw.stat.x == -__builtin_inff() ? 0.0f : raw.stat.x) - kWeightBits,
+                                32u * b + q_row < rows ? raw.stat.y : 0.0f, 0.0f};
+    };
+    if (b_first < b_end) request();
+    // this lane's key, dims 16 s + 8 h ..
+    h8 kh[SLABS], kl[SLABS];
+    const uint32_t first_key = key0 + 32u * wave;
+    {
+        const Q4Cache kc = q4_planes(const_cast<void*>(a.k_cache), a.max_seq, a.n_kv_heads, HD), vc = q4_planes(const_cast<void*>(a.v_cache), a.max_seq, a.n_kv_heads, HD);
+        const size_t at = (size_t)c * a.max_seq + min(first_key + l32, last);
+        _Float16 poison = (_Float16)0.0f;  // (as its token's sum has it)
+#pragma unroll
+        for (int i = 0; i < HD / 32; i++) poison += __builtin_bit_cast(_Float16, vc.scales[at * (HD / 32) + i]) * (_Float16)0.0f;
+#pragma unroll
+        for (int s = 0; s < SLABS; s++)
+            dequantize(kc.quants[at * (HD / 8) + 2u * s + h], __builtin_bit_cast(_Float16, kc.scales[at * (HD / 32) + s / 2]) + poison, kh[s], kl[s]);
     }
-    __syncthreads();
-    v16f acc[U];
+    const uint32_t b_all = first_key + 31u > base ? (uint32_t)(((uint64_t)(first_key + 31u - base) * group + 31u) / 32u) : 0u;  // from there on rows see all of the wave's keys
+    float acc[16];
 #pragma unroll
-    for (int u = 0; u < U; u++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) acc[u][e] = 0.0f;
-    for (uint32_t r0 = r_first + 32u * wave; r0 < rows; r0 += 32u * WAVES) {
-        const uint32_t mine = sees(a, base, r0 + l32, rows, group);
-        Queries<HD> q;
-        q.take(raw, a.scale);
-        const float shift = (stat.x == -__builtin_inff() ? 0.0f : stat.x) - kWeightBits, inverse = stat.y;
-        request(r0 + 32u * WAVES);
-#pragma unroll
-        for (int u = 0; u < U; u++) {
+    for (int e = 0; e < 16; e++) acc[e] = 0.0f;
+    if (b_first < b_end) {
+        store(blocks[0], b_first);
+        if (b_first + 1u < b_end) request();
+        __syncthreads();
+        const auto add = [&](uint32_t b, const Block& now, Block& then) {
+            const v4f row = now.row[l32];
             v16f sc;
 #pragma unroll
             for (int e = 0; e < 16; e++) sc[e] = 0.0f;
 #pragma unroll
             for (int s = 0; s < SLABS; s++) {
-                const h8 kh = *reinterpret_cast<const h8*>(&keys[0][32 * u + l32][16 * s + 8 * h]), kl = *reinterpret_cast<const h8*>(&keys[1][32 * u + l32][16 * s + 8 * h]);
-                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, q.hi[s], sc, 0, 0, 0);
-                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, q.lo[s], sc, 0, 0, 0);
-                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, q.hi[s], sc, 0, 0, 0);
+                const h8 qh = *reinterpret_cast<const h8*>(&now.q[0][l32][16 * s + 8 * h]), ql = *reinterpret_cast<const h8*>(&now.q[1][l32][16 * s + 8 * h]);
+                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl[s], qh, sc, 0, 0, 0);
+                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[s], ql, sc, 0, 0, 0);
+                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[s], qh, sc, 0, 0, 0);
             }
+            if (b + 1u < b_end) store(then, b + 1u);
+            if (b + 2u < b_end) request();
+            if (b < b_all) {  // some query row does not see all of the keys
+                const uint32_t mine = sees(a, base, 32u * b + l32, rows, group);
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], q.factor, -shift)) * inverse;
-                acc[u][e] += key0 + 32u * u + 8u * (e >> 2) + 4u * h + (e & 3) > mine || r0 + l32 >= rows ? 0.0f : w;
+                for (int e = 0; e < 16; e++) {
+                    const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], row[0], -row[1])) * row[2];
+                    acc[e] += first_key + 8u * (e >> 2) + 4u * h + (e & 3) > mine ? 0.0f : w;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; e++) acc[e] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], row[0], -row[1])), row[2], acc[e]);
             }
+            __syncthreads();
+        };
+        for (uint32_t b = b_first; b < b_end; b += 2u) {
+            add(b, blocks[0], blocks[1]);
+            if (b + 1u >= b_end) break;
+            add(b + 1u, blocks[1], blocks[0]);
         }
     }
+    float* const to = shares == 1u ? a.weights + (size_t)c * a.max_seq : sums + (size_t)(share * a.n_kv_heads + c) * stride;
 #pragma unroll
-    for (int u = 0; u < U; u++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const float w = group_sum<32>(acc[u][e]);
-            if (l32 == 0) sums[wave][32 * u + 8 * (e >> 2) + 4 * h + (e & 3)] = w;
+    for (int e = 0; e < 16; e++) {
+        const float w = group_sum<32>(acc[e]);
+        const uint32_t key = first_key + 8u * (e >> 2) + 4u * h + (e & 3);
+        if (l32 == 0 && key <= last) {
+            if (shares == 1u) to[key] += w;
+            else to[key] = w;
         }
-    __syncthreads();
-    if (tid < KT && key0 + tid <= last) {
-        float w = sums[0][tid];
-#pragma unroll
-        for (int i = 1; i < WAVES; i++) w += sums[i][tid];
-        a.weights[first + key0 + tid] += w;
     }
+}
+__global__ __launch_bounds__(256) void attention_q4_add_weights_kernel(Q4AttentionArgs a, const float* sums, uint32_t shares, uint32_t stride) {
+    const uint32_t c = blockIdx.y, t = blockIdx.x * 256u + threadIdx.x, group = a.n_heads / a.n_kv_heads, rows = a.n * group;
+    if (t > sees(a, first_row(a), rows - 1u, rows, group)) return;
+    float w = 0.0f;
+    for (uint32_t i0 = 0; i0 < shares; i0 += 8u) {
+        float x[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; i++) x[i] = sums[(size_t)(min(i0 + i, shares - 1u) * a.n_kv_heads + c) * stride + t];
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; i++) w += i0 + i < shares ? x[i] : 0.0f;
+    }
+    a.weights[(size_t)c * a.max_seq + t] += w;
 }
 
 // Large launches: as many splits as workgroups fit on the GPU, three tiles or more each (a split's state is written and read again).
@@ -999,13 +1065,11 @@ hipError_t launch_head_dim(const Q4AttentionArgs& a, float* d_scores, const Laun
         e = launch_tiles<HD, 4, 1, 1>(a, seen, L);
     }
     if (e != hipSuccess || !a.weights) return e;
-    const uint32_t wide = (uint32_t)((seen + 63u) / 64u);
-    if constexpr (HD <= 128) {  // (of 256 values: the next rows do not fit into the registers)
-        constexpr int kWaves = HD <= 64 ? 16 : 8;
-        if (wide * a.n_kv_heads < kCus)
-            return launch_kernel(L, kFamOther, attention_q4_weights_kernel<HD, kWaves, 1>, dim3((uint32_t)((seen + 31u) / 32u), a.n_kv_heads), dim3(64 * kWaves), a);
-    }
-    return launch_kernel(L, kFamOther, attention_q4_weights_kernel<HD, 8, 2>, dim3(wide, a.n_kv_heads), dim3(512), a);
+    const uint32_t tiles = (uint32_t)((seen + kWeightKeys - 1u) / kWeightKeys), base = a.n_kv_heads * tiles, blocks = (rows + 31u) / 32u, stride = tiles * kWeightKeys;
+    const uint32_t shares = std::min({std::max(kWeightSlots<HD> / base, 1u), kMaxShares, (blocks + 1u) / 2u});
+    e = launch_kernel(L, kFamOther, attention_q4_weights_kernel<HD>, dim3(base * shares), dim3(256), a, d_scores, shares, stride);
+    if (e != hipSuccess || shares == 1u) return e;
+    return launch_kernel(L, kFamOther, attention_q4_add_weights_kernel, dim3((uint32_t)((seen + 255u) / 256u), a.n_kv_heads), dim3(256), a, (const float*)d_scores, shares, stride);
 }
 
 // Floats of the splits' records: what a split launch has at most, for any number of tokens up to n.
@@ -1017,8 +1081,8 @@ size_t part_floats(uint32_t n, uint32_t n_heads, uint32_t head_dim) {
 }  // namespace
 
 size_t attention_q4_scratch_floats(uint32_t n, uint32_t max_seq, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, bool weights) {
-    (void)n_kv_heads;
-    return part_floats(n, n_heads, head_dim) + (weights ? 2 * (size_t)n * n_heads + (size_t)n_heads * max_seq : 0);  // records, statistics, a token's scores
+    // records, statistics, a token's scores or the shares of a prompt's weights
+    return part_floats(n, n_heads, head_dim) + (weights ? 2 * (size_t)n * n_heads + std::max((size_t)n_heads * max_seq, (size_t)kWeightSums) : 0);
 }
 
 hipError_t launch_attention_q4(const float* d_q, uint32_t q_stride, const void* d_k_cache, const void* d_v_cache, float* d_out, uint32_t out_stride,
