@@ -128,7 +128,8 @@ int wick_rocm_kv_q4_read(wick_rocm_ctx *ctx, const void *d_cache, float *d_out, 
  * and all tokens, in an order of their own that is the same in every run: what a row has gathered, for wick_rocm_kv_q4_evict.  Rows appended anew
  * start from what the array holds for them (the caller clears it once, an eviction clears what it frees).
  * d_scratch: wick_rocm_attention_q4_scratch_floats(n, ...) floats (n = 1 for decode; of a longer n than the call's: fine), 16-byte
- * aligned, contents need not be kept; calls that may run at the same time need one each.  d_q, d_out and caches 16-byte aligned, strides multiples of 4.
+ * aligned, contents need not be kept; calls that may run at the same time need one each.  d_q, d_out and caches 16-byte aligned, strides multiples of 4;
+ * with d_weights the output must not overlap the queries, which are read again for them.
  * A row held as NaN gives NaN to every token that sees it, and to no other. */
 size_t wick_rocm_attention_q4_scratch_floats(uint32_t n, uint32_t max_seq, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, int with_weights);
 int wick_rocm_attention_decode_q4(wick_rocm_ctx *ctx, const float *d_q, const void *d_k_cache, const void *d_v_cache, float *d_out, float *d_weights,
@@ -144,7 +145,7 @@ int wick_rocm_attention_prefill_q4(wick_rocm_ctx *ctx, const float *d_q, uint32_
  * came from: nothing is rounded again, and the caller goes on counting positions (for the rotation) while rows are counted anew from
  * seq_len - n_drop.  d_kept ([n_kv_heads][seq_len - n_drop]): the old row of every one that stayed.  Cache rows from seq_len - n_drop on
  * are left as they were, their weights cleared up to seq_len.  n_drop > 0, n_keep + n_recent + n_drop <= seq_len.  d_scratch:
- * wick_rocm_kv_q4_evict_scratch_floats(...) floats (may be null where that is 0). */
+ * wick_rocm_kv_q4_evict_scratch_floats(...) floats, 16-byte aligned, contents need not be kept; calls that may run at the same time need one each. */
 size_t wick_rocm_kv_q4_evict_scratch_floats(uint32_t seq_len, uint32_t n_kv_heads);
 int wick_rocm_kv_q4_evict(wick_rocm_ctx *ctx, void *d_k_cache, void *d_v_cache, float *d_weights, uint32_t *d_kept, float *d_scratch, uint32_t seq_len,
                           uint32_t n_keep, uint32_t n_recent, uint32_t n_drop, uint32_t max_seq, uint32_t n_kv_heads, uint32_t head_dim);

@@ -94,6 +94,7 @@ int main() {
         {"keys off", kArg, [&](Call& a) { a.k = off(a.k, 4); }},
         {"values off", kArg, [&](Call& a) { a.v = off(a.v, 8); }},
         {"cache off", kArg, [&](Call& a) { a.v_cache = off(a.v_cache, 8); }},
+        {"one cache", kArg, [](Call& a) { a.v_cache = a.k_cache; }},
         {"rows past the end", kArg, [](Call& a) { a.row = 61; }},
         {"rows past 2^32", kArg, [](Call& a) { a.row = 4294967295u; }},
         {"more rows than there are", kArg, [](Call& a) { a.n = 65; }},
@@ -121,6 +122,7 @@ int main() {
         {"value cache off", kArg, [&](Call& a) { a.v_cache = off(a.v_cache, 8); }},
         {"scratch off", kArg, [&](Call& a) { a.scratch = off(a.scratch, 4); }},
         {"weights off", kArg, [&](Call& a) { a.weights = off(a.weights, 2); }},
+        {"weights and the output over the queries", kArg, [](Call& a) { a.q = a.out; }},
     });
     auto one = attention, many = attention;
     one.push_back({"rows past the end", kArg, [](Call& a) { a.seq = 65; }});
@@ -147,6 +149,8 @@ int main() {
         {"cache off", kArg, [&](Call& a) { a.k_cache = off(a.k_cache, 4); }},
         {"weights off", kArg, [&](Call& a) { a.weights = off(a.weights, 1); }},
         {"rows off", kArg, [&](Call& a) { a.kept = off(a.kept, 2); }},
+        {"no scratch", kArg, [](Call& a) { a.scratch = nullptr; }},
+        {"scratch off", kArg, [&](Call& a) { a.scratch = off(a.scratch, 8); }},
     }));
     // what needs no launch
     Call none = good;
@@ -167,6 +171,8 @@ int main() {
                     most = floats;
                 }
             }
+    // a token's state of every head, however many
+    if (wick_rocm_attention_q4_scratch_floats(1, 2, 66000, 33000, 32, 1) < (size_t)66000 * (32 + 4 + 2 + 2)) failures++, std::printf("scratch of 66000 heads\n");
     for (void* p : d) wick_rocm_buffer_free(ctx, p);
     wick_rocm_ctx_destroy(ctx);
     return failures ? 1 : 0;

@@ -118,7 +118,7 @@ DECODE = [  # head_dim, heads, KV heads, rows in use, rows
     (64, 16, 8, 1, 64), (64, 16, 8, 2, 64), (64, 16, 8, 31, 256), (64, 32, 8, 64, 64), (64, 16, 8, 65, 4096), (64, 8, 8, 257, 300),
     (64, 24, 3, 1000, 1001), (64, 16, 8, 4097, 8192), (64, 64, 1, 700, 700), (64, 5, 5, 2049, 40000), (64, 34, 2, 300, 512),
     (32, 4, 2, 77, 100), (32, 8, 1, 5000, 5000), (128, 8, 2, 129, 4096), (128, 32, 8, 3001, 3001), (256, 4, 1, 33, 64), (256, 6, 2, 2500, 2600),
-    (32, 80, 1, 170000, 180000),
+    (32, 80, 1, 170000, 180000), (32, 66000, 33000, 2, 2),
 ]
 
 

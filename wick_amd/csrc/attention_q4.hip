@@ -1072,10 +1072,11 @@ hipError_t launch_head_dim(const Q4AttentionArgs& a, float* d_scores, const Laun
     return launch_kernel(L, kFamOther, attention_q4_add_weights_kernel, dim3((uint32_t)((seen + 255u) / 256u), a.n_kv_heads), dim3(256), a, (const float*)d_scores, shares, stride);
 }
 
-// Floats of the splits' records: what a split launch has at most, for any number of tokens up to n.
+// Floats of the splits' records: what a split launch has at most, for any number of tokens up to n, and a token's that gathers weights (which leaves its
+// only split as one, however many its heads).
 size_t part_floats(uint32_t n, uint32_t n_heads, uint32_t head_dim) {
     const size_t rows = (size_t)n * n_heads, most = (size_t)kSplitSlots * kMostRows;
-    return (rows * kMaxSplits < most ? rows * kMaxSplits : most) * (head_dim + 4u);
+    return std::max(std::min(rows * kMaxSplits, most), (size_t)n_heads) * (head_dim + 4u);
 }
 
 }  // namespace

@@ -177,6 +177,7 @@ int wick_rocm_kv_q4_append(wick_rocm_ctx* ctx, const float* d_k, const float* d_
         return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, "kv_q4_append: kv_stride must cover n_kv_heads * head_dim and be a multiple of 4");
     if (misaligned(d_k, 16) || misaligned(d_v, 16) || misaligned(d_k_cache, 16) || misaligned(d_v_cache, 16))
         return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_q4_append: keys, values and caches must be 16-byte aligned");
+    if (d_k_cache == d_v_cache) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_q4_append: keys and values are one cache");
     if (n > max_seq || (!d_row && (uint64_t)row + n > max_seq)) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_q4_append: rows beyond the cache");
     hipError_t e = launch_kv_q4_append(d_k, d_v, kv_stride, d_k_cache, d_v_cache, row, d_row, n, max_seq, n_kv_heads, head_dim, ctx->launch());
     return e == hipSuccess ? WICK_ROCM_OK : fail_hip(ctx, e, "kv_q4_append launch");
@@ -214,6 +215,7 @@ static int attention_q4(wick_rocm_ctx* ctx, const float* d_q, uint32_t q_stride,
         return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "attention_q4: null device pointer");
     if (misaligned(d_q, 16) || misaligned(d_k_cache, 16) || misaligned(d_v_cache, 16) || misaligned(d_out, 16) || misaligned(d_scratch, 16) || misaligned(d_weights, 4))
         return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "attention_q4: q, caches, output and scratch must be 16-byte aligned");
+    if (d_weights && d_out == d_q) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "attention_q4: the queries are read again for the weights, the output must not replace them");
     const float scale = 1.0f / sqrtf((float)head_dim);  // wick/src/model/lfm2.rs:862
     hipError_t e = launch_attention_q4(d_q, q_stride, d_k_cache, d_v_cache, d_out, out_stride, d_weights, d_scratch, pos0, d_pos, n, max_seq, n_heads,
                                        n_kv_heads, head_dim, scale, ctx->launch());
