@@ -299,7 +299,7 @@ def test_heads_past_four_gigabytes(ctx, ops, dev):
 EVICT = [  # head_dim, KV heads, rows in use, rows, kept first, kept last, dropped
     (64, 8, 300, 400, 4, 32, 100), (64, 2, 1, 1, 0, 0, 1), (64, 1, 50, 50, 0, 0, 50), (64, 3, 50, 64, 10, 39, 1), (64, 8, 3000, 3000, 64, 256, 800),
     (32, 2, 1025, 1100, 0, 0, 1), (32, 1, 2500, 2500, 1, 1, 2498), (128, 2, 1024, 1024, 7, 100, 333), (256, 1, 700, 701, 0, 650, 50), (256, 2, 1500, 1600, 1400, 0, 60),
-    (64, 1, 9000, 9000, 4, 1000, 5), (32, 1, 40000, 40000, 0, 0, 20000),
+    (64, 1, 9000, 9000, 4, 1000, 5), (32, 1, 40000, 40000, 0, 0, 20000), (32, 2, 150000, 150001, 5, 77, 60000), (128, 1, 4096, 4096, 0, 0, 4096), (64, 1, 4097, 5000, 4090, 0, 7),
 ]
 
 
@@ -368,6 +368,100 @@ def test_a_captured_step_replayed_while_the_position_moves(ctx, ops, dev):
         total[:, :pos + 1] += R.gathered(p, n_kv)
         assert_f32_parity(d_out.download(np.float32, heads * hd).reshape(heads, hd), ref[0], f"step {s}")
         assert_f32_parity(d_w.download(np.float32, n_kv * max_seq).reshape(n_kv, -1), total, f"weights of step {s}")
+    ctx.graph_destroy(g)
+
+
+def random_cache(rng, max_seq, n_kv, hd):
+    c = R.Cache(max_seq, n_kv, hd)
+    c.raw[:] = rng.integers(0, 256, c.raw.size, np.uint8)
+    return c
+
+
+def assert_evicted(got, before, w, d_w, d_kept, seq, keep, recent, drop):
+    """Caches (device) and weights behind an eviction from `before` (host) by weights w."""
+    n_kv, left = w.shape[0], seq - drop
+    kept = d_kept.download(np.uint32, n_kv * left).reshape(n_kv, left)
+    w_after = w.copy()
+    for c in range(n_kv):
+        assert np.array_equal(kept[c], R.evicted(w[c], seq, keep, recent, drop))
+        w_after[c, :left], w_after[c, left:seq] = w[c, kept[c]], 0
+        for cache in before:
+            cache.words[c, :left], cache.scales[c, :left] = cache.words[c, kept[c]], cache.scales[c, kept[c]]
+    assert np.array_equal(back(d_w, w), w_after)
+    for cache, d in zip(before, got):
+        assert np.array_equal(back(d, cache.raw), cache.raw)
+
+
+@pytest.mark.parametrize("hd,n_kv,seq,drop", [(64, 3, 9000, 2500), (256, 1, 3000, 700), (32, 2, 4097, 4000)])
+def test_a_captured_eviction_replayed(ctx, ops, dev, hd, n_kv, seq, drop):
+    """Its counters and histograms are as it needs them in every replay, with other evictions over the same scratch between."""
+    rng, max_seq, keep, recent = np.random.default_rng(seq), seq + 30, 8, 64
+    small = kv_q4_evict_scratch_floats(500, n_kv)
+    scratch = dev(np.full(max(small, kv_q4_evict_scratch_floats(seq, n_kv)), np.nan, np.float32))
+    d_caches, d_w = [dev(random_cache(rng, max_seq, n_kv, hd).raw) for _ in range(2)], dev(np.zeros((n_kv, max_seq), np.float32))
+    d_kept = dev(np.zeros((n_kv, seq), np.uint32))
+    ctx.sync()
+    ctx.graph_begin()
+    ops.encode_kv_q4_evict(*d_caches, d_w, d_kept, scratch, seq, keep, recent, drop, max_seq, n_kv, hd)
+    g = ctx.graph_end()
+    for _ in range(4):
+        caches, w = [random_cache(rng, max_seq, n_kv, hd) for _ in range(2)], rng.exponential(size=(n_kv, max_seq)).astype(np.float32)
+        for d, c in zip([*d_caches, d_w], [*(c.raw for c in caches), w]):
+            d.upload(c)
+        ctx.graph_launch(g)
+        assert_evicted(d_caches, caches, w, d_w, d_kept, seq, keep, recent, drop)
+        w = back(d_w, w)
+        ops.encode_kv_q4_evict(*d_caches, d_w, d_kept, scratch, 500, 3, 0, 120, max_seq, n_kv, hd)  # eager, between replays
+        assert_evicted(d_caches, caches, w, d_w, d_kept, 500, 3, 0, 120)
+    ctx.graph_destroy(g)
+
+
+def test_two_evictions_at_once(ctx, ops, dev):
+    """Two streams, each with caches and a scratch of its own."""
+    rng, other = np.random.default_rng(1), W.RocmContext(0)
+    hd, n_kv, seq, keep, recent, drop = 128, 4, 20000, 4, 100, 6000
+    try:
+        calls = []
+        for o in (ops, Lfm2Ops(other)):
+            caches, w = [random_cache(rng, seq, n_kv, hd) for _ in range(2)], rng.exponential(size=(n_kv, seq)).astype(np.float32)
+            calls.append((o, caches, w, [dev(c.raw) for c in caches], dev(w), dev(np.zeros((n_kv, seq), np.uint32)), dev(np.zeros(kv_q4_evict_scratch_floats(seq, n_kv), np.float32))))
+        ctx.sync()
+        for o, _, _, d_caches, d_w, d_kept, scratch in calls:
+            o.encode_kv_q4_evict(*d_caches, d_w, d_kept, scratch, seq, keep, recent, drop, seq, n_kv, hd)
+        other.sync()
+        for _, caches, w, d_caches, d_w, d_kept, _ in calls:
+            assert_evicted(d_caches, caches, w, d_w, d_kept, seq, keep, recent, drop)
+    finally:
+        other.close()
+
+
+@pytest.mark.parametrize("hd,heads,n_kv,n,pos0", [(64, 16, 4, 900, 700), (64, 16, 8, 70, 300), (128, 8, 2, 5, 4000)])
+def test_a_captured_prompt_replayed(ctx, ops, dev, hd, heads, n_kv, n, pos0):
+    """Bit for bit the eager call's output and weights, with other prompts over the same scratch between."""
+    max_seq = pos0 + n
+    k, v = filled(3, max_seq, n_kv, hd, max_seq)
+    d_q, d_k, d_v, q = dev(np.zeros((n, heads * hd), np.float32)), dev(k.raw), dev(v.raw), normal(4, 3, n, heads * hd)
+    scratch, d_out, d_w = scratch_for(ctx, dev, n, max_seq, heads, n_kv, hd, True), dev(np.zeros((n, heads * hd), np.float32)), dev(np.zeros((n_kv, max_seq), np.float32))
+
+    def call(of):
+        ops.encode_attention_prefill_q4(d_q, heads * hd, d_k, d_v, d_out, heads * hd, scratch, pos0, of, max_seq, heads, n_kv, hd, weights=d_w)
+
+    def results():
+        return d_out.download(np.uint32, n * heads * hd), d_w.download(np.uint32, n_kv * max_seq)
+
+    ctx.sync()
+    ctx.graph_begin()
+    call(n)
+    g = ctx.graph_end()
+    for x in q:
+        d_q.upload(x)
+        got = []
+        for run in (lambda: call(n), lambda: ctx.graph_launch(g), lambda: ctx.graph_launch(g)):
+            d_w.upload(np.full((n_kv, max_seq), 0.25, np.float32))
+            run()
+            got.append(results())
+            call(max(n // 3, 1))
+        assert all(np.array_equal(a, b) for other in got[1:] for a, b in zip(got[0], other))
     ctx.graph_destroy(g)
 
 
