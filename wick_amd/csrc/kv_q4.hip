@@ -92,7 +92,7 @@ struct Q4EvictArgs {
     void* cache[2];
     float* weights;
     uint32_t* kept;   // [n_kv_heads][seq_len - n_drop]
-    uint32_t* hists;    // of more than kSelectChunk rows: [2][n_kv_heads][parts][kBins]
+    uint32_t* hists;    // of more than kSelectLargest rows: [2][n_kv_heads][parts][kBins]
     SelectRecord* records;  // [n_kv_heads][parts]
     uint32_t* state;    // [2 n_kv_heads]: segments taken, and a line behind it which of `segments` are in registers
     uint32_t segments;  // of rows that stay
@@ -134,40 +134,42 @@ __device__ __forceinline__ uint32_t sum_before(uint32_t v, uint32_t* slots, uint
 // histogram of those bits among the keys that share the bits found so far (11 bits are the exponent and two bits behind it: weights spread over
 // many bins, so that a wave's additions seldom meet).  Of those that have just this key the lower rows leave, as many as are still to go.  A wave's 64
 // consecutive rows are one vote: a row's place is the rows that stay in the votes before, which are added up over the workgroup, and those in front of it in its own.
-// Up to 4096 rows: one workgroup a head, which reads them once; bound by the latency of some 20 barriers and as many trips to LDS (3000 rows of 8 heads 6.4 us).
+// Up to 16384 rows: one workgroup a head, which reads them once; bound by the latency of some 15 barriers and as many trips to LDS, and with more rows by
+// its CU's instructions (8 heads of 3000 rows 6.5 us, 8000 10.4, 16000 14.4; of 32768, 28).
 // More: the head in parts of a workgroup each, a launch to each digit and one to place the rows, every one of which begins with adding up the parts'
-// histograms of the launch before (32768 rows of 8 heads 4.0 + 5.2 + 5.4 + 6.1 us, each bound by the same latencies; by one workgroup a head 28 us, and more
-// with every row).
-constexpr uint32_t kSelectRows = 4, kSelectChunk = kSelectRows * kEvictThreads, kVotes = kSelectRows * kEvictWaves;  // rows of a thread, of a workgroup at a time
-constexpr uint32_t kBins = 2048, kMaxParts = 32;
+// histograms of the launch before (32768 rows of 8 heads 4.0 + 5.2 + 5.4 + 6.1 us, 8000 rows 3.4 + 4.9 + 5.1 + 5.9: each bound by the same latencies).
+constexpr uint32_t kPartRows = 4, kPartChunk = kPartRows * kEvictThreads;  // rows of a thread and of a part's workgroup at a time
+constexpr uint32_t kBins = 2048, kMaxParts = 32, kSelectLargest = 16 * kEvictThreads;
 
 __host__ __device__ inline uint32_t select_parts(uint32_t seq_len) {
-    const uint32_t chunks = (seq_len + kSelectChunk - 1u) / kSelectChunk;
+    const uint32_t chunks = (seq_len + kPartChunk - 1u) / kPartChunk;
     return chunks < kMaxParts ? chunks : kMaxParts;
 }
 
 constexpr uint32_t digit_shift(int digit) { return digit == 0 ? 21u : digit == 1 ? 10u : 0u; }
 
+template <uint32_t ROWS>
 struct SelectShared {
-    uint32_t hist[kBins + 64], slots[3][kEvictWaves], votes[2][kVotes], found[2];
+    uint32_t hist[kBins + 64], slots[3][kEvictWaves], votes[2][ROWS * kEvictWaves], found[2];
 };
 
+template <uint32_t ROWS>
 struct SelectKeys {
-    uint32_t k[kSelectRows], candidates;  // bit i: row i of this thread may leave
+    uint32_t k[ROWS], candidates;  // bit i: row i of this thread may leave
     // (a read behind the last row gives 0, for nobody)
     __device__ __forceinline__ void load(const Q4EvictArgs& a, uint32_t c, uint32_t base) {
         const auto w = __builtin_amdgcn_make_buffer_rsrc(a.weights + (size_t)c * a.max_seq, 0, (int)(4u * a.seq_len), 0x27000);
         const uint32_t first = base + threadIdx.x - a.n_keep, n = a.seq_len - a.n_recent - a.n_keep;
 #pragma unroll
-        for (uint32_t i = 0; i < kSelectRows; i++) k[i] = __builtin_amdgcn_raw_buffer_load_b32(w, 4u * (base + i * kEvictThreads + threadIdx.x), 0, 0);
+        for (uint32_t i = 0; i < ROWS; i++) k[i] = __builtin_amdgcn_raw_buffer_load_b32(w, 4u * (base + i * kEvictThreads + threadIdx.x), 0, 0);
         candidates = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < kSelectRows; i++) candidates |= (uint32_t)(first + i * kEvictThreads < n) << i, k[i] = weight_key(__uint_as_float(k[i]));
+        for (uint32_t i = 0; i < ROWS; i++) candidates |= (uint32_t)(first + i * kEvictThreads < n) << i, k[i] = weight_key(__uint_as_float(k[i]));
     }
     __device__ __forceinline__ void count(uint32_t* hist, int digit, uint32_t prefix) const {
         const uint32_t shift = digit_shift(digit), mask = digit == 2 ? 1023u : 2047u, above = digit == 1 ? 21u : 10u, lane = threadIdx.x & 63u;
 #pragma unroll
-        for (uint32_t i = 0; i < kSelectRows; i++) {
+        for (uint32_t i = 0; i < ROWS; i++) {
             // What does not count goes to a bin of its lane's own (no branch, no two at one address), and so do the lanes that meet the first one: it
             // adds for all of them (rows that are new have no weight at all).
             const bool counts = (candidates >> i & 1u) && (digit == 0 || k[i] >> above == prefix >> above);
@@ -179,64 +181,73 @@ struct SelectKeys {
 };
 
 // The bin that the left-th key is in, this thread having the counts of bins 2 tid and 2 tid + 1; `left` becomes how many of that bin's leave.
-__device__ __forceinline__ uint32_t find_bin(SelectShared& s, uint32_t h0, uint32_t h1, uint32_t* slots, uint32_t& left) {
+__device__ __forceinline__ uint32_t find_bin(uint32_t* found, uint32_t h0, uint32_t h1, uint32_t* slots, uint32_t& left) {
     uint32_t all;
     const uint32_t before = sum_before(h0 + h1, slots, all);
     if (before < left && left <= before + h0 + h1) {  // one thread's (left is at least one and at most how many there are)
         const bool second = left > before + h0;
-        s.found[0] = 2u * threadIdx.x + second, s.found[1] = before + (second ? h0 : 0u);
+        found[0] = 2u * threadIdx.x + second, found[1] = before + (second ? h0 : 0u);
     }
     __syncthreads();
-    const uint32_t bin = s.found[0];
-    left -= s.found[1];
+    const uint32_t bin = found[0];
+    left -= found[1];
     __syncthreads();  // (found is written again)
     return bin;
 }
 
-// Bit i of every thread is row i's vote: how many have been given before this wave's, in lane 16 i + its number (and `before` in all: those of earlier chunks).
+// Bit i of every thread is row i's vote: how many have been given before this wave's, in lane (16 i + its number) / kEach (and `before` in all: those of earlier chunks).
+template <uint32_t ROWS>
 __device__ __forceinline__ uint32_t count_votes(uint32_t* votes, uint32_t bits, uint32_t& before) {
-    static_assert(kVotes == 64 && kEvictWaves == 16, "one lane a vote");
+    constexpr uint32_t kEach = ROWS * kEvictWaves / 64u;  // votes of a lane
+    static_assert(kEvictWaves == 16 && kEach >= 1 && kEach <= 16, "a row's votes are those of whole lanes");
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     uint32_t counts = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < kSelectRows; i++) {
+    for (uint32_t i = 0; i < ROWS; i++) {
         const uint32_t n = (uint32_t)__popcll(__ballot(bits >> i & 1u));
         counts = lane == i ? n : counts;
     }
-    if (lane < kSelectRows) votes[lane * kEvictWaves + wave] = counts;
+    if (lane < ROWS) votes[lane * kEvictWaves + wave] = counts;
     __syncthreads();
-    const uint32_t n = votes[lane], sum = wave_scan(n), at = sum - n + before;
-    before += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+    uint32_t n[kEach], sum = 0, at = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < kEach; j++) n[j] = votes[lane * kEach + j], sum += n[j];
+    const uint32_t scan = wave_scan(sum);
+    uint32_t front = scan - sum + before;
+#pragma unroll
+    for (uint32_t j = 0; j < kEach; j++) at = wave % kEach == j ? front : at, front += n[j];  // (of this wave's among a lane's)
+    before += (uint32_t)__builtin_amdgcn_readlane((int)scan, 63);
     return at;
 }
 
 // Of a chunk, the rows whose keys are larger than `key` stay, and of those equal to it all but the first `left` of the head (equal_before: how many there are
 // in front of the chunk; stay_before: rows that stay in front of it).
-__device__ __forceinline__ void place(SelectShared& s, const Q4EvictArgs& a, uint32_t c, const SelectKeys& keys, uint32_t base, uint32_t key, uint32_t left,
+template <uint32_t ROWS>
+__device__ __forceinline__ void place(SelectShared<ROWS>& s, const Q4EvictArgs& a, uint32_t c, const SelectKeys<ROWS>& keys, uint32_t base, uint32_t key, uint32_t left,
                                       uint32_t& equal_before, uint32_t& stay_before) {
     const uint32_t tid = threadIdx.x;
     const uint64_t in_front = (1ull << (tid & 63u)) - 1ull;
     uint32_t* const kept = a.kept + (size_t)c * (a.seq_len - a.n_drop);
     uint32_t equal = 0, stays = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < kSelectRows; i++) {
+    for (uint32_t i = 0; i < ROWS; i++) {
         equal |= (keys.candidates >> i & (uint32_t)(keys.k[i] == key)) << i;
         stays |= (uint32_t)(base + i * kEvictThreads + tid < a.seq_len && (!(keys.candidates >> i & 1u) || keys.k[i] > key)) << i;
     }
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
-    uint32_t at = count_votes(s.votes[0], equal, equal_before);
+    uint32_t at = count_votes<ROWS>(s.votes[0], equal, equal_before);
     if (__ballot(equal != 0) != 0) {  // (few waves)
 #pragma unroll
-        for (uint32_t i = 0; i < kSelectRows; i++) {
-            const uint32_t rank = (uint32_t)__builtin_amdgcn_readlane((int)at, (int)(kEvictWaves * i + wave)) + (uint32_t)__popcll(__ballot(equal >> i & 1u) & in_front);
+        for (uint32_t i = 0; i < ROWS; i++) {
+            const uint32_t rank = (uint32_t)__builtin_amdgcn_readlane((int)at, (int)(4u * kEvictWaves / ROWS * i + wave * 4u / ROWS)) + (uint32_t)__popcll(__ballot(equal >> i & 1u) & in_front);
             stays |= (equal >> i & (uint32_t)(rank >= left)) << i;
         }
     }
-    at = count_votes(s.votes[1], stays, stay_before);
+    at = count_votes<ROWS>(s.votes[1], stays, stay_before);
 #pragma unroll
-    for (uint32_t i = 0; i < kSelectRows; i++) {
+    for (uint32_t i = 0; i < ROWS; i++) {
         const uint64_t vote = __ballot(stays >> i & 1u);
-        const uint32_t to = (uint32_t)__builtin_amdgcn_readlane((int)at, (int)(kEvictWaves * i + wave)) + (uint32_t)__popcll(vote & in_front);
+        const uint32_t to = (uint32_t)__builtin_amdgcn_readlane((int)at, (int)(4u * kEvictWaves / ROWS * i + wave * 4u / ROWS)) + (uint32_t)__popcll(vote & in_front);
         if (stays >> i & 1u) kept[to] = base + i * kEvictThreads + tid;
     }
 }
@@ -246,11 +257,12 @@ __device__ __forceinline__ void clear_move_state(const Q4EvictArgs& a, uint32_t 
     for (uint32_t i = threadIdx.x; i < n; i += kEvictThreads) a.state[(size_t)c * n + i] = 0u;
 }
 
+template <uint32_t ROWS>
 __global__ __launch_bounds__(kEvictThreads) void kv_q4_select_kernel(Q4EvictArgs a) {
-    __shared__ SelectShared s;
+    __shared__ SelectShared<ROWS> s;
     const uint32_t c = blockIdx.x, tid = threadIdx.x;
     clear_move_state(a, c);
-    SelectKeys keys;
+    SelectKeys<ROWS> keys;
     keys.load(a, c, 0);
     uint32_t prefix = 0, left = a.n_drop;  // bits found so far; how many of the keys that share them leave
 #pragma unroll
@@ -259,7 +271,7 @@ __global__ __launch_bounds__(kEvictThreads) void kv_q4_select_kernel(Q4EvictArgs
         __syncthreads();
         keys.count(s.hist, digit, prefix);
         __syncthreads();
-        prefix |= find_bin(s, s.hist[2u * tid], s.hist[2u * tid + 1u], s.slots[digit], left) << digit_shift(digit);
+        prefix |= find_bin(s.found, s.hist[2u * tid], s.hist[2u * tid + 1u], s.slots[digit], left) << digit_shift(digit);
     }
     uint32_t equal_before = 0, stay_before = 0;
     place(s, a, c, keys, 0, prefix, left, equal_before, stay_before);
@@ -268,13 +280,13 @@ __global__ __launch_bounds__(kEvictThreads) void kv_q4_select_kernel(Q4EvictArgs
 // STEP 0 .. 2: a part's histogram of that digit; 3: its rows placed.  What a part knows goes from launch to launch in a record of its own.
 template <int STEP>
 __global__ __launch_bounds__(kEvictThreads) void kv_q4_select_part_kernel(Q4EvictArgs a) {
-    __shared__ SelectShared s;
+    __shared__ SelectShared<kPartRows> s;
     const uint32_t parts = gridDim.x, part = blockIdx.x, c = blockIdx.y, tid = threadIdx.x;
-    const uint32_t chunks = (a.seq_len + kSelectChunk - 1u) / kSelectChunk, chunk0 = (uint32_t)((uint64_t)chunks * part / parts), chunk_end = (uint32_t)((uint64_t)chunks * (part + 1u) / parts);
+    const uint32_t chunks = (a.seq_len + kPartChunk - 1u) / kPartChunk, chunk0 = (uint32_t)((uint64_t)chunks * part / parts), chunk_end = (uint32_t)((uint64_t)chunks * (part + 1u) / parts);
     const auto hist_of = [&](int step, uint32_t p) { return reinterpret_cast<uint2*>(a.hists + ((size_t)(step & 1) * a.n_kv_heads * parts + (size_t)c * parts + p) * kBins); };
     SelectRecord& record = a.records[(size_t)c * parts + part];
-    SelectKeys keys;
-    keys.load(a, c, chunk0 * kSelectChunk);
+    SelectKeys<kPartRows> keys;
+    keys.load(a, c, chunk0 * kPartChunk);
     uint32_t prefix = 0, left = a.n_drop, smaller_before = 0, equal_before = 0;
     if constexpr (STEP == 0) {
         if (part == 0) clear_move_state(a, c);
@@ -292,7 +304,7 @@ __global__ __launch_bounds__(kEvictThreads) void kv_q4_select_part_kernel(Q4Evic
                 if (p < part) before.x += h[i].x, before.y += h[i].y;
             }
         }
-        const uint32_t bin = find_bin(s, sum.x, sum.y, s.slots[0], left);
+        const uint32_t bin = find_bin(s.found, sum.x, sum.y, s.slots[0], left);
         prefix |= bin << digit_shift(STEP - 1);
         uint32_t smaller;
         (void)sum_before((2u * tid < bin ? before.x : 0u) + (2u * tid + 1u < bin ? before.y : 0u), s.slots[1], smaller);
@@ -306,16 +318,16 @@ __global__ __launch_bounds__(kEvictThreads) void kv_q4_select_part_kernel(Q4Evic
         for (uint32_t i = chunk0;;) {
             keys.count(s.hist, STEP, prefix);
             if (++i >= chunk_end) break;
-            keys.load(a, c, i * kSelectChunk);
+            keys.load(a, c, i * kPartChunk);
         }
         __syncthreads();
         hist_of(STEP, part)[tid] = make_uint2(s.hist[2u * tid], s.hist[2u * tid + 1u]);
     } else {
-        uint32_t stay_before = chunk0 * kSelectChunk - smaller_before - min(equal_before, left);
+        uint32_t stay_before = chunk0 * kPartChunk - smaller_before - min(equal_before, left);
         for (uint32_t i = chunk0;;) {
-            place(s, a, c, keys, i * kSelectChunk, prefix, left, equal_before, stay_before);
+            place(s, a, c, keys, i * kPartChunk, prefix, left, equal_before, stay_before);
             if (++i >= chunk_end) break;
-            keys.load(a, c, i * kSelectChunk);
+            keys.load(a, c, i * kPartChunk);
         }
     }
 }
@@ -433,9 +445,9 @@ hipError_t launch_kv_q4_read(const void* d_cache, float* d_out, uint32_t out_str
 }
 
 // Histograms, records, state of the move.
-static size_t evict_hist_words(uint32_t seq_len, uint32_t n_kv_heads) { return seq_len <= kSelectChunk ? 0 : 2 * (size_t)n_kv_heads * select_parts(seq_len) * kBins; }
+static size_t evict_hist_words(uint32_t seq_len, uint32_t n_kv_heads) { return seq_len <= kSelectLargest ? 0 : 2 * (size_t)n_kv_heads * select_parts(seq_len) * kBins; }
 static size_t evict_record_words(uint32_t seq_len, uint32_t n_kv_heads) {
-    return seq_len <= kSelectChunk ? 0 : (size_t)n_kv_heads * select_parts(seq_len) * (sizeof(SelectRecord) / 4);
+    return seq_len <= kSelectLargest ? 0 : (size_t)n_kv_heads * select_parts(seq_len) * (sizeof(SelectRecord) / 4);
 }
 size_t kv_q4_evict_scratch_floats(uint32_t seq_len, uint32_t n_kv_heads) {
     return evict_hist_words(seq_len, n_kv_heads) + evict_record_words(seq_len, n_kv_heads) +
@@ -450,8 +462,9 @@ hipError_t launch_evict(Q4EvictArgs a, const Launch& L) {
     static_assert(R >= kMoveLeast, "the scratch is sized for it");
     a.segments = (a.seq_len - a.n_drop - a.n_keep + R - 1u) / R;
     hipError_t e = hipSuccess;
-    if (a.seq_len <= kSelectChunk) {
-        e = launch_kernel(L, kFamOther, kv_q4_select_kernel, dim3(a.n_kv_heads), dim3(kEvictThreads), a);
+    if (a.seq_len <= kSelectLargest) {
+        const auto select = a.seq_len <= 4u * kEvictThreads ? kv_q4_select_kernel<4> : a.seq_len <= 8u * kEvictThreads ? kv_q4_select_kernel<8> : kv_q4_select_kernel<16>;
+        e = launch_kernel(L, kFamOther, select, dim3(a.n_kv_heads), dim3(kEvictThreads), a);
     } else {
         for (const auto step : {kv_q4_select_part_kernel<0>, kv_q4_select_part_kernel<1>, kv_q4_select_part_kernel<2>, kv_q4_select_part_kernel<3>})
             if (e == hipSuccess) e = launch_kernel(L, kFamOther, step, dim3(select_parts(a.seq_len), a.n_kv_heads), dim3(kEvictThreads), a);
