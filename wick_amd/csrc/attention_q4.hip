@@ -871,13 +871,20 @@ __global__ __launch_bounds__(256) void attention_q4_finish_kernel(FewArgs args) 
 // All sums in one order.  Bound by vector instructions (exponentials, and the queries' split: a block is split in every workgroup that sees it) and, for few
 // rows, by latency: 555 tokens of 16 heads over 8 of 64 7.4 and 4.5 us for the addition, 1500 of 32 heads 26, 4000 of them 138, 500 of 16 over 4 of 128 9.5 (keys
 // in LDS, the queries split by every wave for itself: 12.7, 54, 257 and 37).  128 keys a workgroup: with 256 and eight waves behind one barrier 9.9, 38, 190 and 17.
+struct WeightArgs {
+    Q4AttentionArgs at;
+    float* sums;  // [shares][n_kv_heads][stride], unless there is one share
+    uint32_t shares, stride;
+};
 constexpr uint32_t kWeightKeys = 128, kMaxShares = 16;
 template <int HD>
 constexpr uint32_t kWeightSlots = kCus * (HD <= 64 ? 4 : HD == 128 ? 3 : 2);  // workgroups that the GPU has at once
 constexpr uint32_t kWeightSums = 4 * kCus * kWeightKeys;  // that the shares of a launch leave at most: no more workgroups than those
 
 template <int HD>
-__global__ __launch_bounds__(256, kWeightSlots<HD> / kCus) void attention_q4_weights_kernel(Q4AttentionArgs a, float* sums, uint32_t shares, uint32_t stride) {
+__global__ __launch_bounds__(256, kWeightSlots<HD> / kCus) void attention_q4_weights_kernel(WeightArgs args) {
+    const Q4AttentionArgs& a = args.at;
+    const uint32_t shares = args.shares;
     constexpr int SLABS = HD / 16, V = HD / 32;  // four values, of a thread's share of a query row
     struct Block {
         _Float16 q[2][32][HD + 8];
@@ -985,7 +992,7 @@ __global__ __launch_bounds__(256, kWeightSlots<HD> / kCus) void attention_q4_wei
             add(b + 1u, blocks[1], blocks[0]);
         }
     }
-    float* const to = shares == 1u ? a.weights + (size_t)c * a.max_seq : sums + (size_t)(share * a.n_kv_heads + c) * stride;
+    float* const to = shares == 1u ? a.weights + (size_t)c * a.max_seq : args.sums + (size_t)(share * a.n_kv_heads + c) * args.stride;
 #pragma unroll
     for (int e = 0; e < 16; e++) {
         const float w = group_sum<32>(acc[e]);
@@ -996,14 +1003,16 @@ __global__ __launch_bounds__(256, kWeightSlots<HD> / kCus) void attention_q4_wei
         }
     }
 }
-__global__ __launch_bounds__(256) void attention_q4_add_weights_kernel(Q4AttentionArgs a, const float* sums, uint32_t shares, uint32_t stride) {
+__global__ __launch_bounds__(256) void attention_q4_add_weights_kernel(WeightArgs args) {
+    const Q4AttentionArgs& a = args.at;
+    const uint32_t shares = args.shares;
     const uint32_t c = blockIdx.y, t = blockIdx.x * 256u + threadIdx.x, group = a.n_heads / a.n_kv_heads, rows = a.n * group;
     if (t > sees(a, first_row(a), rows - 1u, rows, group)) return;
     float w = 0.0f;
     for (uint32_t i0 = 0; i0 < shares; i0 += 8u) {
         float x[8];
 #pragma unroll
-        for (uint32_t i = 0; i < 8u; i++) x[i] = sums[(size_t)(min(i0 + i, shares - 1u) * a.n_kv_heads + c) * stride + t];
+        for (uint32_t i = 0; i < 8u; i++) x[i] = args.sums[(size_t)(min(i0 + i, shares - 1u) * a.n_kv_heads + c) * args.stride + t];
 #pragma unroll
         for (uint32_t i = 0; i < 8u; i++) w += i0 + i < shares ? x[i] : 0.0f;
     }
@@ -1065,11 +1074,11 @@ hipError_t launch_head_dim(const Q4AttentionArgs& a, float* d_scores, const Laun
         e = launch_tiles<HD, 4, 1, 1>(a, seen, L);
     }
     if (e != hipSuccess || !a.weights) return e;
-    const uint32_t tiles = (uint32_t)((seen + kWeightKeys - 1u) / kWeightKeys), base = a.n_kv_heads * tiles, blocks = (rows + 31u) / 32u, stride = tiles * kWeightKeys;
-    const uint32_t shares = std::min({std::max(kWeightSlots<HD> / base, 1u), kMaxShares, (blocks + 1u) / 2u});
-    e = launch_kernel(L, kFamOther, attention_q4_weights_kernel<HD>, dim3(base * shares), dim3(256), a, d_scores, shares, stride);
-    if (e != hipSuccess || shares == 1u) return e;
-    return launch_kernel(L, kFamOther, attention_q4_add_weights_kernel, dim3((uint32_t)((seen + 255u) / 256u), a.n_kv_heads), dim3(256), a, (const float*)d_scores, shares, stride);
+    const uint32_t tiles = (uint32_t)((seen + kWeightKeys - 1u) / kWeightKeys), base = a.n_kv_heads * tiles, blocks = (rows + 31u) / 32u;
+    const WeightArgs w{a, d_scores, std::min({std::max(kWeightSlots<HD> / base, 1u), kMaxShares, (blocks + 1u) / 2u}), tiles * kWeightKeys};
+    e = launch_kernel(L, kFamOther, attention_q4_weights_kernel<HD>, dim3(base * w.shares), dim3(256), w);
+    if (e != hipSuccess || w.shares == 1u) return e;
+    return launch_kernel(L, kFamOther, attention_q4_add_weights_kernel, dim3((uint32_t)((seen + 255u) / 256u), a.n_kv_heads), dim3(256), w);
 }
 
 // Floats of the splits' records: what a split launch has at most, for any number of tokens up to n, and a token's that gathers weights (which leaves its

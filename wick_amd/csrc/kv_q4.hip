@@ -67,17 +67,21 @@ __global__ __launch_bounds__(256) void kv_q4_append_kernel(Q4AppendArgs a) {
 }
 
 // Rows [row, row + n) as floats, token-major: out[j * stride + c * head_dim + i].
-__global__ __launch_bounds__(256) void kv_q4_read_kernel(const void* p, float* __restrict__ out, uint32_t stride, uint32_t row, uint32_t n, uint32_t max_seq,
-                                                         uint32_t n_kv_heads, uint32_t head_dim) {
-    const uint32_t words = head_dim / 8u;
+struct Q4ReadArgs {
+    void* cache;
+    float* out;
+    uint32_t stride, row, n, max_seq, n_kv_heads, head_dim;
+};
+__global__ __launch_bounds__(256) void kv_q4_read_kernel(Q4ReadArgs a) {
+    const uint32_t words = a.head_dim / 8u;
     const uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x;
-    if (i >= (uint64_t)n_kv_heads * n * words) return;
-    const uint32_t w = (uint32_t)(i % words), j = (uint32_t)(i / words % n), c = (uint32_t)(i / words / n);
-    const Q4Cache cache = q4_planes(const_cast<void*>(p), max_seq, n_kv_heads, head_dim);
-    const size_t from = (size_t)c * max_seq + row + j;
+    if (i >= (uint64_t)a.n_kv_heads * a.n * words) return;
+    const uint32_t w = (uint32_t)(i % words), j = (uint32_t)(i / words % a.n), c = (uint32_t)(i / words / a.n);
+    const Q4Cache cache = q4_planes(a.cache, a.max_seq, a.n_kv_heads, a.head_dim);
+    const size_t from = (size_t)c * a.max_seq + a.row + j;
     const uint32_t q = cache.quants[from * words + w];
     const float d = f16_bits_to_f32(cache.scales[from * (words / 4u) + w / 4u]);
-    float* const to = out + (size_t)j * stride + (size_t)c * head_dim + 8u * w;
+    float* const to = a.out + (size_t)j * a.stride + (size_t)c * a.head_dim + 8u * w;
 #pragma unroll
     for (int e = 0; e < 8; e += 4)
         *reinterpret_cast<float4*>(to + e) = make_float4(q4_value(q, e, d), q4_value(q, e + 1, d), q4_value(q, e + 2, d), q4_value(q, e + 3, d));
@@ -440,8 +444,8 @@ hipError_t launch_kv_q4_read(const void* d_cache, float* d_out, uint32_t out_str
                              uint32_t head_dim, const Launch& L) {
     if (n == 0) return hipSuccess;
     const uint64_t threads = (uint64_t)n_kv_heads * n * (head_dim / 8u);
-    return launch_kernel(L, kFamOther, kv_q4_read_kernel, dim3((uint32_t)((threads + 255) / 256)), dim3(256), d_cache, d_out, out_stride, row, n, max_seq,
-                         n_kv_heads, head_dim);
+    const Q4ReadArgs a{const_cast<void*>(d_cache), d_out, out_stride, row, n, max_seq, n_kv_heads, head_dim};
+    return launch_kernel(L, kFamOther, kv_q4_read_kernel, dim3((uint32_t)((threads + 255) / 256)), dim3(256), a);
 }
 
 // Histograms, records, state of the move.
