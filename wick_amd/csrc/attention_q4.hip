@@ -13,8 +13,8 @@
 // a b = a_hi b_hi + a_hi b_lo + a_lo b_hi: each product of halves is exact, sums are f32's, what is dropped is below 2^-22.
 // (One half for the weights or the queries would be off by 2^-12 of each: 100 times what f32 sums are.)
 // Bound by the matrix and vector instructions of a unit of 32 rows and 32 keys (heads of 64: 24 matrix instructions of 32 cycles and 920 cycles of vector ones, of
-// the softmax above all, in 2060 cycles): 2002 tokens of 32 heads over 8 of 64 60 us, 2048 behind 6144 of 16 heads over 4 of 128 311 us (three products at 1160
-// TFLOP/s; power).
+// the softmax above all, in 2060 cycles): 2002 tokens of 32 heads over 8 of 64 62 us, 2048 behind 6144 of 16 heads over 4 of 128 320 us (three
+// products are 310 at the 1160 TFLOP/s of a large library product; power).
 #include <algorithm>
 
 #include "attention_device.h"
