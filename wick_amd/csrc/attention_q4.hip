@@ -152,6 +152,15 @@ struct Raw {
     uint16_t kd[P], vd[P];
 };
 
+// A wave with `left` of its steps to go yields to those of its SIMD that have more (of `longest` at the most): left to themselves, the oldest wave
+// goes first, and when it has gone the last one's latencies are nobody's to hide.
+__device__ __forceinline__ void yield_to_longer(uint32_t left, uint32_t longest) {
+    if (left > longest / 2u) __builtin_amdgcn_s_setprio(3);
+    else if (left > longest / 4u) __builtin_amdgcn_s_setprio(2);
+    else if (left > longest / 8u) __builtin_amdgcn_s_setprio(1);
+    else __builtin_amdgcn_s_setprio(0);
+}
+
 template <int HD, int WQ, int WK, int PER_CU>
 __global__ __launch_bounds__(64 * WQ * WK, PER_CU * WQ * WK / 4) void attention_q4_kernel(Q4AttentionArgs a) {
     constexpr int KT = 32 * WK, NT = 64 * WQ * WK, SLABS = HD / 16, DT = HD / 32, kWords = KT * HD / 8 / NT, W = kWords < 4 ? kWords : 4, P = kWords / W;
@@ -782,7 +791,9 @@ __global__ __launch_bounds__(64 * kFewWaves, HD == 32 ? 4 : HD <= 128 ? 2 : 1) v
             if (d + 1 < CS) unpack_values(d + 1, 3);
         }
     };
+    const uint32_t mine_in_all = u_end - u_first;
     for (uint32_t unit = u_first; unit < u_end; unit += 2u) {
+        yield_to_longer(u_end - unit, mine_in_all);
         attend(unit, units_ahead[0], units_ahead[1]);
         if (unit + 1u >= u_end) break;
         attend(unit + 1u, units_ahead[1], units_ahead[0]);
