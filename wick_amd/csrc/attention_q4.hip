@@ -1034,6 +1034,7 @@ __global__ __launch_bounds__(256) void attention_q4_add_weights_kernel(WeightArg
 template <int HD, int WQ, int WK, int PER_CU>
 hipError_t launch_tiles(Q4AttentionArgs a, uint64_t seen, const Launch& L) {
     constexpr uint32_t RB = 32 * WQ, KT = 32 * WK;
+    static_assert(PER_CU * kCus <= kSplitSlots && RB <= kMostRows, "the scratch is sized for it");
     const uint32_t rows = a.n * (a.n_heads / a.n_kv_heads), blocks = (rows + RB - 1u) / RB, base = a.n_kv_heads * blocks;
     const uint32_t room = kCus * PER_CU / base, most = (uint32_t)((seen + 3u * KT - 1u) / (3u * KT));
     a.splits = std::min({std::max(room, 1u), most, kMaxSplits});
@@ -1051,6 +1052,7 @@ template <int HD>
 hipError_t launch_few(FewArgs f, uint64_t seen, const Launch& L) {
     const Q4AttentionArgs& a = f.at;
     constexpr uint32_t kSpan = kFewKeys * kFewWaves;
+    static_assert(kFewSlots<HD> * kFewRows <= kSplitSlots * kMostRows, "the scratch is sized for it");
     const uint32_t rows = a.n * (a.n_heads / a.n_kv_heads), base = a.n_kv_heads * ((rows + kFewRows - 1u) / kFewRows);
     f.at.splits = std::min({std::max(kFewSlots<HD> / base, 1u), (uint32_t)((seen + kSpan - 1u) / kSpan), kMaxSplits});
     const hipError_t e = launch_kernel(L, kFamOther, attention_q4_few_kernel<HD>, dim3(base * a.splits), dim3(64 * kFewWaves), f);
