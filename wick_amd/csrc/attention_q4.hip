@@ -153,7 +153,7 @@ struct Raw {
 };
 
 // A wave with `left` of its steps to go yields to those of its SIMD that have more (of `longest` at the most): left to themselves, the oldest wave
-// goes first, and when it has gone the last one's latencies are nobody's to hide.
+// goes first, and when it has gone the last one's latencies are nobody's to hide (128000 rows: first waves done at 26 us, last at 41; so 33 and 40).
 __device__ __forceinline__ void yield_to_longer(uint32_t left, uint32_t longest) {
     if (left > longest / 2u) __builtin_amdgcn_s_setprio(3);
     else if (left > longest / 4u) __builtin_amdgcn_s_setprio(2);
@@ -499,8 +499,8 @@ __global__ __launch_bounds__(256) void attention_q4_merge_kernel(Q4AttentionArgs
 // group g HD / 32 of them from word g HD / 32 on, the order of an MFMA's K steps being free), and of the values one word of eight rows, the rows whose weights it
 // holds: two rows' words are transposed to pairs of one dim's values with one byte permutation each.  Keys are multiplied as nibbles less 8, one exact half, a
 // block's 32 dims at a time, and the block's scale is taken into the sum: two products of halves instead of three.
-// Bound at long context by the loads and the unpacking, which overlap in part: one token of 32 heads over 8 of 128 behind 128000 rows (147 MB) 41 us, its
-// loads alone 26; with values through LDS and both planes of the keys 45.  At short context by two or three round trips to memory: 16 heads over 9000 rows 7.2 us.
+// Bound at long context by the loads and the unpacking, which overlap in part: one token of 32 heads over 8 of 128 behind 128000 rows (147 MB) 38 us, its
+// loads alone 26; with values through LDS and both planes of the keys 45, and 42 before waves yielded (see below).  At short context by two or three round trips to memory: 16 heads over 9000 rows 7.2 us.
 struct FewArgs {
     Q4AttentionArgs at;
     float* scores;  // [n_heads][max_seq], of one token's heads in powers of two, for the weights; may be null
