@@ -152,15 +152,6 @@ struct Raw {
     uint16_t kd[P], vd[P];
 };
 
-// A wave with `left` of its steps to go yields to those of its SIMD that have more (of `longest` at the most): left to themselves, the oldest wave
-// goes first, and when it has gone the last one's latencies are nobody's to hide (128000 rows: first waves done at 26 us, last at 41; so 33 and 40).
-__device__ __forceinline__ void yield_to_longer(uint32_t left, uint32_t longest) {
-    if (left > longest / 2u) __builtin_amdgcn_s_setprio(3);
-    else if (left > longest / 4u) __builtin_amdgcn_s_setprio(2);
-    else if (left > longest / 8u) __builtin_amdgcn_s_setprio(1);
-    else __builtin_amdgcn_s_setprio(0);
-}
-
 template <int HD, int WQ, int WK, int PER_CU>
 __global__ __launch_bounds__(64 * WQ * WK, PER_CU * WQ * WK / 4) void attention_q4_kernel(Q4AttentionArgs a) {
     constexpr int KT = 32 * WK, NT = 64 * WQ * WK, SLABS = HD / 16, DT = HD / 32, kWords = KT * HD / 8 / NT, W = kWords < 4 ? kWords : 4, P = kWords / W;
@@ -508,6 +499,15 @@ struct FewArgs {
 constexpr uint32_t kFewRows = 16, kFewKeys = 32, kFewWaves = 4;
 template <int HD>
 constexpr uint32_t kFewSlots = kCus * (HD <= 128 ? 2 : 1);  // workgroups that the GPU has at once
+
+// A wave with `left` of its steps to go yields to those of its SIMD that have more (of `longest` at the most): left to themselves, the oldest wave
+// goes first, and when it has gone the last one's latencies are nobody's to hide (128000 rows: first waves done at 26 us, last at 41; so 33 and 40).
+__device__ __forceinline__ void yield_to_longer(uint32_t left, uint32_t longest) {
+    if (left > longest / 2u) __builtin_amdgcn_s_setprio(3);
+    else if (left > longest / 4u) __builtin_amdgcn_s_setprio(2);
+    else if (left > longest / 8u) __builtin_amdgcn_s_setprio(1);
+    else __builtin_amdgcn_s_setprio(0);
+}
 
 template <int HD>
 __global__ __launch_bounds__(64 * kFewWaves, HD == 32 ? 4 : HD <= 128 ? 2 : 1) void attention_q4_few_kernel(FewArgs args) {
