@@ -880,7 +880,7 @@ __global__ __launch_bounds__(256) void attention_q4_finish_kernel(FewArgs args) 
 // up over the query rows.  Every wave keeps 32 keys as matrix operands in registers; the workgroup walks query rows in blocks of 32 that it splits into
 // halves once for its four waves, through LDS, the next block's on their way meanwhile.  The rows are shared out among `shares` workgroups, whose sums the next launch adds.
 // All sums in one order.  Bound by vector instructions (exponentials, and the queries' split: a block is split in every workgroup that sees it) and, for few
-// rows, by latency: 555 tokens of 16 heads over 8 of 64 7.4 and 4.5 us for the addition, 1500 of 32 heads 26, 4000 of them 138, 500 of 16 over 4 of 128 9.5 (keys
+// rows, by latency: 555 tokens of 16 heads over 8 of 64 7.6 and 3.0 us for the addition, 1500 of 32 heads 26, 4000 of them 138, 500 of 16 over 4 of 128 9.5 (keys
 // in LDS, the queries split by every wave for itself: 12.7, 54, 257 and 37).  128 keys a workgroup: with 256 and eight waves behind one barrier 9.9, 38, 190 and 17.
 struct WeightArgs {
     Q4AttentionArgs at;
