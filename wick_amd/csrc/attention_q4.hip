@@ -881,7 +881,8 @@ __global__ __launch_bounds__(256) void attention_q4_finish_kernel(FewArgs args) 
 // halves once for its four waves, through LDS, the next block's on their way meanwhile.  The rows are shared out among `shares` workgroups, whose sums the next launch adds.
 // All sums in one order.  Bound by vector instructions (exponentials, and the queries' split: a block is split in every workgroup that sees it) and, for few
 // rows, by latency: 555 tokens of 16 heads over 8 of 64 7.6 and 3.0 us for the addition, 1500 of 32 heads 26, 4000 of them 138, 500 of 16 over 4 of 128 9.5 (keys
-// in LDS, the queries split by every wave for itself: 12.7, 54, 257 and 37).  128 keys a workgroup: with 256 and eight waves behind one barrier 9.9, 38, 190 and 17.
+// in LDS, the queries split by every wave for itself: 12.7, 54, 257 and 37).  128 keys a workgroup: with 256 and eight waves behind one barrier 9.9, 38, 190 and 17.  Workgroups with fewer
+// blocks to go yield (834 tokens behind 3353, 24 heads over 3 of 64: 44.8 -> 41.2).
 struct WeightArgs {
     Q4AttentionArgs at;
     float* sums;  // [shares][n_kv_heads][stride], unless there is one share
@@ -998,6 +999,7 @@ __global__ __launch_bounds__(256, kWeightSlots<HD> / kCus) void attention_q4_wei
             __syncthreads();
         };
         for (uint32_t b = b_first; b < b_end; b += 2u) {
+            yield_to_longer(b_end - b, r_end / shares);
             add(b, blocks[0], blocks[1]);
             if (b + 1u >= b_end) break;
             add(b + 1u, blocks[1], blocks[0]);
