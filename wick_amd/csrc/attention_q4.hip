@@ -1049,9 +1049,11 @@ hipError_t launch_tiles(Q4AttentionArgs a, uint64_t seen, const Launch& L) {
                          : launch_kernel(L, kFamOther, attention_q4_merge_kernel<HD, 1>, dim3((merged + 1024u / HD - 1u) / (1024u / HD)), dim3(256), a, RB, KT);
 }
 
-// Small ones: workgroups of 16 query rows and as many splits as fill the GPU, down to a unit of keys for each wave; but none where walking a few units one
-// behind the other takes less than the merge's launch (us, split and alone: a token of 32 heads over 8 of 64 values over 256 rows 7.0 and 4.6, 512 6.9 and
-// 6.0, 768 7.1 and 7.4; of 128 over 256 7.7 and 6.0, 512 7.7 and 8.3; 40 tokens of 32 heads behind 500 10.2 and 7.4; of 256 over 256 10.3 and 10.8).
+// Small ones: workgroups of 16 query rows and as many splits as fill the GPU, down to a unit of keys for each wave; but none where walking some more units one
+// behind the other takes less than the merge, which takes the longer the more rows there are (us, split and alone, 32 heads over 8; of 64 values: a token over
+// 512 rows 6.9 and 6.0, 768 7.1 and 7.4; 30 tokens behind 900 10.0 and 9.4, 1300 11.3 and 11.6; 60 behind 1300 13.3 and 11.8, 2500 15.8 and 18.4; 120 behind
+// 600 15.3 and 8.2, 2500 24.1 and 19.9; of 128: a token over 256 7.7 and 6.0, 512 7.7 and 8.3; 60 behind 800 15.6 and 13.3, 1800 19.9 and 23.6; of 256: 25 behind
+// 300 13.7 and 14.5).
 template <int HD>
 hipError_t launch_few(FewArgs f, uint64_t seen, const Launch& L) {
     const Q4AttentionArgs& a = f.at;
@@ -1059,8 +1061,8 @@ hipError_t launch_few(FewArgs f, uint64_t seen, const Launch& L) {
     static_assert(kFewSlots<HD> * kFewRows <= kSplitSlots * kMostRows, "the scratch is sized for it");
     const uint32_t rows = a.n * (a.n_heads / a.n_kv_heads), base = a.n_kv_heads * ((rows + kFewRows - 1u) / kFewRows);
     const uint32_t spans = (uint32_t)((seen + kSpan - 1u) / kSpan);
-    constexpr uint32_t kAlone = HD <= 64 ? 5 : HD == 128 ? 3 : 1;
-    f.at.splits = spans <= kAlone && !f.scores ? 1u : std::min({std::max(kFewSlots<HD> / base, 1u), spans, kMaxSplits});
+    const uint32_t alone = HD <= 64 ? std::max(5u, 2u + base / 9u) : HD == 128 ? std::max(3u, 1u + base / 12u) : std::max(1u, base / 24u);
+    f.at.splits = spans <= alone && !f.scores ? 1u : std::min({std::max(kFewSlots<HD> / base, 1u), spans, kMaxSplits});
     const hipError_t e = launch_kernel(L, kFamOther, attention_q4_few_kernel<HD>, dim3(base * a.splits), dim3(64 * kFewWaves), f);
     if (e != hipSuccess) return e;
     if (f.scores) return launch_kernel(L, kFamOther, attention_q4_finish_kernel<HD>, dim3(a.n_heads + a.n_kv_heads * (uint32_t)((seen + 255u) / 256u)), dim3(256), f);
