@@ -1032,6 +1032,16 @@ __global__ __launch_bounds__(256) void attention_q4_add_weights_kernel(WeightArg
     a.weights[(size_t)c * a.max_seq + t] += w;
 }
 
+// Up to `few` splits are merged by HD / 4 lanes a row, more by a workgroup a row (us with what is before it, the second and the first: 60 tokens of 32 heads
+// of 64 values behind 2500 in four splits 15.8 and 14.7, 120 behind 5000 in two 35.2 and 32.3, 30 behind 2500 in eight 12.0 and 12.7).
+template <int HD>
+hipError_t launch_merge(const Q4AttentionArgs& a, uint32_t wg_rows, uint32_t tile, uint32_t few, const Launch& L) {
+    constexpr uint32_t kRows = 1024 / HD;  // of a workgroup, HD / 4 lanes each
+    const uint32_t rows = a.n * a.n_heads;
+    return a.splits > few ? launch_kernel(L, kFamOther, attention_q4_merge_kernel<HD, 1024 / HD>, dim3(rows), dim3(256), a, wg_rows, tile)
+                          : launch_kernel(L, kFamOther, attention_q4_merge_kernel<HD, 1>, dim3((rows + kRows - 1u) / kRows), dim3(256), a, wg_rows, tile);
+}
+
 // Large launches: as many splits as workgroups fit on the GPU, three tiles or more each (a split's state is written and read again).
 template <int HD, int WQ, int WK, int PER_CU>
 hipError_t launch_tiles(Q4AttentionArgs a, uint64_t seen, const Launch& L) {
@@ -1044,9 +1054,7 @@ hipError_t launch_tiles(Q4AttentionArgs a, uint64_t seen, const Launch& L) {
     a.first_blocks = base * a.splits > kCus && base * a.splits <= 2u * kCus ? (kCus + per_block - 1u) / per_block : blocks;
     const hipError_t e = launch_kernel(L, kFamOther, attention_q4_kernel<HD, WQ, WK, PER_CU>, dim3(base * a.splits), dim3(64 * WQ * WK), a);
     if (e != hipSuccess || a.splits == 1u) return e;
-    const uint32_t merged = a.n * a.n_heads;
-    return a.splits > 8u ? launch_kernel(L, kFamOther, attention_q4_merge_kernel<HD, 1024 / HD>, dim3(merged), dim3(256), a, RB, KT)
-                         : launch_kernel(L, kFamOther, attention_q4_merge_kernel<HD, 1>, dim3((merged + 1024u / HD - 1u) / (1024u / HD)), dim3(256), a, RB, KT);
+    return launch_merge<HD>(a, RB, KT, 8, L);
 }
 
 // Small ones: workgroups of 16 query rows and as many splits as fill the GPU, down to a unit of keys for each wave; but none where walking some more units one
@@ -1061,12 +1069,12 @@ hipError_t launch_few(FewArgs f, uint64_t seen, const Launch& L) {
     static_assert(kFewSlots<HD> * kFewRows <= kSplitSlots * kMostRows, "the scratch is sized for it");
     const uint32_t rows = a.n * (a.n_heads / a.n_kv_heads), base = a.n_kv_heads * ((rows + kFewRows - 1u) / kFewRows);
     const uint32_t spans = (uint32_t)((seen + kSpan - 1u) / kSpan);
-    const uint32_t alone = HD <= 64 ? std::max(5u, 2u + base / 9u) : HD == 128 ? std::max(3u, 1u + base / 12u) : std::max(1u, base / 24u);
+    const uint32_t alone = HD <= 64 ? std::max(5u, 3u + base / 12u) : HD == 128 ? std::max(3u, 1u + base / 12u) : std::max(1u, base / 24u);
     f.at.splits = spans <= alone && !f.scores ? 1u : std::min({std::max(kFewSlots<HD> / base, 1u), spans, kMaxSplits});
     const hipError_t e = launch_kernel(L, kFamOther, attention_q4_few_kernel<HD>, dim3(base * a.splits), dim3(64 * kFewWaves), f);
     if (e != hipSuccess) return e;
     if (f.scores) return launch_kernel(L, kFamOther, attention_q4_finish_kernel<HD>, dim3(a.n_heads + a.n_kv_heads * (uint32_t)((seen + 255u) / 256u)), dim3(256), f);
-    return a.splits == 1u ? e : launch_kernel(L, kFamOther, attention_q4_merge_kernel<HD, 1024 / HD>, dim3(a.n * a.n_heads), dim3(256), a, kFewRows, kSpan);
+    return a.splits == 1u ? e : launch_merge<HD>(a, kFewRows, kSpan, HD == 256 ? 8u : 4u, L);
 }
 
 // Which kernel: the one for few rows wastes nothing on them and fills the GPU with little work, the tiled one reads and unpacks the cache for up to eight
