@@ -542,3 +542,38 @@ def test_a_session_that_evicts(ctx, ops, dev):
         assert_f32_parity(got_w, w, f"weights behind {n} tokens at row {row}")
         w, pos, row = got_w, pos + n, row + n
     assert pos > max_seq - 20 and row < max_seq
+
+
+# ---- operands of unlike sizes -----------------------------------------------------------------------
+
+def run_attention(ctx, ops, dev, q, k, v, pos0, weights=True):
+    """(out, weights gathered from zero) of n tokens at pos0 .., by the form for one token where it is one."""
+    n, heads, hd = q.shape
+    n_kv, max_seq = k.n_kv, k.max_seq
+    scratch, d_out = scratch_for(ctx, dev, n, max_seq, heads, n_kv, hd, weights), dev(np.full(q.shape, np.nan, np.float32))
+    d_w = dev(np.zeros((n_kv, max_seq), np.float32)) if weights else None
+    if n == 1:
+        ops.encode_attention_q4(dev(q), dev(k.raw), dev(v.raw), d_out, scratch, pos0 + 1, max_seq, heads, n_kv, hd, weights=d_w)
+    else:
+        ops.encode_attention_prefill_q4(dev(q), heads * hd, dev(k.raw), dev(v.raw), d_out, heads * hd, scratch, pos0, n, max_seq, heads, n_kv, hd, weights=d_w)
+    return back(d_out, q), d_w.download(np.float32, n_kv * max_seq).reshape(n_kv, max_seq) if weights else None
+
+
+EITHER_KERNEL = [  # head_dim, heads, KV heads, first row, tokens: a token, a few, more than 12 million pairs
+    (64, 4, 2, 1500, 1), (128, 8, 2, 700, 20), (32, 4, 1, 900, 30), (256, 4, 2, 500, 1),
+    (64, 16, 4, 1200, 700), (128, 16, 4, 1000, 700), (32, 16, 2, 1000, 1000), (256, 8, 2, 1700, 800),
+]
+
+@pytest.mark.parametrize("unit", [2.0 ** -149, 2.0 ** -148, 2.0 ** -140, 2.0 ** -126, 2.0 ** -101])
+@pytest.mark.parametrize("hd,heads,n_kv,pos0,n", EITHER_KERNEL)
+def test_queries_of_the_smallest_floats(ctx, ops, dev, hd, heads, n_kv, pos0, n, unit):
+    """Rows whose largest value is one to three units: every score rounds to nothing, all rows that a token sees weigh alike."""
+    seq = pos0 + n
+    k, v = filled(n, seq, n_kv, hd, seq)
+    q = (np.random.default_rng(1).integers(-3, 4, (n, heads, hd)) * unit).astype(np.float32)
+    q[:, 0] = np.clip(q[:, 0], -unit, unit)
+    assert np.all((q[:, 0] != 0).any(-1)) and np.abs(q[:, 0]).max() == unit
+    ref, p = R.attention(q, k, v, pos0)
+    out, w = run_attention(ctx, ops, dev, q, k, v, pos0)
+    assert_f32_parity(out, ref, "out")
+    assert_f32_parity(w, R.gathered(p, n_kv), "weights")

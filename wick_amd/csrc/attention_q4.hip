@@ -93,6 +93,10 @@ __device__ __forceinline__ float halves_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// The power of two that a query row whose largest magnitude is `top` is taken without, for its halves; its scores' factor has it again.  From below 2^-100 on (where no
+// score is above 2^-70) it stays there: a factor that rounds to zero would make NaN of a masked key's score, which is -infinity.
+__device__ __forceinline__ int query_exponent(float top) { return max(__builtin_amdgcn_frexp_expf(top), -100); }
+
 // 32 query rows as the B operand of the first product: dims 16 s + 8 h .. + 7 of row l32, times 2^-e (the row's largest below 1), and
 // the factor that turns a product into a power of two.
 template <int HD>
@@ -113,7 +117,7 @@ struct Queries {
         for (int i = 0; i < HD / 8; i++)
 #pragma unroll
             for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(raw.x[i][e]));
-        const int e = __builtin_amdgcn_frexp_expf(halves_max(top));
+        const int e = query_exponent(halves_max(top));
         factor = __builtin_amdgcn_ldexpf(scale * kLog2e, e);
 #pragma unroll
         for (int s = 0; s < HD / 16; s++) {
@@ -617,7 +621,7 @@ __global__ __launch_bounds__(64 * kFewWaves, HD == 32 ? 4 : HD <= 128 ? 2 : 1) v
 #pragma unroll
             for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(x[i][e]));
         }
-        const int e = __builtin_amdgcn_frexp_expf(groups_max(top));
+        const int e = query_exponent(groups_max(top));
         factor = __builtin_amdgcn_ldexpf(a.scale * kLog2e, e);
 #pragma unroll
         for (int s = 0; s < SLABS; s++) {
@@ -935,7 +939,7 @@ __global__ __launch_bounds__(256, kWeightSlots<HD> / kCus) void attention_q4_wei
         for (int i = 0; i < V; i++)
 #pragma unroll
             for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(raw.x[i][e]));
-        const int e = __builtin_amdgcn_frexp_expf(group_max8(top));
+        const int e = query_exponent(group_max8(top));
 #pragma unroll
         for (int i = 0; i < V; i++) {
             v4f y;
