@@ -545,6 +545,8 @@ def test_a_session_that_evicts(ctx, ops, dev):
 
 
 # ---- operands of unlike sizes -----------------------------------------------------------------------
+# A query is held as two halves of a row that is scaled by a power of two so that its largest value is below 2^15: of a value x, 22 bits are left, or what is
+# above 2^-25 of the scaled row, so it is off by at most max(2^-22 |x|, 2^-40 of the row's largest).
 
 def run_attention(ctx, ops, dev, q, k, v, pos0, weights=True):
     """(out, weights gathered from zero) of n tokens at pos0 .., by the form for one token where it is one."""
@@ -563,6 +565,26 @@ EITHER_KERNEL = [  # head_dim, heads, KV heads, first row, tokens: a token, a fe
     (64, 4, 2, 1500, 1), (128, 8, 2, 700, 20), (32, 4, 1, 900, 30), (256, 4, 2, 500, 1),
     (64, 16, 4, 1200, 700), (128, 16, 4, 1000, 700), (32, 16, 2, 1000, 1000), (256, 8, 2, 1700, 800),
 ]
+
+
+@pytest.mark.parametrize("r", [10, 100, 1000, 10000])
+@pytest.mark.parametrize("hd,heads,n_kv,pos0,n", EITHER_KERNEL)
+def test_large_key_channels_meet_small_query_channels(ctx, ops, dev, hd, heads, n_kv, pos0, n, r):
+    """Some channels of the keys r times as large as the others and those of the queries r times as small: all of them have their part in a score.  A score
+    q.k / sqrt(hd) of normal values has addends that sum up to about 0.64 sqrt(hd) in magnitude (13 at most: heads of 256, queries of twice the spread: 26), each off by
+    2^-22: 6e-6 if all were off the same way, a tenth of that as they are not; the bar of f32 outputs is 1e-5.  (An absolute 2^-25 of a row's largest: 9e-5 at r = 1000.)"""
+    seq = pos0 + n
+    size = np.ones(hd, np.float32)
+    size[:16 if hd == 32 else 32] = r
+    k, v = R.Cache(seq, n_kv, hd), R.Cache(seq, n_kv, hd)
+    k.append(0, normal(r, seq, n_kv, hd) * size), v.append(0, normal(r + 1, seq, n_kv, hd))
+    assert np.isfinite(k.scales).all()
+    q = normal(r + 2, n, heads, hd) / size
+    ref, p = R.attention(q, k, v, pos0)
+    out, w = run_attention(ctx, ops, dev, q, k, v, pos0)
+    assert_f32_parity(out, ref, "out")
+    assert_f32_parity(w, R.gathered(p, n_kv), "weights")
+
 
 @pytest.mark.parametrize("unit", [2.0 ** -149, 2.0 ** -148, 2.0 ** -140, 2.0 ** -126, 2.0 ** -101])
 @pytest.mark.parametrize("hd,heads,n_kv,pos0,n", EITHER_KERNEL)

@@ -9,7 +9,9 @@
 //                                                   are in the lane's registers (an MFMA's K steps are in any order, so both
 //                                                   operands agree on which key a lane's slot is).
 // Accuracy: a cached value, four bits times an f16 scale, is the sum of two halves exactly (hi = f16(n d), lo = f16(n d - hi), 15 bits
-// in all); a query, scaled by a power of two to below 1, and a softmax weight, times 2^12, are split into two halves that keep 22 bits.
+// in all); a query row, scaled by a power of two to below 2^15, and a softmax weight, times 2^12, are split into two halves, which keep 22 bits of a
+// value x, or what is above 2^-25: a query is off by at most max(2^-22 |x|, 2^-40 of the row's largest).  (With the largest below 1 small values beside
+// it would be off by 2^-25 of it: outputs by 9e-5 where channels of the keys are 1000 times as large as the others and the queries' as small.)
 // a b = a_hi b_hi + a_hi b_lo + a_lo b_hi: each product of halves is exact, sums are f32's, what is dropped is below 2^-22.
 // (One half for the weights or the queries would be off by 2^-12 of each: 100 times what f32 sums are.)
 // Bound by the matrix and vector instructions of a unit of 32 rows and 32 keys (heads of 64: 24 matrix instructions of 32 cycles and 920 cycles of vector ones, of
@@ -25,6 +27,7 @@ namespace wick_rocm {
 
 namespace {
 
+constexpr int kHalfBits = 15;              // queries are split below 2^15, a half's largest power of two, so that small ones keep their bits
 constexpr float kWeightBits = 12.0f;       // softmax weights are taken times 2^12, so that small ones keep their bits in the split
 constexpr uint32_t kMaxSplits = 96;        // workgroups that share the rows of the cache among them
 constexpr uint32_t kCus = 256;
@@ -93,11 +96,12 @@ __device__ __forceinline__ float halves_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// The power of two that a query row whose largest magnitude is `top` is taken without, for its halves; its scores' factor has it again.  From below 2^-100 on (where no
-// score is above 2^-70) it stays there: a factor that rounds to zero would make NaN of a masked key's score, which is -infinity.
-__device__ __forceinline__ int query_exponent(float top) { return max(__builtin_amdgcn_frexp_expf(top), -100); }
+// The power of two that a query row whose largest magnitude is `top` is taken without, for its halves; its scores' factor has it again: the largest is below 2^15 then,
+// and small ones beside it have as many bits of a half below them as there are.  From below 2^-100 on (where no score is above 2^-70) it stays where it is: a factor
+// that rounds to zero would make NaN of a masked key's score, which is -infinity.
+__device__ __forceinline__ int query_exponent(float top) { return max(__builtin_amdgcn_frexp_expf(top), -100) - kHalfBits; }
 
-// 32 query rows as the B operand of the first product: dims 16 s + 8 h .. + 7 of row l32, times 2^-e (the row's largest below 1), and
+// 32 query rows as the B operand of the first product: dims 16 s + 8 h .. + 7 of row l32, times 2^-e (the row's largest below 2^15), and
 // the factor that turns a product into a power of two.
 template <int HD>
 struct Queries {
