@@ -123,9 +123,9 @@ int wick_rocm_kv_q4_read(wick_rocm_ctx *ctx, const void *d_cache, float *d_out, 
                          uint32_t n_kv_heads, uint32_t head_dim);
 
 /* wick_rocm_attention_decode and wick_rocm_attention_prefill over such caches, f32 in and out; sums are f32's, and the cached values are taken as they are held.  A
- * product with one of them is off by at most 2^-21 of itself, or by what 2^-40 of the largest of a head's queries (of one token), 2^-37 of the largest of its
- * softmax weights, makes of the value: outputs are as f32 arithmetic has them, except for what rows of less than 2^-16 of the largest weight add to an output that
- * the heavier ones leave at nearly nothing.  Decode: rows [0, seq_len) or [0, *d_pos]; seq_len 0 gives zeros.
+ * product with one of them is off by at most 2^-21 of itself, or by what 2^-40 of the largest of a head's queries (of one token) or of its softmax weights
+ * makes of the value: outputs are as f32 arithmetic has them, except for what rows of less than 2^-19 of the largest weight add to an output that the heavier ones
+ * leave at nearly nothing.  Decode: rows [0, seq_len) or [0, *d_pos]; seq_len 0 gives zeros.
  * d_weights (may be null): [n_kv_heads][max_seq] floats to which every row's softmax weights are added, over the head's query heads
  * and all tokens, in an order of their own that is the same in every run: what a row has gathered, for wick_rocm_kv_q4_evict.  Rows appended anew
  * start from what the array holds for them (the caller clears it once, an eviction clears what it frees).

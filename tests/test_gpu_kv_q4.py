@@ -545,8 +545,8 @@ def test_a_session_that_evicts(ctx, ops, dev):
 
 
 # ---- operands of unlike sizes -----------------------------------------------------------------------
-# A query is held as two halves of a row that is scaled by a power of two so that its largest value is below 2^15: of a value x, 22 bits are left, or what is
-# above 2^-25 of the scaled row, so it is off by at most max(2^-22 |x|, 2^-40 of the row's largest).
+# An operand is held as two halves of a row that is scaled by a power of two so that its largest value is below 2^15 (a softmax weight: the largest is
+# 2^15): of a value x, 22 bits are left, or what is above 2^-25 of the scaled row, so it is off by at most max(2^-22 |x|, 2^-40 of the row's largest).
 
 def run_attention(ctx, ops, dev, q, k, v, pos0, weights=True):
     """(out, weights gathered from zero) of n tokens at pos0 .., by the form for one token where it is one."""
@@ -584,6 +584,28 @@ def test_large_key_channels_meet_small_query_channels(ctx, ops, dev, hd, heads, 
     out, w = run_attention(ctx, ops, dev, q, k, v, pos0)
     assert_f32_parity(out, ref, "out")
     assert_f32_parity(w, R.gathered(p, n_kv), "weights")
+
+
+@pytest.mark.parametrize("hd,heads,n_kv,pos0,n", [(64, 16, 4, 31, 1), (64, 16, 2, 1999, 1), (32, 16, 1, 31, 1), (128, 16, 4, 31, 1), (256, 16, 2, 31, 1), (128, 16, 4, 20, 12),
+                                                  (64, 16, 4, 700, 900), (128, 16, 4, 700, 900), (32, 16, 4, 500, 1200), (256, 16, 2, 700, 900)])
+def test_a_first_row_that_draws_nearly_all_weight(ctx, ops, dev, hd, heads, n_kv, pos0, n):
+    """Its value is zero, the others' are one and their weights alike, so that their roundings add up.  Each is off by at most 2^-22 of itself or 2^-40 of the largest
+    (relative to the largest: 2^-40).  Besides, the first row's score, `lead`, is off by what f32 leaves of it, and an output by as much, relative: the queries'
+    halves 2^-22; its factor and their product 3 roundings of 2^-24; its sum, of addends of one sign, hd / 16 steps of three matrix instructions that each round, or cut
+    off, the sum so far at 2^-23 (half of the whole on average).  1e-6 for the exponentials, sums and the division (some 2^-23 each)."""
+    seq = pos0 + n
+    k, v = R.Cache(seq, n_kv, hd), R.Cache(seq, n_kv, hd)
+    x = np.zeros((seq, n_kv, hd), np.float32)
+    x[0] = 1.0
+    k.append(0, x), v.append(0, 1.0 - x)
+    lead = np.linspace(10.0, 20.0, heads) + 0.37 * np.arange(n)[:, None] / n  # of the first row's score, by head and token
+    q = np.broadcast_to((lead / np.sqrt(hd))[..., None], (n, heads, hd)).astype(np.float32)
+    ref, _ = R.attention(q, k, v, pos0)
+    out, _ = run_attention(ctx, ops, dev, np.ascontiguousarray(q), k, v, pos0, weights=False)
+    rows = np.arange(pos0, seq)[:, None, None]  # of the others, by token
+    of_a_score = 2.0 ** -22 + 3 * 2.0 ** -24 + 3 * hd / 16 / 2 * 2.0 ** -23
+    off = np.abs(out - ref) / ((lead[..., None] * of_a_score + 1e-6) * np.abs(ref) + 2.0 ** -40 * rows)
+    assert off.max() <= 1, f"{off.max():.2f} of what it may be off by, head and token {np.unravel_index(off.argmax(), off.shape)}"
 
 
 @pytest.mark.parametrize("unit", [2.0 ** -149, 2.0 ** -148, 2.0 ** -140, 2.0 ** -126, 2.0 ** -101])

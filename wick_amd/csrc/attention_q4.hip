@@ -9,8 +9,8 @@
 //                                                   are in the lane's registers (an MFMA's K steps are in any order, so both
 //                                                   operands agree on which key a lane's slot is).
 // Accuracy: a cached value, four bits times an f16 scale, is the sum of two halves exactly (hi = f16(n d), lo = f16(n d - hi), 15 bits
-// in all); a query row, scaled by a power of two to below 2^15, and a softmax weight, times 2^12, are split into two halves, which keep 22 bits of a
-// value x, or what is above 2^-25: a query is off by at most max(2^-22 |x|, 2^-40 of the row's largest).  (With the largest below 1 small values beside
+// in all); a query row, scaled by a power of two to below 2^15, and a softmax weight, times 2^15, are split into two halves, which keep 22 bits of a
+// value x, or what is above 2^-25: it is off by at most max(2^-22 |x|, 2^-40 of the row's largest query or weight).  (With the largest below 1 small values beside
 // it would be off by 2^-25 of it: outputs by 9e-5 where channels of the keys are 1000 times as large as the others and the queries' as small.)
 // a b = a_hi b_hi + a_hi b_lo + a_lo b_hi: each product of halves is exact, sums are f32's, what is dropped is below 2^-22.
 // (One half for the weights or the queries would be off by 2^-12 of each: 100 times what f32 sums are.)
@@ -27,8 +27,8 @@ namespace wick_rocm {
 
 namespace {
 
-constexpr int kHalfBits = 15;              // queries are split below 2^15, a half's largest power of two, so that small ones keep their bits
-constexpr float kWeightBits = 12.0f;       // softmax weights are taken times 2^12, so that small ones keep their bits in the split
+constexpr int kHalfBits = 15;              // queries and weights are split below or at 2^15, a half's largest power of two, so that small ones keep their bits
+constexpr float kWeightBits = kHalfBits;   // softmax weights are taken times 2^15
 constexpr uint32_t kMaxSplits = 96;        // workgroups that share the rows of the cache among them
 constexpr uint32_t kCus = 256;
 constexpr uint32_t kSplitSlots = 2 * kCus; // split launches have no more workgroups than this
@@ -41,7 +41,7 @@ struct Q4AttentionArgs {
     const void* v_cache;
     float* out;      // [n][out_stride]
     float* parts;    // records of the splits, [n * n_heads][splits][4 + head_dim]: {maximum, sum, -, -, values}
-    float* stats;    // {maximum (as a power of two), 1 / (sum 2^12)} of every (token, head)'s softmax, for the weights; may be null
+    float* stats;    // {maximum (as a power of two), 1 / (sum 2^15)} of every (token, head)'s softmax, for the weights; may be null
     float* weights;  // [n_kv_heads][max_seq]
     const uint32_t* d_pos;
     uint32_t pos0, n, q_stride, out_stride, max_seq, n_heads, n_kv_heads, splits;
