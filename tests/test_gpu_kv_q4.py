@@ -621,3 +621,30 @@ def test_queries_of_the_smallest_floats(ctx, ops, dev, hd, heads, n_kv, pos0, n,
     out, w = run_attention(ctx, ops, dev, q, k, v, pos0)
     assert_f32_parity(out, ref, "out")
     assert_f32_parity(w, R.gathered(p, n_kv), "weights")
+
+
+# ---- weights from zero, and many splits -------------------------------------------------------------
+
+@pytest.mark.parametrize("hd,heads,n_kv,seq,max_seq", DECODE + [(64, 4, 1, 20000, 20100), (128, 8, 2, 30000, 30000), (256, 4, 1, 15000, 15000), (32, 8, 4, 12289, 13000)])
+def test_weights_of_one_token_from_zero(ctx, ops, dev, hd, heads, n_kv, seq, max_seq):
+    """Held to the bar by themselves, not as what they change in a sum.  The last four: more than 64 splits in use (128 rows each at the least), each by value and
+    from device memory."""
+    k, v = filled(seq, max_seq, n_kv, hd, seq)
+    q = 2 * normal(seq + 5, 1, heads, hd)
+    out, p = R.attention(q, k, v, seq - 1)
+    scratch, d_k, d_v, d_q = scratch_for(ctx, dev, 1, max_seq, heads, n_kv, hd, True), dev(k.raw), dev(v.raw), dev(q)
+    for d_pos in (None, dev(np.array([seq - 1], np.uint32))):
+        d_out, d_w = dev(np.full(heads * hd, np.nan, np.float32)), dev(np.zeros((n_kv, max_seq), np.float32))
+        ops.encode_attention_q4(d_q, d_k, d_v, d_out, scratch, seq if d_pos is None else 0, max_seq, heads, n_kv, hd, weights=d_w, d_pos=d_pos)
+        assert_f32_parity(d_out.download(np.float32, heads * hd).reshape(heads, hd), out[0], f"d_pos {d_pos}")
+        got = d_w.download(np.float32, n_kv * max_seq).reshape(n_kv, max_seq)
+        assert_f32_parity(got[:, :seq], R.gathered(p, n_kv), "weights")
+        assert not got[:, seq:].any()
+
+
+@pytest.mark.parametrize("hd,heads,n_kv,pos0,n", [(64, 5, 5, 40000, 3), (64, 2, 1, 30000, 40)] + [p[:5] for p in LARGE])
+def test_weights_of_a_prompt_from_zero(ctx, ops, dev, hd, heads, n_kv, pos0, n):
+    k, v = filled(n, pos0 + n, n_kv, hd, pos0 + n)
+    q = 2 * normal(n + 5, n, heads, hd)
+    p = R.attention(q, k, v, pos0)[1]
+    assert_f32_parity(run_attention(ctx, ops, dev, q, k, v, pos0)[1], R.gathered(p, n_kv), "weights")
