@@ -10,6 +10,17 @@ import kv_q4_ref as R
 from conftest import ROOT
 
 
+def run_host(name, tmp_path):
+    """tests/host/<name>.cpp, linked with the library and the pretended runtime, ends with 0."""
+    here, lib, exe = os.path.join(ROOT, "tests", "host"), os.path.join(ROOT, "wick_amd", "lib", "libwick_rocm.a"), str(tmp_path / name)
+    cmd = ["g++", "-std=c++17", "-O1", "-Wall", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", os.path.join(here, name + ".cpp"),
+           os.path.join(here, "fake_hip.cpp"), lib, "-lpthread", "-o", exe]
+    r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    assert r.returncode == 0, r.stdout
+    r = subprocess.run([exe], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=120)
+    assert r.returncode == 0, r.stdout
+
+
 def test_calls_that_are_refused(tmp_path):
     here, lib, exe = os.path.join(ROOT, "tests", "host"), os.path.join(ROOT, "wick_amd", "lib", "libwick_rocm.a"), str(tmp_path / "kv_q4_calls")
     cmd = ["g++", "-std=c++17", "-O1", "-Wall", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", os.path.join(here, "kv_q4_calls.cpp"),
@@ -18,6 +29,10 @@ def test_calls_that_are_refused(tmp_path):
     assert r.returncode == 0, r.stdout
     r = subprocess.run([exe], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=120)
     assert r.returncode == 0, r.stdout
+
+
+def test_what_splits_and_shares_leave_fits_the_scratch(tmp_path):
+    run_host("kv_q4_scratch", tmp_path)
 
 
 @pytest.mark.parametrize("hd", [32, 64, 128, 256])

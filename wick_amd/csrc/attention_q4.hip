@@ -31,8 +31,9 @@ constexpr int kHalfBits = 15;              // queries and weights are split belo
 constexpr float kWeightBits = kHalfBits;   // softmax weights are taken times 2^15
 constexpr uint32_t kMaxSplits = 96;        // workgroups that share the rows of the cache among them
 constexpr uint32_t kCus = 256;
-constexpr uint32_t kSplitSlots = 2 * kCus; // split launches have no more workgroups than this
+constexpr uint32_t kSplitSlots = 2 * kCus; // workgroups that a split launch has at the most by its launcher's rule
 constexpr uint32_t kMostRows = 128;        // query rows of a workgroup at the most
+constexpr uint32_t kMostRecords = kSplitSlots * kMostRows;  // of all splits of a launch
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct Q4AttentionArgs {
@@ -899,7 +900,7 @@ struct WeightArgs {
 constexpr uint32_t kWeightKeys = 128, kMaxShares = 16;
 template <int HD>
 constexpr uint32_t kWeightSlots = kCus * (HD <= 64 ? 4 : HD == 128 ? 3 : 2);  // workgroups that the GPU has at once
-constexpr uint32_t kWeightSums = 4 * kCus * kWeightKeys;  // that the shares of a launch leave at most: no more workgroups than those
+constexpr uint32_t kWeightSums = 4 * kCus * kWeightKeys;  // that the shares of a launch have room for
 
 template <int HD>
 __global__ __launch_bounds__(256, kWeightSlots<HD> / kCus) void attention_q4_weights_kernel(WeightArgs args) {
@@ -1040,6 +1041,10 @@ __global__ __launch_bounds__(256) void attention_q4_add_weights_kernel(WeightArg
     a.weights[(size_t)c * a.max_seq + t] += w;
 }
 
+// As many splits as there are records for, each split leaving one to every row (`rows` in all) in the scratch, or one: whatever a launcher asks for, what it gets fits
+// what part_floats() sizes.
+uint32_t splits_with_records(uint32_t splits, uint64_t rows) { return (uint32_t)std::max<uint64_t>(std::min<uint64_t>({splits, kMaxSplits, kMostRecords / rows}), 1u); }
+
 // Up to `few` splits are merged by HD / 4 lanes a row, more by a workgroup a row (us with what is before it, the second and the first: 60 tokens of 32 heads
 // of 64 values behind 2500 in four splits 15.8 and 14.7, 120 behind 5000 in two 35.2 and 32.3, 30 behind 2500 in eight 12.0 and 12.7).
 template <int HD>
@@ -1054,10 +1059,10 @@ hipError_t launch_merge(const Q4AttentionArgs& a, uint32_t wg_rows, uint32_t til
 template <int HD, int WQ, int WK, int PER_CU>
 hipError_t launch_tiles(Q4AttentionArgs a, uint64_t seen, const Launch& L) {
     constexpr uint32_t RB = 32 * WQ, KT = 32 * WK;
-    static_assert(PER_CU * kCus <= kSplitSlots && RB <= kMostRows, "the scratch is sized for it");
+    static_assert(PER_CU * kCus <= kSplitSlots && RB <= kMostRows, "there are records for all splits that fit on the GPU");
     const uint32_t rows = a.n * (a.n_heads / a.n_kv_heads), blocks = (rows + RB - 1u) / RB, base = a.n_kv_heads * blocks;
     const uint32_t room = kCus * PER_CU / base, most = (uint32_t)((seen + 3u * KT - 1u) / (3u * KT));
-    a.splits = std::min({std::max(room, 1u), most, kMaxSplits});
+    a.splits = splits_with_records(std::min(room, most), (uint64_t)a.n * a.n_heads);
     const uint32_t per_block = a.n_kv_heads * a.splits;
     a.first_blocks = base * a.splits > kCus && base * a.splits <= 2u * kCus ? (kCus + per_block - 1u) / per_block : blocks;
     const hipError_t e = launch_kernel(L, kFamOther, attention_q4_kernel<HD, WQ, WK, PER_CU>, dim3(base * a.splits), dim3(64 * WQ * WK), a);
@@ -1074,11 +1079,11 @@ template <int HD>
 hipError_t launch_few(FewArgs f, uint64_t seen, const Launch& L) {
     const Q4AttentionArgs& a = f.at;
     constexpr uint32_t kSpan = kFewKeys * kFewWaves;
-    static_assert(kFewSlots<HD> * kFewRows <= kSplitSlots * kMostRows, "the scratch is sized for it");
+    static_assert(kFewSlots<HD> * kFewRows <= kMostRecords, "there are records for all splits that fit on the GPU");
     const uint32_t rows = a.n * (a.n_heads / a.n_kv_heads), base = a.n_kv_heads * ((rows + kFewRows - 1u) / kFewRows);
     const uint32_t spans = (uint32_t)((seen + kSpan - 1u) / kSpan);
     const uint32_t alone = HD <= 64 ? std::max(5u, 3u + base / 12u) : HD == 128 ? std::max(3u, 1u + base / 12u) : std::max(1u, base / 24u);
-    f.at.splits = spans <= alone && !f.scores ? 1u : std::min({std::max(kFewSlots<HD> / base, 1u), spans, kMaxSplits});
+    f.at.splits = spans <= alone && !f.scores ? 1u : splits_with_records(std::min(kFewSlots<HD> / base, spans), (uint64_t)a.n * a.n_heads);
     const hipError_t e = launch_kernel(L, kFamOther, attention_q4_few_kernel<HD>, dim3(base * a.splits), dim3(64 * kFewWaves), f);
     if (e != hipSuccess) return e;
     if (f.scores) return launch_kernel(L, kFamOther, attention_q4_finish_kernel<HD>, dim3(a.n_heads + a.n_kv_heads * (uint32_t)((seen + 255u) / 256u)), dim3(256), f);
@@ -1112,7 +1117,8 @@ hipError_t launch_head_dim(const Q4AttentionArgs& a, float* d_scores, const Laun
     }
     if (e != hipSuccess || !a.weights) return e;
     const uint32_t tiles = (uint32_t)((seen + kWeightKeys - 1u) / kWeightKeys), base = a.n_kv_heads * tiles, blocks = (rows + 31u) / 32u;
-    const WeightArgs w{a, d_scores, std::min({std::max(kWeightSlots<HD> / base, 1u), kMaxShares, (blocks + 1u) / 2u}), tiles * kWeightKeys};
+    const uint32_t room = std::min(kWeightSlots<HD>, kWeightSums / kWeightKeys) / base;  // (with one share nothing is left in the scratch)
+    const WeightArgs w{a, d_scores, std::max(std::min({room, kMaxShares, (blocks + 1u) / 2u}), 1u), tiles * kWeightKeys};
     e = launch_kernel(L, kFamOther, attention_q4_weights_kernel<HD>, dim3(base * w.shares), dim3(256), w);
     if (e != hipSuccess || w.shares == 1u) return e;
     return launch_kernel(L, kFamOther, attention_q4_add_weights_kernel, dim3((uint32_t)((seen + 255u) / 256u), a.n_kv_heads), dim3(256), w);
@@ -1121,8 +1127,8 @@ hipError_t launch_head_dim(const Q4AttentionArgs& a, float* d_scores, const Laun
 // Floats of the splits' records: what a split launch has at most, for any number of tokens up to n, and a token's that gathers weights (which leaves its
 // only split as one, however many its heads).
 size_t part_floats(uint32_t n, uint32_t n_heads, uint32_t head_dim) {
-    const size_t rows = (size_t)n * n_heads, most = (size_t)kSplitSlots * kMostRows;
-    return std::max(std::min(rows * kMaxSplits, most), (size_t)n_heads) * (head_dim + 4u);
+    const size_t rows = (size_t)n * n_heads;
+    return std::max(std::min(rows * kMaxSplits, (size_t)kMostRecords), (size_t)n_heads) * (head_dim + 4u);
 }
 
 }  // namespace
