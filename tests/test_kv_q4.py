@@ -35,6 +35,10 @@ def test_what_splits_and_shares_leave_fits_the_scratch(tmp_path):
     run_host("kv_q4_scratch", tmp_path)
 
 
+def test_attention_over_no_row_asks_for_heads_too(tmp_path):
+    run_host("kv_q4_no_rows", tmp_path)
+
+
 @pytest.mark.parametrize("hd", [32, 64, 128, 256])
 def test_a_value_is_off_by_half_a_step_and_the_scale(hd):
     """|x - held| <= d / 2 where the rounding is, d where the largest step is cut off (15 for 16), both with the scale's rounding (2^-11 of up to 8

@@ -232,6 +232,7 @@ int wick_rocm_attention_decode_q4(wick_rocm_ctx* ctx, const float* d_q, const vo
     if (!d_pos && seq_len > max_seq) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "attention_q4: seq_len beyond the cache");
     if ((uint64_t)n_heads * head_dim > UINT32_MAX - 3u) return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, "attention_q4: too many heads");
     if (!d_pos && seq_len == 0) {  // no row to attend over
+        if (n_heads == 0 || n_heads % n_kv_heads != 0) return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, "attention_q4: n_kv_heads must divide n_heads");
         if (!d_out) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "attention_q4: null device pointer");
         hipError_t e = launch_fill_zero(d_out, (size_t)n_heads * head_dim, ctx->launch());
         return e == hipSuccess ? WICK_ROCM_OK : fail_hip(ctx, e, "attention_q4 launch");
