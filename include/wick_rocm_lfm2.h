@@ -112,7 +112,7 @@ int wick_rocm_attention_prefill_quantize_q8_0(wick_rocm_ctx *ctx, const float *d
  * [head_dim / 32] f16, one to a block of 32 values.  A value stands for (nibble - 8) * scale.
  *
  * wick_rocm_kv_q4_append: rows row .. row + n - 1 (or *d_row .., those past the cache are dropped) of both caches from the normed and rotated keys and the values
- * of n tokens (token j's heads at j * kv_stride floats, kv_stride % 4 == 0, 16-byte aligned).  Per block, with m its value of largest
+ * of n tokens (token j's heads at j * kv_stride floats, kv_stride % 4 == 0, 16-byte aligned).  Per block, by GGUF's Q4_0 rule, with m its value of largest
  * magnitude (the positive one of two): d = m / -8, n_i = min(15, trunc(x_i * (1 / d) + 8.5)) in f32, and the scale f16(d) is held; a
  * block whose scale rounds to 0 is held as zeros (scale +0), one with a value that is not finite or beyond +-65504 as NaN.
  * wick_rocm_kv_q4_read: rows row .. row + n - 1 of one cache as floats (out_stride a token, % 4 == 0, 16-byte aligned). */

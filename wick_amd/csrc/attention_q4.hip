@@ -15,8 +15,8 @@
 // a b = a_hi b_hi + a_hi b_lo + a_lo b_hi: each product of halves is exact, sums are f32's, what is dropped is below 2^-22.
 // (One half for the weights or the queries would be off by 2^-12 of each: 100 times what f32 sums are.)
 // Bound by the matrix and vector instructions of a unit of 32 rows and 32 keys (heads of 64: 24 matrix instructions of 32 cycles and 920 cycles of vector ones, of
-// the softmax above all, in 2060 cycles): 2002 tokens of 32 heads over 8 of 64 62 us, 2048 behind 6144 of 16 heads over 4 of 128 320 us (three
-// products are 310 at the 1160 TFLOP/s of a large library product; power).
+// the softmax above all, in 2060 cycles): 2002 tokens of 32 heads over 8 of 64 59 us, 2048 behind 6144 of 16 heads over 4 of 128 300 us (three
+// products are 307 at the 1175 TFLOP/s of a large library product; power).
 #include <algorithm>
 
 #include "attention_device.h"
@@ -29,7 +29,10 @@ namespace {
 
 constexpr int kHalfBits = 15;              // queries and weights are split below or at 2^15, a half's largest power of two, so that small ones keep their bits
 constexpr float kWeightBits = kHalfBits;   // softmax weights are taken times 2^15
-constexpr uint32_t kMaxSplits = 96;        // workgroups that share the rows of the cache among them
+// Workgroups that share the rows of the cache among them at the most, so that a row's records stay few for the merge and the scratch small.  Nothing measured says that 96 is
+// the best: with fewer than six KV heads of up to 128 values (three of 256) it leaves workgroups' places empty (a token over 100000 rows of one KV head 10.5 + 3.8 us, over
+// 12500 of eight 7.2 + 3.5; of 128 values 15.9 + 4.0 and 10.2 + 3.9; of 256, 60000 rows and 7500, 20.1 + 6.2 and 13.1 + 3.9; two KV heads lie between).
+constexpr uint32_t kMaxSplits = 96;
 constexpr uint32_t kCus = 256;
 constexpr uint32_t kSplitSlots = 2 * kCus; // workgroups that a split launch has at the most by its launcher's rule
 constexpr uint32_t kMostRows = 128;        // query rows of a workgroup at the most
@@ -332,7 +335,7 @@ __global__ __launch_bounds__(64 * WQ * WK, PER_CU * WQ * WK / 4) void attention_
     };
 
     // While the arithmetic of tile t runs, the values of t and the keys of t + 1 sit in LDS; the values of t + 1 and the keys of t + 2 are in registers and
-    // go where those of t - 1 and t were; behind them the next are requested.  (Requests past the end repeat the last row.)
+    // go where those of t - 1 and t were; behind them the next are requested.  (Requests past the end give zeros.)
     Share kraw, vraw;
     v16f sc[2];
     fetch(kraw, true);
@@ -499,7 +502,7 @@ __global__ __launch_bounds__(256) void attention_q4_merge_kernel(Q4AttentionArgs
 // group g HD / 32 of them from word g HD / 32 on, the order of an MFMA's K steps being free), and of the values one word of eight rows, the rows whose weights it
 // holds: two rows' words are transposed to pairs of one dim's values with one byte permutation each.  Keys are multiplied as nibbles less 8, one exact half, a
 // block's 32 dims at a time, and the block's scale is taken into the sum: two products of halves instead of three.
-// Bound at long context by the loads and the unpacking, which overlap in part: one token of 32 heads over 8 of 128 behind 128000 rows (147 MB) 38 us, its
+// Bound at long context by the loads and the unpacking, which overlap in part: one token of 32 heads over 8 of 128 behind 128000 rows (147 MB) 39 us, its
 // loads alone 26; with values through LDS and both planes of the keys 45, and 42 before waves yielded (see below).  At short context by two or three round trips to memory: 16 heads over 9000 rows 7.2 us.
 struct FewArgs {
     Q4AttentionArgs at;
@@ -855,7 +858,7 @@ __global__ __launch_bounds__(64 * kFewWaves, HD == 32 ? 4 : HD <= 128 ? 2 : 1) v
 }
 
 // One token's splits merged and, in workgroups of their own, its weights added to what the rows have gathered: from the scores that the launch before left, with
-// each head's maximum and sum worked out from its splits once more.  (9001 rows of 16 heads 3.6 us: a launch and two round trips.)
+// each head's maximum and sum worked out from its splits once more.  (9001 rows of 16 heads 3.4 us: a launch and two round trips.)
 template <int HD>
 __global__ __launch_bounds__(256) void attention_q4_finish_kernel(FewArgs args) {
     const Q4AttentionArgs& a = args.at;
@@ -889,7 +892,7 @@ __global__ __launch_bounds__(256) void attention_q4_finish_kernel(FewArgs args) 
 // up over the query rows.  Every wave keeps 32 keys as matrix operands in registers; the workgroup walks query rows in blocks of 32 that it splits into
 // halves once for its four waves, through LDS, the next block's on their way meanwhile.  The rows are shared out among `shares` workgroups, whose sums the next launch adds.
 // All sums in one order.  Bound by vector instructions (exponentials, and the queries' split: a block is split in every workgroup that sees it) and, for few
-// rows, by latency: 555 tokens of 16 heads over 8 of 64 7.6 and 3.0 us for the addition, 1500 of 32 heads 26, 4000 of them 138, 500 of 16 over 4 of 128 9.5 (keys
+// rows, by latency: 555 tokens of 16 heads over 8 of 64 8.0 and 3.0 us for the addition, 1500 of 32 heads 26, 4000 of them 138, 500 of 16 over 4 of 128 9.5 (keys
 // in LDS, the queries split by every wave for itself: 12.7, 54, 257 and 37).  128 keys a workgroup: with 256 and eight waves behind one barrier 9.9, 38, 190 and 17.  Workgroups with fewer
 // blocks to go yield (834 tokens behind 3353, 24 heads over 3 of 64: 44.8 -> 41.2).
 struct WeightArgs {
@@ -897,7 +900,7 @@ struct WeightArgs {
     float* sums;  // [shares][n_kv_heads][stride], unless there is one share
     uint32_t shares, stride;
 };
-constexpr uint32_t kWeightKeys = 128, kMaxShares = 16;
+constexpr uint32_t kWeightKeys = 128, kMaxShares = 16;  // (one KV head of 64 values: 256 of 1024 places over 2048 rows; other limits were not measured)
 template <int HD>
 constexpr uint32_t kWeightSlots = kCus * (HD <= 64 ? 4 : HD == 128 ? 3 : 2);  // workgroups that the GPU has at once
 constexpr uint32_t kWeightSums = 4 * kCus * kWeightKeys;  // that the shares of a launch have room for
@@ -1055,7 +1058,7 @@ hipError_t launch_merge(const Q4AttentionArgs& a, uint32_t wg_rows, uint32_t til
                           : launch_kernel(L, kFamOther, attention_q4_merge_kernel<HD, 1>, dim3((rows + kRows - 1u) / kRows), dim3(256), a, wg_rows, tile);
 }
 
-// Large launches: as many splits as workgroups fit on the GPU, three tiles or more each (a split's state is written and read again).
+// Large launches: as many splits as workgroups fit on the GPU (kMaxSplits at the most), three tiles or more each (a split's state is written and read again).
 template <int HD, int WQ, int WK, int PER_CU>
 hipError_t launch_tiles(Q4AttentionArgs a, uint64_t seen, const Launch& L) {
     constexpr uint32_t RB = 32 * WQ, KT = 32 * WK;
@@ -1070,7 +1073,7 @@ hipError_t launch_tiles(Q4AttentionArgs a, uint64_t seen, const Launch& L) {
     return launch_merge<HD>(a, RB, KT, 8, L);
 }
 
-// Small ones: workgroups of 16 query rows and as many splits as fill the GPU, down to a unit of keys for each wave; but none where walking some more units one
+// Small ones: workgroups of 16 query rows and as many splits as fill the GPU, but no more than kMaxSplits, down to a unit of keys for each wave; but none where walking some more units one
 // behind the other takes less than the merge, which takes the longer the more rows there are (us, split and alone, 32 heads over 8; of 64 values: a token over
 // 512 rows 6.9 and 6.0, 768 7.1 and 7.4; 30 tokens behind 900 10.0 and 9.4, 1300 11.3 and 11.6; 60 behind 1300 13.3 and 11.8, 2500 15.8 and 18.4; 120 behind
 // 600 15.3 and 8.2, 2500 24.1 and 19.9; of 128: a token over 256 7.7 and 6.0, 512 7.7 and 8.3; 60 behind 800 15.6 and 13.3, 1800 19.9 and 23.6; of 256: 25 behind

@@ -12,10 +12,10 @@ namespace {
 constexpr float kQ4Largest = 65504.0f;  // of a value that a block can hold: eight times its scale is an f16, whatever product takes it
 
 // ---- append, read back ---------------------------------------------------------------------
-// A block's scale is its value of largest magnitude over -8 (the positive one of two), so that this value is held as it is up to
+// GGUF's Q4_0 rule: a block's scale is its value of largest magnitude over -8 (the positive one of two), so that this value is held as it is up to
 // the scale's rounding to f16; the quants come from the unrounded scale: n = min(15, trunc(x * (1 / d) + 8.5)), each step one f32
 // operation.  A block without a scale holds zeros (d rounds to 0), or NaN where a value is none or larger than an f16 holds.
-// Four lanes a block, eight values each.  Bound by memory: 2002 tokens of 8 heads of 64 (10.5 MB) 4.0 us, 3.4 us to read one cache's rows back (5.2 MB).
+// Four lanes a block, eight values each.  Bound by memory: 2002 tokens of 8 heads of 64 (10.5 MB) 4.0 us, 3.5 us to read one cache's rows back (5.2 MB).
 struct Q4AppendArgs {
     const float* src[2];  // keys, values
     void* cache[2];
@@ -141,7 +141,7 @@ __device__ __forceinline__ uint32_t sum_before(uint32_t v, uint32_t* slots, uint
 // Up to 16384 rows: one workgroup a head, which reads them once; bound by the latency of some 15 barriers and as many trips to LDS, and with more rows by
 // its CU's instructions (8 heads of 3000 rows 6.5 us, 8000 10.4, 16000 14.4; of 32768, 28).
 // More: the head in parts of a workgroup each, a launch to each digit and one to place the rows, every one of which begins with adding up the parts'
-// histograms of the launch before (32768 rows of 8 heads 4.0 + 5.2 + 5.4 + 6.1 us, 8000 rows 3.4 + 4.9 + 5.1 + 5.9: each bound by the same latencies).
+// histograms of the launch before (32768 rows of 8 heads 3.7 + 5.3 + 5.5 + 6.3 us, 8000 rows 3.4 + 4.9 + 5.1 + 5.9: each bound by the same latencies).
 constexpr uint32_t kPartRows = 4, kPartChunk = kPartRows * kEvictThreads;  // rows of a thread and of a part's workgroup at a time
 constexpr uint32_t kBins = 2048, kMaxParts = 32, kSelectLargest = 16 * kEvictThreads;
 
@@ -343,7 +343,7 @@ __global__ __launch_bounds__(kEvictThreads) void kv_q4_select_part_kernel(Q4Evic
 // before those writes is asked of the memory: nothing that this launch writes is read in it.)
 // Weights behind the last row that stays are cleared by segments that have nothing to read.
 // Bound by memory latency: taking a segment, its rows' numbers, the rows, the word of the segments in front, one behind the other; 24576 rows of 8 heads of
-// 64 values 12.2 us (18.1 with one workgroup for all rows of a fifth of a head's planes, one chunk of rows behind the other; of one head of 256 values 8.8
+// 64 values 13.4 us (12.2 when it was built, 18.1 with one workgroup for all rows of a fifth of a head's planes, one chunk of rows behind the other; of one head of 256 values 8.8
 // and 50.6).
 constexpr uint32_t kMoveThreads = 256, kMoveLeast = 256;  // threads; rows of a segment at least
 template <int HD>
