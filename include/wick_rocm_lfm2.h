@@ -152,6 +152,79 @@ size_t wick_rocm_kv_q4_evict_scratch_floats(uint32_t seq_len, uint32_t n_kv_head
 int wick_rocm_kv_q4_evict(wick_rocm_ctx *ctx, void *d_k_cache, void *d_v_cache, float *d_weights, uint32_t *d_kept, float *d_scratch, uint32_t seq_len,
                           uint32_t n_keep, uint32_t n_recent, uint32_t n_drop, uint32_t max_seq, uint32_t n_kv_heads, uint32_t head_dim);
 
+/* ---- KV caches in pages ----
+ * Caches of several sequences at once, for continuations of one prompt, sessions that share one, or a queue of sessions: sequences hold pages
+ * of page_rows rows of a pool, and may hold the same ones.  Everything that says who holds what is on the device, so that a captured step serves
+ * every token.  (The reference holds one sequence a cache, wick/src/kv_cache.rs; its prefix cache copies.)
+ *
+ * A plane of the pool is the keys or the values of one layer: [n_pages][n_kv_heads][page_rows][head_dim] elements of kv_dtype (WICK_ROCM_KV_F32
+ * or WICK_ROCM_KV_F16; f16 values are rounded once, to nearest even, when they are appended, and widened exactly), head_dim 32, 64, 128 or 256, 16-byte aligned.
+ * The same pages of all planes belong together.  The caller allocates pool and table:
+ *   d_table [n_seqs][max_pages]  the page of rows [i * page_rows, ..) of sequence s; WICK_ROCM_NO_PAGE: none (all entries behind its last page)
+ *   d_lens  [n_seqs]             rows of sequence s
+ *   d_refs  [n_pages]            table entries that name the page; 0: it is free
+ * An empty pool: entries WICK_ROCM_NO_PAGE, lens and refs 0.  page_rows 16, 32, 64, 128 or 256; n_seqs at most 4096, n_pages 2^24, max_pages * page_rows
+ * and n_seqs * max_pages 2^30.  The struct itself is read during the call only. */
+enum { WICK_ROCM_KV_F32 = 0, WICK_ROCM_KV_F16 = 1 };
+#define WICK_ROCM_NO_PAGE 0xffffffffu
+#define WICK_ROCM_NO_ROW 0xffffffffu
+typedef struct wick_rocm_kv_pages {
+    uint32_t n_seqs, max_pages, n_pages, page_rows;
+    uint32_t *d_table, *d_lens, *d_refs;
+} wick_rocm_kv_pages;
+/* Planes that lie plane_bytes apart (a multiple of 16 that covers a plane), for the calls that move pages. */
+typedef struct wick_rocm_kv_planes {
+    void *d_base;
+    size_t plane_bytes;
+    uint32_t n_planes, n_kv_heads, head_dim;
+    int kv_dtype;
+} wick_rocm_kv_planes;
+
+/* wick_rocm_kv_paged_append: the normed and rotated keys and the values of n tokens into the pages of their sequences (token j's heads at j * kv_stride floats,
+ * kv_stride % 4 == 0, 16-byte aligned).  Sequence s's tokens are [d_first[s], d_first[s + 1]) (n_seqs + 1 ascending numbers; null: one token
+ * each, n = n_seqs) and go to its rows d_start[s] ..; WICK_ROCM_NO_ROW: they are dropped, as are rows that no page is there for.  Tokens of no sequence are left out.  What
+ * wick_rocm_kv_pages_reserve leaves is what d_start takes: it sees to it that nobody else holds the pages that are written to. */
+int wick_rocm_kv_paged_append(wick_rocm_ctx *ctx, const wick_rocm_kv_pages *pages, const float *d_k, const float *d_v, uint32_t kv_stride, void *d_k_pages,
+                              void *d_v_pages, int kv_dtype, const uint32_t *d_start, const uint32_t *d_first, uint32_t n, uint32_t n_kv_heads,
+                              uint32_t head_dim);
+
+/* wick_rocm_attention_decode for one new token of every sequence, over its rows [0, d_lens[s]) (no rows: zeros).  Sequence s's query heads at
+ * d_q + s * q_stride floats, its output at d_out + s * out_stride; f32 in and out, sums and softmax f32's, cached values as they are held.  (f16 pages: a query
+ * element is off by at most 2^-22 of itself or 2^-39 of its head's largest, a softmax weight by the same of itself or of the largest.)  Rows whose entry names no page
+ * of the pool count as not there.  A row that is not finite gives NaN to the sequences that see it, in the heads that read it, and to no other.
+ * The work of all sequences together is split evenly over the GPU, whatever their lengths; a second launch joins what several workgroups share.
+ * d_scratch: wick_rocm_attention_paged_scratch_floats(...) floats (0: not such a shape), contents need not be kept; calls that may run at the same time need one
+ * each.  q, pages, output and scratch 16-byte aligned, strides multiples of 4 that cover the heads. */
+size_t wick_rocm_attention_paged_scratch_floats(uint32_t n_seqs, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim);
+int wick_rocm_attention_decode_paged(wick_rocm_ctx *ctx, const wick_rocm_kv_pages *pages, const float *d_q, uint32_t q_stride, const void *d_k_pages,
+                                     const void *d_v_pages, int kv_dtype, float *d_out, uint32_t out_stride, float *d_scratch, uint32_t n_heads,
+                                     uint32_t n_kv_heads, uint32_t head_dim);
+
+/* Sequences from sequences: s becomes what sequence d_parents[s] was before the call (its pages are held once more, nothing is copied); d_parents[s] == s:
+ * it stays, no such sequence (WICK_ROCM_NO_PAGE, say): it becomes empty.  Copies of a prompt's cache, the survivors of a beam, sessions that move up. */
+int wick_rocm_kv_pages_fork(wick_rocm_ctx *ctx, const wick_rocm_kv_pages *pages, const uint32_t *d_parents);
+/* Sequence s is cut to d_rows[s] rows (one that has no more stays), pages behind them are let go: 0 frees it. */
+int wick_rocm_kv_pages_free(wick_rocm_ctx *ctx, const wick_rocm_kv_pages *pages, const uint32_t *d_rows);
+
+/* Lists of pages that move, as the two calls below leave them and wick_rocm_kv_pages_copy takes them: d_moves[0] is how many, d_moves[1] is said
+ * below, and from word 4 on four words a move: {from, to, rows, 0}.  wick_rocm_kv_pages_moves_words(pages) words (0: not such a pool), 16-byte aligned; what is
+ * behind the list is the calls' workspace.
+ * wick_rocm_kv_pages_reserve: d_counts[s] more rows for every sequence, whose lens grow by them.  New pages are the lowest free ones, for the first sequence
+ * first.  A partial last page that is written to and held by others is copied (rows in use, to a page of the sequence's own); of sequences that write
+ * to one page which nobody else holds, the first keeps it.  d_start[s]: the first of the new rows, or WICK_ROCM_NO_ROW where there are none.  All or nothing: if the
+ * pool (or a sequence's table) has not enough, nothing changes, every d_start is WICK_ROCM_NO_ROW and d_moves[1] says how many pages are wanting (0xffffffff: the
+ * table is too short); else d_moves[1] = 0.
+ * wick_rocm_kv_pages_compact: with U pages in use, the ones at U and above move to the free ones below, in ascending order, so that the rest of the
+ * pool is free in one piece; tables and refs follow.  Pages move whole.  d_moves[1] = U.
+ * planes: what is copied along (null: the caller does it, with wick_rocm_kv_pages_copy for each group of planes).
+ * wick_rocm_kv_pages_copy: the first min(d_moves[0], max_moves) moves in all planes, rows [0, rows) of every head; a move that names no page of the pool is left out.  Pages
+ * that are written must be named once. */
+size_t wick_rocm_kv_pages_moves_words(const wick_rocm_kv_pages *pages);
+int wick_rocm_kv_pages_reserve(wick_rocm_ctx *ctx, const wick_rocm_kv_pages *pages, const uint32_t *d_counts, uint32_t *d_start, uint32_t *d_moves,
+                               const wick_rocm_kv_planes *planes);
+int wick_rocm_kv_pages_compact(wick_rocm_ctx *ctx, const wick_rocm_kv_pages *pages, uint32_t *d_moves, const wick_rocm_kv_planes *planes);
+int wick_rocm_kv_pages_copy(wick_rocm_ctx *ctx, const wick_rocm_kv_pages *pages, const wick_rocm_kv_planes *planes, const uint32_t *d_moves, uint32_t max_moves);
+
 /* The attention block between the Q/K/V projections and the output projection: what wick_rocm_qk_norm_rope followed
  * by wick_rocm_attention_decode compute (wick/src/model/lfm2.rs:783-1006), bit for bit, with the norm, the rotation and
  * the KV append folded into the attention kernel (every workgroup norms and rotates its own query heads and the new key, one
@@ -235,6 +308,28 @@ int wick_rocm_argmax(wick_rocm_ctx *ctx, const float *d_logits, uint32_t n, uint
 int wick_rocm_lm_head_greedy_f32(wick_rocm_ctx *ctx, const wick_rocm_weight *w, const float *d_x, const float *d_norm_weight, float eps,
                                  float *d_logits, uint32_t *d_out, uint32_t *d_token, uint32_t *d_pos);
 
+/* Sampling: the next token of every row of logits ([rows][logits_stride] floats, n in use) from one given uniform number each, where the greedy pick above takes the
+ * largest (the reference's sampler, wick/src/sampler.rs, draws its own on the CPU).  A row's rule (d_params [rows], on the device):
+ *   w_i = exp((l_i - max l) / temperature);    temperature <= 0 or NaN: as if top_k were 1
+ *   K: the top_k largest (0: all);    P: the shortest run of K from the largest down whose mass is at least top_p that of K (>= 1 or NaN: K; at
+ *   least one token);    M: those of P with w_i >= min_p (<= 0 or NaN: P; above 1 counts as 1)
+ *   d_out = the first token, by index, at which the mass of M up to and with it exceeds d_uniform times the whole (d_uniform from [0, 1); what is outside is
+ *   clamped, NaN is 0), d_prob (may be null) = w / mass of M.
+ * Of equal logits the lower index is the larger (wick_rocm_argmax takes the highest).  NaN counts as -infinity, which is never taken; a row of nothing else gives
+ * WICK_ROCM_NO_TOKEN and probability 0.  Masses are sums of whole numbers of 2^-43 of the power of two below the largest weight, so a pick is the same in every run
+ * and on every grid, and tokens of less than 2^-45 of the largest have no mass.
+ * n at most 2^19, rows 65535.  d_scratch: wick_rocm_sample_scratch_bytes(...) bytes (0: not such a shape), 16-byte aligned, contents need not be kept; calls
+ * that may run at the same time need one each. */
+#define WICK_ROCM_NO_TOKEN 0xffffffffu
+typedef struct wick_rocm_sample_params {
+    float temperature;
+    uint32_t top_k;
+    float top_p, min_p;
+} wick_rocm_sample_params;
+size_t wick_rocm_sample_scratch_bytes(uint32_t rows, uint32_t n);
+int wick_rocm_sample(wick_rocm_ctx *ctx, const float *d_logits, uint32_t logits_stride, uint32_t rows, uint32_t n, const wick_rocm_sample_params *d_params,
+                     const float *d_uniform, uint32_t *d_out, float *d_prob, void *d_scratch);
+
 /* ---- the model --------------------------------------------------------------------------- */
 
 typedef struct wick_rocm_lfm2 wick_rocm_lfm2;
@@ -258,7 +353,6 @@ int wick_rocm_lfm2_load(wick_rocm_ctx *ctx, const struct wick_gguf *gguf, uint32
  * attention's cache traffic; every cached value is rounded once, to nearest even, when it is appended (or moved by
  * wick_rocm_lfm2_shift_kv), all arithmetic stays f32.  Snapshots then hold f16 rows (wick_rocm_lfm2_layer_state_bytes says
  * how many bytes). */
-enum { WICK_ROCM_KV_F32 = 0, WICK_ROCM_KV_F16 = 1 };
 int wick_rocm_lfm2_load_kv(wick_rocm_ctx *ctx, const struct wick_gguf *gguf, uint32_t context_size, int kv_dtype, wick_rocm_lfm2 **out);
 int wick_rocm_lfm2_kv_dtype(const wick_rocm_lfm2 *model);
 int wick_rocm_lfm2_free(wick_rocm_ctx *ctx, wick_rocm_lfm2 *model);

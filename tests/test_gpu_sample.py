@@ -1,0 +1,180 @@
+"""Sampling on the GPU against the rule in f64 (paged_ref.py).  A pick may differ where the uniform number lies within 1e-9 of a border of the mass: masses are
+whole numbers of 2^-43 of the largest token's, up to 2^19 of them each off by half of one."""
+import numpy as np
+import pytest
+
+import paged_ref as R
+import wick_amd as W
+from wick_amd import lfm2
+from wick_amd.lfm2 import NO_TOKEN, Lfm2Ops
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture()
+def run(ctx):
+    """(logits, [(temperature, top_k, top_p, min_p)], u) -> (tokens, probabilities)"""
+    ops = Lfm2Ops(ctx)
+
+    def go(logits, params, u, stride=None, prob=True):
+        rows, n = logits.shape
+        stride = stride or n
+        wide = np.full((rows, stride), 1e9, np.float32)  # (what is behind a row would be taken)
+        wide[:, :n] = logits
+        bufs = [ctx.to_device(x) for x in (wide, lfm2.sample_params(params).view(np.uint32), np.asarray(u, np.float32), np.full(rows, 12345, np.uint32),
+                                           np.full(rows, 2.0, np.float32), np.full(lfm2.sample_scratch_bytes(rows, n), 0xff, np.uint8))]
+        ops.sample(bufs[0], stride, rows, n, bufs[1], bufs[2], bufs[3], bufs[4] if prob else None, bufs[5])
+        got = bufs[3].download(np.uint32, rows), bufs[4].download(np.float32, rows)
+        for b in bufs:
+            b.free()
+        return got
+
+    return go
+
+
+def check(got, logits, params, u):
+    held = lfm2.sample_params(params).tolist()  # (as the call has them: f32)
+    for r in range(len(logits)):
+        token, prob, border = R.sample(logits[r], *held[r], u[r])
+        if border < 1e-9:
+            continue
+        assert got[0][r] == token, (r, params[r], u[r], border)
+        assert abs(got[1][r] - prob) <= 2.0 ** -24 * prob + 1e-9 * prob, (r, params[r])  # rounded once
+
+
+def logits_of(seed, rows, n, spread=3.0):
+    return (spread * np.random.default_rng(seed).standard_normal((rows, n))).astype(np.float32)
+
+
+RULES = [(1.0, 0, 1.0, 0.0), (0.8, 40, 0.95, 0.05), (0.3, 0, 0.9, 0.0), (1.6, 0, 0.99, 0.0), (1.0, 1, 1.0, 0.0), (0.0, 50, 0.5, 0.1), (-1.0, 0, 1.0, 0.0), (1.0, 0, 1.0, 0.1),
+         (0.7, 500, 1.0, 0.0), (1.2, 7, 0.6, 0.0), (1.0, 0, 0.0, 0.0), (1.0, 0, 1e-6, 0.0), (2.0, 10 ** 9, 2.0, -1.0), (1.0, 0, 0.5, 1.0), (1.0, 0, 1.0, 7.0),
+         (float("nan"), 5, 0.5, 0.0), (1.0, 20, float("nan"), float("nan")), (0.05, 100, 0.9, 0.01), (50.0, 0, 0.7, 0.0), (1.0, 2, 0.999, 0.5)]
+
+
+@pytest.mark.parametrize("n", [1, 2, 63, 64, 65, 1000, 4095, 4096, 4097, 8193, 50257, 65536])
+def test_rules(run, n):
+    """Every rule, at uniform numbers from one end to the other; rows with a stride of their own."""
+    us = [0.0, 0.1, 0.37, 0.5, 0.93, 1 - 2.0 ** -24]
+    params = [p for p in RULES for _ in us]
+    u = np.array(us * len(RULES), np.float32)
+    logits = logits_of(n, len(params), n)
+    check(run(logits, params, u, stride=n + n % 5), logits, params, u)
+
+
+def test_a_large_vocabulary(run):
+    logits = logits_of(1, 6, 1 << 19)
+    params, u = RULES[:6], np.linspace(0.05, 0.95, 6, dtype=np.float32)
+    check(run(logits, params, u), logits, params, u)
+
+
+def test_many_rows(run):
+    logits = logits_of(2, 3000, 700)
+    params, u = [RULES[r % len(RULES)] for r in range(3000)], np.random.default_rng(3).random(3000, dtype=np.float32)
+    check(run(logits, params, u), logits, params, u)
+
+
+@pytest.mark.parametrize("n", [5, 1024, 1025, 3000, 20000])
+def test_equal_logits(run, n):
+    """Ties go to the lowest index, whatever cuts them: all alike, two values, and whole numbers only."""
+    rng = np.random.default_rng(n)
+    logits = np.stack([np.zeros(n), np.full(n, -3.5), (np.arange(n) % 2) * 1.0, rng.integers(0, 4, n) * 1.0, rng.integers(-3, 1, n) * 0.5, -(np.arange(n) // 7 % 3) * 1.0]).astype(np.float32)
+    logits = np.tile(logits, (len(RULES), 1))
+    params, u = [p for p in RULES for _ in range(6)], np.random.default_rng(1).random(6 * len(RULES), dtype=np.float32)
+    check(run(logits, params, u), logits, params, u)
+
+
+def test_flat_rows_list_more_than_a_workgroup(run):
+    """Logits so close together that the cut's bin holds thousands, none of them alike."""
+    logits = logits_of(4, 8, 30000, spread=0.01)
+    params, u = [(1.0, 777, 1.0, 0.0), (1.0, 20000, 0.5, 0.0), (1.0, 0, 0.3, 0.0), (1.0, 0, 0.999, 0.0), (1.0, 29999, 1.0, 0.0), (0.5, 1, 1.0, 0.0), (1.0, 15000, 0.9, 0.98),
+                 (1.0, 12345, 0.00001, 0.0)], np.linspace(0.01, 0.99, 8, dtype=np.float32)
+    check(run(logits, params, u), logits, params, u)
+
+
+def test_ruled_out_tokens(run):
+    """-infinity and NaN are never taken; a row of nothing else has no token; one alone is taken for certain; the lowest float is a token like others."""
+    n = 5000
+    logits = logits_of(5, 8, n)
+    logits[0] = -np.inf
+    logits[1] = np.nan
+    logits[2], logits[2, 4321] = -np.inf, -7.0
+    logits[3, ::2], logits[3, 1::4] = -np.inf, np.nan
+    logits[4] = np.finfo(np.float32).min
+    logits[5], logits[5, 17] = np.finfo(np.float32).min, 0.0
+    logits[6, :4990] = np.nan
+    logits[7] = np.where(np.arange(n) % 2, -np.inf, np.nan)
+    for rule in RULES:
+        params, u = [rule] * 8, np.array([0.5, 0.5, 0.999, 0.3, 0.25, 0.99, 0.6, 0.1], np.float32)
+        got = run(logits, params, u)
+        check(got, logits, params, u)
+        assert got[0][0] == got[0][1] == got[0][7] == NO_TOKEN and got[1][0] == got[1][1] == got[1][7] == 0
+        assert got[0][2] == 4321 and got[1][2] == 1 and got[0][3] % 4 == 3
+
+
+def test_infinite_logits(run):
+    """+infinity leaves nothing for the finite ones; several share alike."""
+    logits = logits_of(6, 4, 900)
+    logits[0, 700] = logits[1, 5] = logits[1, 800] = np.inf
+    logits[2, :300], logits[2, 400] = np.inf, -np.inf
+    logits[3] = np.inf
+    u = np.array([0.9, 0.6, 0.5, 0.25], np.float32)
+    for rule in [(1.0, 0, 1.0, 0.0), (0.7, 100, 0.9, 0.0), (1e-30, 0, 1.0, 0.5)]:
+        got = run(logits, [rule] * 4, u)
+        check(got, logits, [rule] * 4, u)
+        assert got[0][0] == 700
+
+
+@pytest.mark.parametrize("temperature", [1e-45, 1e-30, 1e-3, 1e6, 3e38, float("inf")])
+def test_extreme_temperatures(run, temperature):
+    logits = np.concatenate([logits_of(7, 2, 3000), logits_of(8, 1, 3000) * 1e30, logits_of(9, 1, 3000) * 1e-30])
+    params, u = [(temperature, 0, 1.0, 0.0), (temperature, 10, 0.9, 0.0), (temperature, 0, 0.7, 0.0), (temperature, 0, 1.0, 0.1)], np.array([0.2, 0.7, 0.5, 0.4], np.float32)
+    check(run(logits, params, u), logits, params, u)
+
+
+def test_logits_far_from_zero(run):
+    """A common offset takes no bits from what is between the logits."""
+    base = np.round(logits_of(10, 4, 3000) * 16) / 16
+    for offset in (-1e4, 300.0, 1e5):
+        logits = (base + np.float32(offset)).astype(np.float32)
+        params, u = RULES[:4], np.array([0.2, 0.7, 0.5, 0.4], np.float32)
+        check(run(logits, params, u), logits, params, u)
+
+
+def test_uniform_numbers_outside_their_range(run):
+    logits = logits_of(11, 6, 300)
+    u = np.array([-0.5, 1.0, 1.5, np.nan, np.inf, -np.inf], np.float32)
+    got = run(logits, [(1.0, 0, 1.0, 0.0)] * 6, u)
+    for r, last in enumerate((False, True, True, False, True, False)):
+        assert got[0][r] == (299 if last else 0)
+
+
+def test_without_probabilities_and_in_every_run_the_same(run):
+    logits = logits_of(12, 50, 50257)
+    params, u = [RULES[r % 4] for r in range(50)], np.random.default_rng(4).random(50, dtype=np.float32)
+    a, b, c = run(logits, params, u), run(logits, params, u), run(logits, params, u, prob=False)
+    assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1]) and np.array_equal(a[0], c[0]) and np.all(c[1] == 2.0)
+
+
+def test_picks_follow_the_probabilities(run):
+    """Over a grid of uniform numbers every token comes up in proportion: the k-th of m equal steps is the f64 rule's."""
+    m = 4000
+    logits = np.repeat(logits_of(13, 1, 37), m, 0)
+    u = ((np.arange(m) + 0.5) / m).astype(np.float32)
+    got = run(logits, [(1.0, 20, 0.9, 0.01)] * m, u)
+    index, w = R.kept(logits[0], 1.0, 20, 0.9, 0.01)
+    assert np.all(np.diff(got[0].astype(int)) >= 0)
+    share = np.bincount(got[0], minlength=37)[index] / m
+    assert np.all(np.abs(share - w / w.sum()) <= 1.5 / m) and set(got[0]) <= set(index)
+
+
+def test_greedy_rows_are_the_largest(ctx, run):
+    """Where the largest logit is one alone, temperature 0 is wick_rocm_argmax."""
+    logits = logits_of(14, 5, 65536)
+    got = run(logits, [(0.0, 0, 1.0, 0.0)] * 5, np.zeros(5))
+    out = ctx.alloc(4)
+    for r in range(5):
+        x = ctx.to_device(logits[r])
+        Lfm2Ops(ctx).argmax(x, 65536, out)
+        assert got[0][r] == out.download(np.uint32, 1)[0] and got[1][r] == 1
+        x.free()
+    out.free()

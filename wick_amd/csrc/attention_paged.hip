@@ -1,0 +1,425 @@
+// Attention of one new token of every sequence over KV caches in pages (wick_rocm_kv_pages), on the matrix cores.
+//
+// With G = n_heads / n_kv_heads, the G query heads of a KV head read the same keys and values: up to 16 of them are one operand of
+// 16x16 matrix instructions, both products transposed (a wave walks 32 rows of the cache at a time, as two halves of 16):
+//   S^T[row][head] = sum_d K[row][d] Q[head][d]        lane l is left with rows 4 (l / 16) + i of each half for head l % 16;
+//   O^T[d][head]  += sum_row V[row][d] P[row][head]    whose operand P is, per lane, the weights as they are in its registers: a matrix
+//                                                      instruction's K steps are in any order, so a lane just reads the values of those rows.
+// Nothing goes through LDS on the way: keys are read 16 bytes a lane in the operand's own order, values as 16 (or fewer) bytes of each of the
+// lane's rows, from which the operand of dimension e is picked lane by lane.
+//   f16 pages: v_mfma_f32_16x16x32_f16; the cached values are exact operands, a query row (scaled by a power of two to below 2^15) and the softmax weights (times
+//   2^15) are split into two halves: a product with one is off by at most 2^-22 of it, or 2^-39 of the row's largest.  Two products.
+//   f32 pages: v_mfma_f32_16x16x4_f32, f32 products as they are.
+// The softmax is a running one: maximum and sum of every head, rescaled when a tile has a larger score.
+//
+// The work of all sequences is one list of units of kUnitRows rows of one KV head (and 16 of its query heads), sequence by sequence, head by head; every
+// workgroup takes an equal, contiguous share, whatever the lengths.  What covers a head's rows completely is written out; a share's
+// first and last piece otherwise leave {maximum, sum, values} in the scratch, which a second launch joins.
+#include <algorithm>
+
+#include "kv_paged_device.h"
+#include "wick_rocm_internal.h"
+
+namespace wick_rocm {
+
+namespace {
+
+constexpr uint32_t kUnitRows = 128, kTileRows = 32, kWaves = 4;  // a unit is a tile of each wave
+constexpr uint32_t kShares = 512;                                // workgroups: two on each of 256 CUs
+constexpr uint32_t kRecordHead = 4;                              // floats of a record in front of its values: maximum, sum, -, -
+constexpr float kHalfScale = 32768.0f;                           // softmax weights are split below or at a half's largest power of two
+constexpr float kLog2e = 1.44269504088896340736f;
+
+struct PagedAttentionArgs {
+    const float* q;
+    const void* pages[2];  // keys, values
+    const uint32_t *table, *lens;
+    float* out;
+    float* parts;  // [shares][2][records of a piece][kRecordHead + head_dim]
+    uint32_t n_seqs, max_pages, n_pages, page_shift, q_stride, out_stride, n_heads, n_kv_heads, group, tiles;  // tiles: of 16 query heads, of a KV head
+    float scale;
+};
+
+__device__ __forceinline__ uint32_t length(const PagedAttentionArgs& a, uint32_t s) { return min(a.lens[s], a.max_pages << a.page_shift); }
+__device__ __forceinline__ uint32_t units_of(uint32_t len) { return (len + kUnitRows - 1u) / kUnitRows; }
+
+// Sum over the wave's lanes up to this one.
+__device__ __forceinline__ uint32_t lanes_upto(uint32_t v) {
+    const uint32_t lane = threadIdx.x & 63u;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t other = __shfl_up(v, d, 64);
+        if (lane >= (uint32_t)d) v += other;
+    }
+    return v;
+}
+
+// Units of all sequences, and of those in front of sequence `upto`.
+__device__ __forceinline__ uint32_t all_units(const PagedAttentionArgs& a, uint32_t heads, uint32_t upto, uint32_t& before) {
+    uint32_t sum = 0, front = 0;
+    for (uint32_t s = threadIdx.x & 63u; s < a.n_seqs; s += 64u) {
+        const uint32_t n = units_of(length(a, s)) * heads;
+        sum += n, front += s < upto ? n : 0u;
+    }
+    before = (uint32_t)__builtin_amdgcn_readlane((int)lanes_upto(front), 63);
+    return (uint32_t)__builtin_amdgcn_readlane((int)lanes_upto(sum), 63);
+}
+
+// The sequence that unit u is one of, and the units in front of it.
+__device__ __forceinline__ uint32_t find_unit(const PagedAttentionArgs& a, uint32_t heads, uint32_t u, uint32_t& before) {
+    before = 0;
+    for (uint32_t base = 0;; base += 64u) {
+        const uint32_t s = base + (threadIdx.x & 63u), n = s < a.n_seqs ? units_of(length(a, s)) * heads : 0u, upto = lanes_upto(n);
+        const uint64_t past = __ballot(before + upto > u);
+        if (past != 0 || base + 64u >= a.n_seqs) {
+            const int lane = past != 0 ? __ffsll((unsigned long long)past) - 1 : 63;
+            before += (uint32_t)__builtin_amdgcn_readlane((int)(upto - n), lane);
+            return base + (uint32_t)lane;
+        }
+        before += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+    }
+}
+
+__device__ __forceinline__ uint32_t share_begin(uint32_t units, uint32_t w, uint32_t shares) { return (uint32_t)((uint64_t)units * w / shares); }
+__device__ __forceinline__ uint32_t share_of(uint32_t units, uint32_t u, uint32_t shares) { return (uint32_t)((((uint64_t)u + 1) * shares - 1) / units); }
+
+template <typename KV, int HD>
+struct Tile {
+    static constexpr bool kF16 = sizeof(KV) == 2;
+    static constexpr int kPer = HD / 16;                         // values of a row that a lane holds
+    static constexpr int kVec = kPer < (kF16 ? 8 : 4) ? kPer : (kF16 ? 8 : 4);  // ... in one load
+    static constexpr int kLoads = kPer / kVec;
+    static constexpr int kSteps = kF16 ? HD / 32 : HD / 16;      // 16-byte loads of a key
+    typedef KV kvec __attribute__((ext_vector_type(kF16 ? 8 : 4)));
+    typedef KV vvec __attribute__((ext_vector_type(kVec)));
+    kvec k[2][kSteps];
+    vvec v[2][4][kLoads];
+};
+
+template <typename KV, int HD>
+struct Query;
+template <int HD>
+struct Query<_Float16, HD> {
+    h8 hi[HD / 32], lo[HD / 32];
+    float factor;
+    __device__ __forceinline__ void load(const float* q, bool there, float scale) {
+        const uint32_t g = (threadIdx.x & 63u) >> 4;
+        v4f x[HD / 32][2];
+        float top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < HD / 32; j++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                x[j][i] = there ? *reinterpret_cast<const v4f*>(q + 32 * j + 8u * g + 4 * i) : v4f{0, 0, 0, 0};
+#pragma unroll
+                for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(x[j][i][e]));
+            }
+        top = groups_max(top);
+        const int e = max(__builtin_amdgcn_frexp_expf(top), -100) - 15;  // (from 2^-100 down no score matters)
+        factor = ldexpf(scale * kLog2e, e);
+#pragma unroll
+        for (int j = 0; j < HD / 32; j++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float y = ldexpf(x[j][i / 4][i % 4], -e);
+                hi[j][i] = (_Float16)y, lo[j][i] = (_Float16)(y - (float)hi[j][i]);
+            }
+    }
+    __device__ __forceinline__ v4f scores(const typename Tile<_Float16, HD>::kvec (&k)[HD / 32]) const {
+        v4f s = {0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < HD / 32; j++) {
+            s = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[j], lo[j], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[j], hi[j], s, 0, 0, 0);
+        }
+        return s;
+    }
+};
+template <int HD>
+struct Query<float, HD> {
+    v4f x[HD / 16];
+    float factor;
+    __device__ __forceinline__ void load(const float* q, bool there, float scale) {
+        const uint32_t g = (threadIdx.x & 63u) >> 4;
+#pragma unroll
+        for (int j = 0; j < HD / 16; j++) x[j] = there ? *reinterpret_cast<const v4f*>(q + 16 * j + 4u * g) : v4f{0, 0, 0, 0};
+        factor = scale * kLog2e;
+    }
+    __device__ __forceinline__ v4f scores(const typename Tile<float, HD>::kvec (&k)[HD / 16]) const {
+        v4f s = {0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < HD / 16; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[j][e], x[j][e], s, 0, 0, 0);
+        return s;
+    }
+};
+
+// What a wave has gathered of a piece: per lane its head's maximum (of a power of two), the sum over its own rows, and 4 dimensions of every tile of the values.
+template <typename KV, int HD>
+struct State {
+    typedef Tile<KV, HD> T;
+    float m = -__builtin_inff(), l = 0.0f;
+    v4f o[T::kPer];
+
+    // The value of dimension (x, e) of m index i is x * 16 kVec + kVec i + e.
+    __device__ __forceinline__ void add(const T& t, const float (&s)[8]) {
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 8; i++) top = fmaxf(top, s[i]);
+        if (__any(top > m)) {
+            const float now = fmaxf(m, groups_max(top)), less = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now);
+#pragma unroll
+            for (int d = 0; d < T::kPer; d++) o[d] *= less;
+            l *= less, m = now;
+        }
+        const float from = m == -__builtin_inff() ? 0.0f : m;
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) p[i] = __builtin_amdgcn_exp2f(s[i] - from);
+        l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+        if constexpr (T::kF16) {
+            h8 hi, lo;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float y = p[i] * kHalfScale;
+                hi[i] = (_Float16)y, lo[i] = (_Float16)(y - (float)hi[i]);
+            }
+#pragma unroll
+            for (int x = 0; x < T::kLoads; x++)
+#pragma unroll
+                for (int e = 0; e < T::kVec; e++) {
+                    const h8 v = {t.v[0][0][x][e], t.v[0][1][x][e], t.v[0][2][x][e], t.v[0][3][x][e], t.v[1][0][x][e], t.v[1][1][x][e], t.v[1][2][x][e], t.v[1][3][x][e]};
+                    v4f& d = o[x * T::kVec + e];
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo, d, 0, 0, 0);
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi, d, 0, 0, 0);
+                }
+        } else {
+#pragma unroll
+            for (int half = 0; half < 2; half++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int x = 0; x < T::kLoads; x++)
+#pragma unroll
+                        for (int e = 0; e < T::kVec; e++) {
+                            v4f& d = o[x * T::kVec + e];
+                            d = __builtin_amdgcn_mfma_f32_16x16x4f32(t.v[half][i][x][e], p[4 * half + i], d, 0, 0, 0);
+                        }
+        }
+    }
+};
+
+// One tile's rows: those at or behind `len` read the last one's (their weights are zero).  `there`: bit h: half h has a page.
+template <typename KV, int HD>
+__device__ __forceinline__ uint32_t load_tile(const PagedAttentionArgs& a, const uint32_t* table, uint32_t c, uint32_t first, uint32_t len, Tile<KV, HD>& t) {
+    typedef Tile<KV, HD> T;
+    const uint32_t lane = threadIdx.x & 63u, l16 = lane & 15u, g = lane >> 4, inside = (1u << a.page_shift) - 1u;
+    uint32_t there = 0;
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+        const uint32_t row0 = first + 16u * half, page = table[min(row0, len - 1u) >> a.page_shift];
+        if (page < a.n_pages) there |= 1u << half;
+        const size_t base = ((size_t)(page < a.n_pages ? page : 0u) * a.n_kv_heads + c) << a.page_shift;
+        const KV* const k = static_cast<const KV*>(a.pages[0]) + (base + (min(row0 + l16, len - 1u) & inside)) * HD + (T::kF16 ? 8u : 4u) * g;
+#pragma unroll
+        for (int j = 0; j < T::kSteps; j++) t.k[half][j] = *reinterpret_cast<const typename T::kvec*>(k + j * (T::kF16 ? 32 : 16));
+    }
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+        const uint32_t row0 = first + 16u * half, page = table[min(row0, len - 1u) >> a.page_shift];
+        const size_t base = ((size_t)(page < a.n_pages ? page : 0u) * a.n_kv_heads + c) << a.page_shift;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const KV* const v = static_cast<const KV*>(a.pages[1]) + (base + (min(row0 + 4u * g + i, len - 1u) & inside)) * HD + T::kVec * l16;
+#pragma unroll
+            for (int x = 0; x < T::kLoads; x++) t.v[half][i][x] = *reinterpret_cast<const typename T::vvec*>(v + x * 16 * T::kVec);
+        }
+    }
+    return there;
+}
+
+// A half without a page: its values are zeros, whatever was read.
+template <typename KV, int HD>
+__device__ __forceinline__ void clear_values(Tile<KV, HD>& t, uint32_t there) {
+#pragma unroll
+    for (int half = 0; half < 2; half++)
+        if ((there >> half & 1u) == 0)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int x = 0; x < Tile<KV, HD>::kLoads; x++) t.v[half][i][x] = typename Tile<KV, HD>::vvec(0);
+}
+
+template <typename KV, int HD>
+__global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attention_paged_kernel(PagedAttentionArgs a) {
+    typedef Tile<KV, HD> T;
+    constexpr uint32_t kRow = HD + 4;  // floats of a head's values in LDS
+    __shared__ __align__(16) float values[kWaves][16][kRow];
+    __shared__ float tops[kWaves][16], sums[kWaves][16];
+    const uint32_t lane = threadIdx.x & 63u, l16 = lane & 15u, g = lane >> 4;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint32_t heads = a.n_kv_heads * a.tiles;
+    uint32_t before;
+    const uint32_t units = all_units(a, heads, 0, before), shares = min(units, kShares);  // (no share is empty)
+    if (blockIdx.x >= shares) return;
+    const uint32_t begin = share_begin(units, blockIdx.x, shares), end = share_begin(units, blockIdx.x + 1u, shares);
+    uint32_t s = find_unit(a, heads, begin, before);
+    const uint32_t records = min(a.group, 16u);
+    for (uint32_t u = begin; u < end && s < a.n_seqs;) {
+        const uint32_t len = length(a, s), chunks = units_of(len);
+        if (u - before >= chunks * heads) {  // (the next sequence; one without rows has no units)
+            before += chunks * heads, s++;
+            continue;
+        }
+        const uint32_t head = (u - before) / chunks, chunk = (u - before) % chunks, take = min(chunks - chunk, end - u);
+        const uint32_t c = head / a.tiles, h0 = c * a.group + head % a.tiles * 16u, h_count = min(a.group - head % a.tiles * 16u, 16u);
+        const uint32_t* const table = a.table + (size_t)s * a.max_pages;
+        Query<KV, HD> q;
+        q.load(a.q + (size_t)s * a.q_stride + (size_t)(h0 + min(l16, h_count - 1u)) * HD, l16 < h_count, a.scale);
+        State<KV, HD> st;
+#pragma unroll
+        for (int d = 0; d < T::kPer; d++) st.o[d] = v4f{0, 0, 0, 0};
+        const uint32_t last = min(len, (chunk + take) * kUnitRows);
+        for (uint32_t first = chunk * kUnitRows + wave * kTileRows; first < last; first += kUnitRows) {
+            T t;
+            const uint32_t there = load_tile(a, table, c, first, len, t);
+            float sc[8];
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                const v4f x = q.scores(t.k[half]);
+#pragma unroll
+                for (int i = 0; i < 4; i++) sc[4 * half + i] = x[i] * q.factor;
+            }
+            if (first + kTileRows > len || there != 3u) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (first + 16u * (i / 4) + 4u * g + i % 4 >= len || (there >> (i / 4) & 1u) == 0) sc[i] = -__builtin_inff();
+                clear_values(t, there);
+            }
+            st.add(t, sc);
+        }
+        // The waves' states, one head after another
+        st.l = groups_sum(st.l);
+        if (g == 0) tops[wave][l16] = st.m, sums[wave][l16] = st.l;
+#pragma unroll
+        for (int x = 0; x < T::kLoads; x++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int e = 0; e < T::kVec; e++) values[wave][l16][x * 16 * T::kVec + T::kVec * (4u * g + r) + e] = st.o[x * T::kVec + e][r];
+        __syncthreads();
+        const bool whole = take == chunks;
+        for (uint32_t i = threadIdx.x; i < h_count * (HD / 4); i += 64u * kWaves) {
+            const uint32_t h = i / (HD / 4), d = i % (HD / 4) * 4u;
+            float top = tops[0][h];
+#pragma unroll
+            for (uint32_t w = 1; w < kWaves; w++) top = fmaxf(top, tops[w][h]);
+            const float from = top == -__builtin_inff() ? 0.0f : top;
+            float sum = 0.0f;
+            v4f v = {0, 0, 0, 0};
+#pragma unroll
+            for (uint32_t w = 0; w < kWaves; w++) {
+                const float less = __builtin_amdgcn_exp2f(tops[w][h] - from);
+                sum += sums[w][h] * less;
+                v += *reinterpret_cast<const v4f*>(&values[w][h][d]) * less;
+            }
+            if (whole) {
+                const float inverse = sum == 0.0f ? 0.0f : 1.0f / (T::kF16 ? sum * kHalfScale : sum);
+                *reinterpret_cast<v4f*>(a.out + (size_t)s * a.out_stride + (size_t)(h0 + h) * HD + d) = v * inverse;
+            } else {
+                float* const to = a.parts + ((size_t)(blockIdx.x * 2u + (u == begin ? 0u : 1u)) * records + h) * (kRecordHead + HD);
+                if (d == 0) to[0] = top, to[1] = T::kF16 ? sum * kHalfScale : sum;
+                *reinterpret_cast<v4f*>(to + kRecordHead + d) = v;
+            }
+        }
+        __syncthreads();
+        u += take;
+    }
+}
+
+// One workgroup a sequence and query head: nothing to do where one share has the whole head, zeros where there is no row.
+template <int HD>
+__global__ __launch_bounds__(256) void attention_paged_join_kernel(PagedAttentionArgs a) {
+    __shared__ float weights[kShares];
+    __shared__ __align__(16) float values[256 / (HD / 4)][HD];
+    __shared__ float tops[4], totals[4];
+    const uint32_t s = blockIdx.x / a.n_heads, h = blockIdx.x % a.n_heads, heads = a.n_kv_heads * a.tiles, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    float* const out = a.out + (size_t)s * a.out_stride + (size_t)h * HD;
+    uint32_t before;
+    const uint32_t units = all_units(a, heads, s, before), chunks = units_of(length(a, s)), shares = min(units, kShares);
+    if (chunks == 0) {
+        if (threadIdx.x < HD / 4) reinterpret_cast<v4f*>(out)[threadIdx.x] = v4f{0, 0, 0, 0};
+        return;
+    }
+    const uint32_t c = h / a.group, in_group = h % a.group, u0 = before + (c * a.tiles + in_group / 16u) * chunks;
+    const uint32_t w0 = share_of(units, u0, shares), w1 = share_of(units, u0 + chunks - 1u, shares), n = w1 - w0 + 1u;
+    if (n == 1) return;
+    const uint32_t records = min(a.group, 16u);
+    const auto record = [&](uint32_t i) {
+        const uint32_t slot = i == 0 && share_begin(units, w0, shares) != u0 ? 1u : 0u;
+        return a.parts + ((size_t)((w0 + i) * 2u + slot) * records + in_group % 16u) * (kRecordHead + HD);
+    };
+    float top = -__builtin_inff();
+    for (uint32_t i = threadIdx.x; i < n; i += 256u) top = fmaxf(top, record(i)[0]);
+    top = wave_max_f32(top);
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    const float from = top == -__builtin_inff() ? 0.0f : top;
+    float sum = 0.0f;
+    for (uint32_t i = threadIdx.x; i < n; i += 256u) {
+        const float* const r = record(i);
+        const float w = __builtin_amdgcn_exp2f(r[0] - from);
+        weights[i] = w, sum += w * r[1];
+    }
+    sum = wave_sum_f32(sum);
+    if (lane == 0) totals[wave] = sum;
+    __syncthreads();
+    sum = (totals[0] + totals[1]) + (totals[2] + totals[3]);
+    constexpr uint32_t kQuads = HD / 4, kGroups = 256 / kQuads;
+    const uint32_t d = threadIdx.x % kQuads, part = threadIdx.x / kQuads;
+    v4f v = {0, 0, 0, 0};
+    for (uint32_t i = part; i < n; i += kGroups) v += *reinterpret_cast<const v4f*>(record(i) + kRecordHead + 4u * d) * weights[i];
+    reinterpret_cast<v4f*>(values[part])[d] = v;
+    __syncthreads();
+    if (threadIdx.x < kQuads) {
+        for (uint32_t p = 1; p < kGroups; p++) v += reinterpret_cast<const v4f*>(values[p])[d];
+        reinterpret_cast<v4f*>(out)[d] = v * (sum == 0.0f ? 0.0f : 1.0f / sum);
+    }
+}
+
+template <typename KV, int HD>
+hipError_t launch_paged(const PagedAttentionArgs& a, const Launch& L) {
+    hipError_t e = launch_kernel(L, kFamOther, attention_paged_kernel<KV, HD>, dim3(kShares), dim3(64 * kWaves), a);
+    if (e != hipSuccess) return e;
+    return launch_kernel(L, kFamOther, attention_paged_join_kernel<HD>, dim3(a.n_seqs * a.n_heads), dim3(256), a);
+}
+
+template <typename KV>
+hipError_t launch_paged(const PagedAttentionArgs& a, uint32_t head_dim, const Launch& L) {
+    return head_dim == 32 ? launch_paged<KV, 32>(a, L) : head_dim == 64 ? launch_paged<KV, 64>(a, L) : head_dim == 128 ? launch_paged<KV, 128>(a, L) : launch_paged<KV, 256>(a, L);
+}
+
+}  // namespace
+
+bool attention_paged_fits(const wick_rocm_kv_pages& p, uint32_t n_heads, uint32_t n_kv_heads) {
+    const uint64_t tiles = (n_heads / n_kv_heads + 15u) / 16u, chunks = ((uint64_t)p.max_pages * p.page_rows + kUnitRows - 1u) / kUnitRows;
+    // (each factor is at most 2^30)
+    return p.n_seqs * chunks <= UINT32_MAX / 2u / (n_kv_heads * tiles) && (uint64_t)p.n_seqs * n_heads <= INT32_MAX;
+}
+
+size_t attention_paged_scratch_floats(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim) {
+    return (size_t)kShares * 2 * std::min(n_heads / n_kv_heads, 16u) * (kRecordHead + head_dim);
+}
+
+hipError_t launch_attention_paged(const wick_rocm_kv_pages& p, const float* d_q, uint32_t q_stride, const void* d_k_pages, const void* d_v_pages, bool kv_f16,
+                                  float* d_out, uint32_t out_stride, float* d_scratch, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, float scale,
+                                  const Launch& L) {
+    const uint32_t group = n_heads / n_kv_heads;
+    const PagedAttentionArgs a{d_q, {d_k_pages, d_v_pages}, p.d_table, p.d_lens, d_out, d_scratch, p.n_seqs, p.max_pages, p.n_pages, (uint32_t)__builtin_ctz(p.page_rows),
+                               q_stride, out_stride, n_heads, n_kv_heads, group, (group + 15u) / 16u, scale};
+    return kv_f16 ? launch_paged<_Float16>(a, head_dim, L) : launch_paged<float>(a, head_dim, L);
+}
+
+}  // namespace wick_rocm

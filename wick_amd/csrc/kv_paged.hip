@@ -1,0 +1,391 @@
+// KV caches in pages that sequences share: rows appended, and what is done to pages themselves -- sequences forked and cut, pages taken for new rows (with
+// a copy of a page that others hold too), the pool moved together.  Who holds what is in the table, lens and refs of wick_rocm_kv_pages, all on the device.
+#include <algorithm>
+
+#include "kv_paged_device.h"
+#include "wick_rocm_internal.h"
+
+namespace wick_rocm {
+
+namespace {
+
+// ---- append --------------------------------------------------------------------------------------
+// One thread a 16-byte load of each source; bound by memory, and by the launch where there are few tokens.
+struct PagedAppendArgs {
+    const float* src[2];  // keys, values
+    void* pages[2];
+    const uint32_t *table, *start, *first;
+    uint32_t n_seqs, max_pages, n_pages, page_shift, n, n_kv_heads, head_dim, stride;
+};
+
+template <typename KV>
+__global__ __launch_bounds__(256) void kv_paged_append_kernel(PagedAppendArgs a) {
+    const uint32_t quads = a.n_kv_heads * a.head_dim / 4u;
+    const uint64_t at = (uint64_t)blockIdx.x * 256u + threadIdx.x;
+    if (at >= (uint64_t)a.n * quads) return;
+    const uint32_t j = (uint32_t)(at / quads), quad = (uint32_t)(at % quads), c = 4u * quad / a.head_dim, i = 4u * quad % a.head_dim;
+    uint32_t s = j, in = 0;
+    if (a.first) {  // the last sequence whose tokens begin at or before this one
+        uint32_t low = 0, high = a.n_seqs;
+        while (high - low > 1) {
+            const uint32_t mid = (low + high) / 2u;
+            (a.first[mid] <= j ? low : high) = mid;
+        }
+        s = low, in = j - a.first[s];
+        if (j < a.first[s] || j >= a.first[s + 1]) return;
+    }
+    const uint32_t start = a.start[s];
+    const uint64_t row = (uint64_t)start + in;
+    if (start == WICK_ROCM_NO_ROW || row >> a.page_shift >= a.max_pages) return;
+    const uint32_t page = a.table[(size_t)s * a.max_pages + (row >> a.page_shift)];
+    if (page >= a.n_pages) return;
+    const size_t to = ((((size_t)page * a.n_kv_heads + c) << a.page_shift) + (row & ((1u << a.page_shift) - 1u))) * a.head_dim + i;
+#pragma unroll
+    for (int which = 0; which < 2; which++) {
+        const float4 x = *reinterpret_cast<const float4*>(a.src[which] + (size_t)j * a.stride + 4u * quad);
+        KV* const p = static_cast<KV*>(a.pages[which]) + to;
+        if constexpr (sizeof(KV) == 4) {
+            *reinterpret_cast<float4*>(p) = x;
+        } else {
+            const h4 h = {(_Float16)x.x, (_Float16)x.y, (_Float16)x.z, (_Float16)x.w};
+            *reinterpret_cast<h4*>(p) = h;
+        }
+    }
+}
+
+// ---- fork, free ----------------------------------------------------------------------------------
+// A table's columns are independent of each other: a workgroup takes a few of them for all sequences, so that it has read every
+// parent's entries before it writes any, and one launch does it in place.  One workgroup more does the same with lens.
+constexpr uint32_t kForkEntries = 8192;  // of a workgroup (LDS); a power of two, at least the most sequences
+struct PagedForkArgs {
+    uint32_t *table, *lens, *refs;
+    const uint32_t* parents;
+    uint32_t n_seqs, max_pages, n_pages, columns;
+};
+
+__global__ __launch_bounds__(256) void kv_pages_fork_kernel(PagedForkArgs a) {
+    __shared__ uint32_t old[kForkEntries];
+    const bool is_lens = blockIdx.x == gridDim.x - 1u;
+    const uint32_t first = blockIdx.x * a.columns, columns = is_lens ? 1u : min(a.columns, a.max_pages - first);
+    uint32_t* const entries = is_lens ? a.lens : a.table + first;
+    const uint32_t stride = is_lens ? 1u : a.max_pages, none = is_lens ? 0u : WICK_ROCM_NO_PAGE;
+    for (uint32_t i = threadIdx.x; i < a.n_seqs * columns; i += 256u) old[i] = entries[(size_t)(i / columns) * stride + i % columns];
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < a.n_seqs * columns; i += 256u) {
+        const uint32_t s = i / columns, parent = a.parents[s];
+        if (parent == s) continue;
+        const uint32_t was = old[i], is = parent < a.n_seqs ? old[parent * columns + i % columns] : none;
+        if (was == is) continue;
+        entries[(size_t)s * stride + i % columns] = is;
+        if (is_lens) continue;
+        if (was < a.n_pages) atomicSub(&a.refs[was], 1u);
+        if (is < a.n_pages) atomicAdd(&a.refs[is], 1u);
+    }
+}
+
+struct PagedFreeArgs {
+    uint32_t *table, *lens, *refs;
+    const uint32_t* rows;
+    uint32_t n_seqs, max_pages, n_pages, page_shift;
+};
+
+__global__ __launch_bounds__(256) void kv_pages_free_kernel(PagedFreeArgs a) {
+    const uint64_t all = (uint64_t)a.n_seqs * a.max_pages;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256u) {
+        const uint32_t s = (uint32_t)(i / a.max_pages), p = (uint32_t)(i % a.max_pages), rows = a.rows[s];
+        if (p == 0 && rows < a.lens[s]) a.lens[s] = rows;
+        if (p < pages_of(rows, a.page_shift)) continue;
+        const uint32_t page = a.table[i];
+        if (page == WICK_ROCM_NO_PAGE) continue;
+        a.table[i] = WICK_ROCM_NO_PAGE;
+        if (page < a.n_pages) atomicSub(&a.refs[page], 1u);
+    }
+}
+
+// ---- the plan of a reservation or a compaction: one workgroup --------------------------------------
+constexpr uint32_t kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
+constexpr uint32_t kRun = 16;  // consecutive pages of a thread at a time
+
+// Sum over the workgroup's threads in front of this one, and over all of them.  `slots`: kPlanWaves, of this call until the next barrier.
+__device__ __forceinline__ uint32_t wave_sum_before(uint32_t v, uint32_t lane) {
+    uint32_t sum = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t other = __shfl_up(sum, d, 64);
+        if (lane >= (uint32_t)d) sum += other;
+    }
+    return sum;
+}
+__device__ __forceinline__ uint32_t sum_before(uint32_t v, uint32_t* slots, uint32_t& total) {
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, upto = wave_sum_before(v, lane);
+    __syncthreads();  // (slots are still read)
+    if (lane == 63u) slots[wave] = upto;
+    __syncthreads();
+    uint32_t before = upto - v;
+    total = 0;
+    for (uint32_t w = 0; w < kPlanWaves; w++) {
+        if (w < wave) before += slots[w];
+        total += slots[w];
+    }
+    return before;
+}
+
+// Bits of the pages [first, first + kRun) that are free; those behind the last page are not.
+__device__ __forceinline__ uint32_t free_bits(const uint32_t* refs, uint64_t first, uint32_t n_pages) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kRun; i++) bits |= (uint32_t)(first + i < n_pages && refs[first + i < n_pages ? first + i : 0] == 0) << i;
+    return bits;
+}
+
+struct PagedPlanArgs {
+    uint32_t *table, *lens, *refs, *start, *moves, *list;  // list: n_pages words behind the moves
+    const uint32_t* counts;
+    uint32_t n_seqs, max_pages, n_pages, page_shift;
+};
+
+// Pages for the new rows of every sequence.  A partial last page of c writers and r holders: where c = r the first writer keeps it and r - 1 copy, else all
+// c do.  Who is who is found in refs itself: every writer takes one off; where nothing is left the writers' largest n_seqs - s is put there.
+__global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(PagedPlanArgs a) {
+    __shared__ uint32_t slots[kPlanWaves], too_short, moved;
+    constexpr uint32_t kOwner = 0x80000000u, kMost = 4;  // sequences of a thread: 4096 in all
+    const uint32_t R = 1u << a.page_shift;
+    const uint64_t capacity = (uint64_t)a.max_pages << a.page_shift;
+    if (threadIdx.x == 0) too_short = 0, moved = 0;
+    __syncthreads();
+    uint32_t len[kMost], count[kMost], page[kMost], need[kMost];
+    bool copies[kMost];
+#pragma unroll
+    for (uint32_t k = 0; k < kMost; k++) {  // consecutive sequences a thread, in order
+        const uint32_t s = threadIdx.x * kMost + k;
+        len[k] = s < a.n_seqs ? a.lens[s] : 0, count[k] = s < a.n_seqs ? a.counts[s] : 0;
+        if ((uint64_t)len[k] + count[k] > capacity) too_short = 1;
+        page[k] = WICK_ROCM_NO_PAGE;
+        if (count[k] != 0 && len[k] % R != 0 && len[k] < capacity) page[k] = a.table[(size_t)s * a.max_pages + (len[k] >> a.page_shift)];
+        if (page[k] >= a.n_pages) page[k] = WICK_ROCM_NO_PAGE;
+        if (page[k] != WICK_ROCM_NO_PAGE) atomicSub(&a.refs[page[k]], 1u);
+    }
+    __threadfence();
+    __syncthreads();
+    bool alone[kMost];
+#pragma unroll
+    for (uint32_t k = 0; k < kMost; k++) alone[k] = page[k] != WICK_ROCM_NO_PAGE && __hip_atomic_load(&a.refs[page[k]], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t k = 0; k < kMost; k++)
+        if (alone[k]) atomicMax(&a.refs[page[k]], kOwner | (a.n_seqs - (threadIdx.x * kMost + k)));
+    __threadfence();
+    __syncthreads();
+    uint32_t mine = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < kMost; k++) {
+        const uint32_t s = threadIdx.x * kMost + k;
+        copies[k] = page[k] != WICK_ROCM_NO_PAGE;
+        if (alone[k] && __hip_atomic_load(&a.refs[page[k]], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (kOwner | (a.n_seqs - s))) copies[k] = false;
+        need[k] = count[k] == 0 ? 0 : pages_of((uint64_t)len[k] + count[k], a.page_shift) - pages_of(len[k], a.page_shift) + copies[k];
+        mine += need[k];
+    }
+    __syncthreads();  // (all have seen who keeps)
+#pragma unroll
+    for (uint32_t k = 0; k < kMost; k++)
+        if (page[k] != WICK_ROCM_NO_PAGE && !copies[k]) __hip_atomic_store(&a.refs[page[k]], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __threadfence();
+    uint32_t wanted;
+    uint32_t at = sum_before(mine, slots, wanted);
+    // the lowest free pages, as many as are wanted
+    uint32_t found = 0;
+    const bool fits_table = too_short == 0;
+    for (uint64_t base = 0; fits_table && base < a.n_pages && found < wanted; base += kRun * kPlanThreads) {
+        const uint64_t first = base + threadIdx.x * kRun;
+        uint32_t bits = free_bits(a.refs, first, a.n_pages), all;
+        uint32_t to = found + sum_before(__popc(bits), slots, all);
+        for (; bits != 0; bits &= bits - 1u, to++)
+            if (to < wanted) a.list[to] = (uint32_t)first + __ffs(bits) - 1u;
+        found += all;
+    }
+    __threadfence();
+    __syncthreads();
+    if (!fits_table || found < wanted) {  // nothing changes: what was taken off refs comes back
+#pragma unroll
+        for (uint32_t k = 0; k < kMost; k++) {
+            const uint32_t s = threadIdx.x * kMost + k;
+            if (copies[k]) atomicAdd(&a.refs[page[k]], 1u);
+            if (s < a.n_seqs) a.start[s] = WICK_ROCM_NO_ROW;
+        }
+        if (threadIdx.x == 0) a.moves[0] = 0, a.moves[1] = fits_table ? wanted - found : 0xffffffffu, a.moves[2] = 0, a.moves[3] = 0;
+        return;
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < kMost; k++) {
+        const uint32_t s = threadIdx.x * kMost + k;
+        if (s >= a.n_seqs) break;
+        a.start[s] = count[k] == 0 ? WICK_ROCM_NO_ROW : len[k];
+        if (count[k] == 0) continue;
+        a.lens[s] = len[k] + count[k];
+        uint32_t* const row = a.table + (size_t)s * a.max_pages;
+        uint32_t p = pages_of(len[k], a.page_shift);
+        if (copies[k]) {
+            const uint32_t to = a.list[at++], m = atomicAdd(&moved, 1u);
+            row[p - 1u] = to, a.refs[to] = 1;
+            uint32_t* const move = a.moves + 4u + 4u * m;
+            move[0] = page[k], move[1] = to, move[2] = len[k] % R, move[3] = 0;
+        }
+        for (uint32_t n = need[k] - copies[k]; n != 0; n--, p++) {
+            const uint32_t to = a.list[at++];
+            row[p] = to, a.refs[to] = 1;
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) a.moves[0] = moved, a.moves[1] = 0, a.moves[2] = 0, a.moves[3] = 0;
+}
+
+// With U pages in use: the i-th page in use at U or above goes to the i-th free one below.
+__global__ __launch_bounds__(kPlanThreads) void kv_pages_compact_kernel(PagedPlanArgs a) {
+    __shared__ uint32_t slots[kPlanWaves];
+    uint32_t free = 0;
+    for (uint64_t base = 0; base < a.n_pages; base += kRun * kPlanThreads) free += __popc(free_bits(a.refs, base + threadIdx.x * kRun, a.n_pages));
+    uint32_t all;
+    sum_before(free, slots, all);
+    const uint32_t used = a.n_pages - all;
+    uint32_t holes = 0, movers = 0;
+    for (uint64_t base = 0; base < a.n_pages; base += kRun * kPlanThreads) {
+        const uint64_t first = base + threadIdx.x * kRun;
+        const uint32_t bits = free_bits(a.refs, first, a.n_pages);
+        const uint32_t inside = first >= a.n_pages ? 0u : first + kRun <= a.n_pages ? 0xffffu : (1u << (a.n_pages - first)) - 1u;
+        const uint32_t below = first >= used ? 0u : first + kRun <= used ? 0xffffu : (1u << (used - first)) - 1u;
+        uint32_t hole = bits & below, mover = ~bits & inside & ~below, n;
+        const uint32_t before = sum_before(__popc(hole) | __popc(mover) << 16, slots, n);  // (at most 2^14 each)
+        uint32_t to = holes + (before & 0xffffu), from = movers + (before >> 16);
+        for (; hole != 0; hole &= hole - 1u) a.moves[4u + 4u * to++ + 1u] = (uint32_t)first + __ffs(hole) - 1u;
+        for (; mover != 0; mover &= mover - 1u) {
+            uint32_t* const move = a.moves + 4u + 4u * from++;
+            move[0] = (uint32_t)first + __ffs(mover) - 1u, move[2] = 1u << a.page_shift, move[3] = 0;
+        }
+        holes += n & 0xffffu, movers += n >> 16;
+    }
+    __threadfence();
+    __syncthreads();
+    for (uint32_t m = threadIdx.x; m < movers; m += kPlanThreads) {
+        const uint32_t from = a.moves[4u + 4u * m], to = a.moves[4u + 4u * m + 1u];
+        a.refs[to] = a.refs[from], a.refs[from] = 0;
+        a.list[from] = to;
+    }
+    if (threadIdx.x == 0) a.moves[0] = movers, a.moves[1] = used, a.moves[2] = 0, a.moves[3] = 0;
+}
+
+// ---- pages moved -----------------------------------------------------------------------------------
+// A unit is 1024 consecutive 16-byte pieces of a page in one plane, taken by the workgroups in turn; behind them, for a compaction, the
+// table's entries.  Bound by memory.
+struct PagedCopyArgs {
+    char* base;
+    size_t plane_bytes;
+    const uint32_t* moves;
+    uint32_t *table;       // entries from moves[1] on are replaced by `list` of them (null: none)
+    const uint32_t* list;
+    uint32_t max_moves, n_planes, n_pages, page_units, row_pieces, rows;  // row_pieces: pieces of a row of one head; rows: of a page
+    uint64_t entries;
+};
+constexpr uint32_t kUnit = 1024;
+
+__global__ __launch_bounds__(256) void kv_pages_copy_kernel(PagedCopyArgs a) {
+    const uint32_t moves = min(a.moves[0], a.max_moves), pieces = a.page_units;
+    const uint32_t per_page = (pieces + kUnit - 1u) / kUnit;
+    const uint64_t units = (uint64_t)moves * a.n_planes * per_page;
+    for (uint64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const uint32_t part = (uint32_t)(u % per_page), plane = (uint32_t)(u / per_page % a.n_planes), m = (uint32_t)(u / per_page / a.n_planes);
+        const uint4 move = *reinterpret_cast<const uint4*>(a.moves + 4u + 4u * (size_t)m);
+        if (move.x >= a.n_pages || move.y >= a.n_pages) continue;
+        char* const p = a.base + plane * a.plane_bytes;
+        const uint4* const from = reinterpret_cast<const uint4*>(p) + (size_t)move.x * pieces;
+        uint4* const to = reinterpret_cast<uint4*>(p) + (size_t)move.y * pieces;
+        uint4 x[kUnit / 256];
+        bool takes[kUnit / 256];
+#pragma unroll
+        for (uint32_t i = 0; i < kUnit / 256; i++) {
+            const uint32_t piece = part * kUnit + i * 256u + threadIdx.x;
+            takes[i] = piece < pieces && piece / a.row_pieces % a.rows < move.z;
+            if (takes[i]) x[i] = from[piece];
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kUnit / 256; i++)
+            if (takes[i]) to[part * kUnit + i * 256u + threadIdx.x] = x[i];
+    }
+    if (a.table == nullptr) return;
+    const uint32_t used = a.moves[1];
+    for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < a.entries; i += (uint64_t)gridDim.x * 256u) {
+        const uint32_t page = a.table[i];
+        if (page >= used && page < a.n_pages) a.table[i] = a.list[page];
+    }
+}
+
+uint32_t page_shift(const wick_rocm_kv_pages& p) { return (uint32_t)__builtin_ctz(p.page_rows); }
+
+size_t most_moves(const wick_rocm_kv_pages& p) { return std::max(p.n_seqs, p.n_pages / 2u); }
+
+uint32_t blocks(uint64_t threads, uint32_t most) { return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(most, (threads + 255u) / 256u)); }
+
+hipError_t launch_copy(const wick_rocm_kv_pages& p, const wick_rocm_kv_planes* planes, const uint32_t* d_moves, uint32_t max_moves, bool table, const Launch& L) {
+    PagedCopyArgs a{};
+    a.moves = d_moves, a.n_pages = p.n_pages, a.rows = p.page_rows;
+    uint64_t units = 0;
+    if (planes) {
+        const uint32_t element = planes->kv_dtype == WICK_ROCM_KV_F16 ? 2u : 4u;
+        a.base = static_cast<char*>(planes->d_base), a.plane_bytes = planes->plane_bytes, a.max_moves = max_moves, a.n_planes = planes->n_planes;
+        a.row_pieces = planes->head_dim * element / 16u, a.page_units = planes->n_kv_heads * p.page_rows * a.row_pieces;
+        units = (uint64_t)max_moves * planes->n_planes * ((a.page_units + kUnit - 1u) / kUnit);
+    } else {
+        a.page_units = 1, a.row_pieces = 1, a.n_planes = 1;
+    }
+    if (table) {
+        a.table = p.d_table, a.list = d_moves + 4u + 4u * most_moves(p), a.entries = (uint64_t)p.n_seqs * p.max_pages;
+        units = std::max(units, (a.entries + 255u) / 256u);
+    }
+    return launch_kernel(L, kFamOther, kv_pages_copy_kernel, dim3(blocks(units * 256u, 2048u)), dim3(256), a);
+}
+
+}  // namespace
+
+hipError_t launch_kv_paged_append(const wick_rocm_kv_pages& p, const float* d_k, const float* d_v, uint32_t kv_stride, void* d_k_pages, void* d_v_pages,
+                                  bool kv_f16, const uint32_t* d_start, const uint32_t* d_first, uint32_t n, uint32_t n_kv_heads, uint32_t head_dim,
+                                  const Launch& L) {
+    if (n == 0) return hipSuccess;
+    const PagedAppendArgs a{{d_k, d_v}, {d_k_pages, d_v_pages}, p.d_table, d_start, d_first, p.n_seqs, p.max_pages, p.n_pages, page_shift(p), n, n_kv_heads,
+                            head_dim, kv_stride};
+    const uint64_t threads = (uint64_t)n * (n_kv_heads * head_dim / 4u);
+    const dim3 grid((uint32_t)((threads + 255u) / 256u));
+    return kv_f16 ? launch_kernel(L, kFamOther, kv_paged_append_kernel<_Float16>, grid, dim3(256), a)
+                  : launch_kernel(L, kFamOther, kv_paged_append_kernel<float>, grid, dim3(256), a);
+}
+
+hipError_t launch_kv_pages_fork(const wick_rocm_kv_pages& p, const uint32_t* d_parents, const Launch& L) {
+    uint32_t columns = 16;
+    while (columns > 1 && columns * p.n_seqs > kForkEntries) columns /= 2u;
+    const PagedForkArgs a{p.d_table, p.d_lens, p.d_refs, d_parents, p.n_seqs, p.max_pages, p.n_pages, columns};
+    return launch_kernel(L, kFamOther, kv_pages_fork_kernel, dim3((p.max_pages + columns - 1u) / columns + 1u), dim3(256), a);
+}
+
+hipError_t launch_kv_pages_free(const wick_rocm_kv_pages& p, const uint32_t* d_rows, const Launch& L) {
+    const PagedFreeArgs a{p.d_table, p.d_lens, p.d_refs, d_rows, p.n_seqs, p.max_pages, p.n_pages, page_shift(p)};
+    return launch_kernel(L, kFamOther, kv_pages_free_kernel, dim3(blocks((uint64_t)p.n_seqs * p.max_pages, 2048u)), dim3(256), a);
+}
+
+size_t kv_pages_moves_words(const wick_rocm_kv_pages& p) { return 4 + 4 * most_moves(p) + p.n_pages; }
+
+hipError_t launch_kv_pages_reserve(const wick_rocm_kv_pages& p, const uint32_t* d_counts, uint32_t* d_start, uint32_t* d_moves, const wick_rocm_kv_planes* planes,
+                                   const Launch& L) {
+    const PagedPlanArgs a{p.d_table, p.d_lens, p.d_refs, d_start, d_moves, d_moves + 4u + 4u * most_moves(p), d_counts, p.n_seqs, p.max_pages, p.n_pages, page_shift(p)};
+    hipError_t e = launch_kernel(L, kFamOther, kv_pages_reserve_kernel, dim3(1), dim3(kPlanThreads), a);
+    return e != hipSuccess || !planes ? e : launch_copy(p, planes, d_moves, p.n_seqs, false, L);
+}
+
+hipError_t launch_kv_pages_compact(const wick_rocm_kv_pages& p, uint32_t* d_moves, const wick_rocm_kv_planes* planes, const Launch& L) {
+    const PagedPlanArgs a{p.d_table, p.d_lens, p.d_refs, nullptr, d_moves, d_moves + 4u + 4u * most_moves(p), nullptr, p.n_seqs, p.max_pages, p.n_pages, page_shift(p)};
+    hipError_t e = launch_kernel(L, kFamOther, kv_pages_compact_kernel, dim3(1), dim3(kPlanThreads), a);
+    return e != hipSuccess ? e : launch_copy(p, planes, d_moves, p.n_pages / 2u, true, L);
+}
+
+hipError_t launch_kv_pages_copy(const wick_rocm_kv_pages& p, const wick_rocm_kv_planes& planes, const uint32_t* d_moves, uint32_t max_moves, const Launch& L) {
+    return max_moves == 0 ? hipSuccess : launch_copy(p, &planes, d_moves, max_moves, false, L);
+}
+
+}  // namespace wick_rocm

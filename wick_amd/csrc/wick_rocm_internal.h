@@ -8,6 +8,8 @@
 
 #include <vector>
 
+#include "../../include/wick_rocm_lfm2.h"
+
 namespace wick_rocm {
 
 constexpr int kTypeQ4_0 = 2;  // ggml ids, wick/src/gguf.rs:36-51
@@ -285,6 +287,29 @@ hipError_t launch_attention_q4(const float* d_q, uint32_t q_stride, const void* 
 size_t kv_q4_evict_scratch_floats(uint32_t seq_len, uint32_t n_kv_heads);
 hipError_t launch_kv_q4_evict(void* d_k_cache, void* d_v_cache, float* d_weights, uint32_t* d_kept, float* d_scratch, uint32_t seq_len, uint32_t n_keep,
                               uint32_t n_recent, uint32_t n_drop, uint32_t max_seq, uint32_t n_kv_heads, uint32_t head_dim, const Launch& L);
+
+// KV caches in pages (kv_paged.hip, attention_paged.hip): head_dim 32 / 64 / 128 / 256, the structs' limits checked by the caller.
+hipError_t launch_kv_paged_append(const wick_rocm_kv_pages& p, const float* d_k, const float* d_v, uint32_t kv_stride, void* d_k_pages, void* d_v_pages,
+                                  bool kv_f16, const uint32_t* d_start, const uint32_t* d_first, uint32_t n, uint32_t n_kv_heads, uint32_t head_dim,
+                                  const Launch& L);
+bool attention_paged_fits(const wick_rocm_kv_pages& p, uint32_t n_heads, uint32_t n_kv_heads);  // its units and heads are within 32 bits
+size_t attention_paged_scratch_floats(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim);
+hipError_t launch_attention_paged(const wick_rocm_kv_pages& p, const float* d_q, uint32_t q_stride, const void* d_k_pages, const void* d_v_pages, bool kv_f16,
+                                  float* d_out, uint32_t out_stride, float* d_scratch, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, float scale,
+                                  const Launch& L);
+hipError_t launch_kv_pages_fork(const wick_rocm_kv_pages& p, const uint32_t* d_parents, const Launch& L);
+hipError_t launch_kv_pages_free(const wick_rocm_kv_pages& p, const uint32_t* d_rows, const Launch& L);
+size_t kv_pages_moves_words(const wick_rocm_kv_pages& p);
+hipError_t launch_kv_pages_reserve(const wick_rocm_kv_pages& p, const uint32_t* d_counts, uint32_t* d_start, uint32_t* d_moves, const wick_rocm_kv_planes* planes,
+                                   const Launch& L);
+hipError_t launch_kv_pages_compact(const wick_rocm_kv_pages& p, uint32_t* d_moves, const wick_rocm_kv_planes* planes, const Launch& L);
+hipError_t launch_kv_pages_copy(const wick_rocm_kv_pages& p, const wick_rocm_kv_planes& planes, const uint32_t* d_moves, uint32_t max_moves, const Launch& L);
+
+// The pick of rows of logits by temperature, top-k, top-p and min-p (sample.hip).
+constexpr uint32_t kSampleMaxTokens = 1u << 19;
+size_t sample_scratch_bytes(uint32_t rows, uint32_t n);
+hipError_t launch_sample(const float* d_logits, uint32_t stride, uint32_t rows, uint32_t n, const wick_rocm_sample_params* d_params, const float* d_uniform,
+                         uint32_t* d_out, float* d_prob, void* d_scratch, const Launch& L);
 
 // n at and above which gemm_q8 uses the MFMA kernel (when k % 128 == 0): the counterpart of GEMM_MIN_N = 16
 // (wick/src/model/metal_lfm2.rs:18-21), set where the two routes cross on this GPU.  The multi-token GEMV streams the weight

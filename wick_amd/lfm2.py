@@ -23,6 +23,14 @@ class Lfm2Config(C.Structure):
                                     "conv_kernel_size")] + [("rope_theta", _F), ("rms_norm_eps", _F)]
 
 
+class _KvPages(C.Structure):
+    _fields_ = [(n, _U32) for n in ("n_seqs", "max_pages", "n_pages", "page_rows")] + [(n, _P) for n in ("d_table", "d_lens", "d_refs")]
+
+
+class _KvPlanes(C.Structure):
+    _fields_ = [("d_base", _P), ("plane_bytes", C.c_size_t)] + [(n, _U32) for n in ("n_planes", "n_kv_heads", "head_dim")] + [("kv_dtype", C.c_int)]
+
+
 _SIGNATURES = {
     "wick_rocm_embed_row": (C.c_int, [_P, _P, _U32, _P, _P]),
     "wick_rocm_rmsnorm": (C.c_int, [_P, _P, _P, _P, _U32, _U32, _U32, _U32, _F]),
@@ -53,6 +61,17 @@ _SIGNATURES = {
     "wick_rocm_attention_prefill_q4": (C.c_int, [_P, _P, _U32, _P, _P, _P, _U32, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32]),
     "wick_rocm_kv_q4_evict_scratch_floats": (C.c_size_t, [_U32, _U32]),
     "wick_rocm_kv_q4_evict": (C.c_int, [_P, _P, _P, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32, _U32]),
+    "wick_rocm_kv_paged_append": (C.c_int, [_P, _P, _P, _P, _U32, _P, _P, C.c_int, _P, _P, _U32, _U32, _U32]),
+    "wick_rocm_attention_paged_scratch_floats": (C.c_size_t, [_U32, _U32, _U32, _U32]),
+    "wick_rocm_attention_decode_paged": (C.c_int, [_P, _P, _P, _U32, _P, _P, C.c_int, _P, _U32, _P, _U32, _U32, _U32]),
+    "wick_rocm_kv_pages_fork": (C.c_int, [_P, _P, _P]),
+    "wick_rocm_kv_pages_free": (C.c_int, [_P, _P, _P]),
+    "wick_rocm_kv_pages_moves_words": (C.c_size_t, [_P]),
+    "wick_rocm_kv_pages_reserve": (C.c_int, [_P, _P, _P, _P, _P, _P]),
+    "wick_rocm_kv_pages_compact": (C.c_int, [_P, _P, _P, _P]),
+    "wick_rocm_kv_pages_copy": (C.c_int, [_P, _P, _P, _P, _U32]),
+    "wick_rocm_sample_scratch_bytes": (C.c_size_t, [_U32, _U32]),
+    "wick_rocm_sample": (C.c_int, [_P, _P, _U32, _U32, _U32, _P, _P, _P, _P, _P]),
     "wick_rocm_lfm2_load": (C.c_int, [_P, _P, _U32, C.POINTER(_P)]),
     "wick_rocm_lfm2_load_kv": (C.c_int, [_P, _P, _U32, C.c_int, C.POINTER(_P)]),
     "wick_rocm_lfm2_kv_dtype": (C.c_int, [_P]),
@@ -118,6 +137,47 @@ def attention_q4_scratch_floats(n: int, max_seq: int, n_heads: int, n_kv_heads: 
 
 def kv_q4_evict_scratch_floats(seq_len: int, n_kv_heads: int) -> int:
     return int(_lib().wick_rocm_kv_q4_evict_scratch_floats(seq_len, n_kv_heads))
+
+
+KV_F32, KV_F16 = 0, 1  # element types of KV caches (wick_rocm_lfm2_load_kv's and the paged caches' kv_dtype)
+NO_PAGE = NO_ROW = NO_TOKEN = 0xFFFFFFFF
+
+
+class KvPages:
+    """A pool of pages and the table of the sequences that hold them (wick_rocm_kv_pages); the arrays are the caller's."""
+
+    def __init__(self, table, lens, refs, n_seqs: int, max_pages: int, n_pages: int, page_rows: int):
+        self.arrays = (table, lens, refs)
+        self.n_seqs, self.max_pages, self.n_pages, self.page_rows = n_seqs, max_pages, n_pages, page_rows
+        self._struct = _KvPages(n_seqs, max_pages, n_pages, page_rows, _ptr(table), _ptr(lens), _ptr(refs))
+        self.handle = C.addressof(self._struct)
+
+
+class KvPlanes:
+    """Planes of a pool that lie plane_bytes apart (wick_rocm_kv_planes)."""
+
+    def __init__(self, base, n_planes: int, plane_bytes: int, n_kv_heads: int, head_dim: int, kv_dtype: int):
+        self.array = base
+        self._struct = _KvPlanes(_ptr(base), plane_bytes, n_planes, n_kv_heads, head_dim, kv_dtype)
+        self.handle = C.addressof(self._struct)
+
+
+def attention_paged_scratch_floats(n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int) -> int:
+    return int(_lib().wick_rocm_attention_paged_scratch_floats(n_seqs, n_heads, n_kv_heads, head_dim))
+
+
+def kv_pages_moves_words(pages: KvPages) -> int:
+    """32-bit words of the list of moves that kv_pages_reserve and kv_pages_compact leave."""
+    return int(_lib().wick_rocm_kv_pages_moves_words(pages.handle))
+
+
+def sample_scratch_bytes(rows: int, n: int) -> int:
+    return int(_lib().wick_rocm_sample_scratch_bytes(rows, n))
+
+
+def sample_params(rows) -> np.ndarray:
+    """[(temperature, top_k, top_p, min_p)] of each row as wick_rocm_sample takes them."""
+    return np.array([tuple(r) for r in rows], dtype=[("temperature", np.float32), ("top_k", np.uint32), ("top_p", np.float32), ("min_p", np.float32)])
 
 
 def rope_theta_scale(head_dim: int, freq_base: float) -> float:
@@ -203,6 +263,43 @@ class Lfm2Ops:
         self.ctx._check(self._l.wick_rocm_kv_q4_evict(self.ctx._h, _ptr(k_cache), _ptr(v_cache), _ptr(weights), _ptr(kept), _ptr(scratch), seq_len, n_keep,
                                                       n_recent, n_drop, max_seq, n_kv_heads, head_dim))
 
+    def encode_kv_paged_append(self, pages: KvPages, k, v, kv_stride: int, k_pages, v_pages, kv_dtype: int, start, n: int, n_kv_heads: int, head_dim: int,
+                               first=None) -> None:
+        """n tokens' normed and rotated keys and their values into the pages of their sequences: rows start[s] .. of tokens first[s] .. (None: one each)."""
+        self.ctx._check(self._l.wick_rocm_kv_paged_append(self.ctx._h, pages.handle, _ptr(k), _ptr(v), kv_stride, _ptr(k_pages), _ptr(v_pages), kv_dtype,
+                                                          _ptr(start), _ptr(first), n, n_kv_heads, head_dim))
+
+    def encode_attention_paged(self, pages: KvPages, q, q_stride: int, k_pages, v_pages, kv_dtype: int, out, out_stride: int, scratch, n_heads: int,
+                               n_kv_heads: int, head_dim: int) -> None:
+        """encode_attention for one new token of every sequence, over the rows that its pages hold."""
+        self.ctx._check(self._l.wick_rocm_attention_decode_paged(self.ctx._h, pages.handle, _ptr(q), q_stride, _ptr(k_pages), _ptr(v_pages), kv_dtype, _ptr(out),
+                                                                 out_stride, _ptr(scratch), n_heads, n_kv_heads, head_dim))
+
+    def kv_pages_fork(self, pages: KvPages, parents) -> None:
+        """Sequence s becomes what sequence parents[s] was (itself: it stays; none: empty); pages are shared, not copied."""
+        self.ctx._check(self._l.wick_rocm_kv_pages_fork(self.ctx._h, pages.handle, _ptr(parents)))
+
+    def kv_pages_free(self, pages: KvPages, rows) -> None:
+        """Sequence s is cut to rows[s] rows."""
+        self.ctx._check(self._l.wick_rocm_kv_pages_free(self.ctx._h, pages.handle, _ptr(rows)))
+
+    def kv_pages_reserve(self, pages: KvPages, counts, start, moves, planes: Optional[KvPlanes] = None) -> None:
+        """Pages of its own for counts[s] more rows of every sequence s, from start[s] on."""
+        self.ctx._check(self._l.wick_rocm_kv_pages_reserve(self.ctx._h, pages.handle, _ptr(counts), _ptr(start), _ptr(moves), planes.handle if planes else None))
+
+    def kv_pages_compact(self, pages: KvPages, moves, planes: Optional[KvPlanes] = None) -> None:
+        """The pages in use moved to the pool's front."""
+        self.ctx._check(self._l.wick_rocm_kv_pages_compact(self.ctx._h, pages.handle, _ptr(moves), planes.handle if planes else None))
+
+    def kv_pages_copy(self, pages: KvPages, planes: KvPlanes, moves, max_moves: int) -> None:
+        """The moves of a list, in all planes."""
+        self.ctx._check(self._l.wick_rocm_kv_pages_copy(self.ctx._h, pages.handle, planes.handle, _ptr(moves), max_moves))
+
+    def sample(self, logits, logits_stride: int, rows: int, n: int, params, uniform, out, prob, scratch) -> None:
+        """The next token of every row by temperature, top-k, top-p and min-p (sample_params) and a uniform number of its own."""
+        self.ctx._check(self._l.wick_rocm_sample(self.ctx._h, _ptr(logits), logits_stride, rows, n, _ptr(params), _ptr(uniform), _ptr(out), _ptr(prob),
+                                                 _ptr(scratch)))
+
     def encode_conv1d_seq(self, proj, buffer, conv_weight, out, hidden: int, kernel_size: int, n: int) -> None:
         """The gated short convolution of n prompt tokens (proj [n][3*hidden] -> out [n][hidden]), then the rolling state."""
         self.ctx._check(self._l.wick_rocm_shortconv_seq(self.ctx._h, _ptr(proj), _ptr(buffer), _ptr(conv_weight), _ptr(out), hidden, kernel_size, n))
@@ -263,9 +360,6 @@ class Lfm2Ops:
         """Output norm + LM head + greedy pick: logits = W rmsnorm(x), out[0] = argmax (and the device-side token / position)."""
         self.ctx._check(self._l.wick_rocm_lm_head_greedy_f32(self.ctx._h, w.handle, _ptr(x), _ptr(norm_weight), eps, _ptr(logits), _ptr(out),
                                                              _ptr(d_token), _ptr(d_pos)))
-
-
-KV_F32, KV_F16 = 0, 1  # wick_rocm_lfm2_load_kv's kv_dtype
 
 
 class RocmLfm2Model:
