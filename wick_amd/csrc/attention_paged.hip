@@ -43,17 +43,6 @@ struct PagedAttentionArgs {
 __device__ __forceinline__ uint32_t length(const PagedAttentionArgs& a, uint32_t s) { return min(a.lens[s], a.max_pages << a.page_shift); }
 __device__ __forceinline__ uint32_t units_of(uint32_t len) { return (len + kUnitRows - 1u) / kUnitRows; }
 
-// Sum over the wave's lanes up to this one.
-__device__ __forceinline__ uint32_t lanes_upto(uint32_t v) {
-    const uint32_t lane = threadIdx.x & 63u;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t other = __shfl_up(v, d, 64);
-        if (lane >= (uint32_t)d) v += other;
-    }
-    return v;
-}
-
 // Units of all sequences, and of those in front of sequence `upto`.
 __device__ __forceinline__ uint32_t all_units(const PagedAttentionArgs& a, uint32_t heads, uint32_t upto, uint32_t& before) {
     uint32_t sum = 0, front = 0;

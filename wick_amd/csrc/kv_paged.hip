@@ -103,38 +103,37 @@ __global__ __launch_bounds__(256) void kv_pages_free_kernel(PagedFreeArgs a) {
 }
 
 // ---- the plan of a reservation or a compaction: one workgroup --------------------------------------
+// A chain of round trips to memory (lengths, the table's entry, its page's count; what is written) and of barriers; refs are read a run of pages a thread, of
+// the first 16384 pages once, at the start.
 constexpr uint32_t kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
-constexpr uint32_t kRun = 16;  // consecutive pages of a thread at a time
+constexpr uint32_t kRun = 16;                    // consecutive pages of a thread at a time
+constexpr uint32_t kListed = 4096;               // pages of a list that are in LDS; those behind them in memory
+constexpr uint32_t kSeqs = 4;                    // sequences of a thread: 4096 in all
+constexpr uint32_t kShared = 2 * kSeqs * kPlanThreads;  // slots for the pages that are shared and written to
 
-// Sum over the workgroup's threads in front of this one, and over all of them.  `slots`: kPlanWaves, of this call until the next barrier.
-__device__ __forceinline__ uint32_t wave_sum_before(uint32_t v, uint32_t lane) {
-    uint32_t sum = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t other = __shfl_up(sum, d, 64);
-        if (lane >= (uint32_t)d) sum += other;
-    }
-    return sum;
-}
+// Sum over the workgroup's threads in front of this one, and over all of them.  `slots`: kPlanWaves, of this call alone until the next barrier.
 __device__ __forceinline__ uint32_t sum_before(uint32_t v, uint32_t* slots, uint32_t& total) {
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, upto = wave_sum_before(v, lane);
-    __syncthreads();  // (slots are still read)
+    const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), upto = lanes_upto(v);
     if (lane == 63u) slots[wave] = upto;
     __syncthreads();
-    uint32_t before = upto - v;
-    total = 0;
-    for (uint32_t w = 0; w < kPlanWaves; w++) {
-        if (w < wave) before += slots[w];
-        total += slots[w];
-    }
-    return before;
+    const uint32_t sums = lanes_upto(lane < kPlanWaves ? slots[lane] : 0u);
+    total = (uint32_t)__builtin_amdgcn_readlane((int)sums, 63);
+    return upto - v + (wave > 0 ? (uint32_t)__builtin_amdgcn_readlane((int)sums, (int)wave - 1) : 0u);
 }
 
 // Bits of the pages [first, first + kRun) that are free; those behind the last page are not.
 __device__ __forceinline__ uint32_t free_bits(const uint32_t* refs, uint64_t first, uint32_t n_pages) {
     uint32_t bits = 0;
+    if (first + kRun <= n_pages) {
 #pragma unroll
-    for (uint32_t i = 0; i < kRun; i++) bits |= (uint32_t)(first + i < n_pages && refs[first + i < n_pages ? first + i : 0] == 0) << i;
+        for (uint32_t i = 0; i < kRun; i += 4) {
+            const u32x4_a4 x = *reinterpret_cast<const u32x4_a4*>(refs + first + i);
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) bits |= (uint32_t)(x.v[e] == 0) << (i + e);
+        }
+    } else {
+        for (uint32_t i = 0; first + i < n_pages; i++) bits |= (uint32_t)(refs[first + i] == 0) << i;
+    }
     return bits;
 }
 
@@ -144,80 +143,81 @@ struct PagedPlanArgs {
     uint32_t n_seqs, max_pages, n_pages, page_shift;
 };
 
-// Pages for the new rows of every sequence.  A partial last page of c writers and r holders: where c = r the first writer keeps it and r - 1 copy, else all
-// c do.  Who is who is found in refs itself: every writer takes one off; where nothing is left the writers' largest n_seqs - s is put there.
+// Pages for the new rows of every sequence.  A partial last page with c writers and r holders: where c = r the first writer keeps it and r - 1 copy, else all c
+// do.  Who is who is found in LDS, by the page's slot of a hash table twice as large as all sequences, for pages that are shared alone.
 __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(PagedPlanArgs a) {
-    __shared__ uint32_t slots[kPlanWaves], too_short, moved;
-    constexpr uint32_t kOwner = 0x80000000u, kMost = 4;  // sequences of a thread: 4096 in all
+    __shared__ uint32_t page_of[kShared], writers[kShared], first_of[kShared], list[kListed], slots[2][kPlanWaves], moved;
     const uint32_t R = 1u << a.page_shift;
     const uint64_t capacity = (uint64_t)a.max_pages << a.page_shift;
-    if (threadIdx.x == 0) too_short = 0, moved = 0;
-    __syncthreads();
-    uint32_t len[kMost], count[kMost], page[kMost], need[kMost];
-    bool copies[kMost];
+    uint32_t len[kSeqs], count[kSeqs], page[kSeqs], held[kSeqs], need[kSeqs];
+    uint32_t bits = free_bits(a.refs, threadIdx.x * kRun, a.n_pages);
+    bool too_long = false, copies[kSeqs], shared = false;
 #pragma unroll
-    for (uint32_t k = 0; k < kMost; k++) {  // consecutive sequences a thread, in order
-        const uint32_t s = threadIdx.x * kMost + k;
+    for (uint32_t k = 0; k < kSeqs; k++) {  // consecutive sequences a thread, in order
+        const uint32_t s = threadIdx.x * kSeqs + k;
         len[k] = s < a.n_seqs ? a.lens[s] : 0, count[k] = s < a.n_seqs ? a.counts[s] : 0;
-        if ((uint64_t)len[k] + count[k] > capacity) too_short = 1;
-        page[k] = WICK_ROCM_NO_PAGE;
-        if (count[k] != 0 && len[k] % R != 0 && len[k] < capacity) page[k] = a.table[(size_t)s * a.max_pages + (len[k] >> a.page_shift)];
-        if (page[k] >= a.n_pages) page[k] = WICK_ROCM_NO_PAGE;
-        if (page[k] != WICK_ROCM_NO_PAGE) atomicSub(&a.refs[page[k]], 1u);
     }
-    __threadfence();
-    __syncthreads();
-    bool alone[kMost];
 #pragma unroll
-    for (uint32_t k = 0; k < kMost; k++) alone[k] = page[k] != WICK_ROCM_NO_PAGE && __hip_atomic_load(&a.refs[page[k]], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0;
-    __syncthreads();
+    for (uint32_t k = 0; k < kSeqs; k++) {
+        const uint32_t s = threadIdx.x * kSeqs + k;
+        too_long = too_long || (uint64_t)len[k] + count[k] > capacity;
+        page[k] = count[k] != 0 && len[k] % R != 0 && len[k] < capacity ? a.table[(size_t)s * a.max_pages + (len[k] >> a.page_shift)] : WICK_ROCM_NO_PAGE;
+    }
 #pragma unroll
-    for (uint32_t k = 0; k < kMost; k++)
-        if (alone[k]) atomicMax(&a.refs[page[k]], kOwner | (a.n_seqs - (threadIdx.x * kMost + k)));
-    __threadfence();
-    __syncthreads();
+    for (uint32_t k = 0; k < kSeqs; k++) {
+        held[k] = page[k] < a.n_pages ? a.refs[page[k]] : 0u;
+        shared = shared || held[k] > 1u, copies[k] = held[k] > 1u;
+    }
+    if (threadIdx.x == 0) moved = 0;
+    if (__syncthreads_or(shared)) {
+        uint32_t size = 64;
+        while (size < 2u * a.n_seqs) size *= 2u;
+        for (uint32_t i = threadIdx.x; i < size; i += kPlanThreads) page_of[i] = WICK_ROCM_NO_PAGE, writers[i] = 0, first_of[i] = WICK_ROCM_NO_PAGE;
+        __syncthreads();
+        uint32_t slot[kSeqs];
+#pragma unroll
+        for (uint32_t k = 0; k < kSeqs; k++) {
+            if (!copies[k]) continue;
+            slot[k] = page[k] * 0x9e3779b1u >> 8 & (size - 1u);
+            for (uint32_t is; (is = atomicCAS(&page_of[slot[k]], WICK_ROCM_NO_PAGE, page[k])) != WICK_ROCM_NO_PAGE && is != page[k];)  // (at most half of the slots are taken)
+                slot[k] = (slot[k] + 1u) & (size - 1u);
+            atomicAdd(&writers[slot[k]], 1u), atomicMin(&first_of[slot[k]], threadIdx.x * kSeqs + k);
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t k = 0; k < kSeqs; k++)
+            if (copies[k]) copies[k] = writers[slot[k]] != held[k] || first_of[slot[k]] != threadIdx.x * kSeqs + k;
+    }
     uint32_t mine = 0;
 #pragma unroll
-    for (uint32_t k = 0; k < kMost; k++) {
-        const uint32_t s = threadIdx.x * kMost + k;
-        copies[k] = page[k] != WICK_ROCM_NO_PAGE;
-        if (alone[k] && __hip_atomic_load(&a.refs[page[k]], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (kOwner | (a.n_seqs - s))) copies[k] = false;
+    for (uint32_t k = 0; k < kSeqs; k++) {
         need[k] = count[k] == 0 ? 0 : pages_of((uint64_t)len[k] + count[k], a.page_shift) - pages_of(len[k], a.page_shift) + copies[k];
         mine += need[k];
     }
-    __syncthreads();  // (all have seen who keeps)
-#pragma unroll
-    for (uint32_t k = 0; k < kMost; k++)
-        if (page[k] != WICK_ROCM_NO_PAGE && !copies[k]) __hip_atomic_store(&a.refs[page[k]], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __threadfence();
+    const bool fits_table = !__syncthreads_or(too_long);
     uint32_t wanted;
-    uint32_t at = sum_before(mine, slots, wanted);
+    uint32_t at = sum_before(mine, slots[0], wanted);
     // the lowest free pages, as many as are wanted
     uint32_t found = 0;
-    const bool fits_table = too_short == 0;
     for (uint64_t base = 0; fits_table && base < a.n_pages && found < wanted; base += kRun * kPlanThreads) {
         const uint64_t first = base + threadIdx.x * kRun;
-        uint32_t bits = free_bits(a.refs, first, a.n_pages), all;
-        uint32_t to = found + sum_before(__popc(bits), slots, all);
-        for (; bits != 0; bits &= bits - 1u, to++)
-            if (to < wanted) a.list[to] = (uint32_t)first + __ffs(bits) - 1u;
+        if (base != 0) bits = free_bits(a.refs, first, a.n_pages);
+        uint32_t all;
+        uint32_t to = found + sum_before(__popc(bits), slots[1], all);
+        for (; bits != 0 && to < wanted; bits &= bits - 1u, to++) (to < kListed ? list[to] : a.list[to]) = (uint32_t)first + __ffs(bits) - 1u;
         found += all;
+        __syncthreads();  // (slots are read, the list is written)
     }
-    __threadfence();
-    __syncthreads();
-    if (!fits_table || found < wanted) {  // nothing changes: what was taken off refs comes back
+    if (!fits_table || found < wanted) {  // nothing changes
 #pragma unroll
-        for (uint32_t k = 0; k < kMost; k++) {
-            const uint32_t s = threadIdx.x * kMost + k;
-            if (copies[k]) atomicAdd(&a.refs[page[k]], 1u);
-            if (s < a.n_seqs) a.start[s] = WICK_ROCM_NO_ROW;
-        }
-        if (threadIdx.x == 0) a.moves[0] = 0, a.moves[1] = fits_table ? wanted - found : 0xffffffffu, a.moves[2] = 0, a.moves[3] = 0;
+        for (uint32_t k = 0; k < kSeqs; k++)
+            if (const uint32_t s = threadIdx.x * kSeqs + k; s < a.n_seqs) a.start[s] = WICK_ROCM_NO_ROW;
+        if (threadIdx.x == 0) *reinterpret_cast<uint4*>(a.moves) = make_uint4(0, fits_table ? wanted - found : 0xffffffffu, 0, 0);
         return;
     }
 #pragma unroll
-    for (uint32_t k = 0; k < kMost; k++) {
-        const uint32_t s = threadIdx.x * kMost + k;
+    for (uint32_t k = 0; k < kSeqs; k++) {
+        const uint32_t s = threadIdx.x * kSeqs + k;
         if (s >= a.n_seqs) break;
         a.start[s] = count[k] == 0 ? WICK_ROCM_NO_ROW : len[k];
         if (count[k] == 0) continue;
@@ -225,98 +225,97 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(PagedPla
         uint32_t* const row = a.table + (size_t)s * a.max_pages;
         uint32_t p = pages_of(len[k], a.page_shift);
         if (copies[k]) {
-            const uint32_t to = a.list[at++], m = atomicAdd(&moved, 1u);
-            row[p - 1u] = to, a.refs[to] = 1;
-            uint32_t* const move = a.moves + 4u + 4u * m;
-            move[0] = page[k], move[1] = to, move[2] = len[k] % R, move[3] = 0;
+            const uint32_t to = at < kListed ? list[at] : a.list[at], m = atomicAdd(&moved, 1u);
+            at++;
+            row[p - 1u] = to, a.refs[to] = 1, atomicSub(&a.refs[page[k]], 1u);
+            *reinterpret_cast<uint4*>(a.moves + 4u + 4u * m) = make_uint4(page[k], to, len[k] % R, 0);
         }
-        for (uint32_t n = need[k] - copies[k]; n != 0; n--, p++) {
-            const uint32_t to = a.list[at++];
+        for (uint32_t n = need[k] - copies[k]; n != 0; n--, p++, at++) {
+            const uint32_t to = at < kListed ? list[at] : a.list[at];
             row[p] = to, a.refs[to] = 1;
         }
     }
     __syncthreads();
-    if (threadIdx.x == 0) a.moves[0] = moved, a.moves[1] = 0, a.moves[2] = 0, a.moves[3] = 0;
+    if (threadIdx.x == 0) *reinterpret_cast<uint4*>(a.moves) = make_uint4(moved, 0, 0, 0);
 }
 
 // With U pages in use: the i-th page in use at U or above goes to the i-th free one below.
 __global__ __launch_bounds__(kPlanThreads) void kv_pages_compact_kernel(PagedPlanArgs a) {
-    __shared__ uint32_t slots[kPlanWaves];
-    uint32_t free = 0;
-    for (uint64_t base = 0; base < a.n_pages; base += kRun * kPlanThreads) free += __popc(free_bits(a.refs, base + threadIdx.x * kRun, a.n_pages));
+    __shared__ uint32_t from_list[kListed], to_list[kListed], slots[2][kPlanWaves];
+    const uint32_t early = free_bits(a.refs, threadIdx.x * kRun, a.n_pages);
+    uint32_t free = __popc(early);
+    for (uint64_t base = kRun * kPlanThreads; base < a.n_pages; base += kRun * kPlanThreads) free += __popc(free_bits(a.refs, base + threadIdx.x * kRun, a.n_pages));
     uint32_t all;
-    sum_before(free, slots, all);
+    sum_before(free, slots[0], all);
     const uint32_t used = a.n_pages - all;
     uint32_t holes = 0, movers = 0;
     for (uint64_t base = 0; base < a.n_pages; base += kRun * kPlanThreads) {
         const uint64_t first = base + threadIdx.x * kRun;
-        const uint32_t bits = free_bits(a.refs, first, a.n_pages);
+        const uint32_t bits = base == 0 ? early : free_bits(a.refs, first, a.n_pages);
         const uint32_t inside = first >= a.n_pages ? 0u : first + kRun <= a.n_pages ? 0xffffu : (1u << (a.n_pages - first)) - 1u;
         const uint32_t below = first >= used ? 0u : first + kRun <= used ? 0xffffu : (1u << (used - first)) - 1u;
         uint32_t hole = bits & below, mover = ~bits & inside & ~below, n;
-        const uint32_t before = sum_before(__popc(hole) | __popc(mover) << 16, slots, n);  // (at most 2^14 each)
+        const uint32_t before = sum_before(__popc(hole) | __popc(mover) << 16, slots[1], n);  // (at most 2^14 each)
         uint32_t to = holes + (before & 0xffffu), from = movers + (before >> 16);
-        for (; hole != 0; hole &= hole - 1u) a.moves[4u + 4u * to++ + 1u] = (uint32_t)first + __ffs(hole) - 1u;
-        for (; mover != 0; mover &= mover - 1u) {
-            uint32_t* const move = a.moves + 4u + 4u * from++;
-            move[0] = (uint32_t)first + __ffs(mover) - 1u, move[2] = 1u << a.page_shift, move[3] = 0;
-        }
+        for (; hole != 0; hole &= hole - 1u, to++) (to < kListed ? to_list[to] : a.moves[4u + 4u * to + 1u]) = (uint32_t)first + __ffs(hole) - 1u;
+        for (; mover != 0; mover &= mover - 1u, from++) (from < kListed ? from_list[from] : a.moves[4u + 4u * from]) = (uint32_t)first + __ffs(mover) - 1u;
         holes += n & 0xffffu, movers += n >> 16;
+        __syncthreads();
     }
-    __threadfence();
-    __syncthreads();
     for (uint32_t m = threadIdx.x; m < movers; m += kPlanThreads) {
-        const uint32_t from = a.moves[4u + 4u * m], to = a.moves[4u + 4u * m + 1u];
+        uint32_t* const move = a.moves + 4u + 4u * m;
+        const uint32_t from = m < kListed ? from_list[m] : move[0], to = m < kListed ? to_list[m] : move[1];
+        *reinterpret_cast<uint4*>(move) = make_uint4(from, to, 1u << a.page_shift, 0);
         a.refs[to] = a.refs[from], a.refs[from] = 0;
         a.list[from] = to;
     }
-    if (threadIdx.x == 0) a.moves[0] = movers, a.moves[1] = used, a.moves[2] = 0, a.moves[3] = 0;
+    if (threadIdx.x == 0) *reinterpret_cast<uint4*>(a.moves) = make_uint4(movers, used, 0, 0);
 }
 
 // ---- pages moved -----------------------------------------------------------------------------------
-// A unit is 1024 consecutive 16-byte pieces of a page in one plane, taken by the workgroups in turn; behind them, for a compaction, the
-// table's entries.  Bound by memory.
+// A workgroup takes 1024 consecutive 16-byte pieces of a page in one plane, of one move after the other; for a compaction, the table's entries behind them.
+// Bound by memory.
 struct PagedCopyArgs {
     char* base;
     size_t plane_bytes;
     const uint32_t* moves;
-    uint32_t *table;       // entries from moves[1] on are replaced by `list` of them (null: none)
+    uint32_t* table;  // entries from moves[1] on are replaced by `list` of them (null: none)
     const uint32_t* list;
-    uint32_t max_moves, n_planes, n_pages, page_units, row_pieces, rows;  // row_pieces: pieces of a row of one head; rows: of a page
+    uint32_t max_moves, n_pages, pieces, parts, row_shift, page_shift;  // pieces: of a page; parts: units of them; row_shift: pieces of a row of one head
     uint64_t entries;
 };
 constexpr uint32_t kUnit = 1024;
 
 __global__ __launch_bounds__(256) void kv_pages_copy_kernel(PagedCopyArgs a) {
-    const uint32_t moves = min(a.moves[0], a.max_moves), pieces = a.page_units;
-    const uint32_t per_page = (pieces + kUnit - 1u) / kUnit;
-    const uint64_t units = (uint64_t)moves * a.n_planes * per_page;
-    for (uint64_t u = blockIdx.x; u < units; u += gridDim.x) {
-        const uint32_t part = (uint32_t)(u % per_page), plane = (uint32_t)(u / per_page % a.n_planes), m = (uint32_t)(u / per_page / a.n_planes);
+    const uint32_t moves = min(a.moves[0], a.max_moves), plane = blockIdx.x / a.parts, first = blockIdx.x % a.parts * kUnit + threadIdx.x;
+    uint4* const pages = reinterpret_cast<uint4*>(a.base + plane * a.plane_bytes) + first;
+    for (uint32_t m = blockIdx.y; m < moves; m += gridDim.y) {
         const uint4 move = *reinterpret_cast<const uint4*>(a.moves + 4u + 4u * (size_t)m);
         if (move.x >= a.n_pages || move.y >= a.n_pages) continue;
-        char* const p = a.base + plane * a.plane_bytes;
-        const uint4* const from = reinterpret_cast<const uint4*>(p) + (size_t)move.x * pieces;
-        uint4* const to = reinterpret_cast<uint4*>(p) + (size_t)move.y * pieces;
-        uint4 x[kUnit / 256];
-        bool takes[kUnit / 256];
-#pragma unroll
-        for (uint32_t i = 0; i < kUnit / 256; i++) {
-            const uint32_t piece = part * kUnit + i * 256u + threadIdx.x;
-            takes[i] = piece < pieces && piece / a.row_pieces % a.rows < move.z;
-            if (takes[i]) x[i] = from[piece];
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < kUnit / 256; i++)
-            if (takes[i]) to[part * kUnit + i * 256u + threadIdx.x] = x[i];
+        const uint4* const from = pages + (size_t)move.x * a.pieces;
+        uint4* const to = pages + (size_t)move.y * a.pieces;
+        const auto takes = [&](uint32_t i) { return first + i < a.pieces && ((first + i) >> a.row_shift & ((1u << a.page_shift) - 1u)) < move.z; };
+        uint4 x0, x1, x2, x3;
+        const bool t0 = takes(0), t1 = takes(256), t2 = takes(512), t3 = takes(768);
+        if (t0) x0 = from[0];
+        if (t1) x1 = from[256];
+        if (t2) x2 = from[512];
+        if (t3) x3 = from[768];
+        if (t0) to[0] = x0;
+        if (t1) to[256] = x1;
+        if (t2) to[512] = x2;
+        if (t3) to[768] = x3;
     }
     if (a.table == nullptr) return;
     const uint32_t used = a.moves[1];
-    for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < a.entries; i += (uint64_t)gridDim.x * 256u) {
+    const uint64_t at = ((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256u + threadIdx.x, step = (uint64_t)gridDim.x * gridDim.y * 256u;
+    for (uint64_t i = at; i < a.entries; i += step) {
         const uint32_t page = a.table[i];
         if (page >= used && page < a.n_pages) a.table[i] = a.list[page];
     }
 }
+
+constexpr uint32_t kCopyGroups = 2048;  // workgroups of a launch that copies, or a round of its planes
 
 uint32_t page_shift(const wick_rocm_kv_pages& p) { return (uint32_t)__builtin_ctz(p.page_rows); }
 
@@ -326,21 +325,20 @@ uint32_t blocks(uint64_t threads, uint32_t most) { return (uint32_t)std::max<uin
 
 hipError_t launch_copy(const wick_rocm_kv_pages& p, const wick_rocm_kv_planes* planes, const uint32_t* d_moves, uint32_t max_moves, bool table, const Launch& L) {
     PagedCopyArgs a{};
-    a.moves = d_moves, a.n_pages = p.n_pages, a.rows = p.page_rows;
-    uint64_t units = 0;
+    a.moves = d_moves, a.n_pages = p.n_pages, a.page_shift = page_shift(p), a.parts = 1;
+    uint32_t x = 1, y = 1;
     if (planes) {
-        const uint32_t element = planes->kv_dtype == WICK_ROCM_KV_F16 ? 2u : 4u;
-        a.base = static_cast<char*>(planes->d_base), a.plane_bytes = planes->plane_bytes, a.max_moves = max_moves, a.n_planes = planes->n_planes;
-        a.row_pieces = planes->head_dim * element / 16u, a.page_units = planes->n_kv_heads * p.page_rows * a.row_pieces;
-        units = (uint64_t)max_moves * planes->n_planes * ((a.page_units + kUnit - 1u) / kUnit);
-    } else {
-        a.page_units = 1, a.row_pieces = 1, a.n_planes = 1;
+        const uint32_t row_pieces = planes->head_dim * (planes->kv_dtype == WICK_ROCM_KV_F16 ? 2u : 4u) / 16u;
+        a.base = static_cast<char*>(planes->d_base), a.plane_bytes = planes->plane_bytes, a.max_moves = max_moves;
+        a.row_shift = (uint32_t)__builtin_ctz(row_pieces), a.pieces = planes->n_kv_heads * p.page_rows * row_pieces, a.parts = (a.pieces + kUnit - 1u) / kUnit;
+        x = planes->n_planes * a.parts;
+        y = std::min(max_moves, std::max(1u, kCopyGroups / x));
     }
     if (table) {
         a.table = p.d_table, a.list = d_moves + 4u + 4u * most_moves(p), a.entries = (uint64_t)p.n_seqs * p.max_pages;
-        units = std::max(units, (a.entries + 255u) / 256u);
+        y = std::max(y, std::min(blocks(a.entries, kCopyGroups) / x, 65535u));
     }
-    return launch_kernel(L, kFamOther, kv_pages_copy_kernel, dim3(blocks(units * 256u, 2048u)), dim3(256), a);
+    return launch_kernel(L, kFamOther, kv_pages_copy_kernel, dim3(x, std::max(y, 1u)), dim3(256), a);
 }
 
 }  // namespace

@@ -37,7 +37,7 @@ int check_planes(wick_rocm_ctx* ctx, const wick_rocm_kv_pages& p, const wick_roc
     if (const char* wrong = heads_shape(planes.n_kv_heads, planes.head_dim, planes.kv_dtype)) return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, wrong);
     if (!planes.d_base || misaligned(planes.d_base, 16)) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages: the planes must be there and 16-byte aligned");
     const uint64_t bytes = (uint64_t)p.page_rows * planes.n_kv_heads * planes.head_dim * (planes.kv_dtype == WICK_ROCM_KV_F16 ? 2u : 4u);
-    if (planes.n_planes == 0 || planes.n_planes > 65535u) return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, "kv_pages: n_planes must be 1 .. 65535");
+    if (planes.n_planes == 0 || planes.n_planes > 1024u) return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, "kv_pages: n_planes must be 1 .. 1024");
     if (planes.n_planes > 1 && (planes.plane_bytes < bytes * p.n_pages || planes.plane_bytes % 16u != 0))
         return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, "kv_pages: plane_bytes must cover a plane and be a multiple of 16");
     return WICK_ROCM_OK;
