@@ -215,25 +215,33 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(PagedPla
         if (threadIdx.x == 0) *reinterpret_cast<uint4*>(a.moves) = make_uint4(0, fits_table ? wanted - found : 0xffffffffu, 0, 0);
         return;
     }
+    // where a sequence's new pages begin, in the list and in its row of the table (in place of what is in LDS no longer needed)
+    uint32_t* const begin = page_of;
+    uint32_t* const entry = writers;
+    __syncthreads();
 #pragma unroll
     for (uint32_t k = 0; k < kSeqs; k++) {
         const uint32_t s = threadIdx.x * kSeqs + k;
-        if (s >= a.n_seqs) break;
-        a.start[s] = count[k] == 0 ? WICK_ROCM_NO_ROW : len[k];
+        begin[s] = at, entry[s] = pages_of(len[k], a.page_shift) - copies[k];
+        if (s < a.n_seqs) a.start[s] = count[k] == 0 ? WICK_ROCM_NO_ROW : len[k];
         if (count[k] == 0) continue;
         a.lens[s] = len[k] + count[k];
-        uint32_t* const row = a.table + (size_t)s * a.max_pages;
-        uint32_t p = pages_of(len[k], a.page_shift);
         if (copies[k]) {
-            const uint32_t to = at < kListed ? list[at] : a.list[at], m = atomicAdd(&moved, 1u);
-            at++;
-            row[p - 1u] = to, a.refs[to] = 1, atomicSub(&a.refs[page[k]], 1u);
-            *reinterpret_cast<uint4*>(a.moves + 4u + 4u * m) = make_uint4(page[k], to, len[k] % R, 0);
+            const uint32_t m = atomicAdd(&moved, 1u);
+            atomicSub(&a.refs[page[k]], 1u);
+            *reinterpret_cast<uint4*>(a.moves + 4u + 4u * m) = make_uint4(page[k], at < kListed ? list[at] : a.list[at], len[k] % R, 0);
         }
-        for (uint32_t n = need[k] - copies[k]; n != 0; n--, p++, at++) {
-            const uint32_t to = at < kListed ? list[at] : a.list[at];
-            row[p] = to, a.refs[to] = 1;
+        at += need[k];
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < wanted; i += kPlanThreads) {  // the last sequence that begins at or in front of it
+        uint32_t low = 0, high = a.n_seqs;
+        while (high - low > 1) {
+            const uint32_t mid = (low + high) / 2u;
+            (begin[mid] <= i ? low : high) = mid;
         }
+        const uint32_t to = i < kListed ? list[i] : a.list[i];
+        a.table[(size_t)low * a.max_pages + entry[low] + (i - begin[low])] = to, a.refs[to] = 1;
     }
     __syncthreads();
     if (threadIdx.x == 0) *reinterpret_cast<uint4*>(a.moves) = make_uint4(moved, 0, 0, 0);

@@ -25,7 +25,7 @@ static_assert(kBins <= 64 * kLaneBins && kMaxParts <= 128);
 constexpr int kFraction = 43;  // masses are whole numbers of 2^-43: up to 2^19 tokens of less than 2 each
 constexpr uint32_t kFew = 512; // top-k up to which all that it leaves is listed: 3. sorts up to 1024 tokens, and the last bin may be half of them
 constexpr double kLog2e = 1.4426950408889634;
-constexpr double kNever = -__builtin_inf(), kInfinite = 0x1p1000;       // y of what is never taken, and of an infinite logit
+constexpr double kInfinite4 = 0x1p1000;                                 // 4 y of an infinite logit
 
 struct SamplePart {
     uint64_t sure;  // mass that is certainly kept
@@ -35,58 +35,85 @@ struct SamplePart {
     uint32_t count[kBins];
 };
 
+// What 2. knows of a row and hands on to 3.: every bin's tokens and mass with those in front of it, and where the cuts can be.
+struct SampleRow {
+    double top4, floor;  // 4 E; the mass that min-p asks for
+    uint32_t k_bin, p_first, p_last, pad;
+    uint64_t mass[64 * kLaneBins];
+    uint32_t count[64 * kLaneBins];
+};
+
 struct SampleArgs {
     const float* logits;
     const wick_rocm_sample_params* params;
     const float* uniform;
     uint32_t* out;
     float* prob;
+    SampleRow* rows;
     SamplePart* parts;  // [rows][n_parts]
     uint32_t* lists;    // [rows][n]: part p's tokens from p kPart on
     uint32_t n, stride, n_parts;
 };
 
 struct Rule {
-    double inverse;  // log2(e) / T
+    double inverse4;  // 4 log2(e) / T
     uint32_t top_k;
     double top_p, min_p;
+    uint32_t n;
     __device__ __forceinline__ bool few() const { return top_k <= kFew; }
     __device__ __forceinline__ bool masses() const { return top_p < 1.0 && !few(); }  // 1. adds up masses,
-    uint32_t n;
     __device__ __forceinline__ bool counts() const { return top_k < n || few(); }     // counts tokens
 };
 __device__ __forceinline__ Rule rule_of(const SampleArgs& a, uint32_t row) {
     const wick_rocm_sample_params p = a.params[row];
-    Rule r{kLog2e, p.top_k == 0 ? a.n : min(p.top_k, a.n), p.top_p >= 0.0f ? fmin((double)p.top_p, 1.0) : p.top_p < 0.0f ? 0.0 : 1.0,
+    Rule r{kSteps * kLog2e, p.top_k == 0 ? a.n : min(p.top_k, a.n), p.top_p >= 0.0f ? fmin((double)p.top_p, 1.0) : p.top_p < 0.0f ? 0.0 : 1.0,
            p.min_p >= 0.0f ? fmin((double)p.min_p, 1.0) : 0.0, a.n};
-    if (p.temperature > 0.0f) r.inverse = kLog2e / (double)p.temperature;
+    if (p.temperature > 0.0f) r.inverse4 = kSteps * kLog2e / (double)p.temperature;
     else r.top_k = 1;
     return r;
 }
 
-__device__ __forceinline__ double power_of(float l, const Rule& r) {
-    if (!(l > -__builtin_inff())) return kNever;
-    return l == __builtin_inff() ? kInfinite : (double)l * r.inverse;
+// What a row's tokens are measured from: E, and whether an infinite logit is the largest.
+struct Origin {
+    double top4;  // 4 E; -infinity: nothing may be taken
+    bool infinite;
+    __device__ __forceinline__ bool none() const { return !(top4 > -__builtin_inf()); }
+};
+__device__ __forceinline__ Origin origin_of(float largest, const Rule& r) {
+    if (!(largest > -__builtin_inff())) return {-__builtin_inf(), false};
+    if (largest == __builtin_inff()) return {kInfinite4, true};
+    return {kSteps * __builtin_floor((double)largest * r.inverse4 / kSteps), false};
 }
-// The bin of a token (kBins: it weighs nothing).  Falls with rising y; every step is exact, so that the bins of another E are the same ones, counted from elsewhere.
-__device__ __forceinline__ uint32_t bin_of(double y, double top) {
-    const double below = (kSteps * top - __builtin_floor(kSteps * y)) + (kSteps - 1);
-    return below < (double)kBins ? (uint32_t)below : kBins;
+// A token's 4 y; of one that is never taken, -infinity or NaN.  (T may be infinite too.)
+__device__ __forceinline__ double quarters(float l, const Rule& r, const Origin& o) {
+    const double y4 = (double)l * r.inverse4;
+    return o.infinite ? (l == __builtin_inff() ? kInfinite4 : -__builtin_inf()) : y4;
 }
-// 2^(y - top) times 2^kFraction, for y of a bin: 2^f for |f| <= 1/2 by the polynomial that interpolates it at the Chebyshev nodes (off by 5e-16), put in place by its
-// exponent.
-__device__ __forceinline__ double exact_weight(double y, double top) {
-    const double v = y - top, n = __builtin_rint(v), f = v - n;
+// Without the conversions of the vector unit, which take four times as long as an addition: a number below 2^51 is rounded to a whole one by adding and taking
+// away 1.5 2^52, and has it as the sum's lower bits.  (What is larger comes out whole too, if not as the nearest.)
+constexpr double kRound = 0x1.8p52;
+__device__ __forceinline__ double whole_below(double y4) {
+    const double r = (y4 + kRound) - kRound;
+    return r > y4 ? r - 1.0 : r;
+}
+// The bin of a token with floor `whole` of its 4 y; kBins or NaN and what is not below it: it weighs nothing.  Falls with rising y; every step is exact, so that the bins of
+// another E are the same ones, counted from elsewhere.
+__device__ __forceinline__ double bin_of(double whole, const Origin& o) { return (o.top4 - whole) + (kSteps - 1); }
+__device__ __forceinline__ uint32_t bin_index(double bin) { return (uint32_t)fmax(bin, 0.0); }  // (beyond 2^51, where wholes are not the nearest, it may be below 0)
+// 2^(y - E) times 2^kFraction, for y of a bin: 2^f for |f| <= 1/2 by the polynomial that interpolates it at the Chebyshev nodes (off by 5e-16), put in place by
+// adding to its exponent.
+__device__ __forceinline__ double exact_weight(double y4, const Origin& o) {
+    const double v = (y4 - o.top4) * (1.0 / kSteps), n = v + kRound, f = v - (n - kRound);
     double p = 0x1.e606452d2a4bep-28;
     p = __builtin_fma(p, f, 0x1.b675bd7308f14p-24), p = __builtin_fma(p, f, 0x1.62bfd472738fap-20), p = __builtin_fma(p, f, 0x1.ffcb54054027cp-17);
     p = __builtin_fma(p, f, 0x1.4309130972582p-13), p = __builtin_fma(p, f, 0x1.5d87fe9d7ab38p-10), p = __builtin_fma(p, f, 0x1.3b2ab6fba1dcfp-7);
     p = __builtin_fma(p, f, 0x1.c6b08d703ce45p-5), p = __builtin_fma(p, f, 0x1.ebfbdff82c598p-3), p = __builtin_fma(p, f, 0x1.62e42fefa3a19p-1);
     p = __builtin_fma(p, f, 1.0);
-    return __builtin_ldexp(p, (int)n + kFraction);
+    return __hiloint2double(__double2hiint(p) + (int)((uint32_t)(__double2loint(n) + kFraction) << 20), __double2loint(p));
 }
 // ... in whole numbers: rounded by adding 2^52.
-__device__ __forceinline__ uint64_t weight_of(double y, double top) {
-    return __builtin_bit_cast(uint64_t, exact_weight(y, top) + 0x1p52) & ((1ull << 52) - 1u);
+__device__ __forceinline__ uint64_t weight_of(double y4, const Origin& o) {
+    return __builtin_bit_cast(uint64_t, exact_weight(y4, o) + 0x1p52) & ((1ull << 52) - 1u);
 }
 
 // (logit, lower index first) as one number, of a logit that may be taken; no key is 0.
@@ -152,15 +179,14 @@ __global__ __launch_bounds__(kPartThreads) void sample_bins_kernel(SampleArgs a)
     __syncthreads();
 #pragma unroll
     for (uint32_t w = 0; w < kPartThreads / 64; w++) top = fmaxf(top, tops[w]);
-    const double e = __builtin_floor(power_of(top, r));
-    if (e > kNever && (counts || masses)) {
+    const Origin o = origin_of(top, r);
+    if (!o.none() && (counts || masses)) {
 #pragma unroll
         for (uint32_t k = 0; k < kPartLoads; k++) {
-            const double y = power_of(l[k], r);
-            const uint32_t b = y > kNever ? bin_of(y, e) : kBins;
-            if (b >= kBins) continue;
-            if (counts) atomicAdd(&count[b], 1u);
-            if (masses) atomicAdd(&mass[b], (unsigned long long)weight_of(y, e));
+            const double y4 = quarters(l[k], r, o), b = bin_of(whole_below(y4), o);
+            if (!(b < (double)kBins)) continue;
+            if (counts) atomicAdd(&count[bin_index(b)], 1u);
+            if (masses) atomicAdd(&mass[bin_index(b)], (unsigned long long)weight_of(y4, o));
         }
     }
     __syncthreads();
@@ -175,7 +201,8 @@ __global__ __launch_bounds__(kPartThreads) void sample_bins_kernel(SampleArgs a)
 // A row's histogram from its parts', every wave with all of it: lane i has bins 3 i .. 3 i + 2, each with those in front of it; and where the cuts can be.
 struct RowBins {
     uint64_t mass[kLaneBins], count[kLaneBins];
-    double top, floor;         // E, and the mass that min-p asks for
+    Origin o;
+    double floor;              // the mass that min-p asks for
     uint32_t k_bin;            // the bin with the top_k-th token; kBins: all are taken
     uint32_t p_first, p_last;  // bins that the nucleus can end in; p_first = kBins: there is none
     bool whole;                // all up to k_bin is listed
@@ -190,7 +217,7 @@ struct RowBins {
     }
     // The first bin up to which there is at least `target`, or kBins.
     static __device__ __forceinline__ uint32_t reaching(const uint64_t (&v)[kLaneBins], uint64_t target) {
-        const uint64_t past = __ballot(v[2] >= target);
+        const uint64_t past = __ballot(v[2] >= target);  // (all lanes are here)
         if (past == 0) return kBins;
         const uint32_t lane = (uint32_t)__ffsll((unsigned long long)past) - 1u;
         return lane * kLaneBins + (read_lane(v[0], lane) >= target ? 0u : read_lane(v[1], lane) >= target ? 1u : 2u);
@@ -213,16 +240,18 @@ __device__ __forceinline__ RowBins row_bins(const SampleArgs& a, uint32_t row, c
     const float largest[2] = {lane < a.n_parts ? parts[lane].largest : -__builtin_inff(), lane + 64u < a.n_parts ? parts[lane + 64u].largest : -__builtin_inff()};
     const float most = wave_max_f32(fmaxf(largest[0], largest[1]));
     RowBins bins;
-    bins.top = __builtin_floor(power_of(most, r));
+    bins.o = origin_of(most, r);
     bins.floor = 0.0, bins.k_bin = bins.p_first = kBins, bins.p_last = 0, bins.whole = r.few();
+#pragma unroll
+    for (uint32_t i = 0; i < kLaneBins; i++) bins.mass[i] = bins.count[i] = 0;
     int off[2];  // whole powers of two that a part's E is below the row's
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-        const double d = bins.top - __builtin_floor(power_of(largest[i], r));  // (infinite or NaN where there is nothing)
+        const double d = (bins.o.top4 - origin_of(largest[i], r).top4) * (1.0 / kSteps);  // (infinite or NaN where there is nothing)
         off[i] = d < (double)kOctaves ? (int)d : kOctaves;
     }
-    if (!(bins.top > kNever)) return bins;
-    bins.floor = r.min_p * (double)weight_of(power_of(most, r), bins.top);
+    if (bins.o.none()) return bins;
+    bins.floor = r.min_p * (double)weight_of(quarters(most, r, bins.o), bins.o);
     const bool counts = r.counts(), masses = r.masses();
     if (!counts && !masses) return bins;
     for (uint32_t b = threadIdx.x; b < 64u * kLaneBins; b += blockDim.x) {
@@ -261,11 +290,27 @@ __device__ __forceinline__ RowBins row_bins(const SampleArgs& a, uint32_t row, c
     return bins;
 }
 
+__device__ __forceinline__ void hand_on(const RowBins& bins, SampleRow& row) {  // one wave
+    const uint32_t lane = threadIdx.x & 63u;
+    if (lane == 0) row.top4 = bins.o.top4, row.floor = bins.floor, row.k_bin = bins.k_bin, row.p_first = bins.p_first, row.p_last = bins.p_last;
+#pragma unroll
+    for (uint32_t i = 0; i < kLaneBins; i++) row.mass[kLaneBins * lane + i] = bins.mass[i], row.count[kLaneBins * lane + i] = (uint32_t)bins.count[i];
+}
+__device__ __forceinline__ RowBins handed_on(const SampleRow& row, const Rule& r) {
+    RowBins bins;
+    const uint32_t lane = threadIdx.x & 63u;
+    bins.o = {row.top4, row.top4 == kInfinite4}, bins.floor = row.floor, bins.k_bin = row.k_bin, bins.p_first = row.p_first, bins.p_last = row.p_last, bins.whole = r.few();
+#pragma unroll
+    for (uint32_t i = 0; i < kLaneBins; i++) bins.mass[i] = row.mass[kLaneBins * lane + i], bins.count[i] = row.count[kLaneBins * lane + i];
+    return bins;
+}
+
 // 2.
 __global__ __launch_bounds__(kPartThreads) void sample_list_kernel(SampleArgs a) {
     __shared__ BinShared shared_bins;
     __shared__ uint64_t slots[kPartThreads / 64];
-    __shared__ uint32_t listed;
+    __shared__ uint2 candidates[kPart];
+    __shared__ uint32_t listed, together;
     const uint32_t row = blockIdx.y, first = blockIdx.x * kPart;
     const float* const logits = a.logits + (size_t)row * a.stride;
     float l[kPartLoads];
@@ -275,25 +320,44 @@ __global__ __launch_bounds__(kPartThreads) void sample_list_kernel(SampleArgs a)
         l[k] = i < a.n ? logits[i] : -__builtin_inff();
     }
     const Rule r = rule_of(a, row);
-    if (threadIdx.x == 0) listed = 0;
+    if (threadIdx.x == 0) listed = 0, together = 0;
     const RowBins bins = row_bins(a, row, r, shared_bins);
-    const double top = bins.top;
-    if (!(top > kNever)) return;
+    if (blockIdx.x == 0 && threadIdx.x < 64u) hand_on(bins, a.rows[row]);
+    if (bins.o.none()) return;
     __syncthreads();
     uint64_t sure = 0;
     uint32_t* const list = a.lists + (size_t)row * a.n + first;
-#pragma unroll
-    for (uint32_t k = 0; k < kPartLoads; k++) {
-        const uint32_t i = first + k * kPartThreads + threadIdx.x;
-        const double y = power_of(l[k], r);
-        const uint32_t b = y > kNever ? bin_of(y, top) : kBins;
-        if (b >= kBins) continue;
-        if (b < bins.sure()) {
-            const uint64_t w = weight_of(y, top);
+    const uint32_t sure_bins = bins.sure();
+    const auto take = [&](float x, uint32_t i) {
+        const double y4 = quarters(x, r, bins.o), b = bin_of(whole_below(y4), bins.o);
+        if (b < (double)sure_bins) {
+            const uint64_t w = weight_of(y4, bins.o);
             sure += (double)w >= bins.floor ? w : 0;
-        } else if (bins.lists(b)) {
+        } else if (b < (double)kBins && bins.lists(bin_index(b))) {
             list[atomicAdd(&listed, 1u)] = i;
         }
+    };
+    // The last bin that matters; as a rule it is far above most tokens.  Those that may be in it or above (by their logit, with room for rounding) are put together
+    // first, so that few waves do the rest.
+    const uint32_t last = bins.k_bin < kBins || bins.p_first == kBins ? bins.k_bin : bins.p_last;
+    if (last == kBins) {
+#pragma unroll
+        for (uint32_t k = 0; k < kPartLoads; k++) take(l[k], first + k * kPartThreads + threadIdx.x);
+    } else {
+        const double lowest = fmin((bins.o.top4 - (double)last) / r.inverse4, kInfinite4);
+        const float low = (float)(lowest - __builtin_fabs(lowest) * 0x1p-20 - 0x1p-140);
+#pragma unroll
+        for (uint32_t k = 0; k < kPartLoads; k++) {
+            const uint64_t here = __ballot(l[k] >= low);
+            if (here == 0) continue;
+            uint32_t at = 0;
+            if ((threadIdx.x & 63u) == 0) at = atomicAdd(&together, (uint32_t)__popcll(here));
+            at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + __builtin_amdgcn_mbcnt_hi((uint32_t)(here >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)here, 0u));
+            if (l[k] >= low) candidates[at] = make_uint2(__float_as_uint(l[k]), first + k * kPartThreads + threadIdx.x);
+        }
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < together; i += kPartThreads) take(__uint_as_float(candidates[i].x), candidates[i].y);
+        __syncthreads();  // (listed)
     }
     uint64_t all;
     sum_before<kPartThreads / 64>(sure, slots, all);
@@ -305,20 +369,43 @@ __global__ __launch_bounds__(kPartThreads) void sample_list_kernel(SampleArgs a)
 constexpr uint32_t kPickThreads = 1024, kPickWaves = kPickThreads / 64, kDigit = 11, kDigits = 1u << kDigit;
 
 struct PickShared {
-    BinShared bins;
-    uint64_t slots[4][kPickWaves], part_mass[kMaxParts], found[4];
-    uint32_t listed[kMaxParts];
-    union {
-        uint64_t key[kPickThreads];
-        struct {
-            uint32_t count[kDigits];
-            unsigned long long mass[kDigits];
-        } digit;
-    };
+    uint64_t slots[4][kPickWaves], part_mass[kMaxParts], found[4], key[64];
+    uint32_t listed[kMaxParts], together;
+    uint32_t count[kDigits];
+    unsigned long long mass[kDigits];
 };
 
-__device__ __forceinline__ uint64_t exchanged(uint64_t v, uint32_t distance) {
-    return (uint64_t)__shfl_xor((unsigned long long)v, (int)distance, 64);
+// Lane i's value from lane i ^ DISTANCE, without LDS.
+template <uint32_t DISTANCE>
+__device__ __forceinline__ uint32_t exchanged(uint32_t v) {
+    if constexpr (DISTANCE == 1) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false);  // quad_perm [1,0,3,2]
+    if constexpr (DISTANCE == 2) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false);  // quad_perm [2,3,0,1]
+    if constexpr (DISTANCE == 4) {  // quads 0 and 2 from the right, 1 and 3 from the left
+        const int right = __builtin_amdgcn_update_dpp(0, (int)v, 0x104, 0xf, 0x5, false);
+        return (uint32_t)__builtin_amdgcn_update_dpp(right, (int)v, 0x114, 0xf, 0xa, false);
+    }
+    if constexpr (DISTANCE == 8) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false);  // row_ror:8
+    if constexpr (DISTANCE == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return (threadIdx.x & 16u) != 0 ? r[0] : r[1];
+    }
+    if constexpr (DISTANCE == 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return (threadIdx.x & 32u) != 0 ? r[0] : r[1];
+    }
+}
+template <uint32_t RUN, uint32_t DISTANCE>
+__device__ __forceinline__ void sort_step(uint64_t& key) {
+    const uint64_t other = (uint64_t)exchanged<DISTANCE>((uint32_t)(key >> 32)) << 32 | exchanged<DISTANCE>((uint32_t)key);
+    const bool larger = ((threadIdx.x & DISTANCE) == 0) == ((threadIdx.x & RUN) == 0 || RUN == 64);
+    if (larger == (other > key)) key = other;  // (equal ones: either)
+    if constexpr (DISTANCE > 1) sort_step<RUN, DISTANCE / 2>(key);
+    else if constexpr (RUN < 64) sort_step<RUN * 2, RUN>(key);
+}
+// Lane i of the wave gets the i-th largest of its keys (a bitonic network).
+__device__ __forceinline__ uint64_t sorted(uint64_t key) {
+    sort_step<2, 1>(key);
+    return key;
 }
 
 struct Picker {
@@ -327,9 +414,9 @@ struct Picker {
     const RowBins& bins;
     PickShared& sh;
     uint32_t row, tokens;  // tokens: listed ones
+    uint64_t mine;         // this thread's, where every token has a thread
 
-    // The key of listed token f.
-    __device__ __forceinline__ uint64_t token(uint32_t f) const {
+    __device__ __forceinline__ uint64_t load(uint32_t f) const {
         uint32_t low = 0, high = a.n_parts;
         while (high - low > 1) {
             const uint32_t mid = (low + high) / 2u;
@@ -338,136 +425,132 @@ struct Picker {
         const uint32_t i = a.lists[(size_t)row * a.n + (size_t)low * kPart + (f - sh.listed[low])];
         return key_of(a.logits[(size_t)row * a.stride + i], i);
     }
-    __device__ __forceinline__ uint64_t weight(uint64_t key) const { return weight_of(power_of(logit_of(key), r), bins.top); }
-    __device__ __forceinline__ uint32_t bin(uint64_t key) const { return bin_of(power_of(logit_of(key), r), bins.top); }
+    // The key of listed token f of this thread.
+    __device__ __forceinline__ uint64_t token(uint32_t f) const { return tokens <= kPickThreads ? mine : load(f); }
+    __device__ __forceinline__ double quarters_of(uint64_t key) const { return quarters(logit_of(key), r, bins.o); }
+    __device__ __forceinline__ uint64_t weight(uint64_t key) const { return weight_of(quarters_of(key), bins.o); }
 
-    // Thread i gets the i-th largest of the workgroup's keys: a bitonic network, whose steps over less than a wave need no barrier.
-    __device__ __forceinline__ uint64_t sorted(uint64_t key) {
-        uint32_t size = 64;
-        while (size < tokens) size *= 2u;
-        const uint32_t i = threadIdx.x;
-        for (uint32_t run = 2; run <= size; run *= 2u)
-            for (uint32_t distance = run / 2u; distance != 0; distance /= 2u) {
-                uint64_t other;
-                if (distance >= 64u) {
-                    __syncthreads();
-                    sh.key[i] = key;
-                    __syncthreads();
-                    other = sh.key[i ^ distance];
-                } else {
-                    other = exchanged(key, distance);
-                }
-                const bool larger = ((i & distance) == 0) == ((i & run) == 0 || run == size);
-                if (larger ? other > key : other < key) key = other;
-            }
-        return key;
-    }
-
-    // The threshold where every listed token has a thread.
-    __device__ __forceinline__ uint64_t few_threshold() {
-        const uint64_t key = sorted(threadIdx.x < tokens ? token(threadIdx.x) : 0);
-        const bool in = threadIdx.x < tokens;
-        const uint32_t b = in ? bin(key) : kBins;
-        const uint64_t w = in ? weight(key) : 0;
-        bool taken = in && b <= bins.k_bin;
-        uint64_t mass = bins.whole || !r.masses() ? 0 : RowBins::before(bins.mass, bins.k_bin);
-        if (bins.k_bin < kBins) {  // of the last bin as many as are missing
-            uint64_t in_front;
-            sum_before<kPickWaves>(in && b < bins.k_bin, sh.slots[0], in_front);
-            const uint64_t missing = r.top_k - RowBins::before(bins.count, bins.k_bin);
-            taken = in && (b < bins.k_bin || (b == bins.k_bin && threadIdx.x - in_front < missing));
-        }
-        if (r.top_p < 1.0) {
-            // masses in front of each: of a whole list as they are, else of a bin in which the nucleus may end, behind what the histogram has in front of it
-            uint64_t kept;
-            const uint64_t of_last = sum_before<kPickWaves>(taken && (bins.whole || b == bins.k_bin) ? w : 0, sh.slots[1], kept);
-            mass += kept;
-            const uint64_t target = share_of_mass(r.top_p, mass);
-            if (bins.whole) {
-                taken = taken && of_last < target;
-            } else {
-                const uint32_t end = max(min(min(RowBins::reaching(bins.mass, target), bins.k_bin), bins.p_last), bins.p_first);
-                uint64_t all;
-                const uint64_t in_front = RowBins::before(bins.mass, end), in_bin = sum_before<kPickWaves>(b == end ? w : 0, sh.slots[2], all);
-                taken = taken && (b < end || (b == end && (in_bin == 0 || in_front + in_bin < target)));
-            }
-        }
-        uint64_t n;
-        sum_before<kPickWaves>(taken, sh.slots[3], n);  // what is taken is in front
-        if (taken && threadIdx.x + 1u == n) sh.found[0] = key;
-        __syncthreads();
-        return sh.found[0];
-    }
-
-    // Of the listed tokens whose keys are from `least` on and whose bin is `bin_` (kBins: any), from the largest key down, as many as are `target` tokens, or as their
-    // masses take to reach `target`: the smallest key of those, and their mass.
-    __device__ __forceinline__ uint64_t select(uint32_t bin_, uint64_t least, uint64_t target, bool by_mass, uint64_t& mass) {
-        uint64_t threshold = 0, left = target;
+    // Of the listed tokens of one bin whose keys are from `least` on, from the largest key down, as many as are `goal` tokens, or as their masses take to reach `goal`: the
+    // smallest key of those, and their mass.
+    __device__ __forceinline__ uint64_t select(uint32_t bin, uint64_t least, uint64_t goal, bool by_mass, uint64_t& mass) {
+        // A bin is 2048 steps of y wide first, of which the one where the goal is reached holds few tokens, as a rule; else their keys' digits, from the highest.
+        uint64_t prefix = 0;  // of the keys that are left, from bit `known` up
+        uint32_t step = 0;
         mass = 0;
-        for (int known = 64, shift = 64 - (int)kDigit;; known = shift, shift = shift > (int)kDigit ? shift - (int)kDigit : 0) {
-            // digits from the highest; the last one overlaps the one before it, whose bits are the same for all that are left
+        for (int known = 64, shift = 64;; known = shift, shift = shift == 64 ? 64 - (int)kDigit : shift > (int)kDigit ? shift - (int)kDigit : 0) {
+            const auto is_left = [&](uint64_t key, double& y4, double& place) {
+                y4 = quarters_of(key);
+                const double whole = whole_below(y4);
+                place = y4 - whole;  // in [0, 1), more of a larger one
+                return key >= least && bin_index(bin_of(whole, bins.o)) == bin && (shift == 64 || (step_of(place) == step && (known == 64 || key >> known == prefix >> known)));
+            };
             __syncthreads();
             if (threadIdx.x < 4) sh.found[threadIdx.x] = 0;
-            for (uint32_t d = threadIdx.x; d < kDigits; d += kPickThreads) sh.digit.count[d] = 0, sh.digit.mass[d] = 0;
+            if (threadIdx.x == 0) sh.together = 0;
+            for (uint32_t d = threadIdx.x; d < kDigits; d += kPickThreads) sh.count[d] = 0, sh.mass[d] = 0;
             __syncthreads();
             for (uint32_t f = threadIdx.x; f < tokens; f += kPickThreads) {
                 const uint64_t key = token(f);
-                if (key < least || (known < 64 && key >> known != threshold >> known) || (bin_ < kBins && bin(key) != bin_)) continue;
-                const uint32_t d = (uint32_t)(key >> shift) & (kDigits - 1u);
-                atomicAdd(&sh.digit.count[d], 1u), atomicAdd(&sh.digit.mass[d], (unsigned long long)weight(key));
+                double y4, place;
+                if (!is_left(key, y4, place)) continue;
+                const uint32_t d = shift == 64 ? step_of(place) : (uint32_t)(key >> shift) & (kDigits - 1u);
+                atomicAdd(&sh.count[d], 1u), atomicAdd(&sh.mass[d], (unsigned long long)weight_of(y4, bins.o));
             }
             __syncthreads();
             // thread t has digits 2047 - 2 t and the one below
             const uint32_t d0 = kDigits - 1u - 2u * threadIdx.x, d1 = d0 - 1u;
-            const uint64_t m0 = sh.digit.mass[d0], m1 = sh.digit.mass[d1], n0 = by_mass ? m0 : sh.digit.count[d0], n1 = by_mass ? m1 : sh.digit.count[d1];
+            const uint64_t m0 = sh.mass[d0], m1 = sh.mass[d1], n0 = by_mass ? m0 : sh.count[d0], n1 = by_mass ? m1 : sh.count[d1];
             uint64_t all, all_mass;
             const uint64_t before = sum_before<kPickWaves>(n0 + n1, sh.slots[0], all), mass_before = sum_before<kPickWaves>(m0 + m1, sh.slots[1], all_mass);
-            const uint64_t goal = left < all ? left : all;  // (what there is may be a little less than the bins' masses said)
+            goal = goal < all ? goal : all;  // (what there is may be a little less than the bins' masses said)
             if (before < goal && goal <= before + n0 + n1) {
                 const bool second = goal > before + n0;
                 sh.found[0] = second ? d1 : d0, sh.found[1] = goal - before - (second ? n0 : 0), sh.found[2] = mass_before + (second ? m0 : 0);
             }
             __syncthreads();
-            const uint64_t digit = sh.found[0];
-            left = sh.found[1], mass += sh.found[2];
-            threshold = (threshold & ~((uint64_t)(kDigits - 1u) << shift)) | digit << shift;
-            if (shift != 0 && sh.digit.count[digit] != 1u) continue;
-            mass += sh.digit.mass[digit];  // the one token that is left
-            if (shift == 0) return threshold;
+            const uint32_t digit = (uint32_t)sh.found[0];
+            goal = sh.found[1], mass += sh.found[2];
+            if (shift == 64) step = digit;
+            else prefix = (prefix & ~((uint64_t)(kDigits - 1u) << shift)) | (uint64_t)digit << shift;
+            if (sh.count[digit] > 64u) continue;  // (a key's last digit leaves one)
+            // what is left has a lane each
             for (uint32_t f = threadIdx.x; f < tokens; f += kPickThreads) {
                 const uint64_t key = token(f);
-                if (key >= least && key >> shift == threshold >> shift && (bin_ == kBins || bin(key) == bin_)) sh.found[3] = key;
+                const double y4 = quarters_of(key), whole = whole_below(y4);
+                if (key >= least && bin_index(bin_of(whole, bins.o)) == bin && step_of(y4 - whole) == step && (shift == 64 || key >> shift == prefix >> shift))
+                    sh.key[atomicAdd(&sh.together, 1u)] = key;
             }
             __syncthreads();
+            if (threadIdx.x < 64u) {
+                const uint64_t key = sorted(threadIdx.x < sh.together ? sh.key[threadIdx.x] : 0), w = key != 0 ? weight(key) : 0, upto = lanes_upto(w);
+                const bool taken = key != 0 && (by_mass ? upto - w < goal : threadIdx.x < goal);
+                const uint64_t takers = __ballot(taken);  // (from lane 0 on)
+                if (threadIdx.x + 1u == (uint32_t)__popcll(takers)) sh.found[3] = key, sh.found[2] = upto;
+            }
+            __syncthreads();
+            mass += sh.found[2];
             return sh.found[3];
         }
     }
+    static __device__ __forceinline__ uint32_t step_of(double place) { return min((uint32_t)(place * (double)kDigits), kDigits - 1u); }
 
-    // The threshold where there are more listed tokens than threads.
-    __device__ __forceinline__ uint64_t many_threshold() {
-        uint64_t threshold = 0, mass = r.masses() ? RowBins::before(bins.mass, bins.k_bin) : 0;
+    // The smallest key that is kept.
+    __device__ __forceinline__ uint64_t threshold() {
+        uint64_t least = 0, mass = r.masses() ? RowBins::before(bins.mass, bins.k_bin) : 0, in_bin;
         if (bins.k_bin < kBins) {
-            uint64_t in_bin;
-            threshold = select(bins.k_bin, 0, r.top_k - RowBins::before(bins.count, bins.k_bin), false, in_bin);
+            least = select(bins.k_bin, 0, r.top_k - RowBins::before(bins.count, bins.k_bin), false, in_bin);
             mass += in_bin;
         }
-        if (r.top_p >= 1.0) return threshold;
-        if (bins.whole) {
-            uint64_t sum = 0;
-            for (uint32_t f = threadIdx.x; f < tokens; f += kPickThreads) {
-                const uint64_t key = token(f);
-                sum += key >= threshold ? weight(key) : 0;
-            }
-            __syncthreads();
-            sum_before<kPickWaves>(sum, sh.slots[2], mass);
-            return select(kBins, threshold, share_of_mass(r.top_p, mass), true, sum);
+        if (r.top_p >= 1.0) return least;
+        if (!bins.whole) {
+            const uint64_t target = share_of_mass(r.top_p, mass);
+            const uint32_t end = max(min(min(RowBins::reaching(bins.mass, target), bins.k_bin), bins.p_last), bins.p_first);
+            const uint64_t in_front = RowBins::before(bins.mass, end);
+            return max(select(end, least, target > in_front ? target - in_front : 1, true, in_bin), least);
         }
-        const uint64_t target = share_of_mass(r.top_p, mass);
-        const uint32_t end = max(min(min(RowBins::reaching(bins.mass, target), bins.k_bin), bins.p_last), bins.p_first);
-        const uint64_t in_front = RowBins::before(bins.mass, end);
-        return select(end, threshold, target > in_front ? target - in_front : 1, true, mass);
+        // nobody has weighed the bins of what top-k leaves
+        __syncthreads();
+        if (threadIdx.x < 64u * kLaneBins) sh.mass[threadIdx.x] = 0;
+        __syncthreads();
+        for (uint32_t f = threadIdx.x; f < tokens; f += kPickThreads) {
+            const uint64_t key = token(f);
+            if (key < least) continue;
+            const double y4 = quarters_of(key);
+            atomicAdd(&sh.mass[bin_index(bin_of(whole_below(y4), bins.o))], (unsigned long long)weight_of(y4, bins.o));
+        }
+        __syncthreads();
+        uint64_t of[kLaneBins], sum = 0;
+        const uint32_t lane = threadIdx.x & 63u;
+#pragma unroll
+        for (uint32_t i = 0; i < kLaneBins; i++) of[i] = sum += sh.mass[kLaneBins * lane + i];
+        const uint64_t front = lanes_upto(sum) - sum;
+#pragma unroll
+        for (uint32_t i = 0; i < kLaneBins; i++) of[i] += front;
+        const uint64_t target = share_of_mass(r.top_p, RowBins::before(of, kBins));
+        const uint32_t end = min(RowBins::reaching(of, target), kBins - 1u);
+        return max(select(end, least, target - RowBins::before(of, end), true, in_bin), least);
     }
 };
+
+// All of it where one wave has every token that may be taken: sorted by key for the cuts, then by index.
+__device__ __forceinline__ void pick_in_a_wave(const SampleArgs& a, uint32_t row, const Rule& r, const RowBins& bins, const Picker& pick, float u) {
+    const uint64_t key = sorted(pick.mine), w = key != 0 ? pick.weight(key) : 0;
+    bool taken = key != 0 && threadIdx.x < r.top_k;
+    if (r.top_p < 1.0) {
+        const uint64_t upto = lanes_upto(taken ? w : 0), target = share_of_mass(r.top_p, read_lane(upto, 63));
+        taken = taken && upto - w < target;
+    }
+    taken = taken && (double)w >= bins.floor;
+    // (the lower half of a key falls with the index; what is not taken goes behind)
+    const uint64_t by_index = sorted(taken ? key << 32 | key >> 32 : 0);
+    const uint64_t back = by_index << 32 | by_index >> 32, weight = by_index != 0 ? pick.weight(back) : 0, upto = lanes_upto(weight), mass = read_lane(upto, 63);
+    const double at = (u > 0.0f ? (double)u : 0.0) * (double)mass;
+    const uint64_t target = at < (double)mass ? min((uint64_t)at, mass - 1u) : mass - 1u;  // the pick is the first to exceed it
+    if (upto - weight <= target && target < upto) {
+        a.out[row] = index_of(back);
+        if (a.prob) a.prob[row] = (float)(exact_weight(pick.quarters_of(back), bins.o) / (double)mass);
+    }
+}
 
 __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a) {
     __shared__ PickShared sh;
@@ -478,9 +561,9 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
     const uint32_t listed = threadIdx.x < a.n_parts ? parts[threadIdx.x].listed : 0;
     const float u = a.uniform[row];
     const Rule r = rule_of(a, row);
-    const RowBins bins = row_bins(a, row, r, sh.bins);
-    const double top = bins.top, floor = bins.floor;
-    if (!(top > kNever)) {
+    const RowBins bins = handed_on(a.rows[row], r);
+    const double floor = bins.floor;
+    if (bins.o.none()) {
         if (threadIdx.x == 0) {
             a.out[row] = WICK_ROCM_NO_TOKEN;
             if (a.prob) a.prob[row] = 0.0f;
@@ -491,8 +574,13 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
     const uint64_t upto = sum_before<kPickWaves>(listed, sh.slots[0], tokens);
     if (threadIdx.x < a.n_parts) sh.listed[threadIdx.x] = (uint32_t)upto, sh.part_mass[threadIdx.x] = sure;
     __syncthreads();
-    Picker pick{a, r, bins, sh, row, (uint32_t)tokens};
-    const uint64_t threshold = tokens == 0 ? 0 : tokens <= kPickThreads ? pick.few_threshold() : pick.many_threshold();
+    Picker pick{a, r, bins, sh, row, (uint32_t)tokens, 0};
+    if (tokens <= kPickThreads && threadIdx.x < tokens) pick.mine = pick.load(threadIdx.x);
+    if (bins.whole && tokens <= 64) {
+        if (threadIdx.x < 64u) pick_in_a_wave(a, row, r, bins, pick, u);
+        return;
+    }
+    const uint64_t threshold = tokens == 0 ? 0 : pick.threshold();
     // what every part keeps
     for (uint32_t f = threadIdx.x; f < tokens; f += kPickThreads) {
         const uint64_t key = pick.token(f), w = key >= threshold ? pick.weight(key) : 0;
@@ -500,7 +588,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
     }
     __syncthreads();
     uint64_t mass;
-    const uint64_t in_part = threadIdx.x < a.n_parts ? sh.part_mass[threadIdx.x] : 0, in_front = sum_before<kPickWaves>(in_part, sh.slots[0], mass);
+    const uint64_t in_part = threadIdx.x < a.n_parts ? sh.part_mass[threadIdx.x] : 0, in_front = sum_before<kPickWaves>(in_part, sh.slots[2], mass);
     const double at = (u > 0.0f ? (double)u : 0.0) * (double)mass;
     const uint64_t target = at < (double)mass ? min((uint64_t)at, mass - 1u) : mass - 1u;  // the pick is the first to exceed it
     if (in_front <= target && target < in_front + in_part) sh.found[0] = threadIdx.x, sh.found[1] = target - in_front;  // (one thread: the mass is not 0)
@@ -514,19 +602,19 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
         weight[k] = 0;
         if (i >= a.n) continue;
         const float l = logits[i];
-        const double y = power_of(l, r);
-        if (!(y > kNever) || bin_of(y, top) >= kBins || key_of(l, i) < threshold) continue;
-        const uint64_t w = weight_of(y, top);
+        const double y4 = quarters(l, r, bins.o);
+        if (!(bin_of(whole_below(y4), bins.o) < (double)kBins) || key_of(l, i) < threshold) continue;
+        const uint64_t w = weight_of(y4, bins.o);
         weight[k] = (double)w >= floor ? w : 0;
         sum += weight[k];
     }
-    uint64_t all, before = sum_before<kPickWaves>(sum, sh.slots[1], all);
+    uint64_t all, before = sum_before<kPickWaves>(sum, sh.slots[3], all);
     if (before <= goal && goal < before + sum) {
         uint32_t i = part * kPart + threadIdx.x * (kPart / kPickThreads);
 #pragma unroll
         for (uint32_t k = 0; k < kPart / kPickThreads; k++) before += weight[k], i += before <= goal;
         a.out[row] = i;
-        if (a.prob) a.prob[row] = (float)(exact_weight(power_of(logits[i], r), top) / (double)mass);
+        if (a.prob) a.prob[row] = (float)(exact_weight(quarters(logits[i], r, bins.o), bins.o) / (double)mass);
     }
 }
 
@@ -534,12 +622,15 @@ size_t parts_of(uint32_t n) { return (n + kPart - 1u) / kPart; }
 
 }  // namespace
 
-size_t sample_scratch_bytes(uint32_t rows, uint32_t n) { return (size_t)rows * (parts_of(n) * sizeof(SamplePart) + (size_t)n * sizeof(uint32_t)); }
+size_t sample_scratch_bytes(uint32_t rows, uint32_t n) {
+    return (size_t)rows * (sizeof(SampleRow) + parts_of(n) * sizeof(SamplePart) + (size_t)n * sizeof(uint32_t));
+}
 
 hipError_t launch_sample(const float* d_logits, uint32_t stride, uint32_t rows, uint32_t n, const wick_rocm_sample_params* d_params, const float* d_uniform,
                          uint32_t* d_out, float* d_prob, void* d_scratch, const Launch& L) {
     if (rows == 0) return hipSuccess;
-    SampleArgs a{d_logits, d_params, d_uniform, d_out, d_prob, static_cast<SamplePart*>(d_scratch), nullptr, n, stride, (uint32_t)parts_of(n)};
+    SampleArgs a{d_logits, d_params, d_uniform, d_out, d_prob, static_cast<SampleRow*>(d_scratch), nullptr, nullptr, n, stride, (uint32_t)parts_of(n)};
+    a.parts = reinterpret_cast<SamplePart*>(a.rows + rows);
     a.lists = reinterpret_cast<uint32_t*>(a.parts + (size_t)rows * a.n_parts);
     hipError_t e = launch_kernel(L, kFamOther, sample_bins_kernel, dim3(a.n_parts, rows), dim3(kPartThreads), a);
     if (e == hipSuccess) e = launch_kernel(L, kFamOther, sample_list_kernel, dim3(a.n_parts, rows), dim3(kPartThreads), a);
