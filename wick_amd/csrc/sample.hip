@@ -10,6 +10,7 @@
 // Where top-k leaves few, tokens are only counted in 1., and all that may be taken are listed: no weights but theirs.  What is listed is at most some hundred
 // tokens as a rule, which 3. sorts, and a row's all in the worst case (all logits alike), for which there is room.
 #include <algorithm>
+#include <type_traits>
 
 #include "wick_rocm_device.h"
 #include "wick_rocm_internal.h"
@@ -22,7 +23,6 @@ constexpr uint32_t kPart = 4096, kMaxParts = kSampleMaxTokens / kPart;  // token
 constexpr int kOctaves = 46, kSteps = 4;                                // bins: kSteps to a power of two
 constexpr uint32_t kBins = kOctaves * kSteps, kLaneBins = 3;            // every wave has them all, three a lane
 static_assert(kBins <= 64 * kLaneBins && kMaxParts <= 128);
-constexpr int kFraction = 43;  // masses are whole numbers of 2^-43: up to 2^19 tokens of less than 2 each
 constexpr uint32_t kFew = 512; // top-k up to which all that it leaves is listed: 3. sorts up to 1024 tokens, and the last bin may be half of them
 constexpr double kLog2e = 1.4426950408889634;
 constexpr double kInfinite4 = 0x1p1000;                                 // 4 y of an infinite logit
@@ -73,48 +73,61 @@ __device__ __forceinline__ Rule rule_of(const SampleArgs& a, uint32_t row) {
     return r;
 }
 
-// What a row's tokens are measured from: E, and whether an infinite logit is the largest.
+// What a row's tokens are measured from: 4 E.  Wild: E is of no use to the short forms below, for an infinite logit is the largest, or E is beyond 2^48.
 struct Origin {
-    double top4;  // 4 E; -infinity: nothing may be taken
-    bool infinite;
+    double top4;  // -infinity: nothing may be taken
+    bool wild;
     __device__ __forceinline__ bool none() const { return !(top4 > -__builtin_inf()); }
 };
+__device__ __forceinline__ Origin origin(double top4) { return {top4, !(__builtin_fabs(top4) < 0x1p50)}; }
 __device__ __forceinline__ Origin origin_of(float largest, const Rule& r) {
-    if (!(largest > -__builtin_inff())) return {-__builtin_inf(), false};
-    if (largest == __builtin_inff()) return {kInfinite4, true};
-    return {kSteps * __builtin_floor((double)largest * r.inverse4 / kSteps), false};
+    if (!(largest > -__builtin_inff())) return origin(-__builtin_inf());
+    if (largest == __builtin_inff()) return origin(kInfinite4);
+    return origin(kSteps * __builtin_floor((double)largest * r.inverse4 / kSteps));
 }
 // A token's 4 y; of one that is never taken, -infinity or NaN.  (T may be infinite too.)
+template <bool WILD>
 __device__ __forceinline__ double quarters(float l, const Rule& r, const Origin& o) {
     const double y4 = (double)l * r.inverse4;
-    return o.infinite ? (l == __builtin_inff() ? kInfinite4 : -__builtin_inf()) : y4;
+    return WILD && o.top4 == kInfinite4 ? (l == __builtin_inff() ? kInfinite4 : -__builtin_inf()) : y4;
 }
-// Without the conversions of the vector unit, which take four times as long as an addition: a number below 2^51 is rounded to a whole one by adding and taking
-// away 1.5 2^52, and has it as the sum's lower bits.  (What is larger comes out whole too, if not as the nearest.)
+// The bin of a token: 4 y rounded to a whole number, counted from 4 E + 4 down, or kBins: it weighs nothing.  The whole number is the token's own, so that the bins of
+// another E are the same ones, counted from elsewhere.  (The short form has it in the lower bits of 4 y + 1.5 2^52, without the vector unit's
+// conversions, which take four times as long as an addition.)
 constexpr double kRound = 0x1.8p52;
-__device__ __forceinline__ double whole_below(double y4) {
-    const double r = (y4 + kRound) - kRound;
-    return r > y4 ? r - 1.0 : r;
+template <bool WILD>
+__device__ __forceinline__ uint32_t bin_of(double y4, const Origin& o) {
+    if constexpr (WILD) {
+        const double below = (o.top4 - __builtin_rint(y4)) + kSteps;
+        return below < (double)kBins ? (uint32_t)fmax(below, 0.0) : kBins;
+    } else {
+        const double from = o.top4 + (kRound + kSteps), at = y4 + kRound;  // (both whole, and their difference)
+        return from - at < (double)kBins ? __double2loint(from) - __double2loint(at) : kBins;
+    }
 }
-// The bin of a token with floor `whole` of its 4 y; kBins or NaN and what is not below it: it weighs nothing.  Falls with rising y; every step is exact, so that the bins of
-// another E are the same ones, counted from elsewhere.
-__device__ __forceinline__ double bin_of(double whole, const Origin& o) { return (o.top4 - whole) + (kSteps - 1); }
-__device__ __forceinline__ uint32_t bin_index(double bin) { return (uint32_t)fmax(bin, 0.0); }  // (beyond 2^51, where wholes are not the nearest, it may be below 0)
-// 2^(y - E) times 2^kFraction, for y of a bin: 2^f for |f| <= 1/2 by the polynomial that interpolates it at the Chebyshev nodes (off by 5e-16), put in place by
-// adding to its exponent.
-__device__ __forceinline__ double exact_weight(double y4, const Origin& o) {
-    const double v = (y4 - o.top4) * (1.0 / kSteps), n = v + kRound, f = v - (n - kRound);
-    double p = 0x1.e606452d2a4bep-28;
-    p = __builtin_fma(p, f, 0x1.b675bd7308f14p-24), p = __builtin_fma(p, f, 0x1.62bfd472738fap-20), p = __builtin_fma(p, f, 0x1.ffcb54054027cp-17);
-    p = __builtin_fma(p, f, 0x1.4309130972582p-13), p = __builtin_fma(p, f, 0x1.5d87fe9d7ab38p-10), p = __builtin_fma(p, f, 0x1.3b2ab6fba1dcfp-7);
-    p = __builtin_fma(p, f, 0x1.c6b08d703ce45p-5), p = __builtin_fma(p, f, 0x1.ebfbdff82c598p-3), p = __builtin_fma(p, f, 0x1.62e42fefa3a19p-1);
-    p = __builtin_fma(p, f, 1.0);
-    return __hiloint2double(__double2hiint(p) + (int)((uint32_t)(__double2loint(n) + kFraction) << 20), __double2loint(p));
-}
-// ... in whole numbers: rounded by adding 2^52.
-__device__ __forceinline__ uint64_t weight_of(double y4, const Origin& o) {
-    return __builtin_bit_cast(uint64_t, exact_weight(y4, o) + 0x1p52) & ((1ull << 52) - 1u);
-}
+// 2^(y - E) times 2^43 (up to 2^19 tokens of less than 2 each), for y of a bin: 2^(g / 4) for |g| <= 2 by the polynomial that interpolates it at the Chebyshev nodes (off by 5e-16), put in place by adding
+// to its exponent; 1.5 2^54 rounds to whole fours.
+struct Power {  // (its coefficients are kept in scalar registers)
+    double c[11] = {0x1p43, 0x1.62e42fefa3a19p40, 0x1.ebfbdff82c598p36, 0x1.c6b08d703ce45p32, 0x1.3b2ab6fba1dcfp28, 0x1.5d87fe9d7ab38p23, 0x1.4309130972582p18,
+                    0x1.ffcb54054027cp12, 0x1.62bfd472738fap7, 0x1.b675bd7308f14p1, 0x1.e606452d2a4bep-5};
+    __device__ __forceinline__ void keep() {
+#pragma unroll
+        for (int i = 0; i < 11; i++) asm("" : "+s"(c[i]));
+    }
+    __device__ __forceinline__ double exact(double y4, const Origin& o) const {
+        const double d = y4 - o.top4, n = d + 0x1.8p54, g = d - (n - 0x1.8p54);
+        double p = c[10];
+#pragma unroll
+        for (int i = 9; i >= 0; i--) p = __builtin_fma(p, g, c[i]);
+        return __hiloint2double(__double2hiint(p) + (int)((uint32_t)__double2loint(n) << 20), __double2loint(p));
+    }
+    // ... in whole numbers: rounded by adding 2^52.
+    __device__ __forceinline__ uint64_t whole(double y4, const Origin& o) const {
+        return __builtin_bit_cast(uint64_t, exact(y4, o) + 0x1p52) & ((1ull << 52) - 1u);
+    }
+};
+__device__ __forceinline__ double exact_weight(double y4, const Origin& o) { return Power().exact(y4, o); }
+__device__ __forceinline__ uint64_t weight_of(double y4, const Origin& o) { return Power().whole(y4, o); }
 
 // (logit, lower index first) as one number, of a logit that may be taken; no key is 0.
 __device__ __forceinline__ uint64_t key_of(float l, uint32_t i) {
@@ -180,14 +193,21 @@ __global__ __launch_bounds__(kPartThreads) void sample_bins_kernel(SampleArgs a)
 #pragma unroll
     for (uint32_t w = 0; w < kPartThreads / 64; w++) top = fmaxf(top, tops[w]);
     const Origin o = origin_of(top, r);
-    if (!o.none() && (counts || masses)) {
+    const auto add = [&](auto wild) {
+        Power power;
+        power.keep();
 #pragma unroll
         for (uint32_t k = 0; k < kPartLoads; k++) {
-            const double y4 = quarters(l[k], r, o), b = bin_of(whole_below(y4), o);
-            if (!(b < (double)kBins)) continue;
-            if (counts) atomicAdd(&count[bin_index(b)], 1u);
-            if (masses) atomicAdd(&mass[bin_index(b)], (unsigned long long)weight_of(y4, o));
+            const double y4 = quarters<decltype(wild)::value>(l[k], r, o);
+            const uint32_t b = bin_of<decltype(wild)::value>(y4, o);
+            if (b >= kBins) continue;
+            if (counts) atomicAdd(&count[b], 1u);
+            if (masses) atomicAdd(&mass[b], (unsigned long long)power.whole(y4, o));
         }
+    };
+    if (!o.none() && (counts || masses)) {
+        if (o.wild) add(std::true_type());
+        else add(std::false_type());
     }
     __syncthreads();
     SamplePart& part = a.parts[(size_t)row * a.n_parts + blockIdx.x];
@@ -251,7 +271,7 @@ __device__ __forceinline__ RowBins row_bins(const SampleArgs& a, uint32_t row, c
         off[i] = d < (double)kOctaves ? (int)d : kOctaves;
     }
     if (bins.o.none()) return bins;
-    bins.floor = r.min_p * (double)weight_of(quarters(most, r, bins.o), bins.o);
+    bins.floor = r.min_p * (double)weight_of(quarters<true>(most, r, bins.o), bins.o);
     const bool counts = r.counts(), masses = r.masses();
     if (!counts && !masses) return bins;
     for (uint32_t b = threadIdx.x; b < 64u * kLaneBins; b += blockDim.x) {
@@ -299,7 +319,7 @@ __device__ __forceinline__ void hand_on(const RowBins& bins, SampleRow& row) {  
 __device__ __forceinline__ RowBins handed_on(const SampleRow& row, const Rule& r) {
     RowBins bins;
     const uint32_t lane = threadIdx.x & 63u;
-    bins.o = {row.top4, row.top4 == kInfinite4}, bins.floor = row.floor, bins.k_bin = row.k_bin, bins.p_first = row.p_first, bins.p_last = row.p_last, bins.whole = r.few();
+    bins.o = origin(row.top4), bins.floor = row.floor, bins.k_bin = row.k_bin, bins.p_first = row.p_first, bins.p_last = row.p_last, bins.whole = r.few();
 #pragma unroll
     for (uint32_t i = 0; i < kLaneBins; i++) bins.mass[i] = row.mass[kLaneBins * lane + i], bins.count[i] = row.count[kLaneBins * lane + i];
     return bins;
@@ -309,7 +329,8 @@ __device__ __forceinline__ RowBins handed_on(const SampleRow& row, const Rule& r
 __global__ __launch_bounds__(kPartThreads) void sample_list_kernel(SampleArgs a) {
     __shared__ BinShared shared_bins;
     __shared__ uint64_t slots[kPartThreads / 64];
-    __shared__ uint2 candidates[kPart];
+    __shared__ float candidates[kPart];
+    __shared__ uint16_t places[kPart];
     __shared__ uint32_t listed, together;
     const uint32_t row = blockIdx.y, first = blockIdx.x * kPart;
     const float* const logits = a.logits + (size_t)row * a.stride;
@@ -328,23 +349,26 @@ __global__ __launch_bounds__(kPartThreads) void sample_list_kernel(SampleArgs a)
     uint64_t sure = 0;
     uint32_t* const list = a.lists + (size_t)row * a.n + first;
     const uint32_t sure_bins = bins.sure();
-    const auto take = [&](float x, uint32_t i) {
-        const double y4 = quarters(x, r, bins.o), b = bin_of(whole_below(y4), bins.o);
-        if (b < (double)sure_bins) {
-            const uint64_t w = weight_of(y4, bins.o);
+    Power power;
+    power.keep();
+    const auto take = [&](auto wild, float x, uint32_t i) {
+        const double y4 = quarters<decltype(wild)::value>(x, r, bins.o);
+        const uint32_t b = bin_of<decltype(wild)::value>(y4, bins.o);
+        if (b < sure_bins) {
+            const uint64_t w = power.whole(y4, bins.o);
             sure += (double)w >= bins.floor ? w : 0;
-        } else if (b < (double)kBins && bins.lists(bin_index(b))) {
+        } else if (b < kBins && bins.lists(b)) {
             list[atomicAdd(&listed, 1u)] = i;
         }
     };
     // The last bin that matters; as a rule it is far above most tokens.  Those that may be in it or above (by their logit, with room for rounding) are put together
     // first, so that few waves do the rest.
     const uint32_t last = bins.k_bin < kBins || bins.p_first == kBins ? bins.k_bin : bins.p_last;
-    if (last == kBins) {
+    if (last == kBins && !bins.o.wild) {
 #pragma unroll
-        for (uint32_t k = 0; k < kPartLoads; k++) take(l[k], first + k * kPartThreads + threadIdx.x);
+        for (uint32_t k = 0; k < kPartLoads; k++) take(std::false_type(), l[k], first + k * kPartThreads + threadIdx.x);
     } else {
-        const double lowest = fmin((bins.o.top4 - (double)last) / r.inverse4, kInfinite4);
+        const double lowest = fmin((bins.o.top4 - (double)last) / r.inverse4, kInfinite4);  // (a bin goes half a step further down than its whole number, which is at 4 E + 4 - bin)
         const float low = (float)(lowest - __builtin_fabs(lowest) * 0x1p-20 - 0x1p-140);
 #pragma unroll
         for (uint32_t k = 0; k < kPartLoads; k++) {
@@ -353,10 +377,13 @@ __global__ __launch_bounds__(kPartThreads) void sample_list_kernel(SampleArgs a)
             uint32_t at = 0;
             if ((threadIdx.x & 63u) == 0) at = atomicAdd(&together, (uint32_t)__popcll(here));
             at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + __builtin_amdgcn_mbcnt_hi((uint32_t)(here >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)here, 0u));
-            if (l[k] >= low) candidates[at] = make_uint2(__float_as_uint(l[k]), first + k * kPartThreads + threadIdx.x);
+            if (l[k] >= low) candidates[at] = l[k], places[at] = (uint16_t)(k * kPartThreads + threadIdx.x);
         }
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < together; i += kPartThreads) take(__uint_as_float(candidates[i].x), candidates[i].y);
+        for (uint32_t i = threadIdx.x; i < together; i += kPartThreads) {
+            if (bins.o.wild) take(std::true_type(), candidates[i], first + places[i]);
+            else take(std::false_type(), candidates[i], first + places[i]);
+        }
         __syncthreads();  // (listed)
     }
     uint64_t all;
@@ -427,7 +454,7 @@ struct Picker {
     }
     // The key of listed token f of this thread.
     __device__ __forceinline__ uint64_t token(uint32_t f) const { return tokens <= kPickThreads ? mine : load(f); }
-    __device__ __forceinline__ double quarters_of(uint64_t key) const { return quarters(logit_of(key), r, bins.o); }
+    __device__ __forceinline__ double quarters_of(uint64_t key) const { return quarters<true>(logit_of(key), r, bins.o); }
     __device__ __forceinline__ uint64_t weight(uint64_t key) const { return weight_of(quarters_of(key), bins.o); }
 
     // Of the listed tokens of one bin whose keys are from `least` on, from the largest key down, as many as are `goal` tokens, or as their masses take to reach `goal`: the
@@ -439,10 +466,8 @@ struct Picker {
         mass = 0;
         for (int known = 64, shift = 64;; known = shift, shift = shift == 64 ? 64 - (int)kDigit : shift > (int)kDigit ? shift - (int)kDigit : 0) {
             const auto is_left = [&](uint64_t key, double& y4, double& place) {
-                y4 = quarters_of(key);
-                const double whole = whole_below(y4);
-                place = y4 - whole;  // in [0, 1), more of a larger one
-                return key >= least && bin_index(bin_of(whole, bins.o)) == bin && (shift == 64 || (step_of(place) == step && (known == 64 || key >> known == prefix >> known)));
+                y4 = quarters_of(key), place = y4 - __builtin_rint(y4);  // within half a step, more of a larger one
+                return key >= least && bin_of<true>(y4, bins.o) == bin && (shift == 64 || (step_of(place) == step && (known == 64 || key >> known == prefix >> known)));
             };
             __syncthreads();
             if (threadIdx.x < 4) sh.found[threadIdx.x] = 0;
@@ -476,8 +501,8 @@ struct Picker {
             // what is left has a lane each
             for (uint32_t f = threadIdx.x; f < tokens; f += kPickThreads) {
                 const uint64_t key = token(f);
-                const double y4 = quarters_of(key), whole = whole_below(y4);
-                if (key >= least && bin_index(bin_of(whole, bins.o)) == bin && step_of(y4 - whole) == step && (shift == 64 || key >> shift == prefix >> shift))
+                const double y4 = quarters_of(key);
+                if (key >= least && bin_of<true>(y4, bins.o) == bin && step_of(y4 - __builtin_rint(y4)) == step && (shift == 64 || key >> shift == prefix >> shift))
                     sh.key[atomicAdd(&sh.together, 1u)] = key;
             }
             __syncthreads();
@@ -492,7 +517,7 @@ struct Picker {
             return sh.found[3];
         }
     }
-    static __device__ __forceinline__ uint32_t step_of(double place) { return min((uint32_t)(place * (double)kDigits), kDigits - 1u); }
+    static __device__ __forceinline__ uint32_t step_of(double place) { return min((uint32_t)(place * (double)kDigits + (double)(kDigits / 2u)), kDigits - 1u); }
 
     // The smallest key that is kept.
     __device__ __forceinline__ uint64_t threshold() {
@@ -516,7 +541,7 @@ struct Picker {
             const uint64_t key = token(f);
             if (key < least) continue;
             const double y4 = quarters_of(key);
-            atomicAdd(&sh.mass[bin_index(bin_of(whole_below(y4), bins.o))], (unsigned long long)weight_of(y4, bins.o));
+            atomicAdd(&sh.mass[bin_of<true>(y4, bins.o)], (unsigned long long)weight_of(y4, bins.o));
         }
         __syncthreads();
         uint64_t of[kLaneBins], sum = 0;
@@ -602,8 +627,8 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
         weight[k] = 0;
         if (i >= a.n) continue;
         const float l = logits[i];
-        const double y4 = quarters(l, r, bins.o);
-        if (!(bin_of(whole_below(y4), bins.o) < (double)kBins) || key_of(l, i) < threshold) continue;
+        const double y4 = quarters<true>(l, r, bins.o);
+        if (bin_of<true>(y4, bins.o) >= kBins || key_of(l, i) < threshold) continue;
         const uint64_t w = weight_of(y4, bins.o);
         weight[k] = (double)w >= floor ? w : 0;
         sum += weight[k];
@@ -614,7 +639,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
 #pragma unroll
         for (uint32_t k = 0; k < kPart / kPickThreads; k++) before += weight[k], i += before <= goal;
         a.out[row] = i;
-        if (a.prob) a.prob[row] = (float)(exact_weight(quarters(logits[i], r, bins.o), bins.o) / (double)mass);
+        if (a.prob) a.prob[row] = (float)(exact_weight(quarters<true>(logits[i], r, bins.o), bins.o) / (double)mass);
     }
 }
 
