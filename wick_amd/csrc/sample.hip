@@ -393,7 +393,9 @@ __global__ __launch_bounds__(kPartThreads) void sample_list_kernel(SampleArgs a)
 }
 
 // 3.
-constexpr uint32_t kPickThreads = 1024, kPickWaves = kPickThreads / 64, kDigit = 11, kDigits = 1u << kDigit;
+// (Four waves: with sixteen, whose sums over the workgroup are sixteen times the same work, 64 rows took 13.8 us.)
+constexpr uint32_t kPickThreads = 1024, kPickWaves = kPickThreads / 64, kDigit = 11, kDigits = 1u << kDigit, kOwn = 1;
+constexpr uint32_t kEach = kPart / kPickThreads, kDigitsEach = kDigits / kPickThreads;
 
 struct PickShared {
     uint64_t slots[4][kPickWaves], part_mass[kMaxParts], found[4], key[64];
@@ -441,7 +443,7 @@ struct Picker {
     const RowBins& bins;
     PickShared& sh;
     uint32_t row, tokens;  // tokens: listed ones
-    uint64_t mine;         // this thread's, where every token has a thread
+    uint64_t own[kOwn];    // this thread's first ones
 
     __device__ __forceinline__ uint64_t load(uint32_t f) const {
         uint32_t low = 0, high = a.n_parts;
@@ -452,8 +454,14 @@ struct Picker {
         const uint32_t i = a.lists[(size_t)row * a.n + (size_t)low * kPart + (f - sh.listed[low])];
         return key_of(a.logits[(size_t)row * a.stride + i], i);
     }
-    // The key of listed token f of this thread.
-    __device__ __forceinline__ uint64_t token(uint32_t f) const { return tokens <= kPickThreads ? mine : load(f); }
+    // All listed tokens, each by a thread of its own.
+    template <typename F>
+    __device__ __forceinline__ void for_all(F f) const {
+#pragma unroll
+        for (uint32_t i = 0; i < kOwn; i++)
+            if (threadIdx.x + i * kPickThreads < tokens) f(own[i]);
+        for (uint32_t t = threadIdx.x + kOwn * kPickThreads; t < tokens; t += kPickThreads) f(load(t));
+    }
     __device__ __forceinline__ double quarters_of(uint64_t key) const { return quarters<true>(logit_of(key), r, bins.o); }
     __device__ __forceinline__ uint64_t weight(uint64_t key) const { return weight_of(quarters_of(key), bins.o); }
 
@@ -474,23 +482,27 @@ struct Picker {
             if (threadIdx.x == 0) sh.together = 0;
             for (uint32_t d = threadIdx.x; d < kDigits; d += kPickThreads) sh.count[d] = 0, sh.mass[d] = 0;
             __syncthreads();
-            for (uint32_t f = threadIdx.x; f < tokens; f += kPickThreads) {
-                const uint64_t key = token(f);
+            for_all([&](uint64_t key) {
                 double y4, place;
-                if (!is_left(key, y4, place)) continue;
+                if (!is_left(key, y4, place)) return;
                 const uint32_t d = shift == 64 ? step_of(place) : (uint32_t)(key >> shift) & (kDigits - 1u);
                 atomicAdd(&sh.count[d], 1u), atomicAdd(&sh.mass[d], (unsigned long long)weight_of(y4, bins.o));
-            }
+            });
             __syncthreads();
-            // thread t has digits 2047 - 2 t and the one below
-            const uint32_t d0 = kDigits - 1u - 2u * threadIdx.x, d1 = d0 - 1u;
-            const uint64_t m0 = sh.mass[d0], m1 = sh.mass[d1], n0 = by_mass ? m0 : sh.count[d0], n1 = by_mass ? m1 : sh.count[d1];
+            // thread t has the digits from 2047 - 8 t down
+            uint64_t sum = 0, masses = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < kDigitsEach; i++) {
+                const uint32_t d = kDigits - 1u - kDigitsEach * threadIdx.x - i;
+                masses += sh.mass[d], sum += by_mass ? sh.mass[d] : sh.count[d];
+            }
             uint64_t all, all_mass;
-            const uint64_t before = sum_before<kPickWaves>(n0 + n1, sh.slots[0], all), mass_before = sum_before<kPickWaves>(m0 + m1, sh.slots[1], all_mass);
+            uint64_t before = sum_before<kPickWaves>(sum, sh.slots[0], all), mass_before = sum_before<kPickWaves>(masses, sh.slots[1], all_mass);
             goal = goal < all ? goal : all;  // (what there is may be a little less than the bins' masses said)
-            if (before < goal && goal <= before + n0 + n1) {
-                const bool second = goal > before + n0;
-                sh.found[0] = second ? d1 : d0, sh.found[1] = goal - before - (second ? n0 : 0), sh.found[2] = mass_before + (second ? m0 : 0);
+            if (before < goal && goal <= before + sum) {
+                uint32_t d = kDigits - 1u - kDigitsEach * threadIdx.x;
+                for (uint64_t n; before + (n = by_mass ? sh.mass[d] : sh.count[d]) < goal; d--) before += n, mass_before += sh.mass[d];
+                sh.found[0] = d, sh.found[1] = goal - before, sh.found[2] = mass_before;
             }
             __syncthreads();
             const uint32_t digit = (uint32_t)sh.found[0];
@@ -499,12 +511,11 @@ struct Picker {
             else prefix = (prefix & ~((uint64_t)(kDigits - 1u) << shift)) | (uint64_t)digit << shift;
             if (sh.count[digit] > 64u) continue;  // (a key's last digit leaves one)
             // what is left has a lane each
-            for (uint32_t f = threadIdx.x; f < tokens; f += kPickThreads) {
-                const uint64_t key = token(f);
+            for_all([&](uint64_t key) {
                 const double y4 = quarters_of(key);
                 if (key >= least && bin_of<true>(y4, bins.o) == bin && step_of(y4 - __builtin_rint(y4)) == step && (shift == 64 || key >> shift == prefix >> shift))
                     sh.key[atomicAdd(&sh.together, 1u)] = key;
-            }
+            });
             __syncthreads();
             if (threadIdx.x < 64u) {
                 const uint64_t key = sorted(threadIdx.x < sh.together ? sh.key[threadIdx.x] : 0), w = key != 0 ? weight(key) : 0, upto = lanes_upto(w);
@@ -537,12 +548,11 @@ struct Picker {
         __syncthreads();
         if (threadIdx.x < 64u * kLaneBins) sh.mass[threadIdx.x] = 0;
         __syncthreads();
-        for (uint32_t f = threadIdx.x; f < tokens; f += kPickThreads) {
-            const uint64_t key = token(f);
-            if (key < least) continue;
+        for_all([&](uint64_t key) {
+            if (key < least) return;
             const double y4 = quarters_of(key);
             atomicAdd(&sh.mass[bin_of<true>(y4, bins.o)], (unsigned long long)weight_of(y4, bins.o));
-        }
+        });
         __syncthreads();
         uint64_t of[kLaneBins], sum = 0;
         const uint32_t lane = threadIdx.x & 63u;
@@ -559,7 +569,7 @@ struct Picker {
 
 // All of it where one wave has every token that may be taken: sorted by key for the cuts, then by index.
 __device__ __forceinline__ void pick_in_a_wave(const SampleArgs& a, uint32_t row, const Rule& r, const RowBins& bins, const Picker& pick, float u) {
-    const uint64_t key = sorted(pick.mine), w = key != 0 ? pick.weight(key) : 0;
+    const uint64_t key = sorted(pick.own[0]), w = key != 0 ? pick.weight(key) : 0;
     bool taken = key != 0 && threadIdx.x < r.top_k;
     if (r.top_p < 1.0) {
         const uint64_t upto = lanes_upto(taken ? w : 0), target = share_of_mass(r.top_p, read_lane(upto, 63));
@@ -599,18 +609,20 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
     const uint64_t upto = sum_before<kPickWaves>(listed, sh.slots[0], tokens);
     if (threadIdx.x < a.n_parts) sh.listed[threadIdx.x] = (uint32_t)upto, sh.part_mass[threadIdx.x] = sure;
     __syncthreads();
-    Picker pick{a, r, bins, sh, row, (uint32_t)tokens, 0};
-    if (tokens <= kPickThreads && threadIdx.x < tokens) pick.mine = pick.load(threadIdx.x);
+    Picker pick{a, r, bins, sh, row, (uint32_t)tokens, {}};
+#pragma unroll
+    for (uint32_t i = 0; i < kOwn; i++)
+        if (threadIdx.x + i * kPickThreads < tokens) pick.own[i] = pick.load(threadIdx.x + i * kPickThreads);
     if (bins.whole && tokens <= 64) {
         if (threadIdx.x < 64u) pick_in_a_wave(a, row, r, bins, pick, u);
         return;
     }
     const uint64_t threshold = tokens == 0 ? 0 : pick.threshold();
     // what every part keeps
-    for (uint32_t f = threadIdx.x; f < tokens; f += kPickThreads) {
-        const uint64_t key = pick.token(f), w = key >= threshold ? pick.weight(key) : 0;
+    pick.for_all([&](uint64_t key) {
+        const uint64_t w = key >= threshold ? pick.weight(key) : 0;
         if ((double)w >= floor && w != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.part_mass[index_of(key) / kPart]), (unsigned long long)w);
-    }
+    });
     __syncthreads();
     uint64_t mass;
     const uint64_t in_part = threadIdx.x < a.n_parts ? sh.part_mass[threadIdx.x] : 0, in_front = sum_before<kPickWaves>(in_part, sh.slots[2], mass);
@@ -620,24 +632,34 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
     __syncthreads();
     const uint32_t part = min((uint32_t)sh.found[0], a.n_parts - 1u);
     const uint64_t goal = sh.found[1];
-    uint64_t weight[kPart / kPickThreads], sum = 0;
+    float l[kEach];
+    const uint32_t first = part * kPart + threadIdx.x * kEach;
+    if (first + kEach <= a.n) {
 #pragma unroll
-    for (uint32_t k = 0; k < kPart / kPickThreads; k++) {
-        const uint32_t i = part * kPart + threadIdx.x * (kPart / kPickThreads) + k;
+        for (uint32_t k = 0; k < kEach; k += 4) {
+            const u32x4_a4 x = *reinterpret_cast<const u32x4_a4*>(logits + first + k);
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) l[k + e] = __uint_as_float(x.v[e]);
+        }
+    } else {
+#pragma unroll
+        for (uint32_t k = 0; k < kEach; k++) l[k] = first + k < a.n ? logits[first + k] : -__builtin_inff();
+    }
+    uint64_t weight[kEach], sum = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < kEach; k++) {
         weight[k] = 0;
-        if (i >= a.n) continue;
-        const float l = logits[i];
-        const double y4 = quarters<true>(l, r, bins.o);
-        if (bin_of<true>(y4, bins.o) >= kBins || key_of(l, i) < threshold) continue;
+        const double y4 = quarters<true>(l[k], r, bins.o);
+        if (bin_of<true>(y4, bins.o) >= kBins || key_of(l[k], first + k) < threshold) continue;
         const uint64_t w = weight_of(y4, bins.o);
         weight[k] = (double)w >= floor ? w : 0;
         sum += weight[k];
     }
     uint64_t all, before = sum_before<kPickWaves>(sum, sh.slots[3], all);
     if (before <= goal && goal < before + sum) {
-        uint32_t i = part * kPart + threadIdx.x * (kPart / kPickThreads);
+        uint32_t i = first;
 #pragma unroll
-        for (uint32_t k = 0; k < kPart / kPickThreads; k++) before += weight[k], i += before <= goal;
+        for (uint32_t k = 0; k < kEach; k++) before += weight[k], i += before <= goal;
         a.out[row] = i;
         if (a.prob) a.prob[row] = (float)(exact_weight(quarters<true>(logits[i], r, bins.o), bins.o) / (double)mass);
     }
