@@ -155,6 +155,7 @@ __device__ __forceinline__ uint64_t lanes_upto(uint64_t v) {
     v += moved_or_zero<0x142, 0xa>(v), v += moved_or_zero<0x143, 0xc>(v);
     return v;
 }
+__device__ __forceinline__ uint32_t lanes_upto(uint32_t v) { return (uint32_t)lanes_upto((uint64_t)v); }
 // Sum over the workgroup's threads in front of this one, and over all of them.  `slots`: one per wave, of this call alone until the next barrier.
 template <uint32_t WAVES>
 __device__ __forceinline__ uint64_t sum_before(uint64_t v, uint64_t* slots, uint64_t& total) {
@@ -248,7 +249,7 @@ __device__ __forceinline__ uint64_t share_of_mass(double share, uint64_t mass) {
     return t == 0 ? 1u : t < mass ? t : mass;
 }
 
-constexpr uint32_t kAtOnce = 8;
+constexpr uint32_t kAtOnce = 16;
 struct BinShared {
     uint64_t mass[64 * kLaneBins];
     uint32_t count[64 * kLaneBins];
@@ -329,8 +330,8 @@ __device__ __forceinline__ RowBins handed_on(const SampleRow& row, const Rule& r
 __global__ __launch_bounds__(kPartThreads) void sample_list_kernel(SampleArgs a) {
     __shared__ BinShared shared_bins;
     __shared__ uint64_t slots[kPartThreads / 64];
-    __shared__ float candidates[kPart];
-    __shared__ uint16_t places[kPart];
+    __shared__ float candidates[kPart / 2];
+    __shared__ uint16_t places[kPart / 2];
     __shared__ uint32_t listed, together;
     const uint32_t row = blockIdx.y, first = blockIdx.x * kPart;
     const float* const logits = a.logits + (size_t)row * a.stride;
@@ -371,18 +372,27 @@ __global__ __launch_bounds__(kPartThreads) void sample_list_kernel(SampleArgs a)
         const double lowest = fmin((bins.o.top4 - (double)last) / r.inverse4, kInfinite4);  // (a bin goes half a step further down than its whole number, which is at 4 E + 4 - bin)
         const float low = (float)(lowest - __builtin_fabs(lowest) * 0x1p-20 - 0x1p-140);
 #pragma unroll
-        for (uint32_t k = 0; k < kPartLoads; k++) {
-            const uint64_t here = __ballot(l[k] >= low);
-            if (here == 0) continue;
+        for (uint32_t half = 0; half < 2; half++) {
+            if (half != 0) {
+                __syncthreads();
+                if (threadIdx.x == 0) together = 0;
+                __syncthreads();
+            }
+            uint32_t count = 0;
+#pragma unroll
+            for (uint32_t k = half * kPartLoads / 2; k < (half + 1) * kPartLoads / 2; k++) count += l[k] >= low;
+            const uint32_t upto = lanes_upto(count);
             uint32_t at = 0;
-            if ((threadIdx.x & 63u) == 0) at = atomicAdd(&together, (uint32_t)__popcll(here));
-            at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + __builtin_amdgcn_mbcnt_hi((uint32_t)(here >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)here, 0u));
-            if (l[k] >= low) candidates[at] = l[k], places[at] = (uint16_t)(k * kPartThreads + threadIdx.x);
-        }
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < together; i += kPartThreads) {
-            if (bins.o.wild) take(std::true_type(), candidates[i], first + places[i]);
-            else take(std::false_type(), candidates[i], first + places[i]);
+            if ((threadIdx.x & 63u) == 63u) at = atomicAdd(&together, upto);
+            at = (uint32_t)__builtin_amdgcn_readlane((int)at, 63) + upto - count;
+#pragma unroll
+            for (uint32_t k = half * kPartLoads / 2; k < (half + 1) * kPartLoads / 2; k++)
+                if (l[k] >= low) candidates[at] = l[k], places[at] = (uint16_t)(k * kPartThreads + threadIdx.x), at++;
+            __syncthreads();
+            for (uint32_t i = threadIdx.x; i < together; i += kPartThreads) {
+                if (bins.o.wild) take(std::true_type(), candidates[i], first + places[i]);
+                else take(std::false_type(), candidates[i], first + places[i]);
+            }
         }
         __syncthreads();  // (listed)
     }
@@ -394,7 +404,7 @@ __global__ __launch_bounds__(kPartThreads) void sample_list_kernel(SampleArgs a)
 
 // 3.
 // (Sixteen waves: 64 rows' nuclei and 200 rows' mixed rules take 13.1 and 16.2 us; with four 15.9 and 25.1, with eight 12.9 and 17.7.)
-constexpr uint32_t kPickThreads = 1024, kPickWaves = kPickThreads / 64, kDigit = 11, kDigits = 1u << kDigit, kOwn = 1;
+constexpr uint32_t kPickThreads = 1024, kPickWaves = kPickThreads / 64, kDigit = 10, kDigits = 1u << kDigit, kOwn = 1;
 constexpr uint32_t kEach = kPart / kPickThreads, kDigitsEach = kDigits / kPickThreads;
 
 struct PickShared {
@@ -468,7 +478,7 @@ struct Picker {
     // Of the listed tokens of one bin whose keys are from `least` on, from the largest key down, as many as are `goal` tokens, or as their masses take to reach `goal`: the
     // smallest key of those, and their mass.
     __device__ __forceinline__ uint64_t select(uint32_t bin, uint64_t least, uint64_t goal, bool by_mass, uint64_t& mass) {
-        // A bin is 2048 steps of y wide first, of which the one where the goal is reached holds few tokens, as a rule; else their keys' digits, from the highest.
+        // A bin is 1024 steps of y wide first, of which the one where the goal is reached holds few tokens, as a rule; else their keys' digits, from the highest.
         uint64_t prefix = 0;  // of the keys that are left, from bit `known` up
         uint32_t step = 0;
         mass = 0;
@@ -489,7 +499,7 @@ struct Picker {
                 atomicAdd(&sh.count[d], 1u), atomicAdd(&sh.mass[d], (unsigned long long)weight_of(y4, bins.o));
             });
             __syncthreads();
-            // thread t has the digits from 2047 - 8 t down
+            // the digits from the highest
             uint64_t sum = 0, masses = 0;
 #pragma unroll
             for (uint32_t i = 0; i < kDigitsEach; i++) {
@@ -497,7 +507,7 @@ struct Picker {
                 masses += sh.mass[d], sum += by_mass ? sh.mass[d] : sh.count[d];
             }
             uint64_t all, all_mass;
-            uint64_t before = sum_before<kPickWaves>(sum, sh.slots[0], all), mass_before = sum_before<kPickWaves>(masses, sh.slots[1], all_mass);
+            uint64_t before = sum_before<kPickWaves>(sum, sh.slots[0], all), mass_before = by_mass ? before : sum_before<kPickWaves>(masses, sh.slots[1], all_mass);
             goal = goal < all ? goal : all;  // (what there is may be a little less than the bins' masses said)
             if (before < goal && goal <= before + sum) {
                 uint32_t d = kDigits - 1u - kDigitsEach * threadIdx.x;
