@@ -249,13 +249,15 @@ __device__ __forceinline__ uint64_t share_of_mass(double share, uint64_t mass) {
     return t == 0 ? 1u : t < mass ? t : mass;
 }
 
-constexpr uint32_t kAtOnce = 16;
+constexpr uint32_t kAtOnce = 8;
 struct BinShared {
     uint64_t mass[64 * kLaneBins];
     uint32_t count[64 * kLaneBins];
 };
 
-__device__ __forceinline__ RowBins row_bins(const SampleArgs& a, uint32_t row, const Rule& r, BinShared& sh) {
+// `meanwhile`: what else is to be asked of memory, behind the parts' histograms, whose registers it may have.
+template <typename F>
+__device__ __forceinline__ RowBins row_bins(const SampleArgs& a, uint32_t row, const Rule& r, BinShared& sh, F meanwhile) {
     const SamplePart* const parts = a.parts + (size_t)row * a.n_parts;
     const uint32_t lane = threadIdx.x & 63u;
     const float largest[2] = {lane < a.n_parts ? parts[lane].largest : -__builtin_inff(), lane + 64u < a.n_parts ? parts[lane + 64u].largest : -__builtin_inff()};
@@ -274,7 +276,10 @@ __device__ __forceinline__ RowBins row_bins(const SampleArgs& a, uint32_t row, c
     if (bins.o.none()) return bins;
     bins.floor = r.min_p * (double)weight_of(quarters<true>(most, r, bins.o), bins.o);
     const bool counts = r.counts(), masses = r.masses();
-    if (!counts && !masses) return bins;
+    if (!counts && !masses) {
+        meanwhile();
+        return bins;
+    }
     for (uint32_t b = threadIdx.x; b < 64u * kLaneBins; b += blockDim.x) {
         uint64_t mass = 0;
         uint32_t count = 0;
@@ -294,6 +299,7 @@ __device__ __forceinline__ RowBins row_bins(const SampleArgs& a, uint32_t row, c
         }
         sh.count[b] = count, sh.mass[b] = mass;
     }
+    meanwhile();
     __syncthreads();
     uint64_t sum = 0, tokens = 0;
 #pragma unroll
@@ -327,7 +333,7 @@ __device__ __forceinline__ RowBins handed_on(const SampleRow& row, const Rule& r
 }
 
 // 2.
-__global__ __launch_bounds__(kPartThreads) void sample_list_kernel(SampleArgs a) {
+__global__ __launch_bounds__(kPartThreads, 8) void sample_list_kernel(SampleArgs a) {
     __shared__ BinShared shared_bins;
     __shared__ uint64_t slots[kPartThreads / 64];
     __shared__ float candidates[kPart / 2];
@@ -335,15 +341,16 @@ __global__ __launch_bounds__(kPartThreads) void sample_list_kernel(SampleArgs a)
     __shared__ uint32_t listed, together;
     const uint32_t row = blockIdx.y, first = blockIdx.x * kPart;
     const float* const logits = a.logits + (size_t)row * a.stride;
-    float l[kPartLoads];
-#pragma unroll
-    for (uint32_t k = 0; k < kPartLoads; k++) {
-        const uint32_t i = first + k * kPartThreads + threadIdx.x;
-        l[k] = i < a.n ? logits[i] : -__builtin_inff();
-    }
     const Rule r = rule_of(a, row);
     if (threadIdx.x == 0) listed = 0, together = 0;
-    const RowBins bins = row_bins(a, row, r, shared_bins);
+    float l[kPartLoads];
+    const RowBins bins = row_bins(a, row, r, shared_bins, [&] {
+#pragma unroll
+        for (uint32_t k = 0; k < kPartLoads; k++) {
+            const uint32_t i = first + k * kPartThreads + threadIdx.x;
+            l[k] = i < a.n ? logits[i] : -__builtin_inff();
+        }
+    });
     if (blockIdx.x == 0 && threadIdx.x < 64u) hand_on(bins, a.rows[row]);
     if (bins.o.none()) return;
     __syncthreads();
