@@ -25,7 +25,7 @@ namespace wick_rocm {
 namespace {
 
 constexpr uint32_t kUnitRows = 128, kTileRows = 32, kWaves = 4;  // a unit is a tile of each wave
-constexpr uint32_t kShares = 512;                                // workgroups: two on each of 256 CUs
+constexpr uint32_t kShares = 512;                                 // workgroups: two on each of 256 CUs
 constexpr uint32_t kRecordHead = 4;                              // floats of a record in front of its values: maximum, sum, -, -
 constexpr float kHalfScale = 32768.0f;                           // softmax weights are split below or at a half's largest power of two
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -54,23 +54,35 @@ __device__ __forceinline__ uint32_t all_units(const PagedAttentionArgs& a, uint3
     return (uint32_t)__builtin_amdgcn_readlane((int)lanes_upto(sum), 63);
 }
 
-// The sequence that unit u is one of, and the units in front of it.
-__device__ __forceinline__ uint32_t find_unit(const PagedAttentionArgs& a, uint32_t heads, uint32_t u, uint32_t& before) {
-    before = 0;
-    for (uint32_t base = 0;; base += 64u) {
-        const uint32_t s = base + (threadIdx.x & 63u), n = s < a.n_seqs ? units_of(length(a, s)) * heads : 0u, upto = lanes_upto(n);
-        const uint64_t past = __ballot(before + upto > u);
-        if (past != 0 || base + 64u >= a.n_seqs) {
-            const int lane = past != 0 ? __ffsll((unsigned long long)past) - 1 : 63;
-            before += (uint32_t)__builtin_amdgcn_readlane((int)(upto - n), lane);
-            return base + (uint32_t)lane;
-        }
-        before += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
-    }
-}
-
+// The workgroup's share of the units, [begin, end), the sequence that it begins in and the units in front of that one; up to 64 sequences, a lane each, are read once.
+struct Share {
+    uint32_t units, begin, end, s, before;
+};
 __device__ __forceinline__ uint32_t share_begin(uint32_t units, uint32_t w, uint32_t shares) { return (uint32_t)((uint64_t)units * w / shares); }
 __device__ __forceinline__ uint32_t share_of(uint32_t units, uint32_t u, uint32_t shares) { return (uint32_t)((((uint64_t)u + 1) * shares - 1) / units); }
+__device__ __forceinline__ Share my_share(const PagedAttentionArgs& a, uint32_t heads) {
+    const uint32_t lane = threadIdx.x & 63u, first = lane < a.n_seqs ? units_of(length(a, lane)) * heads : 0u;
+    uint32_t sum = first;
+    for (uint32_t s = lane + 64u; s < a.n_seqs; s += 64u) sum += units_of(length(a, s)) * heads;
+    const uint32_t upto_first = lanes_upto(first);
+    Share x{};
+    x.units = (uint32_t)__builtin_amdgcn_readlane((int)(a.n_seqs <= 64u ? upto_first : lanes_upto(sum)), 63);
+    const uint32_t shares = min(x.units, kShares);  // (no share is empty)
+    if (blockIdx.x >= shares) return x;
+    x.begin = share_begin(x.units, blockIdx.x, shares), x.end = share_begin(x.units, blockIdx.x + 1u, shares);
+    uint32_t n = first, upto = upto_first;
+    for (uint32_t base = 0;;) {
+        const uint64_t past = __ballot(x.before + upto > x.begin);
+        if (past != 0 || base + 64u >= a.n_seqs) {
+            const int at = past != 0 ? __ffsll((unsigned long long)past) - 1 : 63;
+            x.before += (uint32_t)__builtin_amdgcn_readlane((int)(upto - n), at), x.s = base + (uint32_t)at;
+            return x;
+        }
+        x.before += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+        base += 64u;
+        n = base + lane < a.n_seqs ? units_of(length(a, base + lane)) * heads : 0u, upto = lanes_upto(n);
+    }
+}
 
 template <typename KV, int HD>
 struct Tile {
@@ -89,20 +101,22 @@ template <typename KV, int HD>
 struct Query;
 template <int HD>
 struct Query<_Float16, HD> {
+    v4f x[HD / 32][2];
     h8 hi[HD / 32], lo[HD / 32];
     float factor;
-    __device__ __forceinline__ void load(const float* q, bool there, float scale) {
+    __device__ __forceinline__ void load(const float* q, bool there) {
         const uint32_t g = (threadIdx.x & 63u) >> 4;
-        v4f x[HD / 32][2];
+#pragma unroll
+        for (int j = 0; j < HD / 32; j++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) x[j][i] = there ? *reinterpret_cast<const v4f*>(q + 32 * j + 8u * g + 4 * i) : v4f{0, 0, 0, 0};
+    }
+    __device__ __forceinline__ void split(float scale) {
         float top = 0.0f;
 #pragma unroll
         for (int j = 0; j < HD / 32; j++)
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                x[j][i] = there ? *reinterpret_cast<const v4f*>(q + 32 * j + 8u * g + 4 * i) : v4f{0, 0, 0, 0};
-#pragma unroll
-                for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(x[j][i][e]));
-            }
+            for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[j][i / 4][i % 4]));
         top = groups_max(top);
         const int e = max(__builtin_amdgcn_frexp_expf(top), -100) - 15;  // (from 2^-100 down no score matters)
         factor = ldexpf(scale * kLog2e, e);
@@ -128,12 +142,12 @@ template <int HD>
 struct Query<float, HD> {
     v4f x[HD / 16];
     float factor;
-    __device__ __forceinline__ void load(const float* q, bool there, float scale) {
+    __device__ __forceinline__ void load(const float* q, bool there) {
         const uint32_t g = (threadIdx.x & 63u) >> 4;
 #pragma unroll
         for (int j = 0; j < HD / 16; j++) x[j] = there ? *reinterpret_cast<const v4f*>(q + 16 * j + 4u * g) : v4f{0, 0, 0, 0};
-        factor = scale * kLog2e;
     }
+    __device__ __forceinline__ void split(float scale) { factor = scale * kLog2e; }
     __device__ __forceinline__ v4f scores(const typename Tile<float, HD>::kvec (&k)[HD / 16]) const {
         v4f s = {0, 0, 0, 0};
 #pragma unroll
@@ -199,33 +213,39 @@ struct State {
     }
 };
 
-// One tile's rows: those at or behind `len` read the last one's (their weights are zero).  `there`: bit h: half h has a page.
-template <typename KV, int HD>
-__device__ __forceinline__ uint32_t load_tile(const PagedAttentionArgs& a, const uint32_t* table, uint32_t c, uint32_t first, uint32_t len, Tile<KV, HD>& t) {
-    typedef Tile<KV, HD> T;
-    const uint32_t lane = threadIdx.x & 63u, l16 = lane & 15u, g = lane >> 4, inside = (1u << a.page_shift) - 1u;
-    uint32_t there = 0;
+// Where a tile's rows are: those at or behind `len` are the last one's (their weights are zero), those without a page the first page's.
+struct Place {
+    size_t base[2];  // rows in front of each half's page of this KV head
+    uint32_t first, there;  // bit h of `there`: half h has a page
+};
+__device__ __forceinline__ Place place(const PagedAttentionArgs& a, const uint32_t* table, uint32_t c, uint32_t first, uint32_t len) {
+    Place p{{0, 0}, first, 0};
 #pragma unroll
     for (int half = 0; half < 2; half++) {
-        const uint32_t row0 = first + 16u * half, page = table[min(row0, len - 1u) >> a.page_shift];
-        if (page < a.n_pages) there |= 1u << half;
-        const size_t base = ((size_t)(page < a.n_pages ? page : 0u) * a.n_kv_heads + c) << a.page_shift;
-        const KV* const k = static_cast<const KV*>(a.pages[0]) + (base + (min(row0 + l16, len - 1u) & inside)) * HD + (T::kF16 ? 8u : 4u) * g;
+        const uint32_t page = table[min(first + 16u * half, len - 1u) >> a.page_shift];
+        p.there |= (uint32_t)(page < a.n_pages) << half;
+        p.base[half] = ((size_t)(page < a.n_pages ? page : 0u) * a.n_kv_heads + c) << a.page_shift;
+    }
+    return p;
+}
+template <typename KV, int HD>
+__device__ __forceinline__ void load_tile(const PagedAttentionArgs& a, const Place& p, uint32_t len, Tile<KV, HD>& t) {
+    typedef Tile<KV, HD> T;
+    const uint32_t l16 = threadIdx.x & 15u, g = (threadIdx.x & 63u) >> 4, inside = (1u << a.page_shift) - 1u;
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+        const KV* const k = static_cast<const KV*>(a.pages[0]) + (p.base[half] + (min(p.first + 16u * half + l16, len - 1u) & inside)) * HD + (T::kF16 ? 8u : 4u) * g;
 #pragma unroll
         for (int j = 0; j < T::kSteps; j++) t.k[half][j] = *reinterpret_cast<const typename T::kvec*>(k + j * (T::kF16 ? 32 : 16));
     }
 #pragma unroll
-    for (int half = 0; half < 2; half++) {
-        const uint32_t row0 = first + 16u * half, page = table[min(row0, len - 1u) >> a.page_shift];
-        const size_t base = ((size_t)(page < a.n_pages ? page : 0u) * a.n_kv_heads + c) << a.page_shift;
+    for (int half = 0; half < 2; half++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const KV* const v = static_cast<const KV*>(a.pages[1]) + (base + (min(row0 + 4u * g + i, len - 1u) & inside)) * HD + T::kVec * l16;
+            const KV* const v = static_cast<const KV*>(a.pages[1]) + (p.base[half] + (min(p.first + 16u * half + 4u * g + i, len - 1u) & inside)) * HD + T::kVec * l16;
 #pragma unroll
             for (int x = 0; x < T::kLoads; x++) t.v[half][i][x] = *reinterpret_cast<const typename T::vvec*>(v + x * 16 * T::kVec);
         }
-    }
-    return there;
 }
 
 // A half without a page: its values are zeros, whatever was read.
@@ -240,39 +260,39 @@ __device__ __forceinline__ void clear_values(Tile<KV, HD>& t, uint32_t there) {
                 for (int x = 0; x < Tile<KV, HD>::kLoads; x++) t.v[half][i][x] = typename Tile<KV, HD>::vvec(0);
 }
 
-template <typename KV, int HD>
-__global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attention_paged_kernel(PagedAttentionArgs a) {
+// A workgroup's share of all units, or, where the table has room for few rows (SHORT), all rows of one sequence's KV head (and 16 of its query heads): no piece is left.
+template <typename KV, int HD, uint32_t WAVES, bool SHORT>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : HD == 256 ? 1 : 2) void attention_paged_kernel(PagedAttentionArgs a) {
     typedef Tile<KV, HD> T;
-    constexpr uint32_t kRow = HD + 4;  // floats of a head's values in LDS
-    __shared__ __align__(16) float values[kWaves][16][kRow];
-    __shared__ float tops[kWaves][16], sums[kWaves][16];
+    constexpr uint32_t kRow = HD + 4, kStep = WAVES * kTileRows;  // floats of a head's values in LDS; rows of all waves
+    static_assert(SHORT || kStep == kUnitRows);
+    __shared__ __align__(16) float values[WAVES][16][kRow];
+    __shared__ float tops[WAVES][16], sums[WAVES][16];
     const uint32_t lane = threadIdx.x & 63u, l16 = lane & 15u, g = lane >> 4;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const uint32_t heads = a.n_kv_heads * a.tiles;
-    uint32_t before;
-    const uint32_t units = all_units(a, heads, 0, before), shares = min(units, kShares);  // (no share is empty)
-    if (blockIdx.x >= shares) return;
-    const uint32_t begin = share_begin(units, blockIdx.x, shares), end = share_begin(units, blockIdx.x + 1u, shares);
-    uint32_t s = find_unit(a, heads, begin, before);
-    const uint32_t records = min(a.group, 16u);
-    for (uint32_t u = begin; u < end && s < a.n_seqs;) {
+    const uint32_t heads = a.n_kv_heads * a.tiles, records = min(a.group, 16u);
+    const Share sh = SHORT ? Share{0, 0, 1, blockIdx.x / heads, 0} : my_share(a, heads);
+    uint32_t s = sh.s, before = sh.before;
+    for (uint32_t u = sh.begin; u < sh.end && s < a.n_seqs;) {
         const uint32_t len = length(a, s), chunks = units_of(len);
-        if (u - before >= chunks * heads) {  // (the next sequence; one without rows has no units)
+        if (!SHORT && u - before >= chunks * heads) {  // (the next sequence; one without rows has no units)
             before += chunks * heads, s++;
             continue;
         }
-        const uint32_t head = (u - before) / chunks, chunk = (u - before) % chunks, take = min(chunks - chunk, end - u);
+        const uint32_t head = SHORT ? blockIdx.x % heads : (u - before) / chunks, chunk = SHORT ? 0u : (u - before) % chunks, take = SHORT ? 1u : min(chunks - chunk, sh.end - u);
         const uint32_t c = head / a.tiles, h0 = c * a.group + head % a.tiles * 16u, h_count = min(a.group - head % a.tiles * 16u, 16u);
         const uint32_t* const table = a.table + (size_t)s * a.max_pages;
         Query<KV, HD> q;
-        q.load(a.q + (size_t)s * a.q_stride + (size_t)(h0 + min(l16, h_count - 1u)) * HD, l16 < h_count, a.scale);
+        q.load(a.q + (size_t)s * a.q_stride + (size_t)(h0 + min(l16, h_count - 1u)) * HD, l16 < h_count);
+        q.split(a.scale);
         State<KV, HD> st;
 #pragma unroll
         for (int d = 0; d < T::kPer; d++) st.o[d] = v4f{0, 0, 0, 0};
-        const uint32_t last = min(len, (chunk + take) * kUnitRows);
-        for (uint32_t first = chunk * kUnitRows + wave * kTileRows; first < last; first += kUnitRows) {
+        const uint32_t last = SHORT ? len : min(len, (chunk + take) * kUnitRows);
+        for (uint32_t first = chunk * kUnitRows + wave * kTileRows; first < last; first += kStep) {
             T t;
-            const uint32_t there = load_tile(a, table, c, first, len, t);
+            const Place p = place(a, table, c, first, len);
+            load_tile(a, p, len, t);
             float sc[8];
 #pragma unroll
             for (int half = 0; half < 2; half++) {
@@ -280,35 +300,42 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attention_page
 #pragma unroll
                 for (int i = 0; i < 4; i++) sc[4 * half + i] = x[i] * q.factor;
             }
-            if (first + kTileRows > len || there != 3u) {
+            if (first + kTileRows > len || p.there != 3u) {
 #pragma unroll
                 for (int i = 0; i < 8; i++)
-                    if (first + 16u * (i / 4) + 4u * g + i % 4 >= len || (there >> (i / 4) & 1u) == 0) sc[i] = -__builtin_inff();
-                clear_values(t, there);
+                    if (first + 16u * (i / 4) + 4u * g + i % 4 >= len || (p.there >> (i / 4) & 1u) == 0) sc[i] = -__builtin_inff();
+                clear_values(t, p.there);
             }
             st.add(t, sc);
         }
         // The waves' states, one head after another
         st.l = groups_sum(st.l);
         if (g == 0) tops[wave][l16] = st.m, sums[wave][l16] = st.l;
+        constexpr int kWide = T::kVec < 4 ? T::kVec : 4;
+        typedef float wide __attribute__((ext_vector_type(kWide)));
 #pragma unroll
         for (int x = 0; x < T::kLoads; x++)
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
-                for (int e = 0; e < T::kVec; e++) values[wave][l16][x * 16 * T::kVec + T::kVec * (4u * g + r) + e] = st.o[x * T::kVec + e][r];
+                for (int e = 0; e < T::kVec; e += kWide) {
+                    wide w;
+#pragma unroll
+                    for (int k = 0; k < kWide; k++) w[k] = st.o[x * T::kVec + e + k][r];
+                    *reinterpret_cast<wide*>(&values[wave][l16][x * 16 * T::kVec + T::kVec * (4u * g + r) + e]) = w;
+                }
         __syncthreads();
-        const bool whole = take == chunks;
-        for (uint32_t i = threadIdx.x; i < h_count * (HD / 4); i += 64u * kWaves) {
+        const bool whole = SHORT || take == chunks;
+        for (uint32_t i = threadIdx.x; i < h_count * (HD / 4); i += 64u * WAVES) {
             const uint32_t h = i / (HD / 4), d = i % (HD / 4) * 4u;
             float top = tops[0][h];
 #pragma unroll
-            for (uint32_t w = 1; w < kWaves; w++) top = fmaxf(top, tops[w][h]);
+            for (uint32_t w = 1; w < WAVES; w++) top = fmaxf(top, tops[w][h]);
             const float from = top == -__builtin_inff() ? 0.0f : top;
             float sum = 0.0f;
             v4f v = {0, 0, 0, 0};
 #pragma unroll
-            for (uint32_t w = 0; w < kWaves; w++) {
+            for (uint32_t w = 0; w < WAVES; w++) {
                 const float less = __builtin_amdgcn_exp2f(tops[w][h] - from);
                 sum += sums[w][h] * less;
                 v += *reinterpret_cast<const v4f*>(&values[w][h][d]) * less;
@@ -317,11 +344,12 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attention_page
                 const float inverse = sum == 0.0f ? 0.0f : 1.0f / (T::kF16 ? sum * kHalfScale : sum);
                 *reinterpret_cast<v4f*>(a.out + (size_t)s * a.out_stride + (size_t)(h0 + h) * HD + d) = v * inverse;
             } else {
-                float* const to = a.parts + ((size_t)(blockIdx.x * 2u + (u == begin ? 0u : 1u)) * records + h) * (kRecordHead + HD);
+                float* const to = a.parts + ((size_t)(blockIdx.x * 2u + (u == sh.begin ? 0u : 1u)) * records + h) * (kRecordHead + HD);
                 if (d == 0) to[0] = top, to[1] = T::kF16 ? sum * kHalfScale : sum;
                 *reinterpret_cast<v4f*>(to + kRecordHead + d) = v;
             }
         }
+        if (SHORT) return;
         __syncthreads();
         u += take;
     }
@@ -349,27 +377,42 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(PagedAttentio
         const uint32_t slot = i == 0 && share_begin(units, w0, shares) != u0 ? 1u : 0u;
         return a.parts + ((size_t)((w0 + i) * 2u + slot) * records + in_group % 16u) * (kRecordHead + HD);
     };
-    float top = -__builtin_inff();
-    for (uint32_t i = threadIdx.x; i < n; i += 256u) top = fmaxf(top, record(i)[0]);
-    top = wave_max_f32(top);
+    // A thread's records' heads, and its part of the first records' values, are read in one go.
+    constexpr uint32_t kQuads = HD / 4, kGroups = 256 / kQuads, kAhead = 4;
+    static_assert(kShares <= 512);
+    const uint32_t d = threadIdx.x % kQuads, part = threadIdx.x / kQuads;
+    float tops_of[2] = {-__builtin_inff(), -__builtin_inff()}, sums_of[2] = {0.0f, 0.0f};
+    v4f ahead[kAhead];
+#pragma unroll
+    for (uint32_t x = 0; x < 2; x++)
+        if (threadIdx.x + 256u * x < n) {
+            const float* const r = record(threadIdx.x + 256u * x);
+            tops_of[x] = r[0], sums_of[x] = r[1];
+        }
+#pragma unroll
+    for (uint32_t x = 0; x < kAhead; x++)
+        if (part + x * kGroups < n) ahead[x] = *reinterpret_cast<const v4f*>(record(part + x * kGroups) + kRecordHead + 4u * d);
+    float top = wave_max_f32(fmaxf(tops_of[0], tops_of[1]));
     if (lane == 0) tops[wave] = top;
     __syncthreads();
     top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
     const float from = top == -__builtin_inff() ? 0.0f : top;
     float sum = 0.0f;
-    for (uint32_t i = threadIdx.x; i < n; i += 256u) {
-        const float* const r = record(i);
-        const float w = __builtin_amdgcn_exp2f(r[0] - from);
-        weights[i] = w, sum += w * r[1];
-    }
+#pragma unroll
+    for (uint32_t x = 0; x < 2; x++)
+        if (threadIdx.x + 256u * x < n) {
+            const float w = __builtin_amdgcn_exp2f(tops_of[x] - from);
+            weights[threadIdx.x + 256u * x] = w, sum += w * sums_of[x];
+        }
     sum = wave_sum_f32(sum);
     if (lane == 0) totals[wave] = sum;
     __syncthreads();
     sum = (totals[0] + totals[1]) + (totals[2] + totals[3]);
-    constexpr uint32_t kQuads = HD / 4, kGroups = 256 / kQuads;
-    const uint32_t d = threadIdx.x % kQuads, part = threadIdx.x / kQuads;
     v4f v = {0, 0, 0, 0};
-    for (uint32_t i = part; i < n; i += kGroups) v += *reinterpret_cast<const v4f*>(record(i) + kRecordHead + 4u * d) * weights[i];
+#pragma unroll
+    for (uint32_t x = 0; x < kAhead; x++)
+        if (part + x * kGroups < n) v += ahead[x] * weights[part + x * kGroups];
+    for (uint32_t i = part + kAhead * kGroups; i < n; i += kGroups) v += *reinterpret_cast<const v4f*>(record(i) + kRecordHead + 4u * d) * weights[i];
     reinterpret_cast<v4f*>(values[part])[d] = v;
     __syncthreads();
     if (threadIdx.x < kQuads) {
@@ -378,9 +421,16 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(PagedAttentio
     }
 }
 
+// Waves of a workgroup for short tables, as many as the registers allow, and the rows up to which a table is one: two tiles a wave.
+template <typename KV, int HD>
+constexpr uint32_t kShortWaves = HD * sizeof(KV) <= 128 ? 16 : HD * sizeof(KV) <= 256 ? 8 : 4;
+
 template <typename KV, int HD>
 hipError_t launch_paged(const PagedAttentionArgs& a, const Launch& L) {
-    hipError_t e = launch_kernel(L, kFamOther, attention_paged_kernel<KV, HD>, dim3(kShares), dim3(64 * kWaves), a);
+    constexpr uint32_t W = kShortWaves<KV, HD>;
+    if (((uint64_t)a.max_pages << a.page_shift) <= 2u * W * kTileRows)
+        return launch_kernel(L, kFamOther, attention_paged_kernel<KV, HD, W, true>, dim3(a.n_seqs * a.n_kv_heads * a.tiles), dim3(64 * W), a);
+    hipError_t e = launch_kernel(L, kFamOther, attention_paged_kernel<KV, HD, kWaves, false>, dim3(kShares), dim3(64 * kWaves), a);
     if (e != hipSuccess) return e;
     return launch_kernel(L, kFamOther, attention_paged_join_kernel<HD>, dim3(a.n_seqs * a.n_heads), dim3(256), a);
 }
