@@ -14,7 +14,13 @@
 //
 // The work of all sequences is one list of units of kUnitRows rows of one KV head (and 16 of its query heads), sequence by sequence, head by head; every
 // workgroup takes an equal, contiguous share, whatever the lengths.  What covers a head's rows completely is written out; a share's
-// first and last piece otherwise leave {maximum, sum, values} in the scratch, which a second launch joins.
+// first and last piece otherwise leave {maximum, sum, values} in the scratch, which a second launch joins.  (Joined by the last workgroup of a head to arrive
+// instead, over device-scope atomics, 128,000 rows took 104 us, not 98.7: what the others wrote has to be read past the caches.)
+//
+// Reading the pages bounds it: every cached element is read once.  32 sequences of up to 8192 rows (8 KV heads of 64, f16: 278 MB) take 53.9 us, 5.2 TB/s,
+// and 4.8 us to join; 64 of up to 2002 rows in f32 (271 MB) 53 us, 5.1 TB/s; one of 128,000 rows (8 KV heads of 128, f16: 524 MB) 91 us, 5.8 TB/s, and 7.4 us
+// to join.  Loads of the next tile ahead of a tile's products (f32: 53 to 56 us) and waves that yield to those with more left (no difference) do not pay:
+// with 8 waves a CU the loads of one fill the products of another.
 #include <algorithm>
 
 #include "kv_paged_device.h"
@@ -25,7 +31,7 @@ namespace wick_rocm {
 namespace {
 
 constexpr uint32_t kUnitRows = 128, kTileRows = 32, kWaves = 4;  // a unit is a tile of each wave
-constexpr uint32_t kShares = 512;                                 // workgroups: two on each of 256 CUs
+constexpr uint32_t kShares = 512;                                 // workgroups, two on each of 256 CUs (one where the registers of a row of 256 leave room for one)
 constexpr uint32_t kRecordHead = 4;                              // floats of a record in front of its values: maximum, sum, -, -
 constexpr float kHalfScale = 32768.0f;                           // softmax weights are split below or at a half's largest power of two
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -36,7 +42,7 @@ struct PagedAttentionArgs {
     const uint32_t *table, *lens;
     float* out;
     float* parts;  // [shares][2][records of a piece][kRecordHead + head_dim]
-    uint32_t n_seqs, max_pages, n_pages, page_shift, q_stride, out_stride, n_heads, n_kv_heads, group, tiles;  // tiles: of 16 query heads, of a KV head
+    uint32_t n_seqs, max_pages, n_pages, page_shift, q_stride, out_stride, n_heads, n_kv_heads, group, tiles, shares;  // tiles: of 16 query heads, of a KV head
     float scale;
 };
 
@@ -54,25 +60,27 @@ __device__ __forceinline__ uint32_t all_units(const PagedAttentionArgs& a, uint3
     return (uint32_t)__builtin_amdgcn_readlane((int)lanes_upto(sum), 63);
 }
 
-// The workgroup's share of the units, [begin, end), the sequence that it begins in and the units in front of that one; up to 64 sequences, a lane each, are read once.
+// Share `w` of the units, [begin, end), the sequence of its first unit (or its last one) and the units in front of that sequence; up to 64 sequences, a
+// lane each, are read once.
 struct Share {
     uint32_t units, begin, end, s, before;
 };
 __device__ __forceinline__ uint32_t share_begin(uint32_t units, uint32_t w, uint32_t shares) { return (uint32_t)((uint64_t)units * w / shares); }
 __device__ __forceinline__ uint32_t share_of(uint32_t units, uint32_t u, uint32_t shares) { return (uint32_t)((((uint64_t)u + 1) * shares - 1) / units); }
-__device__ __forceinline__ Share my_share(const PagedAttentionArgs& a, uint32_t heads) {
+__device__ __forceinline__ Share share(const PagedAttentionArgs& a, uint32_t heads, uint32_t w, bool its_last) {
     const uint32_t lane = threadIdx.x & 63u, first = lane < a.n_seqs ? units_of(length(a, lane)) * heads : 0u;
     uint32_t sum = first;
     for (uint32_t s = lane + 64u; s < a.n_seqs; s += 64u) sum += units_of(length(a, s)) * heads;
     const uint32_t upto_first = lanes_upto(first);
     Share x{};
     x.units = (uint32_t)__builtin_amdgcn_readlane((int)(a.n_seqs <= 64u ? upto_first : lanes_upto(sum)), 63);
-    const uint32_t shares = min(x.units, kShares);  // (no share is empty)
-    if (blockIdx.x >= shares) return x;
-    x.begin = share_begin(x.units, blockIdx.x, shares), x.end = share_begin(x.units, blockIdx.x + 1u, shares);
+    const uint32_t shares = min(x.units, a.shares);  // (no share is empty)
+    if (w >= shares) return x;
+    x.begin = share_begin(x.units, w, shares), x.end = share_begin(x.units, w + 1u, shares);
+    const uint32_t unit = its_last ? x.end - 1u : x.begin;
     uint32_t n = first, upto = upto_first;
     for (uint32_t base = 0;;) {
-        const uint64_t past = __ballot(x.before + upto > x.begin);
+        const uint64_t past = __ballot(x.before + upto > unit);
         if (past != 0 || base + 64u >= a.n_seqs) {
             const int at = past != 0 ? __ffsll((unsigned long long)past) - 1 : 63;
             x.before += (uint32_t)__builtin_amdgcn_readlane((int)(upto - n), at), x.s = base + (uint32_t)at;
@@ -189,14 +197,17 @@ struct State {
                 hi[i] = (_Float16)y, lo[i] = (_Float16)(y - (float)hi[i]);
             }
 #pragma unroll
-            for (int x = 0; x < T::kLoads; x++)
+            for (int x = 0; x < T::kLoads; x++) {
+                // (whole vectors first: elements picked from the array itself keep it out of registers)
+                const typename T::vvec r0 = t.v[0][0][x], r1 = t.v[0][1][x], r2 = t.v[0][2][x], r3 = t.v[0][3][x], r4 = t.v[1][0][x], r5 = t.v[1][1][x], r6 = t.v[1][2][x], r7 = t.v[1][3][x];
 #pragma unroll
                 for (int e = 0; e < T::kVec; e++) {
-                    const h8 v = {t.v[0][0][x][e], t.v[0][1][x][e], t.v[0][2][x][e], t.v[0][3][x][e], t.v[1][0][x][e], t.v[1][1][x][e], t.v[1][2][x][e], t.v[1][3][x][e]};
+                    const h8 v = {r0[e], r1[e], r2[e], r3[e], r4[e], r5[e], r6[e], r7[e]};
                     v4f& d = o[x * T::kVec + e];
                     d = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo, d, 0, 0, 0);
                     d = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi, d, 0, 0, 0);
                 }
+            }
         } else {
 #pragma unroll
             for (int half = 0; half < 2; half++)
@@ -271,7 +282,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : HD == 256 ? 1 : 2) vo
     const uint32_t lane = threadIdx.x & 63u, l16 = lane & 15u, g = lane >> 4;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t heads = a.n_kv_heads * a.tiles, records = min(a.group, 16u);
-    const Share sh = SHORT ? Share{0, 0, 1, blockIdx.x / heads, 0} : my_share(a, heads);
+    const Share sh = SHORT ? Share{0, 0, 1, blockIdx.x / heads, 0} : share(a, heads, blockIdx.x, false);
     uint32_t s = sh.s, before = sh.before;
     for (uint32_t u = sh.begin; u < sh.end && s < a.n_seqs;) {
         const uint32_t len = length(a, s), chunks = units_of(len);
@@ -353,29 +364,41 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : HD == 256 ? 1 : 2) vo
         __syncthreads();
         u += take;
     }
+    for (uint32_t e = blockIdx.x; e < a.n_seqs; e += gridDim.x)  // sequences without rows
+        if (a.lens[e] == 0)
+            for (uint32_t i = threadIdx.x; i < a.n_heads * (HD / 4); i += 64u * WAVES) reinterpret_cast<v4f*>(a.out + (size_t)e * a.out_stride)[i] = v4f{0, 0, 0, 0};
 }
 
-// One workgroup a sequence and query head: nothing to do where one share has the whole head, zeros where there is no row.
-template <int HD>
+// Joins the pieces of a KV head (and 16 of its query heads) for one of the query heads, blockIdx.y.  Where there are more such heads than shares, the first
+// of which a share leaves for the next one is the head that its last unit is in: one workgroup a share (BY_SHARE), otherwise one a head.  With 400
+// sequences of 32 heads and up to 1024 rows, one workgroup a head took 20.9 us, one a share 11.3 us.
+template <int HD, bool BY_SHARE>
 __global__ __launch_bounds__(256) void attention_paged_join_kernel(PagedAttentionArgs a) {
     __shared__ float weights[kShares];
     __shared__ __align__(16) float values[256 / (HD / 4)][HD];
     __shared__ float tops[4], totals[4];
-    const uint32_t s = blockIdx.x / a.n_heads, h = blockIdx.x % a.n_heads, heads = a.n_kv_heads * a.tiles, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    float* const out = a.out + (size_t)s * a.out_stride + (size_t)h * HD;
-    uint32_t before;
-    const uint32_t units = all_units(a, heads, s, before), chunks = units_of(length(a, s)), shares = min(units, kShares);
-    if (chunks == 0) {
-        if (threadIdx.x < HD / 4) reinterpret_cast<v4f*>(out)[threadIdx.x] = v4f{0, 0, 0, 0};
-        return;
+    const uint32_t heads = a.n_kv_heads * a.tiles, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    uint32_t s, head, units, u0, chunks, w0;
+    if constexpr (BY_SHARE) {
+        const Share sh = share(a, heads, blockIdx.x, true);
+        if (sh.begin == sh.end) return;
+        s = sh.s, units = sh.units, w0 = blockIdx.x, chunks = units_of(length(a, s));
+        head = (sh.end - 1u - sh.before) / chunks, u0 = sh.before + head * chunks;
+        if (u0 < sh.begin || u0 + chunks == sh.end) return;  // begun by an earlier share, or whole
+    } else {
+        uint32_t before;
+        s = blockIdx.x / heads, head = blockIdx.x % heads, units = all_units(a, heads, s, before), chunks = units_of(length(a, s)), u0 = before + head * chunks;
+        if (chunks == 0) return;
+        w0 = share_of(units, u0, min(units, a.shares));
     }
-    const uint32_t c = h / a.group, in_group = h % a.group, u0 = before + (c * a.tiles + in_group / 16u) * chunks;
-    const uint32_t w0 = share_of(units, u0, shares), w1 = share_of(units, u0 + chunks - 1u, shares), n = w1 - w0 + 1u;
-    if (n == 1) return;
+    const uint32_t shares = min(units, a.shares), n = share_of(units, u0 + chunks - 1u, shares) - w0 + 1u;
+    const uint32_t in_tile = blockIdx.y, h = head / a.tiles * a.group + head % a.tiles * 16u + in_tile;
+    if (n == 1 || head % a.tiles * 16u + in_tile >= a.group) return;
+    float* const out = a.out + (size_t)s * a.out_stride + (size_t)h * HD;
     const uint32_t records = min(a.group, 16u);
     const auto record = [&](uint32_t i) {
         const uint32_t slot = i == 0 && share_begin(units, w0, shares) != u0 ? 1u : 0u;
-        return a.parts + ((size_t)((w0 + i) * 2u + slot) * records + in_group % 16u) * (kRecordHead + HD);
+        return a.parts + ((size_t)((w0 + i) * 2u + slot) * records + in_tile) * (kRecordHead + HD);
     };
     // A thread's records' heads, and its part of the first records' values, are read in one go.
     constexpr uint32_t kQuads = HD / 4, kGroups = 256 / kQuads, kAhead = 4;
@@ -421,7 +444,9 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(PagedAttentio
     }
 }
 
-// Waves of a workgroup for short tables, as many as the registers allow, and the rows up to which a table is one: two tiles a wave.
+// Waves of a workgroup for short tables, as many as the registers allow.  A table is short where its rows are at most two tiles a wave: one launch without a join.
+// For 32 heads of 64 in f16, 1 sequence of 512 rows takes 6.2 us, in shares 4.7 and 4.2 for the join; 32 of 1024 rows 12.8, in shares 13.6 and 4.2; 400 of up to
+// 1024 rows 98, in shares 107 and 11.
 template <typename KV, int HD>
 constexpr uint32_t kShortWaves = HD * sizeof(KV) <= 128 ? 16 : HD * sizeof(KV) <= 256 ? 8 : 4;
 
@@ -430,9 +455,11 @@ hipError_t launch_paged(const PagedAttentionArgs& a, const Launch& L) {
     constexpr uint32_t W = kShortWaves<KV, HD>;
     if (((uint64_t)a.max_pages << a.page_shift) <= 2u * W * kTileRows)
         return launch_kernel(L, kFamOther, attention_paged_kernel<KV, HD, W, true>, dim3(a.n_seqs * a.n_kv_heads * a.tiles), dim3(64 * W), a);
-    hipError_t e = launch_kernel(L, kFamOther, attention_paged_kernel<KV, HD, kWaves, false>, dim3(kShares), dim3(64 * kWaves), a);
+    hipError_t e = launch_kernel(L, kFamOther, attention_paged_kernel<KV, HD, kWaves, false>, dim3(a.shares), dim3(64 * kWaves), a);
     if (e != hipSuccess) return e;
-    return launch_kernel(L, kFamOther, attention_paged_join_kernel<HD>, dim3(a.n_seqs * a.n_heads), dim3(256), a);
+    const uint32_t heads = a.n_seqs * a.n_kv_heads * a.tiles, records = std::min(a.group, 16u);
+    return heads > a.shares ? launch_kernel(L, kFamOther, attention_paged_join_kernel<HD, true>, dim3(a.shares, records), dim3(256), a)
+                           : launch_kernel(L, kFamOther, attention_paged_join_kernel<HD, false>, dim3(heads, records), dim3(256), a);
 }
 
 template <typename KV>
@@ -456,8 +483,11 @@ hipError_t launch_attention_paged(const wick_rocm_kv_pages& p, const float* d_q,
                                   float* d_out, uint32_t out_stride, float* d_scratch, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, float scale,
                                   const Launch& L) {
     const uint32_t group = n_heads / n_kv_heads;
+    // Two workgroups of rows of 256 do not fit on a CU, and twice the shares only leave more to join: f16, 128,000 rows 185 and 7.8 us (512 shares: 190 and
+    // 12.8), 128 sequences of up to 1024 rows 127 and 5.7 (144 and 8).  With rows of 128 it would be 53 us against 62.
+    const uint32_t shares = head_dim == 256 ? kShares / 2 : kShares;
     const PagedAttentionArgs a{d_q, {d_k_pages, d_v_pages}, p.d_table, p.d_lens, d_out, d_scratch, p.n_seqs, p.max_pages, p.n_pages, (uint32_t)__builtin_ctz(p.page_rows),
-                               q_stride, out_stride, n_heads, n_kv_heads, group, (group + 15u) / 16u, scale};
+                               q_stride, out_stride, n_heads, n_kv_heads, group, (group + 15u) / 16u, shares, scale};
     return kv_f16 ? launch_paged<_Float16>(a, head_dim, L) : launch_paged<float>(a, head_dim, L);
 }
 
