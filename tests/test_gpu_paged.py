@@ -187,6 +187,34 @@ def test_attention_of_many_sequences(ctx, ops, dev, dtype):
     assert_f32_parity(attend(ctx, ops, dev, OnDevice(dev, pool), q), pool.attention(q))
 
 
+@pytest.mark.parametrize("dtype", [KV_F32, KV_F16])
+@pytest.mark.parametrize("hd,heads,n_kv,page_rows,lens", ATTENTION, ids=[f"{c[0]}-{c[1]}-{c[2]}-{c[3]}-{len(c[4])}x{max(c[4])}" for c in ATTENTION])
+def test_attention_under_a_wide_table(ctx, ops, dev, hd, heads, n_kv, page_rows, lens, dtype):
+    """Room for many more rows than there are: what is taken in one launch above is split over shares and joined."""
+    pool = filled(len(lens) + hd, lens, page_rows, n_kv, hd, dtype)
+    pool.max_pages += 2048 // page_rows
+    q = normal(11, len(lens), heads, hd) * 1.5
+    got = attend(ctx, ops, dev, OnDevice(dev, pool), q, extra=4)
+    want = pool.attention(q)
+    for s, n in enumerate(lens):
+        assert_f32_parity(got[s], want[s], f"sequence {s}") if n else np.testing.assert_array_equal(got[s], 0)
+
+
+@pytest.mark.parametrize("dtype", [KV_F32, KV_F16])
+@pytest.mark.parametrize("seqs,hd,heads,n_kv", [(600, 32, 1, 1), (130, 64, 8, 4), (40, 64, 40, 8), (300, 128, 17, 1), (70, 256, 4, 4)])
+def test_more_heads_than_shares(ctx, ops, dev, dtype, seqs, hd, heads, n_kv):
+    """Sequences of all lengths and of none, also at both ends; heads that end where a share does and heads over several shares."""
+    lens = [int(n) for n in np.random.default_rng(seqs).integers(0, 400, seqs)]
+    for s in (0, 7, 8, 70, seqs - 1):
+        lens[s % seqs] = 0
+    lens[1], lens[seqs // 2] = 128, 3000
+    pool = filled(34, lens, 64, n_kv, hd, dtype)
+    q = normal(35, seqs, heads, hd)
+    got, want = attend(ctx, ops, dev, OnDevice(dev, pool), q, extra=8), pool.attention(q)
+    for s, n in enumerate(lens):
+        assert_f32_parity(got[s], want[s], f"sequence {s}") if n else np.testing.assert_array_equal(got[s], 0)
+
+
 def test_attention_over_shared_pages(ctx, ops, dev):
     pool = filled(14, [900, 901, 400, 33], 32, 2, 64, KV_F16, share={1: 0, 2: 0, 3: 1})
     q = normal(15, 4, 8, 64)
