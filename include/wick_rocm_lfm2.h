@@ -188,11 +188,20 @@ int wick_rocm_kv_paged_append(wick_rocm_ctx *ctx, const wick_rocm_kv_pages *page
                               void *d_v_pages, int kv_dtype, const uint32_t *d_start, const uint32_t *d_first, uint32_t n, uint32_t n_kv_heads,
                               uint32_t head_dim);
 
+/* wick_rocm_qk_norm_rope for such tokens: token j's query heads (d_q + j * q_stride) and key heads normed and rotated in place, at the row that it goes to as its
+ * position, then keys and values appended as above; tokens that are dropped stay as they were, rows that no page is there for are not stored.  Bit-identical to
+ * wick_rocm_qk_norm_rope token by token.  Pages 16-byte aligned, the rest 4. */
+int wick_rocm_qk_norm_rope_paged(wick_rocm_ctx *ctx, const wick_rocm_kv_pages *pages, float *d_q, uint32_t q_stride, float *d_k, const float *d_v,
+                                 uint32_t kv_stride, const float *d_q_norm, const float *d_k_norm, void *d_k_pages, void *d_v_pages, int kv_dtype,
+                                 const uint32_t *d_start, const uint32_t *d_first, uint32_t n, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                                 float eps, float theta_scale);
+
 /* wick_rocm_attention_decode for one new token of every sequence, over its rows [0, d_lens[s]) (no rows: zeros).  Sequence s's query heads at
  * d_q + s * q_stride floats, its output at d_out + s * out_stride; f32 in and out, sums and softmax f32's, cached values as they are held.  (f16 pages: a query
  * element is off by at most 2^-22 of itself or 2^-39 of its head's largest, a softmax weight by the same of itself or of the largest.)  Rows whose entry names no page
- * of the pool count as not there.  A row that is not finite gives NaN to the sequences that see it, in the heads that read it, and to no other.
- * The work of all sequences together is split evenly over the GPU, whatever their lengths; a second launch joins what several workgroups share.
+ * of the pool count as not there.  A row that is not finite may make outputs that are not finite of the sequences that see it, in the heads that read it, and of no other.
+ * The work of all sequences together is split evenly over the GPU, whatever their lengths, and a second launch joins what several workgroups share; a table of few
+ * rows (at most 256 to 1024, by head_dim) takes one launch.
  * d_scratch: wick_rocm_attention_paged_scratch_floats(...) floats (0: not such a shape), contents need not be kept; calls that may run at the same time need one
  * each.  q, pages, output and scratch 16-byte aligned, strides multiples of 4 that cover the heads. */
 size_t wick_rocm_attention_paged_scratch_floats(uint32_t n_seqs, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim);

@@ -153,6 +153,57 @@ def test_appended_rows_without_a_page_are_dropped(ops, dev):
     assert np.array_equal(back(d.planes, pool.planes), pool.planes, equal_nan=True)
 
 
+# ---- tokens normed, rotated and appended ------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [KV_F32, KV_F16])
+@pytest.mark.parametrize("heads,n_kv,hd,page_rows,pad,one_each", [
+    (16, 8, 64, 16, 0, False), (4, 2, 64, 64, 3, True), (40, 8, 64, 32, 0, True), (3, 3, 128, 32, 5, False), (6, 2, 256, 16, 0, True), (17, 1, 32, 256, 1, False)])
+def test_tokens_of_several_sequences_normed_and_rotated(ctx, ops, dev, dtype, heads, n_kv, hd, page_rows, pad, one_each):
+    """One launch for tokens at rows of their own as wick_rocm_qk_norm_rope and wick_rocm_kv_paged_append token by token, bit for bit; few tokens and many."""
+    eps, ts, kv_dim = 1e-5, lfm2.rope_theta_scale(hd, 1_000_000.0), n_kv * hd
+    counts = [1] * 9 if one_each else [3, 0, 300, 1, 40]
+    lens = [500, 3, 0, 15, 16, 17, 31, 700, 1][:len(counts)]
+    n, S = sum(counts), len(counts)
+    pool = filled(50, [a + b for a, b in zip(lens, counts)], page_rows, n_kv, hd, dtype)
+    d, d2 = OnDevice(dev, pool), OnDevice(dev, pool)
+    start = u32(*lens)
+    start[1] = NONE  # sequence 1's are dropped
+    table = pool.table
+    table[4, lens[4] // page_rows] = NONE  # there is no page for the first of sequence 4's
+    for x in (d, d2):
+        x.table.upload(table)
+    width = heads * hd + 2 * kv_dim + pad  # one [q | k | v] row a token
+    rows = normal(51, n + 2, width)  # two more tokens than there are: of no sequence
+    first = u32(0, *np.cumsum(counts))
+    d_rows, d_rows2, qn, kn, none = dev(rows), dev(rows), dev(1 + 0.2 * normal(52, hd)), dev(1 + 0.2 * normal(53, hd)), dev(np.zeros(kv_dim, np.float32))
+
+    def parts(r, j=0):
+        p = r.ptr + 4 * j * width
+        return p, p + 4 * heads * hd, p + 4 * (heads * hd + kv_dim)
+
+    q, k, v = parts(d_rows)
+    ops.encode_qk_norm_rope_paged(d.pages, q, width, k, v, width, qn, kn, d.plane(0), d.plane(1), dtype, dev(start), n if one_each else n + 2, heads, n_kv, hd, eps, ts,
+                                  first=None if one_each else dev(first))
+    got = back(d_rows, rows)
+    for s in range(S):
+        for i in range(counts[s] if start[s] != NONE else 0):
+            j = int(first[s]) + i
+            # (a position at or behind its cache's rows is not stored)
+            q, k, v = parts(d_rows2, j)
+            ops.encode_qk_norm_rope(q, k, v, qn, kn, none, none, 0, 0, hd, heads, n_kv, eps, ts, d_pos=dev(u32(lens[s] + i)))
+            one = u32(*[NONE] * S)
+            one[s] = lens[s] + i
+            kv = back(d_rows2, rows)[j, heads * hd:heads * hd + 2 * kv_dim]
+            ops.encode_kv_paged_append(d2.pages, dev(kv[:kv_dim]), dev(kv[kv_dim:]), kv_dim, d2.plane(0), d2.plane(1), dtype, dev(one), 1, n_kv, hd,
+                                       first=dev(u32(*[0] * (s + 1), *[1] * (S - s))))
+    want = back(d_rows2, rows)
+    assert np.array_equal(got.view(np.uint32), want.view(np.uint32)) and not np.array_equal(got, rows)
+    assert np.array_equal(got[n:], rows[n:]) and np.array_equal(got[first[1]:first[2]], rows[first[1]:first[2]])
+    bits = {4: np.uint32, 2: np.uint16}[pool.planes.itemsize]
+    a, b = back(d.planes, pool.planes).view(bits), back(d2.planes, pool.planes).view(bits)
+    assert np.array_equal(a, b) and not np.array_equal(a, pool.planes.view(bits))
+
+
 # ---- attention -----------------------------------------------------------------------------------
 
 ATTENTION = [  # head_dim, heads, KV heads, page_rows, lengths
@@ -555,6 +606,40 @@ def test_continuations_of_a_prompt(ctx, ops, dev, dtype):
     check(141)
     used = len({p for row in back(d.table, pool.table).tolist() for p in row if p != NONE})
     assert (back(d.refs, pool.refs) > 0).sum() == used
+
+
+def test_steps_of_sessions_as_each_by_itself(ctx, ops, dev):
+    """The attention block of several steps of five sessions at once -- rows reserved, tokens normed, rotated and appended, attention -- against
+    wick_rocm_attention_block of each over a cache of its own; one session sits out a step, one ends."""
+    heads, n_kv, hd, max_seq, eps = 16, 4, 64, 256, 1e-5
+    S, kv_dim, width, ts = 5, n_kv * hd, heads * hd + 2 * n_kv * hd, lfm2.rope_theta_scale(hd, 1_000_000.0)
+    pool = R.Pool(S, 8, 30, 16, n_kv, hd, KV_F32)
+    d = OnDevice(dev, pool)
+    start, moves = dev(np.zeros(S, np.uint32)), dev(np.zeros(kv_pages_moves_words(d.pages), np.uint32))
+    scratch, sc = dev(np.zeros(attention_paged_scratch_floats(S, heads, n_kv, hd), np.float32)), dev(np.zeros(lfm2.attention_block_scratch_bytes(max_seq, heads, hd), np.uint8))
+    qn, kn = dev(1 + 0.2 * normal(60, hd)), dev(1 + 0.2 * normal(61, hd))
+    caches, rows_of = [[dev(np.zeros(max_seq * kv_dim, np.float32)) for _ in range(2)] for _ in range(S)], [0] * S
+    out, one = dev(np.zeros((S, heads * hd), np.float32)), dev(np.zeros(heads * hd, np.float32))
+    for step in range(40):
+        counts = [int(not (s == step % 7 and step % 2)) for s in range(S)]
+        if step == 25:
+            ops.kv_pages_free(d.pages, dev(u32(NONE, NONE, 0, NONE, NONE)))
+            ops.kv_pages_compact(d.pages, moves, d.all)
+            rows_of[2] = 0
+        x = normal(100 + step, S, width)
+        ops.kv_pages_reserve(d.pages, dev(u32(*counts)), start, moves, d.all)
+        d_x = dev(x)
+        q, k, v = d_x.ptr, d_x.ptr + 4 * heads * hd, d_x.ptr + 4 * (heads * hd + kv_dim)
+        ops.encode_qk_norm_rope_paged(d.pages, q, width, k, v, width, qn, kn, d.plane(0), d.plane(1), KV_F32, start, S, heads, n_kv, hd, eps, ts)
+        ops.encode_attention_paged(d.pages, q, width, d.plane(0), d.plane(1), KV_F32, out, heads * hd, scratch, heads, n_kv, hd)
+        got = out.download(np.float32, S * heads * hd).reshape(S, -1)
+        for s in range(S):
+            if not counts[s]:
+                continue
+            o = [dev(np.ascontiguousarray(p)) for p in np.split(x[s], [heads * hd, heads * hd + kv_dim])]
+            ops.encode_attention_block(o[0], o[1], o[2], qn, kn, caches[s][0], caches[s][1], one, sc, rows_of[s], max_seq, hd, heads, n_kv, eps, ts)
+            rows_of[s] += 1
+            assert_f32_parity(got[s], one.download(np.float32, heads * hd), f"step {step}, session {s}")
 
 
 def test_a_captured_step_replayed(ctx, ops, dev):

@@ -471,8 +471,8 @@ hipError_t launch_paged(const PagedAttentionArgs& a, uint32_t head_dim, const La
 
 bool attention_paged_fits(const wick_rocm_kv_pages& p, uint32_t n_heads, uint32_t n_kv_heads) {
     const uint64_t tiles = (n_heads / n_kv_heads + 15u) / 16u, chunks = ((uint64_t)p.max_pages * p.page_rows + kUnitRows - 1u) / kUnitRows;
-    // (each factor is at most 2^30)
-    return p.n_seqs * chunks <= UINT32_MAX / 2u / (n_kv_heads * tiles) && (uint64_t)p.n_seqs * n_heads <= INT32_MAX;
+    // (each factor is at most 2^30; a launch has less than 2^32 threads, of which 1024 may go to a sequence's KV head)
+    return p.n_seqs * chunks <= UINT32_MAX / 2u / (n_kv_heads * tiles) && (uint64_t)p.n_seqs * n_kv_heads * tiles <= 1u << 21;
 }
 
 size_t attention_paged_scratch_floats(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim) {

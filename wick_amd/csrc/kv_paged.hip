@@ -14,8 +14,8 @@ namespace {
 struct PagedAppendArgs {
     const float* src[2];  // keys, values
     void* pages[2];
-    const uint32_t *table, *start, *first;
-    uint32_t n_seqs, max_pages, n_pages, page_shift, n, n_kv_heads, head_dim, stride;
+    PagedRows rows;
+    uint32_t n, n_kv_heads, head_dim, stride;
 };
 
 template <typename KV>
@@ -24,22 +24,10 @@ __global__ __launch_bounds__(256) void kv_paged_append_kernel(PagedAppendArgs a)
     const uint64_t at = (uint64_t)blockIdx.x * 256u + threadIdx.x;
     if (at >= (uint64_t)a.n * quads) return;
     const uint32_t j = (uint32_t)(at / quads), quad = (uint32_t)(at % quads), c = 4u * quad / a.head_dim, i = 4u * quad % a.head_dim;
-    uint32_t s = j, in = 0;
-    if (a.first) {  // the last sequence whose tokens begin at or before this one
-        uint32_t low = 0, high = a.n_seqs;
-        while (high - low > 1) {
-            const uint32_t mid = (low + high) / 2u;
-            (a.first[mid] <= j ? low : high) = mid;
-        }
-        s = low, in = j - a.first[s];
-        if (j < a.first[s] || j >= a.first[s + 1]) return;
-    }
-    const uint32_t start = a.start[s];
-    const uint64_t row = (uint64_t)start + in;
-    if (start == WICK_ROCM_NO_ROW || row >> a.page_shift >= a.max_pages) return;
-    const uint32_t page = a.table[(size_t)s * a.max_pages + (row >> a.page_shift)];
-    if (page >= a.n_pages) return;
-    const size_t to = ((((size_t)page * a.n_kv_heads + c) << a.page_shift) + (row & ((1u << a.page_shift) - 1u))) * a.head_dim + i;
+    uint32_t page;
+    const uint32_t row = paged_row(a.rows, j, page);
+    if (row == WICK_ROCM_NO_ROW || page >= a.rows.n_pages) return;
+    const size_t to = paged_at(a.rows, page, row, a.n_kv_heads, c, a.head_dim) + i;
 #pragma unroll
     for (int which = 0; which < 2; which++) {
         const float4 x = *reinterpret_cast<const float4*>(a.src[which] + (size_t)j * a.stride + 4u * quad);
@@ -355,7 +343,7 @@ hipError_t launch_kv_paged_append(const wick_rocm_kv_pages& p, const float* d_k,
                                   bool kv_f16, const uint32_t* d_start, const uint32_t* d_first, uint32_t n, uint32_t n_kv_heads, uint32_t head_dim,
                                   const Launch& L) {
     if (n == 0) return hipSuccess;
-    const PagedAppendArgs a{{d_k, d_v}, {d_k_pages, d_v_pages}, p.d_table, d_start, d_first, p.n_seqs, p.max_pages, p.n_pages, page_shift(p), n, n_kv_heads,
+    const PagedAppendArgs a{{d_k, d_v}, {d_k_pages, d_v_pages}, {p.d_table, d_start, d_first, p.n_seqs, p.max_pages, p.n_pages, page_shift(p)}, n, n_kv_heads,
                             head_dim, kv_stride};
     const uint64_t threads = (uint64_t)n * (n_kv_heads * head_dim / 4u);
     const dim3 grid((uint32_t)((threads + 255u) / 256u));

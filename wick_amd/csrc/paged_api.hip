@@ -43,6 +43,20 @@ int check_planes(wick_rocm_ctx* ctx, const wick_rocm_kv_pages& p, const wick_roc
     return WICK_ROCM_OK;
 }
 
+// What both calls that put tokens into pages ask of them.
+int check_tokens(wick_rocm_ctx* ctx, const wick_rocm_kv_pages& p, const float* d_k, const float* d_v, uint32_t kv_stride, const void* d_k_pages,
+                 const void* d_v_pages, int kv_dtype, const uint32_t* d_start, const uint32_t* d_first, uint32_t n, uint32_t n_kv_heads, uint32_t head_dim) {
+    if (const char* wrong = heads_shape(n_kv_heads, head_dim, kv_dtype)) return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, wrong);
+    if (!d_k || !d_v || !d_k_pages || !d_v_pages || !d_start) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages: null keys, values, pages or start");
+    if (kv_stride < (uint64_t)n_kv_heads * head_dim) return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, "kv_pages: kv_stride must cover n_kv_heads * head_dim");
+    if (misaligned(d_k_pages, 16) || misaligned(d_v_pages, 16)) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages: pages must be 16-byte aligned");
+    if (misaligned(d_start, 4) || misaligned(d_first, 4)) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages: start and first must be 4-byte aligned");
+    if (d_k_pages == d_v_pages) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages: keys and values are one plane");
+    if (!d_first && n != p.n_seqs) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages: without d_first there is one token a sequence");
+    if (n > 1u << 23 || (uint64_t)n * n_kv_heads * head_dim > (uint64_t)1 << 33) return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, "kv_pages: too many tokens at once");
+    return WICK_ROCM_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -52,19 +66,30 @@ int wick_rocm_kv_paged_append(wick_rocm_ctx* ctx, const wick_rocm_kv_pages* page
                               uint32_t head_dim) {
     WR_ENTER(ctx);
     if (int rc = check_pool(ctx, pages)) return rc;
-    if (const char* wrong = heads_shape(n_kv_heads, head_dim, kv_dtype)) return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, wrong);
-    if (!d_k || !d_v || !d_k_pages || !d_v_pages || !d_start) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_paged_append: null device pointer");
-    if (kv_stride < (uint64_t)n_kv_heads * head_dim || kv_stride % 4u != 0)
-        return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, "kv_paged_append: kv_stride must cover n_kv_heads * head_dim and be a multiple of 4");
-    if (misaligned(d_k, 16) || misaligned(d_v, 16) || misaligned(d_k_pages, 16) || misaligned(d_v_pages, 16))
-        return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_paged_append: keys, values and pages must be 16-byte aligned");
-    if (misaligned(d_start, 4) || misaligned(d_first, 4)) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_paged_append: start and first must be 4-byte aligned");
-    if (d_k_pages == d_v_pages) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_paged_append: keys and values are one plane");
-    if (!d_first && n != pages->n_seqs) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_paged_append: without d_first there is one token a sequence");
-    if ((uint64_t)n * n_kv_heads * head_dim > (uint64_t)1 << 40) return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, "kv_paged_append: too many values");
+    if (int rc = check_tokens(ctx, *pages, d_k, d_v, kv_stride, d_k_pages, d_v_pages, kv_dtype, d_start, d_first, n, n_kv_heads, head_dim)) return rc;
+    if (kv_stride % 4u != 0 || misaligned(d_k, 16) || misaligned(d_v, 16))
+        return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_paged_append: keys and values must be 16-byte aligned, kv_stride a multiple of 4");
     hipError_t e = launch_kv_paged_append(*pages, d_k, d_v, kv_stride, d_k_pages, d_v_pages, kv_dtype == WICK_ROCM_KV_F16, d_start, d_first, n, n_kv_heads,
                                           head_dim, ctx->launch());
     return e == hipSuccess ? WICK_ROCM_OK : fail_hip(ctx, e, "kv_paged_append launch");
+}
+
+int wick_rocm_qk_norm_rope_paged(wick_rocm_ctx* ctx, const wick_rocm_kv_pages* pages, float* d_q, uint32_t q_stride, float* d_k, const float* d_v,
+                                 uint32_t kv_stride, const float* d_q_norm, const float* d_k_norm, void* d_k_pages, void* d_v_pages, int kv_dtype,
+                                 const uint32_t* d_start, const uint32_t* d_first, uint32_t n, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, float eps,
+                                 float theta_scale) {
+    WR_ENTER(ctx);
+    if (int rc = check_pool(ctx, pages)) return rc;
+    if (int rc = check_tokens(ctx, *pages, d_k, d_v, kv_stride, d_k_pages, d_v_pages, kv_dtype, d_start, d_first, n, n_kv_heads, head_dim)) return rc;
+    if (n_heads == 0 || n_heads > 65535u || n_heads % n_kv_heads != 0)
+        return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, "qk_norm_rope_paged: n_heads must be 1 .. 65535, and n_kv_heads divide it");
+    if (q_stride < (uint64_t)n_heads * head_dim) return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, "qk_norm_rope_paged: q_stride must cover a token's heads");
+    if (!d_q || !d_q_norm || !d_k_norm || misaligned(d_q, 4) || misaligned(d_k, 4) || misaligned(d_v, 4) || misaligned(d_q_norm, 4) || misaligned(d_k_norm, 4))
+        return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "qk_norm_rope_paged: queries, keys, values and norms must be there and 4-byte aligned");
+    if (d_q == d_k) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "qk_norm_rope_paged: queries and keys are one array");
+    hipError_t e = launch_qk_norm_rope_paged(*pages, d_q, q_stride, d_k, d_v, kv_stride, d_q_norm, d_k_norm, d_k_pages, d_v_pages, kv_dtype == WICK_ROCM_KV_F16,
+                                             d_start, d_first, n, n_heads, n_kv_heads, head_dim, eps, theta_scale, ctx->launch());
+    return e == hipSuccess ? WICK_ROCM_OK : fail_hip(ctx, e, "qk_norm_rope_paged launch");
 }
 
 size_t wick_rocm_attention_paged_scratch_floats(uint32_t n_seqs, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim) {
@@ -95,6 +120,7 @@ int wick_rocm_kv_pages_fork(wick_rocm_ctx* ctx, const wick_rocm_kv_pages* pages,
     WR_ENTER(ctx);
     if (int rc = check_pool(ctx, pages)) return rc;
     if (!d_parents || misaligned(d_parents, 4)) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages_fork: the parents must be there and 4-byte aligned");
+    if (d_parents == pages->d_lens || d_parents == pages->d_table) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages_fork: the parents must be an array of their own");
     hipError_t e = launch_kv_pages_fork(*pages, d_parents, ctx->launch());
     return e == hipSuccess ? WICK_ROCM_OK : fail_hip(ctx, e, "kv_pages_fork launch");
 }

@@ -292,6 +292,10 @@ hipError_t launch_kv_q4_evict(void* d_k_cache, void* d_v_cache, float* d_weights
 hipError_t launch_kv_paged_append(const wick_rocm_kv_pages& p, const float* d_k, const float* d_v, uint32_t kv_stride, void* d_k_pages, void* d_v_pages,
                                   bool kv_f16, const uint32_t* d_start, const uint32_t* d_first, uint32_t n, uint32_t n_kv_heads, uint32_t head_dim,
                                   const Launch& L);
+hipError_t launch_qk_norm_rope_paged(const wick_rocm_kv_pages& p, float* d_q, uint32_t q_stride, float* d_k, const float* d_v, uint32_t kv_stride,
+                                     const float* d_q_norm, const float* d_k_norm, void* d_k_pages, void* d_v_pages, bool kv_f16, const uint32_t* d_start,
+                                     const uint32_t* d_first, uint32_t n, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, float eps, float theta_scale,
+                                     const Launch& L);
 bool attention_paged_fits(const wick_rocm_kv_pages& p, uint32_t n_heads, uint32_t n_kv_heads);  // its units and heads are within 32 bits
 size_t attention_paged_scratch_floats(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim);
 hipError_t launch_attention_paged(const wick_rocm_kv_pages& p, const float* d_q, uint32_t q_stride, const void* d_k_pages, const void* d_v_pages, bool kv_f16,

@@ -61,6 +61,7 @@ _SIGNATURES = {
     "wick_rocm_attention_prefill_q4": (C.c_int, [_P, _P, _U32, _P, _P, _P, _U32, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32]),
     "wick_rocm_kv_q4_evict_scratch_floats": (C.c_size_t, [_U32, _U32]),
     "wick_rocm_kv_q4_evict": (C.c_int, [_P, _P, _P, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32, _U32]),
+    "wick_rocm_qk_norm_rope_paged": (C.c_int, [_P, _P, _P, _U32, _P, _P, _U32, _P, _P, _P, _P, C.c_int, _P, _P, _U32, _U32, _U32, _U32, _F, _F]),
     "wick_rocm_kv_paged_append": (C.c_int, [_P, _P, _P, _P, _U32, _P, _P, C.c_int, _P, _P, _U32, _U32, _U32]),
     "wick_rocm_attention_paged_scratch_floats": (C.c_size_t, [_U32, _U32, _U32, _U32]),
     "wick_rocm_attention_decode_paged": (C.c_int, [_P, _P, _P, _U32, _P, _P, C.c_int, _P, _U32, _P, _U32, _U32, _U32]),
@@ -268,6 +269,13 @@ class Lfm2Ops:
         """n tokens' normed and rotated keys and their values into the pages of their sequences: rows start[s] .. of tokens first[s] .. (None: one each)."""
         self.ctx._check(self._l.wick_rocm_kv_paged_append(self.ctx._h, pages.handle, _ptr(k), _ptr(v), kv_stride, _ptr(k_pages), _ptr(v_pages), kv_dtype,
                                                           _ptr(start), _ptr(first), n, n_kv_heads, head_dim))
+
+    def encode_qk_norm_rope_paged(self, pages: KvPages, q, q_stride: int, k, v, kv_stride: int, q_norm, k_norm, k_pages, v_pages, kv_dtype: int, start, n: int,
+                                  n_heads: int, n_kv_heads: int, head_dim: int, eps: float, theta_scale: float, first=None) -> None:
+        """encode_qk_norm_rope for n tokens of several sequences, each at the row that it goes to, appended to their pages as by encode_kv_paged_append."""
+        self.ctx._check(self._l.wick_rocm_qk_norm_rope_paged(self.ctx._h, pages.handle, _ptr(q), q_stride, _ptr(k), _ptr(v), kv_stride, _ptr(q_norm), _ptr(k_norm),
+                                                             _ptr(k_pages), _ptr(v_pages), kv_dtype, _ptr(start), _ptr(first), n, n_heads, n_kv_heads, head_dim,
+                                                             eps, theta_scale))
 
     def encode_attention_paged(self, pages: KvPages, q, q_stride: int, k_pages, v_pages, kv_dtype: int, out, out_stride: int, scratch, n_heads: int,
                                n_kv_heads: int, head_dim: int) -> None:
