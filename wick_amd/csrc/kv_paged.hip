@@ -10,7 +10,8 @@ namespace wick_rocm {
 namespace {
 
 // ---- append --------------------------------------------------------------------------------------
-// One thread a 16-byte load of each source; bound by memory, and by the launch where there are few tokens.
+// One thread a 16-byte load of each source; bound by memory (2002 tokens of 8 heads of 64 in f32, 16 MB: 4.8 us, 3.4 TB/s), and by the launch where there are few
+// tokens (64: 3.8 us).
 struct PagedAppendArgs {
     const float* src[2];  // keys, values
     void* pages[2];
@@ -43,7 +44,8 @@ __global__ __launch_bounds__(256) void kv_paged_append_kernel(PagedAppendArgs a)
 
 // ---- fork, free ----------------------------------------------------------------------------------
 // A table's columns are independent of each other: a workgroup takes a few of them for all sequences, so that it has read every
-// parent's entries before it writes any, and one launch does it in place.  One workgroup more does the same with lens.
+// parent's entries before it writes any, and one launch does it in place.  One workgroup more does the same with lens.  Bound by its round trips: 3.9 us for 17
+// sequences of 32 pages, 4.9 for 8 of 1000.
 constexpr uint32_t kForkEntries = 8192;  // of a workgroup (LDS); a power of two, at least the most sequences
 struct PagedForkArgs {
     uint32_t *table, *lens, *refs;
@@ -92,7 +94,8 @@ __global__ __launch_bounds__(256) void kv_pages_free_kernel(PagedFreeArgs a) {
 
 // ---- the plan of a reservation or a compaction: one workgroup --------------------------------------
 // A chain of round trips to memory (lengths, the table's entry, its page's count; what is written) and of barriers; refs are read a run of pages a thread, of
-// the first 16384 pages once, at the start.
+// the first 16384 pages once, at the start.  A row for each of 16 continuations (a shared page copied) takes 9.0 us, 2002 rows for one of 32 sequences 6.5, a compaction
+// of 8000 pages 4.9.
 constexpr uint32_t kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
 constexpr uint32_t kRun = 16;                    // consecutive pages of a thread at a time
 constexpr uint32_t kListed = 4096;               // pages of a list that are in LDS; those behind them in memory
@@ -270,7 +273,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_compact_kernel(PagedPla
 
 // ---- pages moved -----------------------------------------------------------------------------------
 // A workgroup takes 1024 consecutive 16-byte pieces of a page in one plane, of one move after the other; for a compaction, the table's entries behind them.
-// Bound by memory.
+// Bound by memory: 393 MB read and written in 81 us, 4.8 TB/s, the rate of a large copy; 50 MB in 11 us.
 struct PagedCopyArgs {
     char* base;
     size_t plane_bytes;
