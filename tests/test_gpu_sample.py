@@ -91,6 +91,17 @@ def test_flat_rows_list_more_than_a_workgroup(run):
     check(run(logits, params, u), logits, params, u)
 
 
+def test_long_lists(run):
+    """Many times what a workgroup holds at once is listed: alike, two values, nearly alike, alike but for a few, and alike from somewhere on."""
+    n, rng = 150001, np.random.default_rng(6)
+    logits = np.stack([np.full(n, 2.5), np.where(np.arange(n) % 3 == 0, 1.0, 0.9), rng.standard_normal(n) * 1e-6, np.where(rng.random(n) > 1 - 1e-4, 1.0, 0.0),
+                       np.where(np.arange(n) > 100000, 0.0, -1e-3 * rng.random(n))]).astype(np.float32)
+    params = [(1.0, 100000, 1.0, 0.0), (1.0, 0, 0.37, 0.0), (1.0, 40, 0.95, 0.05), (0.7, 140000, 0.8, 0.9)]
+    logits, params = np.tile(logits, (len(params), 1)), [p for p in params for _ in range(5)]
+    u = rng.random(len(params)).astype(np.float32)
+    check(run(logits, params, u), logits, params, u)
+
+
 def test_ruled_out_tokens(run):
     """-infinity and NaN are never taken; a row of nothing else has no token; one alone is taken for certain; the lowest float is a token like others."""
     n = 5000

@@ -9,6 +9,10 @@
 //   3. one workgroup a row: the cuts exactly, from the listed tokens; the mass of every part; the part in which the pick is, token by token.
 // Where top-k leaves few, tokens are only counted in 1., and all that may be taken are listed: no weights but theirs.  What is listed is at most some hundred
 // tokens as a rule, which 3. sorts, and a row's all in the worst case (all logits alike), for which there is room.
+//
+// Three dependent launches bound a single row (65536 tokens, top-k 40: 4.3, 7.8 and 4.8 us, each a chain of round trips); f64 arithmetic, of which every weight takes some
+// twenty instructions, many (64 rows of 65536 under top-p: 9.4, 12.5 and 12.6 us; reading them alone would take 3.5).  65536 tokens that are all alike take 0.37 ms,
+// 0.39 in 64 rows: passes over a long list.
 #include <algorithm>
 #include <type_traits>
 
@@ -51,7 +55,7 @@ struct SampleArgs {
     float* prob;
     SampleRow* rows;
     SamplePart* parts;  // [rows][n_parts]
-    uint32_t* lists;    // [rows][n]: part p's tokens from p kPart on
+    uint64_t* lists;    // [rows][n] keys: part p's tokens from p kPart on
     uint32_t n, stride, n_parts;
 };
 
@@ -355,7 +359,7 @@ __global__ __launch_bounds__(kPartThreads, 8) void sample_list_kernel(SampleArgs
     if (bins.o.none()) return;
     __syncthreads();
     uint64_t sure = 0;
-    uint32_t* const list = a.lists + (size_t)row * a.n + first;
+    uint64_t* const list = a.lists + (size_t)row * a.n + first;
     const uint32_t sure_bins = bins.sure();
     Power power;
     power.keep();
@@ -366,7 +370,7 @@ __global__ __launch_bounds__(kPartThreads, 8) void sample_list_kernel(SampleArgs
             const uint64_t w = power.whole(y4, bins.o);
             sure += (double)w >= bins.floor ? w : 0;
         } else if (b < kBins && bins.lists(b)) {
-            list[atomicAdd(&listed, 1u)] = i;
+            list[atomicAdd(&listed, 1u)] = key_of(x, i);
         }
     };
     // The last bin that matters; as a rule it is far above most tokens.  Those that may be in it or above (by their logit, with room for rounding) are put together
@@ -411,7 +415,7 @@ __global__ __launch_bounds__(kPartThreads, 8) void sample_list_kernel(SampleArgs
 
 // 3.
 // (Sixteen waves: 64 rows' nuclei and 200 rows' mixed rules take 13.1 and 16.2 us; with four 15.9 and 25.1, with eight 12.9 and 17.7.)
-constexpr uint32_t kPickThreads = 1024, kPickWaves = kPickThreads / 64, kDigit = 10, kDigits = 1u << kDigit, kOwn = 1;
+constexpr uint32_t kPickThreads = 1024, kPickWaves = kPickThreads / 64, kDigit = 10, kDigits = 1u << kDigit, kOwn = 1, kLoadsAtOnce = 8;
 constexpr uint32_t kEach = kPart / kPickThreads, kDigitsEach = kDigits / kPickThreads;
 
 struct PickShared {
@@ -468,16 +472,37 @@ struct Picker {
             const uint32_t mid = (low + high) / 2u;
             (sh.listed[mid] <= f ? low : high) = mid;
         }
-        const uint32_t i = a.lists[(size_t)row * a.n + (size_t)low * kPart + (f - sh.listed[low])];
-        return key_of(a.logits[(size_t)row * a.stride + i], i);
+        return a.lists[(size_t)row * a.n + (size_t)low * kPart + (f - sh.listed[low])];
     }
-    // All listed tokens, each by a thread of its own.
+    // All listed tokens, each by a thread of its own; f's second argument: behind the first ones.
     template <typename F>
     __device__ __forceinline__ void for_all(F f) const {
 #pragma unroll
         for (uint32_t i = 0; i < kOwn; i++)
-            if (threadIdx.x + i * kPickThreads < tokens) f(own[i]);
-        for (uint32_t t = threadIdx.x + kOwn * kPickThreads; t < tokens; t += kPickThreads) f(load(t));
+            if (threadIdx.x + i * kPickThreads < tokens) f(own[i], std::false_type());
+        for (uint32_t t = threadIdx.x + kOwn * kPickThreads; t < tokens; t += kLoadsAtOnce * kPickThreads) {
+            uint64_t key[kLoadsAtOnce];
+#pragma unroll
+            for (uint32_t i = 0; i < kLoadsAtOnce; i++) key[i] = t + i * kPickThreads < tokens ? load(t + i * kPickThreads) : 0;
+#pragma unroll
+            for (uint32_t i = 0; i < kLoadsAtOnce; i++)
+                if (key[i] != 0) f(key[i], std::true_type());
+        }
+    }
+    // *sum += v of every lane that is here.  Where there are many tokens, lanes with the same v at the same place (tokens that are alike) are one addition.
+    template <typename MANY>
+    static __device__ __forceinline__ void add_to(unsigned long long* sum, uint64_t v, MANY) {
+        if constexpr (!MANY::value) {
+            atomicAdd(sum, (unsigned long long)v);
+            return;
+        }
+        const uint64_t here = __ballot(true), first = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+        const uint32_t place = (uint32_t)(uintptr_t)sum;
+        if (__ballot(v == first && place == (uint32_t)__builtin_amdgcn_readfirstlane((int)place)) == here) {
+            if ((threadIdx.x & 63u) == (uint32_t)__ffsll((unsigned long long)here) - 1u) atomicAdd(sum, (unsigned long long)(first * (uint32_t)__popcll(here)));
+        } else {
+            atomicAdd(sum, (unsigned long long)v);
+        }
     }
     __device__ __forceinline__ double quarters_of(uint64_t key) const { return quarters<true>(logit_of(key), r, bins.o); }
     __device__ __forceinline__ uint64_t weight(uint64_t key) const { return weight_of(quarters_of(key), bins.o); }
@@ -489,7 +514,8 @@ struct Picker {
         uint64_t prefix = 0;  // of the keys that are left, from bit `known` up
         uint32_t step = 0;
         mass = 0;
-        for (int known = 64, shift = 64;; known = shift, shift = shift == 64 ? 64 - (int)kDigit : shift > (int)kDigit ? shift - (int)kDigit : 0) {
+        const auto next = [](int known) { return known > (int)kDigit ? known - (int)kDigit : 0; };
+        for (int known = 64, shift = 64;;) {
             const auto is_left = [&](uint64_t key, double& y4, double& place) {
                 y4 = quarters_of(key), place = y4 - __builtin_rint(y4);  // within half a step, more of a larger one
                 return key >= least && bin_of<true>(y4, bins.o) == bin && (shift == 64 || (step_of(place) == step && (known == 64 || key >> known == prefix >> known)));
@@ -499,11 +525,11 @@ struct Picker {
             if (threadIdx.x == 0) sh.together = 0;
             for (uint32_t d = threadIdx.x; d < kDigits; d += kPickThreads) sh.count[d] = 0, sh.mass[d] = 0;
             __syncthreads();
-            for_all([&](uint64_t key) {
+            for_all([&](uint64_t key, auto many) {
                 double y4, place;
                 if (!is_left(key, y4, place)) return;
                 const uint32_t d = shift == 64 ? step_of(place) : (uint32_t)(key >> shift) & (kDigits - 1u);
-                atomicAdd(&sh.count[d], 1u), atomicAdd(&sh.mass[d], (unsigned long long)weight_of(y4, bins.o));
+                atomicAdd(&sh.count[d], 1u), add_to(&sh.mass[d], weight_of(y4, bins.o), many);
             });
             __syncthreads();
             // the digits from the highest
@@ -526,9 +552,28 @@ struct Picker {
             goal = sh.found[1], mass += sh.found[2];
             if (shift == 64) step = digit;
             else prefix = (prefix & ~((uint64_t)(kDigits - 1u) << shift)) | (uint64_t)digit << shift;
-            if (sh.count[digit] > 64u) continue;  // (a key's last digit leaves one)
+            if (sh.count[digit] > 64u) {  // (a key's last digit leaves one)
+                if (shift != 64) {
+                    known = shift, shift = next(known);
+                    continue;
+                }
+                // the digits begin where those that are left differ: only in their indexes, if many are alike
+                __syncthreads();
+                if (threadIdx.x == 0) sh.found[0] = 0, sh.found[1] = ~0ull;
+                __syncthreads();
+                uint64_t any = 0, every = ~0ull;
+                for_all([&](uint64_t key, auto) {
+                    const double y4 = quarters_of(key);
+                    if (key >= least && bin_of<true>(y4, bins.o) == bin && step_of(y4 - __builtin_rint(y4)) == step) any |= key, every &= key;
+                });
+                atomicOr(reinterpret_cast<unsigned long long*>(&sh.found[0]), (unsigned long long)any);
+                atomicAnd(reinterpret_cast<unsigned long long*>(&sh.found[1]), (unsigned long long)every);
+                __syncthreads();
+                prefix = sh.found[0], known = 64 - __builtin_clzll(sh.found[0] ^ sh.found[1]), shift = next(known);  // (more than 64 differ)
+                continue;
+            }
             // what is left has a lane each
-            for_all([&](uint64_t key) {
+            for_all([&](uint64_t key, auto) {
                 const double y4 = quarters_of(key);
                 if (key >= least && bin_of<true>(y4, bins.o) == bin && step_of(y4 - __builtin_rint(y4)) == step && (shift == 64 || key >> shift == prefix >> shift))
                     sh.key[atomicAdd(&sh.together, 1u)] = key;
@@ -565,10 +610,10 @@ struct Picker {
         __syncthreads();
         if (threadIdx.x < 64u * kLaneBins) sh.mass[threadIdx.x] = 0;
         __syncthreads();
-        for_all([&](uint64_t key) {
+        for_all([&](uint64_t key, auto many) {
             if (key < least) return;
             const double y4 = quarters_of(key);
-            atomicAdd(&sh.mass[bin_of<true>(y4, bins.o)], (unsigned long long)weight_of(y4, bins.o));
+            add_to(&sh.mass[bin_of<true>(y4, bins.o)], weight_of(y4, bins.o), many);
         });
         __syncthreads();
         uint64_t of[kLaneBins], sum = 0;
@@ -636,9 +681,9 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
     }
     const uint64_t threshold = tokens == 0 ? 0 : pick.threshold();
     // what every part keeps
-    pick.for_all([&](uint64_t key) {
+    pick.for_all([&](uint64_t key, auto many) {
         const uint64_t w = key >= threshold ? pick.weight(key) : 0;
-        if ((double)w >= floor && w != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.part_mass[index_of(key) / kPart]), (unsigned long long)w);
+        if ((double)w >= floor && w != 0) Picker::add_to(reinterpret_cast<unsigned long long*>(&sh.part_mass[index_of(key) / kPart]), w, many);
     });
     __syncthreads();
     uint64_t mass;
@@ -687,7 +732,7 @@ size_t parts_of(uint32_t n) { return (n + kPart - 1u) / kPart; }
 }  // namespace
 
 size_t sample_scratch_bytes(uint32_t rows, uint32_t n) {
-    return (size_t)rows * (sizeof(SampleRow) + parts_of(n) * sizeof(SamplePart) + (size_t)n * sizeof(uint32_t));
+    return (size_t)rows * (sizeof(SampleRow) + parts_of(n) * sizeof(SamplePart) + (size_t)n * sizeof(uint64_t));
 }
 
 hipError_t launch_sample(const float* d_logits, uint32_t stride, uint32_t rows, uint32_t n, const wick_rocm_sample_params* d_params, const float* d_uniform,
@@ -695,7 +740,7 @@ hipError_t launch_sample(const float* d_logits, uint32_t stride, uint32_t rows, 
     if (rows == 0) return hipSuccess;
     SampleArgs a{d_logits, d_params, d_uniform, d_out, d_prob, static_cast<SampleRow*>(d_scratch), nullptr, nullptr, n, stride, (uint32_t)parts_of(n)};
     a.parts = reinterpret_cast<SamplePart*>(a.rows + rows);
-    a.lists = reinterpret_cast<uint32_t*>(a.parts + (size_t)rows * a.n_parts);
+    a.lists = reinterpret_cast<uint64_t*>(a.parts + (size_t)rows * a.n_parts);
     hipError_t e = launch_kernel(L, kFamOther, sample_bins_kernel, dim3(a.n_parts, rows), dim3(kPartThreads), a);
     if (e == hipSuccess) e = launch_kernel(L, kFamOther, sample_list_kernel, dim3(a.n_parts, rows), dim3(kPartThreads), a);
     if (e == hipSuccess) e = launch_kernel(L, kFamOther, sample_pick_kernel, dim3(rows), dim3(kPickThreads), a);
