@@ -164,7 +164,7 @@ int wick_rocm_kv_q4_evict(wick_rocm_ctx *ctx, void *d_k_cache, void *d_v_cache, 
  *   d_lens  [n_seqs]             rows of sequence s
  *   d_refs  [n_pages]            table entries that name the page; 0: it is free
  * An empty pool: entries WICK_ROCM_NO_PAGE, lens and refs 0.  page_rows 16, 32, 64, 128 or 256; n_seqs at most 4096, n_pages 2^24, max_pages * page_rows
- * and n_seqs * max_pages 2^30.  The struct itself is read during the call only. */
+ * and n_seqs * max_pages 2^30.  The struct itself is read during the call only.  Calls on one pool follow each other, on one context's stream or ordered by the caller. */
 enum { WICK_ROCM_KV_F32 = 0, WICK_ROCM_KV_F16 = 1 };
 #define WICK_ROCM_NO_PAGE 0xffffffffu
 #define WICK_ROCM_NO_ROW 0xffffffffu

@@ -200,6 +200,7 @@ int main() {
         {"too many planes", kShape, [](Call& a) { a.planes.n_planes = 1025; }},
         {"planes that overlap", kShape, [](Call& a) { a.planes.plane_bytes -= 16; }},
         {"planes off each other", kShape, [](Call& a) { a.planes.plane_bytes += 8; }},
+        {"pages past any memory", kShape, [](Call& a) { a.pages.page_rows = 256, a.planes = {a.planes.d_base, (size_t)1 << 45, 1024, 65535, 256, WICK_ROCM_KV_F32}; }},
     });
     each("fork", fork, with(counts, {
         {"parents in the lengths", kArg, [](Call& a) { a.counts = a.pages.d_lens; }},

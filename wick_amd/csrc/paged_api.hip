@@ -40,6 +40,7 @@ int check_planes(wick_rocm_ctx* ctx, const wick_rocm_kv_pages& p, const wick_roc
     if (planes.n_planes == 0 || planes.n_planes > 1024u) return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, "kv_pages: n_planes must be 1 .. 1024");
     if (planes.n_planes > 1 && (planes.plane_bytes < bytes * p.n_pages || planes.plane_bytes % 16u != 0))
         return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, "kv_pages: plane_bytes must cover a plane and be a multiple of 16");
+    if (planes.n_planes * ((bytes + 16383u) / 16384u) > 1u << 23) return fail(ctx, WICK_ROCM_ERR_BAD_SHAPE, "kv_pages: a page of all planes is more than 2^37 bytes");
     return WICK_ROCM_OK;
 }
 
