@@ -395,11 +395,10 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(PagedAttentio
     const uint32_t in_tile = blockIdx.y, h = head / a.tiles * a.group + head % a.tiles * 16u + in_tile;
     if (n == 1 || head % a.tiles * 16u + in_tile >= a.group) return;
     float* const out = a.out + (size_t)s * a.out_stride + (size_t)h * HD;
-    const uint32_t records = min(a.group, 16u);
-    const auto record = [&](uint32_t i) {
-        const uint32_t slot = i == 0 && share_begin(units, w0, shares) != u0 ? 1u : 0u;
-        return a.parts + ((size_t)((w0 + i) * 2u + slot) * records + in_tile) * (kRecordHead + HD);
-    };
+    const uint32_t stride = 2u * min(a.group, 16u) * (kRecordHead + HD);  // of the first pieces of two shares; a share's second is half of it behind
+    const float* const parts = a.parts + (size_t)w0 * stride + in_tile * (kRecordHead + HD);
+    const uint32_t front = share_begin(units, w0, shares) != u0 ? stride / 2u : 0u;
+    const auto record = [&](uint32_t i) { return parts + (i == 0 ? front : i * stride); };
     // A thread's records' heads, and its part of the first records' values, are read in one go.
     constexpr uint32_t kQuads = HD / 4, kGroups = 256 / kQuads, kAhead = 4;
     static_assert(kShares <= 512);
