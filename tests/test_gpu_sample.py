@@ -91,6 +91,22 @@ def test_flat_rows_list_more_than_a_workgroup(run):
     check(run(logits, params, u), logits, params, u)
 
 
+@pytest.mark.parametrize("min_p", [2.0 ** -149, 1e-13, 2.0 ** -43, 1e-6, 0.01, 0.25, 0.5, float(np.nextafter(np.float32(0.5), np.float32(1))), 0.999, 1.0])
+def test_the_floor_alone(run, min_p):
+    """Tokens on the floor and a step off it, on both sides; rows of infinities and of values whose 4 y leave what is exact."""
+    n = 9000
+    logits = logits_of(15, 6, n)
+    logits[1] = (np.log(min_p) + 3 + np.arange(-4500, 4500) * 2.0 ** -20).astype(np.float32)
+    logits[1, 4321] = 3.0
+    logits[2] = np.log(2.0) * -(np.arange(n) % 60)
+    logits[3] *= 1e18
+    logits[4, :4000] = np.inf
+    logits[5, 7:] = -np.inf
+    u = np.array([0.7, 0.9, 0.5, 0.3, 0.6, 0.2], np.float32)
+    params = [(1.0, 0, 1.0, min_p)] * 6
+    check(run(logits, params, u), logits, params, u)
+
+
 def test_long_lists(run):
     """Many times what a workgroup holds at once is listed: alike, two values, nearly alike, alike but for a few, and alike from somewhere on."""
     n, rng = 150001, np.random.default_rng(6)

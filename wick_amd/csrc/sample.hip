@@ -376,11 +376,15 @@ __global__ __launch_bounds__(kPartThreads, 8) void sample_list_kernel(SampleArgs
     // The last bin that matters; as a rule it is far above most tokens.  Those that may be in it or above (by their logit, with room for rounding) are put together
     // first, so that few waves do the rest.
     const uint32_t last = bins.k_bin < kBins || bins.p_first == kBins ? bins.k_bin : bins.p_last;
-    if (last == kBins && !bins.o.wild) {
+    // Where nothing is cut, only the weights that min-p leaves matter: from an octave below its floor up (200 rows of 50257 under min-p alone: 34.5 us with all of them, 27.6).
+    const bool uncut = bins.k_bin == kBins && bins.p_first == kBins;
+    if (last == kBins && !bins.o.wild && !(uncut && bins.floor > 0.0)) {
 #pragma unroll
         for (uint32_t k = 0; k < kPartLoads; k++) take(std::false_type(), l[k], first + k * kPartThreads + threadIdx.x);
     } else {
-        const double lowest = fmin((bins.o.top4 - (double)last) / r.inverse4, kInfinite4);  // (a bin goes half a step further down than its whole number, which is at 4 E + 4 - bin)
+        // (a bin goes half a step further down than its whole number, which is at 4 E + 4 - bin; the floor is 2^43 times one of 2^(y - E))
+        const double below = uncut && bins.floor > 0.0 ? (double)(kSteps * (45 - __builtin_amdgcn_frexp_exp(bins.floor))) : (double)last;
+        const double lowest = fmin((bins.o.top4 - below) / r.inverse4, kInfinite4);
         const float low = (float)(lowest - __builtin_fabs(lowest) * 0x1p-20 - 0x1p-140);
 #pragma unroll
         for (uint32_t half = 0; half < 2; half++) {
