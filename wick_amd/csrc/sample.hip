@@ -10,9 +10,9 @@
 // Where top-k leaves few, tokens are only counted in 1., and all that may be taken are listed: no weights but theirs.  What is listed is at most some hundred
 // tokens as a rule, which 3. sorts, and a row's all in the worst case (all logits alike), for which there is room.
 //
-// Three dependent launches bound a single row (65536 tokens, top-k 40: 4.3, 7.8 and 4.8 us, each a chain of round trips); f64 arithmetic, of which every weight takes some
-// twenty instructions, many (64 rows of 65536 under top-p: 9.4, 12.5 and 12.6 us; reading them alone would take 3.5).  65536 tokens that are all alike take 0.37 ms,
-// 0.39 in 64 rows: passes over a long list.
+// Three dependent launches bound a single row (65536 tokens, top-k 40: 4.3, 7.8 and 4.7 us, each a chain of round trips); f64 arithmetic, of which every weight takes some
+// twenty instructions, many (64 rows of 65536 under top-p: 9.4, 12.6 and 11.6 us; reading them alone would take 3.5).  65536 tokens that are all alike take 0.38 ms,
+// 0.41 in 64 rows: passes over a long list.
 #include <algorithm>
 #include <type_traits>
 
@@ -419,7 +419,7 @@ __global__ __launch_bounds__(kPartThreads, 8) void sample_list_kernel(SampleArgs
 
 // 3.
 // (Sixteen waves: 64 rows' nuclei and 200 rows' mixed rules take 13.1 and 16.2 us; with four 15.9 and 25.1, with eight 12.9 and 17.7.)
-constexpr uint32_t kPickThreads = 1024, kPickWaves = kPickThreads / 64, kDigit = 10, kDigits = 1u << kDigit, kOwn = 1, kLoadsAtOnce = 8;
+constexpr uint32_t kPickThreads = 1024, kPickWaves = kPickThreads / 64, kDigit = 10, kDigits = 1u << kDigit, kOwn = 1, kLoadsAtOnce = 2;
 constexpr uint32_t kEach = kPart / kPickThreads, kDigitsEach = kDigits / kPickThreads;
 
 struct PickShared {
@@ -462,6 +462,9 @@ __device__ __forceinline__ uint64_t sorted(uint64_t key) {
     return key;
 }
 
+// MANY: more tokens are listed than threads.  The usual row, which has fewer, keeps code of its own: with the loops over long lists in it 64 rows took 12.2 us, not 11.6, and
+// 200 16.3, not 15.7.
+template <bool MANY>
 struct Picker {
     const SampleArgs& a;
     const Rule& r;
@@ -478,25 +481,25 @@ struct Picker {
         }
         return a.lists[(size_t)row * a.n + (size_t)low * kPart + (f - sh.listed[low])];
     }
-    // All listed tokens, each by a thread of its own; f's second argument: behind the first ones.
+    // All listed tokens, each by a thread of its own.
     template <typename F>
     __device__ __forceinline__ void for_all(F f) const {
 #pragma unroll
         for (uint32_t i = 0; i < kOwn; i++)
-            if (threadIdx.x + i * kPickThreads < tokens) f(own[i], std::false_type());
+            if (threadIdx.x + i * kPickThreads < tokens) f(own[i]);
+        if constexpr (!MANY) return;
         for (uint32_t t = threadIdx.x + kOwn * kPickThreads; t < tokens; t += kLoadsAtOnce * kPickThreads) {
             uint64_t key[kLoadsAtOnce];
 #pragma unroll
             for (uint32_t i = 0; i < kLoadsAtOnce; i++) key[i] = t + i * kPickThreads < tokens ? load(t + i * kPickThreads) : 0;
 #pragma unroll
             for (uint32_t i = 0; i < kLoadsAtOnce; i++)
-                if (key[i] != 0) f(key[i], std::true_type());
+                if (key[i] != 0) f(key[i]);
         }
     }
     // *sum += v of every lane that is here.  Where there are many tokens, lanes with the same v at the same place (tokens that are alike) are one addition.
-    template <typename MANY>
-    static __device__ __forceinline__ void add_to(unsigned long long* sum, uint64_t v, MANY) {
-        if constexpr (!MANY::value) {
+    static __device__ __forceinline__ void add_to(unsigned long long* sum, uint64_t v) {
+        if constexpr (!MANY) {
             atomicAdd(sum, (unsigned long long)v);
             return;
         }
@@ -529,11 +532,11 @@ struct Picker {
             if (threadIdx.x == 0) sh.together = 0;
             for (uint32_t d = threadIdx.x; d < kDigits; d += kPickThreads) sh.count[d] = 0, sh.mass[d] = 0;
             __syncthreads();
-            for_all([&](uint64_t key, auto many) {
+            for_all([&](uint64_t key) {
                 double y4, place;
                 if (!is_left(key, y4, place)) return;
                 const uint32_t d = shift == 64 ? step_of(place) : (uint32_t)(key >> shift) & (kDigits - 1u);
-                atomicAdd(&sh.count[d], 1u), add_to(&sh.mass[d], weight_of(y4, bins.o), many);
+                atomicAdd(&sh.count[d], 1u), add_to(&sh.mass[d], weight_of(y4, bins.o));
             });
             __syncthreads();
             // the digits from the highest
@@ -566,7 +569,7 @@ struct Picker {
                 if (threadIdx.x == 0) sh.found[0] = 0, sh.found[1] = ~0ull;
                 __syncthreads();
                 uint64_t any = 0, every = ~0ull;
-                for_all([&](uint64_t key, auto) {
+                for_all([&](uint64_t key) {
                     const double y4 = quarters_of(key);
                     if (key >= least && bin_of<true>(y4, bins.o) == bin && step_of(y4 - __builtin_rint(y4)) == step) any |= key, every &= key;
                 });
@@ -577,7 +580,7 @@ struct Picker {
                 continue;
             }
             // what is left has a lane each
-            for_all([&](uint64_t key, auto) {
+            for_all([&](uint64_t key) {
                 const double y4 = quarters_of(key);
                 if (key >= least && bin_of<true>(y4, bins.o) == bin && step_of(y4 - __builtin_rint(y4)) == step && (shift == 64 || key >> shift == prefix >> shift))
                     sh.key[atomicAdd(&sh.together, 1u)] = key;
@@ -614,10 +617,10 @@ struct Picker {
         __syncthreads();
         if (threadIdx.x < 64u * kLaneBins) sh.mass[threadIdx.x] = 0;
         __syncthreads();
-        for_all([&](uint64_t key, auto many) {
+        for_all([&](uint64_t key) {
             if (key < least) return;
             const double y4 = quarters_of(key);
-            add_to(&sh.mass[bin_of<true>(y4, bins.o)], weight_of(y4, bins.o), many);
+            add_to(&sh.mass[bin_of<true>(y4, bins.o)], weight_of(y4, bins.o));
         });
         __syncthreads();
         uint64_t of[kLaneBins], sum = 0;
@@ -634,7 +637,7 @@ struct Picker {
 };
 
 // All of it where one wave has every token that may be taken: sorted by key for the cuts, then by index.
-__device__ __forceinline__ void pick_in_a_wave(const SampleArgs& a, uint32_t row, const Rule& r, const RowBins& bins, const Picker& pick, float u) {
+__device__ __forceinline__ void pick_in_a_wave(const SampleArgs& a, uint32_t row, const Rule& r, const RowBins& bins, const Picker<false>& pick, float u) {
     const uint64_t key = sorted(pick.own[0]), w = key != 0 ? pick.weight(key) : 0;
     bool taken = key != 0 && threadIdx.x < r.top_k;
     if (r.top_p < 1.0) {
@@ -653,41 +656,25 @@ __device__ __forceinline__ void pick_in_a_wave(const SampleArgs& a, uint32_t row
     }
 }
 
-__global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a) {
-    __shared__ PickShared sh;
-    const uint32_t row = blockIdx.x;
+// The cuts and the pick, from the tokens that are listed and the masses that parts keep for certain (in sh).
+template <bool MANY>
+__device__ __forceinline__ void pick_of(const SampleArgs& a, uint32_t row, const Rule& r, const RowBins& bins, PickShared& sh, uint32_t tokens, float u) {
     const float* const logits = a.logits + (size_t)row * a.stride;
-    const SamplePart* const parts = a.parts + (size_t)row * a.n_parts;
-    const uint64_t sure = threadIdx.x < a.n_parts ? parts[threadIdx.x].sure : 0;
-    const uint32_t listed = threadIdx.x < a.n_parts ? parts[threadIdx.x].listed : 0;
-    const float u = a.uniform[row];
-    const Rule r = rule_of(a, row);
-    const RowBins bins = handed_on(a.rows[row], r);
     const double floor = bins.floor;
-    if (bins.o.none()) {
-        if (threadIdx.x == 0) {
-            a.out[row] = WICK_ROCM_NO_TOKEN;
-            if (a.prob) a.prob[row] = 0.0f;
-        }
-        return;
-    }
-    uint64_t tokens;
-    const uint64_t upto = sum_before<kPickWaves>(listed, sh.slots[0], tokens);
-    if (threadIdx.x < a.n_parts) sh.listed[threadIdx.x] = (uint32_t)upto, sh.part_mass[threadIdx.x] = sure;
-    __syncthreads();
-    Picker pick{a, r, bins, sh, row, (uint32_t)tokens, {}};
+    Picker<MANY> pick{a, r, bins, sh, row, tokens, {}};
 #pragma unroll
     for (uint32_t i = 0; i < kOwn; i++)
         if (threadIdx.x + i * kPickThreads < tokens) pick.own[i] = pick.load(threadIdx.x + i * kPickThreads);
-    if (bins.whole && tokens <= 64) {
-        if (threadIdx.x < 64u) pick_in_a_wave(a, row, r, bins, pick, u);
-        return;
-    }
+    if constexpr (!MANY)
+        if (bins.whole && tokens <= 64) {
+            if (threadIdx.x < 64u) pick_in_a_wave(a, row, r, bins, pick, u);
+            return;
+        }
     const uint64_t threshold = tokens == 0 ? 0 : pick.threshold();
     // what every part keeps
-    pick.for_all([&](uint64_t key, auto many) {
+    pick.for_all([&](uint64_t key) {
         const uint64_t w = key >= threshold ? pick.weight(key) : 0;
-        if ((double)w >= floor && w != 0) Picker::add_to(reinterpret_cast<unsigned long long*>(&sh.part_mass[index_of(key) / kPart]), w, many);
+        if ((double)w >= floor && w != 0) Picker<MANY>::add_to(reinterpret_cast<unsigned long long*>(&sh.part_mass[index_of(key) / kPart]), w);
     });
     __syncthreads();
     uint64_t mass;
@@ -729,6 +716,30 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
         a.out[row] = i;
         if (a.prob) a.prob[row] = (float)(exact_weight(quarters<true>(logits[i], r, bins.o), bins.o) / (double)mass);
     }
+}
+
+__global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a) {
+    __shared__ PickShared sh;
+    const uint32_t row = blockIdx.x;
+    const SamplePart* const parts = a.parts + (size_t)row * a.n_parts;
+    const uint64_t sure = threadIdx.x < a.n_parts ? parts[threadIdx.x].sure : 0;
+    const uint32_t listed = threadIdx.x < a.n_parts ? parts[threadIdx.x].listed : 0;
+    const float u = a.uniform[row];
+    const Rule r = rule_of(a, row);
+    const RowBins bins = handed_on(a.rows[row], r);
+    if (bins.o.none()) {
+        if (threadIdx.x == 0) {
+            a.out[row] = WICK_ROCM_NO_TOKEN;
+            if (a.prob) a.prob[row] = 0.0f;
+        }
+        return;
+    }
+    uint64_t tokens;
+    const uint64_t upto = sum_before<kPickWaves>(listed, sh.slots[0], tokens);
+    if (threadIdx.x < a.n_parts) sh.listed[threadIdx.x] = (uint32_t)upto, sh.part_mass[threadIdx.x] = sure;
+    __syncthreads();
+    if (tokens > kOwn * kPickThreads) return pick_of<true>(a, row, r, bins, sh, (uint32_t)tokens, u);
+    pick_of<false>(a, row, r, bins, sh, (uint32_t)tokens, u);
 }
 
 size_t parts_of(uint32_t n) { return (n + kPart - 1u) / kPart; }
