@@ -252,6 +252,22 @@ def test_attention_under_a_wide_table(ctx, ops, dev, hd, heads, n_kv, page_rows,
 
 
 @pytest.mark.parametrize("dtype", [KV_F32, KV_F16])
+@pytest.mark.parametrize("longest,spread", [(40, 1), (2, 1), (40, 500)])
+def test_attention_of_many_sequences_under_a_wide_table(ctx, ops, dev, dtype, longest, spread):
+    """4096 sequences, of which all, or one in 500, have rows: the others lie between those that a share has."""
+    lens = [int(n) if s % spread == 0 else 0 for s, n in enumerate(np.random.default_rng(36).integers(0, longest, 4096))]
+    lens[4095], lens[2001] = 200, 2500
+    pool = filled(37, lens, 16, 2, 32, dtype)
+    pool.max_pages = 300
+    q = normal(38, 4096, 4, 32)
+    got, want = attend(ctx, ops, dev, OnDevice(dev, pool), q, extra=4), pool.attention(q)
+    assert_f32_parity(got, want)
+    assert np.all(got[np.array(lens) == 0] == 0)
+    for s in (2001, 4095):
+        assert_f32_parity(got[s], want[s])
+
+
+@pytest.mark.parametrize("dtype", [KV_F32, KV_F16])
 @pytest.mark.parametrize("seqs,hd,heads,n_kv", [(600, 32, 1, 1), (130, 64, 8, 4), (40, 64, 40, 8), (300, 128, 17, 1), (70, 256, 4, 4)])
 def test_more_heads_than_shares(ctx, ops, dev, dtype, seqs, hd, heads, n_kv):
     """Sequences of all lengths and of none, also at both ends; heads that end where a share does and heads over several shares."""
