@@ -60,36 +60,47 @@ __device__ __forceinline__ uint32_t all_units(const PagedAttentionArgs& a, uint3
     return (uint32_t)__builtin_amdgcn_readlane((int)lanes_upto(sum), 63);
 }
 
-// Share `w` of the units, [begin, end), the sequence of its first unit (or its last one) and the units in front of that sequence; up to 64 sequences, a
-// lane each, are read once.
+// Share `w` of the units, [begin, end), the sequence of its first unit (or its last one) and the units in front of that sequence.  64 sequences at a time, a lane
+// each, the lengths of several 64s on their way together; the 64 that have the unit are then looked at once more.
 struct Share {
     uint32_t units, begin, end, s, before;
 };
 __device__ __forceinline__ uint32_t share_begin(uint32_t units, uint32_t w, uint32_t shares) { return (uint32_t)((uint64_t)units * w / shares); }
 __device__ __forceinline__ uint32_t share_of(uint32_t units, uint32_t u, uint32_t shares) { return (uint32_t)((((uint64_t)u + 1) * shares - 1) / units); }
 __device__ __forceinline__ Share share(const PagedAttentionArgs& a, uint32_t heads, uint32_t w, bool its_last) {
-    const uint32_t lane = threadIdx.x & 63u, first = lane < a.n_seqs ? units_of(length(a, lane)) * heads : 0u;
-    uint32_t sum = first;
-    for (uint32_t s = lane + 64u; s < a.n_seqs; s += 64u) sum += units_of(length(a, s)) * heads;
-    const uint32_t upto_first = lanes_upto(first);
+    const uint32_t lane = threadIdx.x & 63u, runs = (a.n_seqs + 63u) / 64u;
+    const auto units_at = [&](uint32_t s) { return s < a.n_seqs ? units_of(length(a, s)) * heads : 0u; };
+    uint32_t n = units_at(lane), upto = lanes_upto(n);
+    uint32_t sum = lane == 0 ? (uint32_t)__builtin_amdgcn_readlane((int)upto, 63) : 0u;  // of the lane's 64
+#pragma unroll 8
+    for (uint32_t i = 1; i < runs; i++) {
+        const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)lanes_upto(units_at(64u * i + lane)), 63);
+        sum = lane == i ? all : sum;
+    }
+    const uint32_t runs_upto = lanes_upto(sum);
     Share x{};
-    x.units = (uint32_t)__builtin_amdgcn_readlane((int)(a.n_seqs <= 64u ? upto_first : lanes_upto(sum)), 63);
+    x.units = (uint32_t)__builtin_amdgcn_readlane((int)runs_upto, 63);
     const uint32_t shares = min(x.units, a.shares);  // (no share is empty)
     if (w >= shares) return x;
     x.begin = share_begin(x.units, w, shares), x.end = share_begin(x.units, w + 1u, shares);
     const uint32_t unit = its_last ? x.end - 1u : x.begin;
-    uint32_t n = first, upto = upto_first;
-    for (uint32_t base = 0;;) {
-        const uint64_t past = __ballot(x.before + upto > unit);
-        if (past != 0 || base + 64u >= a.n_seqs) {
-            const int at = past != 0 ? __ffsll((unsigned long long)past) - 1 : 63;
-            x.before += (uint32_t)__builtin_amdgcn_readlane((int)(upto - n), at), x.s = base + (uint32_t)at;
-            return x;
-        }
-        x.before += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
-        base += 64u;
-        n = base + lane < a.n_seqs ? units_of(length(a, base + lane)) * heads : 0u, upto = lanes_upto(n);
+    const int run = __ffsll((unsigned long long)__ballot(runs_upto > unit)) - 1;
+    x.before = (uint32_t)__builtin_amdgcn_readlane((int)(runs_upto - sum), run);
+    if (run != 0) n = units_at(64u * (uint32_t)run + lane), upto = lanes_upto(n);
+    const int at = __ffsll((unsigned long long)__ballot(x.before + upto > unit)) - 1;
+    x.before += (uint32_t)__builtin_amdgcn_readlane((int)(upto - n), at), x.s = 64u * (uint32_t)run + (uint32_t)at;
+    return x;
+}
+
+// The first sequence from `s` on that has rows, or n_seqs; 64 at a time.  (20 sequences of 2000 rows among 1024: 20.4 us, 28.5 one by one; among 4000, with the search
+// above, 33 and 69.  32 with rows each take 0.7 of 59 us longer for it.)
+__device__ __forceinline__ uint32_t next_with_rows(const PagedAttentionArgs& a, uint32_t s) {
+    const uint32_t lane = threadIdx.x & 63u;
+    for (; s < a.n_seqs; s += 64u) {
+        const uint64_t some = __ballot(s + lane < a.n_seqs && a.lens[min(s + lane, a.n_seqs - 1u)] != 0);
+        if (some != 0) return s + (uint32_t)__ffsll((unsigned long long)some) - 1u;
     }
+    return a.n_seqs;
 }
 
 template <typename KV, int HD>
@@ -286,8 +297,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : HD == 256 ? 1 : 2) vo
     uint32_t s = sh.s, before = sh.before;
     for (uint32_t u = sh.begin; u < sh.end && s < a.n_seqs;) {
         const uint32_t len = length(a, s), chunks = units_of(len);
-        if (!SHORT && u - before >= chunks * heads) {  // (the next sequence; one without rows has no units)
-            before += chunks * heads, s++;
+        if (!SHORT && u - before >= chunks * heads) {
+            before += chunks * heads, s = chunks != 0 ? s + 1u : next_with_rows(a, s + 1u);
             continue;
         }
         const uint32_t head = SHORT ? blockIdx.x % heads : (u - before) / chunks, chunk = SHORT ? 0u : (u - before) % chunks, take = SHORT ? 1u : min(chunks - chunk, sh.end - u);
