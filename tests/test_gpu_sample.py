@@ -205,3 +205,52 @@ def test_greedy_rows_are_the_largest(ctx, run):
         assert got[0][r] == out.download(np.uint32, 1)[0] and got[1][r] == 1
         x.free()
     out.free()
+
+
+# (temperature, top_k, top_p, min_p) where the nucleus and min-p both cut, under a top_k that leaves at most 512 tokens
+NUCLEUS_AND_FLOOR = [(0.8, 40, 0.95, 0.05), (1.0, 40, 0.5, 0.3), (1.0, 500, 0.9, 0.1), (0.1, 40, 0.9, 0.01), (1.0, 512, 0.8, 0.999)]
+
+
+@pytest.mark.parametrize("n", [40, 512, 513, 5000, 20000])
+def test_fewer_live_tokens_than_top_k(run, n):
+    """Rows of which a grammar leaves fewer tokens than top_k: top-p's share is of all of them, min-p cuts what top-p leaves.  (At most 300 masses, each off by half of
+    2^-43 where the largest is at least 1: within 2e-11 of the whole.)"""
+    rng = np.random.default_rng(n)
+    rules = NUCLEUS_AND_FLOOR + ([(1.0, 0, 0.7, 0.2)] if n <= 512 else [])
+    us, logits, params = [0.05, 0.4, 0.75, 0.97], [], []
+    for live in (2, 3, 5, 8, 13, 21, 30, 39, 64, 65, 120, 300):
+        for rule in rules if live < n else []:
+            for spread in (1.0, 2.5):
+                row = np.full(n, -np.inf, np.float32)
+                row[rng.permutation(n)[:live]] = spread * rng.standard_normal(live)
+                logits += [row] * len(us)
+                params += [rule] * len(us)
+    u = np.array(us * (len(params) // len(us)), np.float32)
+    logits = np.stack(logits)
+    check(run(logits, params, u), logits, params, u)
+
+
+@pytest.mark.parametrize("n", [30, 512, 1000, 70000])
+def test_a_tail_below_the_floor_counts_for_the_nucleus(run, n):
+    """Light tokens that min-p rules out are part of the mass that top-p takes its share of."""
+    tail_of_27 = np.log(np.array([1, 0.06, 0.055] + [0.01] * 27))
+    two_and_20 = np.log(np.array([1, 0.9] + [0.1] * 20))
+    us = (np.arange(32, dtype=np.float32) + 0.5) / 32
+    for live, rule, kept in ((tail_of_27, (1.0, 40, 0.9, 0.05), [1, 0.06, 0.055]), (two_and_20, (1.0, 40, 0.5, 0.3), [1, 0.9])):
+        logits = np.full((32, n), -np.inf, np.float32)
+        at = np.random.default_rng(n).permutation(n)[:live.size]
+        logits[:, at] = live
+        got = run(logits, [rule] * 32, us)
+        assert set(got[0]) <= set(at[:len(kept)])
+        check(got, logits, [rule] * 32, us)
+        for token, w in zip(at, kept):  # (logits are f32: weights within 2^-23 or so)
+            assert np.all(np.abs(got[1][got[0] == token] - w / sum(kept)) <= 1e-6)
+        assert len(set(got[0])) == len(kept)
+
+
+@pytest.mark.parametrize("temperature", [0.02, 0.1])
+def test_cold_rows_of_a_whole_vocabulary(run, temperature):
+    """At low temperatures few of many finite tokens have mass."""
+    logits = logits_of(16, 120, 50257, spread=4.0)
+    params, u = [(temperature, 40, 0.9, 0.05), (temperature, 200, 0.6, 0.02), (temperature, 512, 0.99, 0.1)] * 40, np.random.default_rng(17).random(120, dtype=np.float32)
+    check(run(logits, params, u), logits, params, u)

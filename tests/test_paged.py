@@ -103,3 +103,14 @@ def test_picks_are_as_often_as_their_weights():
     want = np.zeros(30)
     want[index] = w / w.sum() * n
     assert np.all(np.abs(picks - want) <= 1) and (picks > 0).sum() == index.size < 12
+
+
+@pytest.mark.parametrize("n", [30, 512, 1000])
+def test_top_p_is_of_all_that_top_k_leaves(n):
+    """Tokens that min-p rules out afterwards are part of the mass that top-p takes its share of."""
+    for live, rule, tokens in (([1, 0.06, 0.055] + [0.01] * 27, (1.0, 40, 0.9, 0.05), 3), ([1, 0.9] + [0.1] * 20, (1.0, 40, 0.5, 0.3), 2)):
+        logits = np.full(n, -INF, np.float32)
+        logits[:len(live)] = np.log(live)
+        index, w = R.kept(logits, *rule)
+        assert index.tolist() == list(range(tokens)) and np.allclose(w, live[:tokens], rtol=1e-6)
+        assert np.isclose(R.sample(logits, *rule, 0.0)[1], 1 / sum(live[:tokens]), rtol=1e-6)

@@ -376,8 +376,9 @@ __global__ __launch_bounds__(kPartThreads, 8) void sample_list_kernel(SampleArgs
     // The last bin that matters; as a rule it is far above most tokens.  Those that may be in it or above (by their logit, with room for rounding) are put together
     // first, so that few waves do the rest.
     const uint32_t last = bins.k_bin < kBins || bins.p_first == kBins ? bins.k_bin : bins.p_last;
-    // Where nothing is cut, only the weights that min-p leaves matter: from an octave below its floor up (200 rows of 50257 under min-p alone: 34.5 us with all of them, 27.6).
-    const bool uncut = bins.k_bin == kBins && bins.p_first == kBins;
+    // Where min-p alone cuts, only the weights that it leaves matter: from an octave below its floor up (200 rows of 50257 under min-p alone: 34.5 us with all of them, 27.6).  Top-p's
+    // share is of what is below the floor too, and where tokens are only counted no bin says that it cuts.
+    const bool uncut = bins.k_bin == kBins && bins.p_first == kBins && r.top_p >= 1.0;
     if (last == kBins && !bins.o.wild && !(uncut && bins.floor > 0.0)) {
 #pragma unroll
         for (uint32_t k = 0; k < kPartLoads; k++) take(std::false_type(), l[k], first + k * kPartThreads + threadIdx.x);
