@@ -198,7 +198,7 @@ int wick_rocm_qk_norm_rope_paged(wick_rocm_ctx *ctx, const wick_rocm_kv_pages *p
 
 /* wick_rocm_attention_decode for one new token of every sequence, over its rows [0, d_lens[s]) (no rows: zeros).  Sequence s's query heads at
  * d_q + s * q_stride floats, its output at d_out + s * out_stride; f32 in and out, sums and softmax f32's, cached values as they are held.  (f16 pages: a query
- * element is off by at most 2^-22 of itself or 2^-39 of its head's largest, a softmax weight by the same of itself or of the largest.)  Rows whose entry names no page
+ * element is off by at most 2^-22 of itself, a softmax weight too, or by 2^-19 of itself where it is less than 2^-18 of the largest.)  Rows whose entry names no page
  * of the pool count as not there.  A row that is not finite may make outputs that are not finite of the sequences that see it, in the heads that read it, and of no other.
  * The work of all sequences together is split evenly over the GPU, whatever their lengths, and a second launch joins what several workgroups share; a table of few
  * rows (at most 256 to 1024, by head_dim) takes one launch.

@@ -714,3 +714,98 @@ def test_two_contexts_at_once(ctx, dev):
         ctx.sync(), other.sync()
         for pool, _, q, _, d_out, _ in sides:
             assert_f32_parity(back(d_out, q), pool.attention(q))
+
+
+@pytest.mark.parametrize("hd,heads,n_kv,page_rows", [(64, 8, 2, 16), (32, 3, 3, 32), (128, 8, 1, 64), (256, 4, 2, 16)])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("dtype", [KV_F32, KV_F16])
+def test_a_large_query_element_takes_no_bits_from_the_others(ctx, ops, dev, dtype, wide, hd, heads, n_kv, page_rows):
+    """Where a channel of the keys is zero, what the query has there makes no difference, however large it is; one head has ordinary queries beside the others'."""
+    pool = filled(90, [150, 500, 7], page_rows, n_kv, hd, dtype)
+    pool.planes[0, ..., 5] = 0
+    pool.max_pages += 2048 // page_rows if wide else 0
+    d, q = OnDevice(dev, pool), normal(91, 3, heads, hd)
+    for large in (0.0, 2.0 ** 12, 2.0 ** 19, 2.0 ** 24, 2.0 ** 40, 2.0 ** 100, 3e38):
+        q[:, 1:, 5] = large
+        got, want = attend(ctx, ops, dev, d, q), pool.attention(q)
+        for h in range(heads):
+            assert_f32_parity(got[:, h], want[:, h], f"{large}, head {h}")
+
+
+@pytest.mark.parametrize("bits", [4, 20, 30, 40, 60])
+@pytest.mark.parametrize("hd,heads,n_kv,page_rows", [(64, 8, 2, 16), (32, 3, 3, 32), (128, 8, 1, 64), (256, 4, 2, 16)])
+@pytest.mark.parametrize("dtype", [KV_F32, KV_F16])
+def test_values_that_light_rows_alone_hold(ctx, ops, dev, dtype, hd, heads, n_kv, page_rows, bits):
+    """One row draws nearly all weight and holds zeros in half of the channels; the others' weights are 2^-bits of it and are all that these channels have.
+    An exponent of at most bits + 2 in magnitude is rounded at most eight times (square root, its inverse, log2(e), their product, the product with q, k's sum, the largest taken off), and
+    exp2 is off by less than 2^-22, two halves of a weight by 2^-19: a weight by (8 ln2 (bits + 2) + 4 + 32) 2^-24 of itself.  Sums of n rows in f32 add n 2^-24 in whatever
+    order, the joins a few more."""
+    n = 61
+    pool = filled(92, [n, 1], page_rows, n_kv, hd, dtype)
+    pool.max_pages += 2048 // page_rows if bits % 20 == 0 else 0
+    q = np.zeros((2, heads, hd), np.float32)
+    q[..., 3] = 64.0
+    for i, page in enumerate(pool.held[0]):  # row r's exponent: a multiple of 2^-3 about `bits` below row 33's
+        pool.planes[0, page] = 0
+        for r in range(page_rows):
+            x = bits + (i * page_rows + r) % 9 / 8 if i * page_rows + r != 33 else 0.0
+            pool.planes[0, page, :, r, 3] = np.round(-x * np.log(2) * np.sqrt(hd) / 64 * 1024) / 1024
+    page, r = pool.held[0][33 // page_rows], 33 % page_rows
+    pool.planes[1, page, :, r, :hd // 2] = 0
+    got, want = attend(ctx, ops, dev, OnDevice(dev, pool), q), pool.attention(q)
+    magnitude = R.Pool.attention(_absolute(pool), q)
+    steps = 8 * np.log(2) * (bits + 2) + 4 + 32 + n + 8
+    off = np.abs(got[0] - want[0]) / magnitude[0]
+    assert off.max() <= steps * 2.0 ** -24, (off.max() * 2.0 ** 24, steps)
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("hd,heads,n_kv,page_rows", [(64, 8, 2, 16), (32, 3, 3, 32), (128, 8, 1, 64), (256, 4, 2, 16)])
+@pytest.mark.parametrize("dtype", [KV_F32, KV_F16])
+def test_every_weight_keeps_its_bits(ctx, ops, dev, dtype, wide, hd, heads, n_kv, page_rows):
+    """Values of which each row has one, in a channel of its own, under weights from 1 down to 2^-90 in any order: outputs are the weights themselves.  As above but for the
+    sums: a channel has one term, the weights' sum is 1 to 3 and of few that matter."""
+    pool = filled(94, [hd], page_rows, n_kv, hd, dtype)
+    pool.max_pages += 2048 // page_rows if wide else 0
+    q = np.zeros((1, heads, hd), np.float32)
+    q[..., 3] = 64.0
+    octaves = np.random.default_rng(95).permutation(hd) * (90 / hd)
+    keys = np.round(-octaves * np.log(2) * np.sqrt(hd) / 64 * 64) / 64
+    for i, page in enumerate(pool.held[0]):
+        pool.planes[:, page] = 0
+        for r in range(min(page_rows, hd - i * page_rows)):
+            pool.planes[0, page, :, r, 3] = keys[i * page_rows + r]
+            pool.planes[1, page, :, r, i * page_rows + r] = 1 + r / 64
+    got, want = attend(ctx, ops, dev, OnDevice(dev, pool), q)[0], pool.attention(q)[0]
+    steps = 8 * np.log(2) * (octaves + 3) + 4 + 32 + 64
+    assert np.all(np.abs(got - want) <= steps * 2.0 ** -24 * want), (np.abs(got / want - 1) * 2.0 ** 24 / steps).max()
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("hd,heads,n_kv,page_rows", [(64, 8, 2, 16), (32, 3, 3, 32), (128, 8, 1, 64), (256, 4, 2, 16), (64, 34, 2, 32)])
+@pytest.mark.parametrize("dtype", [KV_F32, KV_F16])
+def test_queries_as_small_as_keys_are_large(ctx, ops, dev, dtype, wide, hd, heads, n_kv, page_rows):
+    """Channels whose keys are 2^28 times as large as others', and their queries as small: all of them make the scores alike.  Some heads have but one such element, some none."""
+    lens = [300, 40]
+    pool = filled(96, lens, page_rows, n_kv, hd, dtype)
+    pool.max_pages += 2048 // page_rows if wide else 0
+    e = np.random.default_rng(97).integers(0, 29, hd)
+    x = np.clip(np.random.default_rng(98).standard_normal(pool.planes[0].shape), -3.99, 3.99)  # (times 2^14 an f16)
+    pool.planes[0] = np.where(np.isnan(pool.planes[0]), np.nan, x * 2.0 ** (e - 14)).astype(R.TYPES[dtype])
+    q = (normal(99, 2, heads, hd) * 2.0 ** (14 - e)).astype(np.float32)
+    one = int(np.argmax(e))
+    if heads > 4:
+        q[:, 1] = np.where(np.arange(hd) == one, q[:, 1], np.where(e == e.min(), q[:, 1], 0))
+        q[:, 2] = np.where(e <= e.min() + 3, q[:, 2], 0)
+    got, want = attend(ctx, ops, dev, OnDevice(dev, pool), q), pool.attention(q)
+    for s in range(2):
+        for h in range(heads):
+            assert_f32_parity(got[s, h], want[s, h], f"sequence {s}, head {h}")
+
+
+def _absolute(pool):
+    """The pool with its values' magnitudes."""
+    p = R.Pool(pool.S, pool.max_pages, pool.n_pages, pool.R, pool.n_kv, pool.hd, pool.dtype)
+    p.held, p.lens, p.planes = pool.held, pool.lens, pool.planes.copy()
+    p.planes[1] = np.abs(p.planes[1])
+    return p

@@ -8,7 +8,9 @@
 // Nothing goes through LDS on the way: keys are read 16 bytes a lane in the operand's own order, values as 16 (or fewer) bytes of each of the
 // lane's rows, from which the operand of dimension e is picked lane by lane.
 //   f16 pages: v_mfma_f32_16x16x32_f16; the cached values are exact operands, a query row (scaled by a power of two to below 2^15) and the softmax weights (times
-//   2^15) are split into two halves: a product with one is off by at most 2^-22 of it, or 2^-39 of the row's largest.  Two products.
+//   2^15) are split into two halves: a product with one is off by at most 2^-22 of it.  Two products.  What is so far below the row's largest that halves would lose its bits
+//   goes through f32 products instead: elements of the query (Query) and the weights of a tile (State).  (All of it in f32 products: 73 us for the 59.3 of 32 sequences
+//   below, 108 for the 99.5 of one, 11.4 for 7.3 with 701 rows.)
 //   f32 pages: v_mfma_f32_16x16x4_f32, f32 products as they are.
 // The softmax is a running one: maximum and sum of every head, rescaled when a tile has a larger score.
 //
@@ -22,6 +24,7 @@
 // to join.  Loads of the next tile ahead of a tile's products (f32: 53 to 56 us) and waves that yield to those with more left (no difference) do not pay:
 // with 8 waves a CU the loads of one fill the products of another.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_paged_device.h"
 #include "wick_rocm_internal.h"
@@ -34,6 +37,9 @@ constexpr uint32_t kUnitRows = 128, kTileRows = 32, kWaves = 4;  // a unit is a 
 constexpr uint32_t kShares = 512;                                 // workgroups, two on each of 256 CUs (one where the registers of a row of 256 leave room for one)
 constexpr uint32_t kRecordHead = 4;                              // floats of a record in front of its values: maximum, sum, -, -
 constexpr float kHalfScale = 32768.0f;                           // softmax weights are split below or at a half's largest power of two
+// Two halves of a value of 2^-3 to 2^15 are off by at most 2^-22 of it, of a smaller one by 2^-25.
+constexpr int kQueryBits = 18;   // queries down to 2^-18 of a head's largest are halves
+constexpr int kWeightBits = 21;  // weights down to 2^-21 of the largest are: off by 2^-19 then, as f32's rounding of such an exponent makes them (with 18, ordinary scores have tiles of f32)
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct PagedAttentionArgs {
@@ -118,11 +124,14 @@ struct Tile {
 
 template <typename KV, int HD>
 struct Query;
+// Elements below 2^-18 of their head's largest are left out of the halves; f32 products add them to the scores, four dimensions at a time and only where there are
+// any: `rest_of` (LDS, HD / 4 floats of each lane) has them.  32 sequences of up to 8192 rows of 64: 50.4 us without, 53.6 with one such element in every head, 69.8 with 63.
 template <int HD>
 struct Query<_Float16, HD> {
     v4f x[HD / 32][2];
     h8 hi[HD / 32], lo[HD / 32];
-    float factor;
+    float factor, rest_factor;
+    uint64_t rest;  // bit 8 j + i: some of dims 32 j + 8 g + i
     __device__ __forceinline__ void load(const float* q, bool there) {
         const uint32_t g = (threadIdx.x & 63u) >> 4;
 #pragma unroll
@@ -130,15 +139,31 @@ struct Query<_Float16, HD> {
 #pragma unroll
             for (int i = 0; i < 2; i++) x[j][i] = there ? *reinterpret_cast<const v4f*>(q + 32 * j + 8u * g + 4 * i) : v4f{0, 0, 0, 0};
     }
-    __device__ __forceinline__ void split(float scale) {
+    __device__ __forceinline__ void split(float scale, float* rest_of) {
         float top = 0.0f;
+        uint32_t least = 0xffffffffu;  // of the magnitudes that are not zero
 #pragma unroll
         for (int j = 0; j < HD / 32; j++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[j][i / 4][i % 4]));
+            for (int i = 0; i < 8; i++) {
+                const float y = x[j][i / 4][i % 4];
+                top = fmaxf(top, fabsf(y)), least = min(least, 2u * __float_as_uint(y) - 1u);
+            }
         top = groups_max(top);
         const int e = max(__builtin_amdgcn_frexp_expf(top), -100) - 15;  // (from 2^-100 down no score matters)
-        factor = ldexpf(scale * kLog2e, e);
+        const float enough = ldexpf(1.0f, e + 15 - kQueryBits);
+        rest_factor = scale * kLog2e, factor = ldexpf(rest_factor, e), rest = 0;
+        if (__any(least < 2u * __float_as_uint(enough) - 1u))
+#pragma unroll
+            for (int j = 0; j < HD / 32; j++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float y = x[j][i / 4][i % 4];
+                    const bool small = fabsf(y) < enough && y != 0.0f;
+                    rest |= (uint64_t)(__any(small) != 0) << (8 * j + i);
+                    rest_of[(8 * j + i) * 64 + (threadIdx.x & 63u)] = small ? y : 0.0f;
+                    x[j][i / 4][i % 4] = small ? 0.0f : y;
+                }
 #pragma unroll
         for (int j = 0; j < HD / 32; j++)
 #pragma unroll
@@ -156,17 +181,32 @@ struct Query<_Float16, HD> {
         }
         return s;
     }
+    __device__ __forceinline__ void add_rest(const typename Tile<_Float16, HD>::kvec (&k)[2][HD / 32], const float* rest_of, float (&sc)[8]) const {
+        v4f s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+        for (int j = 0; j < HD / 32; j++)
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if ((rest >> (8 * j + i) & 1u) != 0) {
+                    const float y = rest_of[(8 * j + i) * 64 + (threadIdx.x & 63u)];
+#pragma unroll
+                    for (int half = 0; half < 2; half++) s[half] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)k[half][j][i], y, s[half], 0, 0, 0);
+                }
+#pragma unroll
+        for (int i = 0; i < 8; i++) sc[i] += s[i / 4][i % 4] * rest_factor;
+    }
 };
 template <int HD>
 struct Query<float, HD> {
     v4f x[HD / 16];
     float factor;
+    static constexpr uint64_t rest = 0;
     __device__ __forceinline__ void load(const float* q, bool there) {
         const uint32_t g = (threadIdx.x & 63u) >> 4;
 #pragma unroll
         for (int j = 0; j < HD / 16; j++) x[j] = there ? *reinterpret_cast<const v4f*>(q + 16 * j + 4u * g) : v4f{0, 0, 0, 0};
     }
-    __device__ __forceinline__ void split(float scale) { factor = scale * kLog2e; }
+    __device__ __forceinline__ void split(float scale, float*) { factor = scale * kLog2e; }
     __device__ __forceinline__ v4f scores(const typename Tile<float, HD>::kvec (&k)[HD / 16]) const {
         v4f s = {0, 0, 0, 0};
 #pragma unroll
@@ -175,6 +215,7 @@ struct Query<float, HD> {
             for (int e = 0; e < 4; e++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[j][e], x[j][e], s, 0, 0, 0);
         return s;
     }
+    __device__ __forceinline__ void add_rest(const typename Tile<float, HD>::kvec (&)[2][HD / 16], const float*, float (&)[8]) const {}
 };
 
 // What a wave has gathered of a piece: per lane its head's maximum (of a power of two), the sum over its own rows, and 4 dimensions of every tile of the values.
@@ -185,7 +226,8 @@ struct State {
     v4f o[T::kPer];
 
     // The value of dimension (x, e) of m index i is x * 16 kVec + kVec i + e.
-    __device__ __forceinline__ void add(const T& t, const float (&s)[8]) {
+    // `least`: no score of a row that is there is below it.
+    __device__ __forceinline__ void add(const T& t, const float (&s)[8], float least) {
         float top = s[0];
 #pragma unroll
         for (int i = 1; i < 8; i++) top = fmaxf(top, s[i]);
@@ -201,37 +243,40 @@ struct State {
         for (int i = 0; i < 8; i++) p[i] = __builtin_amdgcn_exp2f(s[i] - from);
         l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
         if constexpr (T::kF16) {
-            h8 hi, lo;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float y = p[i] * kHalfScale;
-                hi[i] = (_Float16)y, lo[i] = (_Float16)(y - (float)hi[i]);
-            }
+            for (int i = 0; i < 8; i++) p[i] *= kHalfScale;
+            if (!__any(least < m - kWeightBits)) {  // (32 sequences of scores that spread by 2^20 and more take 57.0 us, not 50.4)
+                h8 hi, lo;
 #pragma unroll
-            for (int x = 0; x < T::kLoads; x++) {
-                // (whole vectors first: elements picked from the array itself keep it out of registers)
-                const typename T::vvec r0 = t.v[0][0][x], r1 = t.v[0][1][x], r2 = t.v[0][2][x], r3 = t.v[0][3][x], r4 = t.v[1][0][x], r5 = t.v[1][1][x], r6 = t.v[1][2][x], r7 = t.v[1][3][x];
+                for (int i = 0; i < 8; i++) hi[i] = (_Float16)p[i], lo[i] = (_Float16)(p[i] - (float)hi[i]);
 #pragma unroll
-                for (int e = 0; e < T::kVec; e++) {
-                    const h8 v = {r0[e], r1[e], r2[e], r3[e], r4[e], r5[e], r6[e], r7[e]};
-                    v4f& d = o[x * T::kVec + e];
-                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo, d, 0, 0, 0);
-                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi, d, 0, 0, 0);
+                for (int x = 0; x < T::kLoads; x++) {
+                    // (whole vectors first: elements picked from the array itself keep it out of registers)
+                    const typename T::vvec r0 = t.v[0][0][x], r1 = t.v[0][1][x], r2 = t.v[0][2][x], r3 = t.v[0][3][x], r4 = t.v[1][0][x], r5 = t.v[1][1][x], r6 = t.v[1][2][x], r7 = t.v[1][3][x];
+#pragma unroll
+                    for (int e = 0; e < T::kVec; e++) {
+                        const h8 v = {r0[e], r1[e], r2[e], r3[e], r4[e], r5[e], r6[e], r7[e]};
+                        v4f& d = o[x * T::kVec + e];
+                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo, d, 0, 0, 0);
+                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi, d, 0, 0, 0);
+                    }
                 }
+                return;
             }
-        } else {
-#pragma unroll
-            for (int half = 0; half < 2; half++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int x = 0; x < T::kLoads; x++)
-#pragma unroll
-                        for (int e = 0; e < T::kVec; e++) {
-                            v4f& d = o[x * T::kVec + e];
-                            d = __builtin_amdgcn_mfma_f32_16x16x4f32(t.v[half][i][x][e], p[4 * half + i], d, 0, 0, 0);
-                        }
         }
+#pragma unroll
+        for (int half = 0; half < 2; half++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int x = 0; x < T::kLoads; x++) {
+                    const typename T::vvec r = t.v[half][i][x];
+#pragma unroll
+                    for (int e = 0; e < T::kVec; e++) {
+                        v4f& d = o[x * T::kVec + e];
+                        d = __builtin_amdgcn_mfma_f32_16x16x4f32((float)r[e], p[4 * half + i], d, 0, 0, 0);
+                    }
+                }
     }
 };
 
@@ -283,8 +328,10 @@ __device__ __forceinline__ void clear_values(Tile<KV, HD>& t, uint32_t there) {
 }
 
 // A workgroup's share of all units, or, where the table has room for few rows (SHORT), all rows of one sequence's KV head (and 16 of its query heads): no piece is left.
+// Waves of a SIMD: exactly as many as there are.  (With registers for a third one in mind the compiler loads values behind the first products: 61.0 us, not 59.3.)
+constexpr int waves_of_simd(int hd, int waves) { return waves == 16 ? 4 : hd == 256 ? 1 : 2; }
 template <typename KV, int HD, uint32_t WAVES, bool SHORT>
-__global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : HD == 256 ? 1 : 2) void attention_paged_kernel(PagedAttentionArgs a) {
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(waves_of_simd(HD, WAVES), waves_of_simd(HD, WAVES)))) void attention_paged_kernel(PagedAttentionArgs a) {
     typedef Tile<KV, HD> T;
     constexpr uint32_t kRow = HD + 4, kStep = WAVES * kTileRows;  // floats of a head's values in LDS; rows of all waves
     static_assert(SHORT || kStep == kUnitRows);
@@ -306,30 +353,39 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : HD == 256 ? 1 : 2) vo
         const uint32_t* const table = a.table + (size_t)s * a.max_pages;
         Query<KV, HD> q;
         q.load(a.q + (size_t)s * a.q_stride + (size_t)(h0 + min(l16, h_count - 1u)) * HD, l16 < h_count);
-        q.split(a.scale);
+        float* const rest_of = &values[wave][0][0];  // (its own wave's, until the state goes there)
+        q.split(a.scale, rest_of);
         State<KV, HD> st;
 #pragma unroll
         for (int d = 0; d < T::kPer; d++) st.o[d] = v4f{0, 0, 0, 0};
         const uint32_t last = SHORT ? len : min(len, (chunk + take) * kUnitRows);
-        for (uint32_t first = chunk * kUnitRows + wave * kTileRows; first < last; first += kStep) {
-            T t;
-            const Place p = place(a, table, c, first, len);
-            load_tile(a, p, len, t);
-            float sc[8];
+        const auto walk = [&](auto rest) __attribute__((always_inline)) {  // (a loop for either: a branch inside cost all queries 2 to 9 %, for values were loaded behind products)
+            for (uint32_t first = chunk * kUnitRows + wave * kTileRows; first < last; first += kStep) {
+                T t;
+                const Place p = place(a, table, c, first, len);
+                load_tile(a, p, len, t);
+                float sc[8];
 #pragma unroll
-            for (int half = 0; half < 2; half++) {
-                const v4f x = q.scores(t.k[half]);
+                for (int half = 0; half < 2; half++) {
+                    const v4f x = q.scores(t.k[half]);
 #pragma unroll
-                for (int i = 0; i < 4; i++) sc[4 * half + i] = x[i] * q.factor;
+                    for (int i = 0; i < 4; i++) sc[4 * half + i] = x[i] * q.factor;
+                }
+                if constexpr (decltype(rest)::value) q.add_rest(t.k, rest_of, sc);
+                float least = sc[0];
+#pragma unroll
+                for (int i = 1; i < 8; i++) least = fminf(least, sc[i]);
+                if (first + kTileRows > len || p.there != 3u) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        if (first + 16u * (i / 4) + 4u * g + i % 4 >= len || (p.there >> (i / 4) & 1u) == 0) sc[i] = -__builtin_inff();
+                    clear_values(t, p.there);
+                }
+                st.add(t, sc, least);
             }
-            if (first + kTileRows > len || p.there != 3u) {
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (first + 16u * (i / 4) + 4u * g + i % 4 >= len || (p.there >> (i / 4) & 1u) == 0) sc[i] = -__builtin_inff();
-                clear_values(t, p.there);
-            }
-            st.add(t, sc);
-        }
+        };
+        if (q.rest == 0) walk(std::false_type());
+        else walk(std::bool_constant<T::kF16>());
         // The waves' states, one head after another
         st.l = groups_sum(st.l);
         if (g == 0) tops[wave][l16] = st.m, sums[wave][l16] = st.l;
