@@ -220,7 +220,7 @@ int wick_rocm_kv_pages_free(wick_rocm_ctx *ctx, const wick_rocm_kv_pages *pages,
  * behind the list is the calls' workspace.
  * wick_rocm_kv_pages_reserve: d_counts[s] more rows for every sequence, whose lens grow by them.  New pages are the lowest free ones, for the first sequence
  * first.  A partial last page that is written to and held by others is copied (rows in use, to a page of the sequence's own); of sequences that write
- * to one page which nobody else holds, the first keeps it.  d_start[s]: the first of the new rows, or WICK_ROCM_NO_ROW where there are none.  All or nothing: if the
+ * to one page which nobody else holds, the first keeps it.  The moves are in the sequences' order.  d_start[s]: the first of the new rows, or WICK_ROCM_NO_ROW where there are none.  All or nothing: if the
  * pool (or a sequence's table) has not enough, nothing changes, every d_start is WICK_ROCM_NO_ROW and d_moves[1] says how many pages are wanting (0xffffffff: the
  * table is too short); else d_moves[1] = 0.
  * wick_rocm_kv_pages_compact: with U pages in use, the ones at U and above move to the free ones below, in ascending order, so that the rest of the

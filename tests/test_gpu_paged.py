@@ -809,3 +809,23 @@ def _absolute(pool):
     p.held, p.lens, p.planes = pool.held, pool.lens, pool.planes.copy()
     p.planes[1] = np.abs(p.planes[1])
     return p
+
+
+@pytest.mark.parametrize("seqs,n_pages", [(40, 50), (300, 400), (4096, 8400)])
+def test_moves_of_a_reservation_are_in_the_sequences_order(ops, dev, seqs, n_pages):
+    """Many that write to a few shared pages: the list is the lists' own, move by move, in every run."""
+    rng = np.random.default_rng(seqs)
+    parents = [0, 1, 2] + [int(p) for p in rng.integers(0, 3, seqs - 3)]
+    counts = [int(c) for c in rng.integers(0, 3, seqs)]
+    for _ in range(3):
+        pool = R.Pool(seqs, 4, n_pages, 16, 1, 32, KV_F16, n_planes=1)
+        pool.reserve([20, 7, 33] + [0] * (seqs - 3))
+        pool.fork(parents)
+        d = OnDevice(dev, pool)
+        start, moves = dev(np.zeros(seqs, np.uint32)), dev(np.zeros(kv_pages_moves_words(d.pages), np.uint32))
+        want = pool.reserve(counts)
+        ops.kv_pages_reserve(d.pages, dev(u32(*counts)), start, moves)
+        assert want[2] == 0 and len(want[1]) > seqs // 2
+        assert moves_of(moves) == (want[1], 0)
+        assert np.array_equal(start.download(np.uint32, seqs), u32(*want[0]))
+        d.check(planes=False)

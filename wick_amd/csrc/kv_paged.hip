@@ -137,7 +137,7 @@ struct PagedPlanArgs {
 // Pages for the new rows of every sequence.  A partial last page with c writers and r holders: where c = r the first writer keeps it and r - 1 copy, else all c
 // do.  Who is who is found in LDS, by the page's slot of a hash table twice as large as all sequences, for pages that are shared alone.
 __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(PagedPlanArgs a) {
-    __shared__ uint32_t page_of[kShared], writers[kShared], first_of[kShared], list[kListed], slots[2][kPlanWaves], moved;
+    __shared__ uint32_t page_of[kShared], writers[kShared], first_of[kShared], list[kListed], slots[3][kPlanWaves];
     const uint32_t R = 1u << a.page_shift;
     const uint64_t capacity = (uint64_t)a.max_pages << a.page_shift;
     uint32_t len[kSeqs], count[kSeqs], page[kSeqs], held[kSeqs], need[kSeqs];
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(PagedPla
         held[k] = page[k] < a.n_pages ? a.refs[page[k]] : 0u;
         shared = shared || held[k] > 1u, copies[k] = held[k] > 1u;
     }
-    if (threadIdx.x == 0) moved = 0;
+    uint32_t move = 0, moves = 0;  // this thread's first one, and all: in the sequences' order
     if (__syncthreads_or(shared)) {
         uint32_t size = 64;
         while (size < 2u * a.n_seqs) size *= 2u;
@@ -178,6 +178,10 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(PagedPla
 #pragma unroll
         for (uint32_t k = 0; k < kSeqs; k++)
             if (copies[k]) copies[k] = writers[slot[k]] != held[k] || first_of[slot[k]] != threadIdx.x * kSeqs + k;
+        uint32_t mine = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < kSeqs; k++) mine += copies[k];
+        move = sum_before(mine, slots[2], moves);
     }
     uint32_t mine = 0;
 #pragma unroll
@@ -218,9 +222,8 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(PagedPla
         if (count[k] == 0) continue;
         a.lens[s] = len[k] + count[k];
         if (copies[k]) {
-            const uint32_t m = atomicAdd(&moved, 1u);
             atomicSub(&a.refs[page[k]], 1u);
-            *reinterpret_cast<uint4*>(a.moves + 4u + 4u * m) = make_uint4(page[k], at < kListed ? list[at] : a.list[at], len[k] % R, 0);
+            *reinterpret_cast<uint4*>(a.moves + 4u + 4u * move++) = make_uint4(page[k], at < kListed ? list[at] : a.list[at], len[k] % R, 0);
         }
         at += need[k];
     }
@@ -234,8 +237,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(PagedPla
         const uint32_t to = i < kListed ? list[i] : a.list[i];
         a.table[(size_t)low * a.max_pages + entry[low] + (i - begin[low])] = to, a.refs[to] = 1;
     }
-    __syncthreads();
-    if (threadIdx.x == 0) *reinterpret_cast<uint4*>(a.moves) = make_uint4(moved, 0, 0, 0);
+    if (threadIdx.x == 0) *reinterpret_cast<uint4*>(a.moves) = make_uint4(moves, 0, 0, 0);
 }
 
 // With U pages in use: the i-th page in use at U or above goes to the i-th free one below.
