@@ -164,7 +164,8 @@ int wick_rocm_kv_q4_evict(wick_rocm_ctx *ctx, void *d_k_cache, void *d_v_cache, 
  *   d_lens  [n_seqs]             rows of sequence s
  *   d_refs  [n_pages]            table entries that name the page; 0: it is free
  * An empty pool: entries WICK_ROCM_NO_PAGE, lens and refs 0.  page_rows 16, 32, 64, 128 or 256; n_seqs at most 4096, n_pages 2^24, max_pages * page_rows
- * and n_seqs * max_pages 2^30.  The struct itself is read during the call only.  Calls on one pool follow each other, on one context's stream or ordered by the caller. */
+ * and n_seqs * max_pages 2^30.  The struct itself is read during the call only.  Calls on one pool follow each other, on one context's stream or ordered by the caller.
+ * What a call writes overlaps nothing else that it is given, unless it is said to be in place. */
 enum { WICK_ROCM_KV_F32 = 0, WICK_ROCM_KV_F16 = 1 };
 #define WICK_ROCM_NO_PAGE 0xffffffffu
 #define WICK_ROCM_NO_ROW 0xffffffffu
@@ -201,7 +202,7 @@ int wick_rocm_qk_norm_rope_paged(wick_rocm_ctx *ctx, const wick_rocm_kv_pages *p
  * element is off by at most 2^-22 of itself, a softmax weight too, or by 2^-19 of itself where it is less than 2^-18 of the largest.)  Rows whose entry names no page
  * of the pool count as not there.  A row that is not finite may make outputs that are not finite of the sequences that see it, in the heads that read it, and of no other.
  * The work of all sequences together is split evenly over the GPU, whatever their lengths, and a second launch joins what several workgroups share; a table of few
- * rows (at most 256 to 1024, by head_dim) takes one launch.
+ * rows (at most 256 to 1024, by head_dim) takes one launch.  The output may be in place of the queries, at their stride.
  * d_scratch: wick_rocm_attention_paged_scratch_floats(...) floats (0: not such a shape), contents need not be kept; calls that may run at the same time need one
  * each.  q, pages, output and scratch 16-byte aligned, strides multiples of 4 that cover the heads. */
 size_t wick_rocm_attention_paged_scratch_floats(uint32_t n_seqs, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim);

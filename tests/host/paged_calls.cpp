@@ -110,6 +110,9 @@ int main() {
         {"no refs", kArg, [](Call& a) { a.pages.d_refs = nullptr; }},
         {"table off", kArg, [](Call& a) { a.pages.d_table = off(a.pages.d_table, 2); }},
         {"refs off", kArg, [](Call& a) { a.pages.d_refs = off(a.pages.d_refs, 1); }},
+        {"lens in the table", kArg, [](Call& a) { a.pages.d_lens = a.pages.d_table; }},
+        {"refs in the table", kArg, [](Call& a) { a.pages.d_refs = a.pages.d_table; }},
+        {"refs in the lens", kArg, [](Call& a) { a.pages.d_refs = a.pages.d_lens; }},
         {"pages of 8 rows", kShape, [](Call& a) { a.pages.page_rows = 8; }},
         {"pages of 48 rows", kShape, [](Call& a) { a.pages.page_rows = 48; }},
         {"pages of 512 rows", kShape, [](Call& a) { a.pages.page_rows = 512; }},
@@ -184,6 +187,12 @@ int main() {
         {"heads past 2^32", kShape, [](Call& a) { a.n_heads = 1u << 26; }},
         {"too many rows and heads in all", kShape, [](Call& a) { a.pages.n_seqs = 4096, a.pages.max_pages = 1u << 18, a.n_heads = a.n_kv = 64, a.q_stride = a.out_stride = 4096; }},
         {"too many heads of all sequences", kShape, [](Call& a) { a.pages.n_seqs = 4096, a.n_heads = a.n_kv = 513, a.q_stride = a.out_stride = 513 * 64; }},
+        {"output in place at another stride", kArg, [](Call& a) { a.out = a.q, a.out_stride = 512; }},
+        {"output in the keys", kArg, [](Call& a) { a.out = (float*)a.k_pages; }},
+        {"output in the values", kArg, [](Call& a) { a.out = (float*)a.v_pages; }},
+        {"scratch in the queries", kArg, [](Call& a) { a.scratch = a.q; }},
+        {"scratch in the output", kArg, [](Call& a) { a.scratch = a.out; }},
+        {"scratch in the keys", kArg, [](Call& a) { a.scratch = (float*)a.k_pages; }},
     }));
     const Wrongs counts = with(pool, {
         {"no numbers", kArg, [](Call& a) { a.counts = nullptr; }},
@@ -205,15 +214,22 @@ int main() {
     each("fork", fork, with(counts, {
         {"parents in the lengths", kArg, [](Call& a) { a.counts = a.pages.d_lens; }},
         {"parents in the table", kArg, [](Call& a) { a.counts = a.pages.d_table; }},
+        {"parents in the refs", kArg, [](Call& a) { a.counts = a.pages.d_refs; }},
     }));
     each("free", free_rows, with(counts, {{"rows in the lengths", kArg, [](Call& a) { a.counts = a.pages.d_lens; }}}));
+    each("free", free_rows, {{"rows in the table", kArg, [](Call& a) { a.counts = a.pages.d_table; }}, {"rows in the refs", kArg, [](Call& a) { a.counts = a.pages.d_refs; }}});
     each("reserve", reserve, with(with(with(counts, moves), planes), {
         {"no start", kArg, [](Call& a) { a.start = nullptr; }},
         {"start off", kArg, [](Call& a) { a.start = off(a.start, 1); }},
         {"start in the counts", kArg, [](Call& a) { a.start = a.counts; }},
         {"start in the lengths", kArg, [](Call& a) { a.start = a.pages.d_lens; }},
+        {"start in the table", kArg, [](Call& a) { a.start = a.pages.d_table; }},
+        {"start in the refs", kArg, [](Call& a) { a.start = a.pages.d_refs; }},
+        {"start in the moves", kArg, [](Call& a) { a.start = a.moves; }},
+        {"moves in the refs", kArg, [](Call& a) { a.moves = a.pages.d_refs; }},
     }));
     each("compact", compact, with(moves, planes));
+    each("compact", compact, {{"moves in the table", kArg, [](Call& a) { a.moves = a.pages.d_table; }}, {"moves in the lengths", kArg, [](Call& a) { a.moves = a.pages.d_lens; }}});
     each("copy", copy, with(with(moves, planes), {{"no planes at all", kArg, [](Call& a) { a.no_planes = true; }}}));
     each("sample", sample, {
         {"no logits", kArg, [](Call& a) { a.logits = nullptr; }},
@@ -231,6 +247,12 @@ int main() {
         {"too many tokens", kShape, [](Call& a) { a.tokens = a.logits_stride = (1u << 19) + 1; }},
         {"too many rows", kShape, [](Call& a) { a.rows = 65536; }},
         {"short stride", kShape, [](Call& a) { a.logits_stride = 999; }},
+        {"picks and probabilities in one place", kArg, [](Call& a) { a.prob = (float*)a.token; }},
+        {"picks in the logits", kArg, [](Call& a) { a.token = (uint32_t*)a.logits; }},
+        {"picks in the rules", kArg, [](Call& a) { a.token = (uint32_t*)a.params; }},
+        {"probabilities in the logits", kArg, [](Call& a) { a.prob = (float*)a.logits; }},
+        {"scratch in the logits", kArg, [](Call& a) { a.work = (void*)a.logits; }},
+        {"scratch in the picks", kArg, [](Call& a) { a.work = a.token; }},
     });
     // what may be left out, or is at its limit
     const auto goes = [&](const char* what, int (*call)(wick_rocm_ctx*, const Call&), long launches, const std::function<void(Call&)>& change) {
@@ -249,6 +271,9 @@ int main() {
     goes("rows reserved and copied", reserve, 2, [](Call&) {});
     goes("a short table in one launch", attention, 1, [](Call&) {});
     goes("a long table in two", attention, 2, [](Call& a) { a.pages.max_pages = 1000; });
+    goes("an output in place of the queries", attention, 1, [](Call& a) { a.out = a.q; });
+    goes("one sequence's in place at any stride", attention, 1, [](Call& a) { a.out = a.q, a.out_stride = 512, a.pages.n_seqs = 1; });
+    goes("picks in place of the uniform numbers", sample, 3, [](Call& a) { a.token = (uint32_t*)a.uniform; });
     goes("the largest pool", attention, 2, [](Call& a) { a.pages = {4096, 1u << 18, 1u << 24, 16, a.pages.d_table, a.pages.d_lens, a.pages.d_refs}, a.n_heads = a.n_kv = 1; });
     goes("no rows to pick from", sample, 0, [](Call& a) { a.rows = 0; });
     goes("one row at any stride, no probabilities", sample, 3, [](Call& a) { a.rows = 1, a.logits_stride = 0, a.prob = nullptr; });

@@ -829,3 +829,18 @@ def test_moves_of_a_reservation_are_in_the_sequences_order(ops, dev, seqs, n_pag
         assert moves_of(moves) == (want[1], 0)
         assert np.array_equal(start.download(np.uint32, seqs), u32(*want[0]))
         d.check(planes=False)
+
+
+@pytest.mark.parametrize("dtype", [KV_F32, KV_F16])
+@pytest.mark.parametrize("hd,heads,n_kv,page_rows,lens", ATTENTION[2:20:3])
+@pytest.mark.parametrize("wide", [False, True])
+def test_attention_in_place_of_its_queries(ctx, ops, dev, wide, hd, heads, n_kv, page_rows, lens, dtype):
+    """In one launch, over shares and joined: the same bits as into an array of its own."""
+    pool = filled(len(lens) + hd, lens, page_rows, n_kv, hd, dtype)
+    pool.max_pages += 2048 // page_rows if wide else 0
+    d, q = OnDevice(dev, pool), normal(11, len(lens), heads, hd) * np.float32(1.5)
+    want = attend(ctx, ops, dev, d, q)
+    d_q, width = dev(q), heads * hd
+    scratch = dev(np.full(attention_paged_scratch_floats(len(lens), heads, n_kv, hd), np.nan, np.float32))
+    ops.encode_attention_paged(d.pages, d_q, width, d.plane(0), d.plane(1), dtype, d_q, width, scratch, heads, n_kv, hd)
+    assert np.array_equal(back(d_q, q), want)

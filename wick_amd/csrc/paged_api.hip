@@ -1,5 +1,7 @@
 // C ABI of include/wick_rocm_lfm2.h: KV caches in pages, and sampling.  Host code only.
+#include <algorithm>
 #include <cmath>
+#include <initializer_list>
 
 #include "wick_rocm_ctx.h"
 
@@ -8,6 +10,9 @@ namespace {
 constexpr uint32_t kMaxSeqs = 4096, kMaxPages = 1u << 24, kMaxRows = 1u << 30;
 
 bool misaligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a != 0; }
+
+// An array that a call writes is none of the others (null: not given).
+bool among(const void* p, std::initializer_list<const void*> others) { return p && std::find(others.begin(), others.end(), p) != others.end(); }
 
 // What every call asks of a pool and its table; null: nothing is wrong.
 const char* pool_shape(const wick_rocm_kv_pages& p) {
@@ -31,6 +36,7 @@ int check_pool(wick_rocm_ctx* ctx, const wick_rocm_kv_pages* p) {
     if (!p->d_table || !p->d_lens || !p->d_refs) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages: null table, lens or refs");
     if (misaligned(p->d_table, 4) || misaligned(p->d_lens, 4) || misaligned(p->d_refs, 4))
         return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages: table, lens and refs must be 4-byte aligned");
+    if (among(p->d_table, {p->d_lens, p->d_refs}) || p->d_lens == p->d_refs) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages: table, lens and refs are one array");
     return WICK_ROCM_OK;
 }
 int check_planes(wick_rocm_ctx* ctx, const wick_rocm_kv_pages& p, const wick_rocm_kv_planes& planes) {
@@ -111,6 +117,10 @@ int wick_rocm_attention_decode_paged(wick_rocm_ctx* ctx, const wick_rocm_kv_page
     if (!d_q || !d_k_pages || !d_v_pages || !d_out || !d_scratch) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "attention_paged: null device pointer");
     if (misaligned(d_q, 16) || misaligned(d_k_pages, 16) || misaligned(d_v_pages, 16) || misaligned(d_out, 16) || misaligned(d_scratch, 16))
         return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "attention_paged: q, pages, output and scratch must be 16-byte aligned");
+    if (d_out == d_q && out_stride != q_stride && pages->n_seqs > 1)  // (else a sequence's queries are read before its output is written)
+        return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "attention_paged: an output in place of the queries needs their stride");
+    if (among(d_scratch, {d_q, d_out, d_k_pages, d_v_pages}) || among(d_out, {d_k_pages, d_v_pages}))
+        return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "attention_paged: output and scratch must be arrays of their own");
     const float scale = 1.0f / sqrtf((float)head_dim);  // wick/src/model/lfm2.rs:862
     hipError_t e = launch_attention_paged(*pages, d_q, q_stride, d_k_pages, d_v_pages, kv_dtype == WICK_ROCM_KV_F16, d_out, out_stride, d_scratch, n_heads,
                                           n_kv_heads, head_dim, scale, ctx->launch());
@@ -121,7 +131,7 @@ int wick_rocm_kv_pages_fork(wick_rocm_ctx* ctx, const wick_rocm_kv_pages* pages,
     WR_ENTER(ctx);
     if (int rc = check_pool(ctx, pages)) return rc;
     if (!d_parents || misaligned(d_parents, 4)) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages_fork: the parents must be there and 4-byte aligned");
-    if (d_parents == pages->d_lens || d_parents == pages->d_table) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages_fork: the parents must be an array of their own");
+    if (among(d_parents, {pages->d_table, pages->d_lens, pages->d_refs})) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages_fork: the parents must be an array of their own");
     hipError_t e = launch_kv_pages_fork(*pages, d_parents, ctx->launch());
     return e == hipSuccess ? WICK_ROCM_OK : fail_hip(ctx, e, "kv_pages_fork launch");
 }
@@ -130,7 +140,7 @@ int wick_rocm_kv_pages_free(wick_rocm_ctx* ctx, const wick_rocm_kv_pages* pages,
     WR_ENTER(ctx);
     if (int rc = check_pool(ctx, pages)) return rc;
     if (!d_rows || misaligned(d_rows, 4)) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages_free: the rows must be there and 4-byte aligned");
-    if (d_rows == pages->d_lens) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages_free: the rows are the lengths themselves");
+    if (among(d_rows, {pages->d_table, pages->d_lens, pages->d_refs})) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages_free: the rows must be an array of their own");
     hipError_t e = launch_kv_pages_free(*pages, d_rows, ctx->launch());
     return e == hipSuccess ? WICK_ROCM_OK : fail_hip(ctx, e, "kv_pages_free launch");
 }
@@ -144,7 +154,8 @@ int wick_rocm_kv_pages_reserve(wick_rocm_ctx* ctx, const wick_rocm_kv_pages* pag
     if (!d_counts || !d_start || !d_moves) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages_reserve: null device pointer");
     if (misaligned(d_counts, 4) || misaligned(d_start, 4) || misaligned(d_moves, 16))
         return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages_reserve: counts and start must be 4-byte, moves 16-byte aligned");
-    if (d_start == d_counts || d_start == pages->d_lens) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages_reserve: start must be an array of its own");
+    if (among(d_start, {d_counts, d_moves, pages->d_table, pages->d_lens, pages->d_refs})) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages_reserve: start must be an array of its own");
+    if (among(d_moves, {pages->d_table, pages->d_lens, pages->d_refs})) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages_reserve: the moves must be an array of their own");
     if (planes)
         if (int rc = check_planes(ctx, *pages, *planes)) return rc;
     hipError_t e = launch_kv_pages_reserve(*pages, d_counts, d_start, d_moves, planes, ctx->launch());
@@ -155,6 +166,7 @@ int wick_rocm_kv_pages_compact(wick_rocm_ctx* ctx, const wick_rocm_kv_pages* pag
     WR_ENTER(ctx);
     if (int rc = check_pool(ctx, pages)) return rc;
     if (!d_moves || misaligned(d_moves, 16)) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages_compact: the moves must be there and 16-byte aligned");
+    if (among(d_moves, {pages->d_table, pages->d_lens, pages->d_refs})) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "kv_pages_compact: the moves must be an array of their own");
     if (planes)
         if (int rc = check_planes(ctx, *pages, *planes)) return rc;
     hipError_t e = launch_kv_pages_compact(*pages, d_moves, planes, ctx->launch());
@@ -182,6 +194,8 @@ int wick_rocm_sample(wick_rocm_ctx* ctx, const float* d_logits, uint32_t logits_
     if (!d_logits || !d_params || !d_uniform || !d_out || !d_scratch) return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "sample: null device pointer");
     if (misaligned(d_logits, 4) || misaligned(d_params, 4) || misaligned(d_uniform, 4) || misaligned(d_out, 4) || misaligned(d_prob, 4) || misaligned(d_scratch, 16))
         return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "sample: arrays must be 4-byte, scratch 16-byte aligned");
+    if (among(d_out, {d_logits, d_params, d_prob, d_scratch}) || among(d_prob, {d_logits, d_params, d_scratch}) || among(d_scratch, {d_logits, d_params, d_uniform}))
+        return fail(ctx, WICK_ROCM_ERR_INVALID_ARG, "sample: what is written must be arrays of their own");
     hipError_t e = launch_sample(d_logits, logits_stride, rows, n, d_params, d_uniform, d_out, d_prob, d_scratch, ctx->launch());
     return e == hipSuccess ? WICK_ROCM_OK : fail_hip(ctx, e, "sample launch");
 }
