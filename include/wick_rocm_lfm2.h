@@ -227,8 +227,8 @@ int wick_rocm_kv_pages_free(wick_rocm_ctx *ctx, const wick_rocm_kv_pages *pages,
  * wick_rocm_kv_pages_compact: with U pages in use, the ones at U and above move to the free ones below, in ascending order, so that the rest of the
  * pool is free in one piece; tables and refs follow.  Pages move whole.  d_moves[1] = U.
  * planes: what is copied along (null: the caller does it, with wick_rocm_kv_pages_copy for each group of planes).
- * wick_rocm_kv_pages_copy: the first min(d_moves[0], max_moves) moves in all planes, rows [0, rows) of every head; a move that names no page of the pool is left out.  Pages
- * that are written must be named once. */
+ * wick_rocm_kv_pages_copy: the first min(d_moves[0], max_moves) moves in all planes, rows [0, rows) of every head; a move that names no page of the pool is left out.  Moves
+ * run in no order: a page that one of them writes is named by no other, neither to write nor to read (a chain a -> b, b -> c takes two calls). */
 size_t wick_rocm_kv_pages_moves_words(const wick_rocm_kv_pages *pages);
 int wick_rocm_kv_pages_reserve(wick_rocm_ctx *ctx, const wick_rocm_kv_pages *pages, const uint32_t *d_counts, uint32_t *d_start, uint32_t *d_moves,
                                const wick_rocm_kv_planes *planes);

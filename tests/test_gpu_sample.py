@@ -1,5 +1,7 @@
 """Sampling on the GPU against the rule in f64 (paged_ref.py).  A pick may differ where the uniform number lies within 1e-9 of a border of the mass: masses are
 whole numbers of 2^-43 of the largest token's, up to 2^19 of them each off by half of one."""
+# (That is n 2^-44 of the largest weight for n tokens, at most 2^-25: 1e-9 of the mass bounds up to 17000 tokens whatever their weights.  The longer rows here stay below it because
+# their masses are many times the largest weight, and because rounded weights are off to either side.)
 import numpy as np
 import pytest
 

@@ -19,8 +19,8 @@
 // first and last piece otherwise leave {maximum, sum, values} in the scratch, which a second launch joins.  (Joined by the last workgroup of a head to arrive
 // instead, over device-scope atomics, 128,000 rows took 104 us, not 98.7: what the others wrote has to be read past the caches.)
 //
-// Reading the pages bounds it: every cached element is read once.  32 sequences of up to 8192 rows (8 KV heads of 64, f16: 278 MB) take 53.9 us, 5.2 TB/s,
-// and 4.8 us to join; 64 of up to 2002 rows in f32 (271 MB) 53 us, 5.1 TB/s; one of 128,000 rows (8 KV heads of 128, f16: 524 MB) 91 us, 5.8 TB/s, and 7.4 us
+// Reading the pages bounds it: every cached element is read once.  32 sequences of up to 8192 rows (8 KV heads of 64, f16: 278 MB) take 55 us, 5.0 TB/s,
+// and 4.9 us to join; 64 of up to 2002 rows in f32 (271 MB) 53 us, 5.1 TB/s; one of 128,000 rows (8 KV heads of 128, f16: 524 MB) 92 us, 5.7 TB/s, and 7.6 us
 // to join.  Loads of the next tile ahead of a tile's products (f32: 53 to 56 us) and waves that yield to those with more left (no difference) do not pay:
 // with 8 waves a CU the loads of one fill the products of another.
 #include <algorithm>

@@ -94,7 +94,7 @@ __global__ __launch_bounds__(256) void kv_pages_free_kernel(PagedFreeArgs a) {
 
 // ---- the plan of a reservation or a compaction: one workgroup --------------------------------------
 // A chain of round trips to memory (lengths, the table's entry, its page's count; what is written) and of barriers; refs are read a run of pages a thread, of
-// the first 16384 pages once, at the start.  A row for each of 16 continuations (a shared page copied) takes 9.0 us, 2002 rows for one of 32 sequences 6.5, a compaction
+// the first 16384 pages once, at the start.  A row for each of 16 continuations (a shared page copied) takes 9.2 us, 2002 rows for one of 32 sequences 6.5, a compaction
 // of 8000 pages 4.9.
 constexpr uint32_t kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
 constexpr uint32_t kRun = 16;                    // consecutive pages of a thread at a time
