@@ -327,9 +327,10 @@ __device__ __forceinline__ void clear_values(Tile<KV, HD>& t, uint32_t there) {
                 for (int x = 0; x < Tile<KV, HD>::kLoads; x++) t.v[half][i][x] = typename Tile<KV, HD>::vvec(0);
 }
 
-// A workgroup's share of all units, or, where the table has room for few rows (SHORT), all rows of one sequence's KV head (and 16 of its query heads): no piece is left.
 // Waves of a SIMD: exactly as many as there are.  (With registers for a third one in mind the compiler loads values behind the first products: 61.0 us, not 59.3.)
 constexpr int waves_of_simd(int hd, int waves) { return waves == 16 ? 4 : hd == 256 ? 1 : 2; }
+
+// A workgroup's share of all units, or, where the table has room for few rows (SHORT), all rows of one sequence's KV head (and 16 of its query heads): no piece is left.
 template <typename KV, int HD, uint32_t WAVES, bool SHORT>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(waves_of_simd(HD, WAVES), waves_of_simd(HD, WAVES)))) void attention_paged_kernel(PagedAttentionArgs a) {
     typedef Tile<KV, HD> T;
